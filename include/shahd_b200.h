@@ -302,6 +302,166 @@ int shahd_attention_decode(ShahdAttention* a, const float* q, const float* k, co
                            void* stream);
 const char* shahd_last_error(void);
 
+/* ================================================================================================
+ * 3. Serving operators on caller-owned device buffers: prompts of different lengths in one call, and trees of drafted
+ *    tokens against a paged cache. They fit together as one serving step:
+ *      shahd_rope_apply (q, k turned; k, v into the cache) -> shahd_prompt_attention           for new prompts,
+ *      shahd_rope_apply -> shahd_tree_attention -> (the model's logits) -> shahd_verify_tree
+ *                       -> shahd_rope_apply with positions = commit (accepted rows into the cache) for drafted tokens.
+ *    All pointers in the call structures are device pointers of one device (checked; the current device does not matter
+ *    and is left as it is), the structures themselves lie on the host and are only read during the call. Calls are
+ *    asynchronous on `stream` (0 = the legacy stream), allocate nothing, keep nothing between calls and can be captured
+ *    into CUDA graphs. Sequences are packed: rows offsets[s] .. offsets[s+1]-1 are sequence s (offsets int32 [n+1] on the
+ *    device, ascending, offsets[n] <= rows; empty sequences are allowed). Rows behind the last sequence are neither
+ *    read nor written. Operands and results must not overlap unless a function says so.
+ * ============================================================================================== */
+
+#define SHAHD_BF16 0
+#define SHAHD_F16 1
+#define SHAHD_F32 2
+
+/* Rows of heads: value i of head h of row r is data[r * row_stride + h * head_stride + i] (strides in elements). */
+typedef struct ShahdRows {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} ShahdRows;
+
+/* One layer of a paged K/V cache of 16-bit values in the layout of the FusedAttention operator: page p is
+ * [kv_heads][K|V][64][head_dim] at pool + p * page_stride (elements, a multiple of 8; pool 16-byte aligned), and
+ * block_table[s * max_blocks + b] (int32, device) names the page with positions 64 b .. 64 b + 63 of sequence s. Entries
+ * outside 0 .. pages-1 name no page: nothing is written there and nothing is attended to there. */
+typedef struct ShahdKvCache {
+  void* pool;
+  int64_t page_stride;
+  const int32_t* block_table;
+  int32_t max_blocks;
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t head_dim;
+} ShahdKvCache;
+
+/* The cache of a FusedAttention operator (bf16; sequence s is its slot s), for the operators below. It belongs to `a` and
+ * ends with it. Rows appended through it count for shahd_attention_decode once shahd_attention_set_lengths has
+ * been told so. */
+int shahd_attention_cache(ShahdAttention* a, ShahdKvCache* out);
+/* Sets the cached positions of sequences 0..n-1 (host lengths, 0 .. capacity), in the order of `stream` (0 = the operator's
+ * own stream). */
+int shahd_attention_set_lengths(ShahdAttention* a, const int32_t* lengths, int32_t n, void* stream);
+
+/* ---- rotary positions (ApplyRope, RotaryEmbedding.ts:63-75, with further layouts and scalings) ---- */
+#define SHAHD_ROPE_INTERLEAVED 0 /* pairs (2i, 2i+1), as the session and FusedAttention turn them */
+#define SHAHD_ROPE_HALF 1        /* pairs (i, i + rotary_dim/2) */
+#define SHAHD_ROPE_UNSCALED 0    /* f_i = base^(-2i/rotary_dim) */
+#define SHAHD_ROPE_LINEAR 1      /* f_i / factor (positions interpolated) */
+#define SHAHD_ROPE_STRETCHED 2   /* base * factor^(r/(r-2)) for base: the slowest pair is slowed by factor, the fastest not */
+#define SHAHD_ROPE_BY_PARTS 3    /* pairs that make more than beta_fast turns in original_positions keep f_i, those that make
+                                    fewer than beta_slow get f_i / factor, a linear ramp over the pairs between */
+typedef struct ShahdRopeCfg {
+  int32_t head_dim;           /* 2 .. 256 */
+  int32_t rotary_dim;         /* even, <= head_dim: the first rotary_dim values of a head are turned */
+  int32_t layout;
+  int32_t scaling;
+  int32_t original_positions; /* SHAHD_ROPE_BY_PARTS */
+  int32_t reserved;
+  double base;                /* 10000 in the reference */
+  double factor;              /* >= 1; unused without scaling */
+  double beta_fast, beta_slow; /* SHAHD_ROPE_BY_PARTS, usually 32 and 1 */
+  double magnitude;           /* cos and sin are multiplied by it; 1 for none */
+} ShahdRopeCfg;
+typedef struct ShahdRope ShahdRope;
+/* The frequencies of one configuration, computed in 64 bits on the host; on no device, may be used from any thread. */
+int shahd_rope_create(const ShahdRopeCfg* cfg, ShahdRope** out);
+int shahd_rope_destroy(ShahdRope* rope);
+
+typedef struct ShahdRopeCall {
+  int32_t dtype;      /* of q, k, v and their results: SHAHD_BF16, SHAHD_F16 or SHAHD_F32 */
+  int32_t rows;
+  int32_t num_heads;  /* 0: no queries */
+  int32_t kv_heads;   /* 0: no keys */
+  int32_t n;          /* sequences; 0 without offsets */
+  int32_t reserved;
+  const int32_t* positions; /* [rows]; a row of negative position is left as it is everywhere */
+  const int32_t* offsets;   /* [n+1]; may be null without a cache: then every row counts */
+  ShahdRows q, q_out;       /* [rows, num_heads, head_dim]; q_out may be q */
+  ShahdRows k, k_out;       /* [rows, kv_heads, head_dim]; k_out may be k, or its data null with a cache */
+  ShahdRows v;              /* [rows, kv_heads, head_dim], read when there is a cache */
+  ShahdKvCache cache;       /* pool null: none. The turned k and v go to their row's position; values of dtype, bf16 for
+                               SHAHD_F32. Positions beyond max_blocks * 64 or on no page are not written. Two rows of
+                               one sequence must not have one position. */
+} ShahdRopeCall;
+/* Turns pair (a, b) of each head by position * f_i: (a cos - b sin, a sin + b cos) * magnitude; products in 32 bits, rounded
+ * once. Any strides of at least head_dim and any element alignment (16-byte aligned operands run faster). */
+int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* call, void* stream);
+
+/* ---- causal attention over packed prompts (MultiHeadAttention.ts:46-74 with one length per sequence) ---- */
+typedef struct ShahdPromptCall {
+  int32_t dtype;     /* SHAHD_BF16 or SHAHD_F16 */
+  int32_t rows;
+  int32_t n;
+  int32_t num_heads; /* query head h reads kv head h / (num_heads / kv_heads), at most 8 per kv head */
+  int32_t kv_heads;
+  int32_t head_dim;  /* 32, 64 or 128 */
+  double scale;      /* of the scores; 0: 1/sqrt(head_dim) */
+  const int32_t* offsets;
+  ShahdRows q, k, v, out; /* 16-byte aligned, strides multiples of 8 */
+} ShahdPromptCall;
+/* out[i] = sum over j <= i of softmax_j(scale q[i].k[j]) v[j] within each sequence. Softmax and sums in 32 bits; the
+ * probabilities meet v in dtype. A value of k or v that is not finite can reach every row of its own sequence, the
+ * earlier ones too, but no other sequence. */
+int shahd_prompt_attention(const ShahdPromptCall* call, void* stream);
+
+/* ---- attention of drafted token trees over the cache (verify passes; one node per sequence is a decode step) ---- */
+typedef struct ShahdTreeCall {
+  int32_t dtype;     /* of q, k, v, out and the cache: SHAHD_BF16 or SHAHD_F16 */
+  int32_t rows;
+  int32_t n;
+  int32_t num_heads; /* kv_heads and head_dim (32, 64 or 128) are the cache's; at most 8 query heads per kv head */
+  int32_t max_nodes; /* no sequence has more rows than this, 1 .. 64 (rows beyond it would be left as they are) */
+  int32_t reserved;
+  double scale;      /* 0: 1/sqrt(head_dim) */
+  const int32_t* offsets;
+  const int32_t* lengths;  /* [n] cached positions per sequence (values are cut to 0 .. max_blocks * 64) */
+  const uint64_t* masks;   /* [rows] bit j: the row attends to row j of its sequence (itself included only by its bit) */
+  ShahdRows q, k, v, out;  /* 16-byte aligned, strides multiples of 8; k and v are the nodes' own, not in the cache */
+  ShahdKvCache cache;
+  void* workspace;         /* 16-byte aligned, shahd_tree_attention_workspace bytes; in use until the call has run */
+  int64_t workspace_bytes;
+} ShahdTreeCall;
+/* Bytes of workspace for a call with these n, num_heads, max_nodes and cache sizes (0: none), or a negative status; dtype,
+ * pointers, rows and scale are not looked at. The device is the current one. */
+int64_t shahd_tree_attention_workspace(const ShahdTreeCall* call);
+/* out[i] = sum of softmax(scale q[i].k[j]) v[j] over the cached positions of the row's sequence and the rows of its mask;
+ * a row that attends to nothing gives 0. Positions at or beyond the length are never used, whatever their pages
+ * hold. */
+int shahd_tree_attention(const ShahdTreeCall* call, void* stream);
+
+/* ---- verification of drafted trees (SpeculativeSample, SpeculativeSampling.ts:82-112, for trees and device rows) ---- */
+typedef struct ShahdVerifyCall {
+  int32_t dtype;  /* of target and draft: SHAHD_BF16, SHAHD_F16 or SHAHD_F32 */
+  int32_t rows;
+  int32_t n;
+  int32_t vocab;
+  const void* target;     /* [rows, vocab] probabilities: row i is the target's distribution after node i */
+  const void* draft;      /* [rows, vocab]: the draft's distribution after node i, from which i's children were drawn */
+  int64_t target_stride, draft_stride; /* elements between rows */
+  const int32_t* offsets; /* node 0 of a sequence is its root: the last token already taken */
+  const int32_t* parents; /* [rows] index within the sequence, below the node's own; the root's is not read */
+  const int32_t* tokens;  /* [rows]; the root's is not read */
+  const float* uniforms;  /* [rows] in [0, 1): a node's decides on it, the root's draws the next token */
+  const int32_t* lengths; /* [n] cached positions; may be null without commit and new_lengths */
+  int32_t* path;          /* [rows] out: the taken nodes in order, the root's 0 first, then -1 */
+  int32_t* count;         /* [n] out: taken nodes without the root */
+  int32_t* next_ids;      /* [n] out: the token drawn after the last taken node (-1 for an empty sequence) */
+  int32_t* commit;        /* [rows] out, may be null: lengths[s] + depth for taken nodes, the root too, else -1 */
+  int32_t* new_lengths;   /* [n] out, may be null: lengths[s] + count + 1 (lengths[s] for an empty sequence) */
+} ShahdVerifyCall;
+/* Each child x of the current node, in index order, is taken with probability min(1, p(x)/q(x)); a refusal replaces p by
+ * max(0, p - q) over its sum. The next token is drawn from what p is at the end (the target's row itself when nothing is
+ * left), in index order against the root's number. Values that are not positive numbers count as 0; nodes whose token is
+ * outside the vocabulary or whose parent is not below them are passed over. */
+int shahd_verify_tree(const ShahdVerifyCall* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

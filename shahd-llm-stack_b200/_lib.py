@@ -44,6 +44,56 @@ class ShahdSessionOpts(ctypes.Structure):
     _fields_ = [("max_seqs", _i32), ("kv_pages", _i32), ("device", _i32), ("flags", _i32)]
 
 
+SHAHD_BF16 = 0
+SHAHD_F16 = 1
+SHAHD_F32 = 2
+
+
+class ShahdRows(ctypes.Structure):
+    """Rows of heads in device memory: value i of head h of row r at data[r * row_stride + h * head_stride + i]."""
+
+    _fields_ = [("data", _vp), ("row_stride", _i64), ("head_stride", _i64)]
+
+
+class ShahdKvCache(ctypes.Structure):
+    """One layer of a paged K/V cache: pages [kv_heads][K|V][64][head_dim] of 16-bit values, a block table per sequence."""
+
+    _fields_ = [("pool", _vp), ("page_stride", _i64), ("block_table", _vp), ("max_blocks", _i32), ("pages", _i32),
+                ("kv_heads", _i32), ("head_dim", _i32)]
+
+
+class ShahdRopeCfg(ctypes.Structure):
+    _fields_ = [("head_dim", _i32), ("rotary_dim", _i32), ("layout", _i32), ("scaling", _i32), ("original_positions", _i32),
+                ("reserved", _i32), ("base", ctypes.c_double), ("factor", ctypes.c_double), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class ShahdRopeCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("num_heads", _i32), ("kv_heads", _i32), ("n", _i32), ("reserved", _i32),
+                ("positions", _vp), ("offsets", _vp), ("q", ShahdRows), ("q_out", ShahdRows), ("k", ShahdRows),
+                ("k_out", ShahdRows), ("v", ShahdRows), ("cache", ShahdKvCache)]
+
+
+class ShahdPromptCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("n", _i32), ("num_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("scale", ctypes.c_double), ("offsets", _vp), ("q", ShahdRows), ("k", ShahdRows), ("v", ShahdRows),
+                ("out", ShahdRows)]
+
+
+class ShahdTreeCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("n", _i32), ("num_heads", _i32), ("max_nodes", _i32), ("reserved", _i32),
+                ("scale", ctypes.c_double), ("offsets", _vp), ("lengths", _vp), ("masks", _vp), ("q", ShahdRows),
+                ("k", ShahdRows), ("v", ShahdRows), ("out", ShahdRows), ("cache", ShahdKvCache), ("workspace", _vp),
+                ("workspace_bytes", _i64)]
+
+
+class ShahdVerifyCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("n", _i32), ("vocab", _i32), ("target", _vp), ("draft", _vp),
+                ("target_stride", _i64), ("draft_stride", _i64), ("offsets", _vp), ("parents", _vp), ("tokens", _vp),
+                ("uniforms", _vp), ("lengths", _vp), ("path", _vp), ("count", _vp), ("next_ids", _vp), ("commit", _vp),
+                ("new_lengths", _vp)]
+
+
 # name -> (restype, argtypes); every symbol include/shahd_b200.h declares
 SIGNATURES = {
     "MatMulF64": (None, [_dp, _dp, _dp, _i32, _i32, _i32]),
@@ -97,6 +147,15 @@ SIGNATURES = {
     "shahd_attention_length": (_i32, [_vp, _i32]),
     "shahd_attention_prefill": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp]),
     "shahd_attention_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "shahd_attention_cache": (ctypes.c_int, [_vp, ctypes.POINTER(ShahdKvCache)]),
+    "shahd_attention_set_lengths": (ctypes.c_int, [_vp, _ip, _i32, _vp]),
+    "shahd_rope_create": (ctypes.c_int, [ctypes.POINTER(ShahdRopeCfg), ctypes.POINTER(_vp)]),
+    "shahd_rope_destroy": (ctypes.c_int, [_vp]),
+    "shahd_rope_apply": (ctypes.c_int, [_vp, ctypes.POINTER(ShahdRopeCall), _vp]),
+    "shahd_prompt_attention": (ctypes.c_int, [ctypes.POINTER(ShahdPromptCall), _vp]),
+    "shahd_tree_attention_workspace": (_i64, [ctypes.POINTER(ShahdTreeCall)]),
+    "shahd_tree_attention": (ctypes.c_int, [ctypes.POINTER(ShahdTreeCall), _vp]),
+    "shahd_verify_tree": (ctypes.c_int, [ctypes.POINTER(ShahdVerifyCall), _vp]),
     "shahd_last_error": (ctypes.c_char_p, []),
 }
 

@@ -15,8 +15,10 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
 ]
+# each a translation unit with its own device module; compiled at the same time
+UNITS = ["shahd_b200.cu", "serving_ops.cu"]
 
 
 def _sources() -> list[str]:
@@ -38,7 +40,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         return SO_PATH
     nvcc = os.environ.get("NVCC", "nvcc")
     tmp = SO_PATH + ".tmp"
-    cmd = [nvcc, *NVCC_FLAGS, *(extra or []), "-o", tmp, os.path.join(CSRC, "shahd_b200.cu")]
+    cmd = [nvcc, *NVCC_FLAGS, *(extra or []), "-o", tmp, *(os.path.join(CSRC, u) for u in UNITS)]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)

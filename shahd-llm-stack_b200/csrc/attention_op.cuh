@@ -340,4 +340,44 @@ int shahd_attention_decode(ShahdAttention* a, const float* q, const float* k, co
   return CheckLaunch("shahd_attention_decode");
 }
 
+int shahd_attention_cache(ShahdAttention* a, ShahdKvCache* out) {
+  using namespace shahd;
+  if (!a || !out) {
+    SetError("shahd_attention_cache: null argument");
+    return SHAHD_EINVAL;
+  }
+  *out = ShahdKvCache{a->pool, (int64_t)a->page_elems, a->d_block_table, a->max_blocks, a->max_seqs * a->max_blocks, a->Hk, a->d};
+  return SHAHD_OK;
+}
+
+int shahd_attention_set_lengths(ShahdAttention* a, const int32_t* lengths, int32_t n, void* stream) {
+  using namespace shahd;
+  if (!a || !lengths) {
+    SetError("shahd_attention_set_lengths: null argument");
+    return SHAHD_EINVAL;
+  }
+  if (n < 1 || n > a->max_seqs) {
+    SetError("shahd_attention_set_lengths: need 1 <= n <= %d sequences (got %d)", a->max_seqs, n);
+    return SHAHD_EINVAL;
+  }
+  for (int i = 0; i < n; i++)
+    if (lengths[i] < 0 || lengths[i] > a->C) {
+      SetError("shahd_attention_set_lengths: sequence %d: length %d is not in 0 .. %d", i, lengths[i], a->C);
+      return SHAHD_EINVAL;
+    }
+  std::lock_guard<std::mutex> g(a->mu);
+  SHAHD_CUDA_TRY(cudaSetDevice(a->device));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : a->stream;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  SHAHD_CUDA_TRY(cudaStreamIsCapturing(st, &capturing));
+  if (capturing != cudaStreamCaptureStatusNone) {
+    SetError("shahd_attention_set_lengths: the operator's host lengths cannot be part of a captured graph");
+    return SHAHD_EINVAL;
+  }
+  // from pageable memory: the call returns with the lengths taken over
+  SHAHD_CUDA_TRY(cudaMemcpyAsync(a->d_len, lengths, sizeof(int) * (size_t)n, cudaMemcpyHostToDevice, st));
+  for (int i = 0; i < n; i++) a->h_len[i] = lengths[i];
+  return SHAHD_OK;
+}
+
 }  // extern "C"

@@ -16,6 +16,8 @@
 
 namespace shahd {
 
+int OpsDeviceError();  // the flag of the kernels of serving_ops.cu
+
 int g_umma_min_rows = 17;
 bool g_use_pdl = true;
 int g_decode_chains = 0;  // 0 = automatic
@@ -359,7 +361,7 @@ void ShahdSetPersistentPrefillProjections(int enable) { g_persist_linear = enabl
 int ShahdDeviceErrorFlag(void) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_shahd_device_error, sizeof(int)) != cudaSuccess) return -1;
-  return v;
+  return v != 0 ? v : OpsDeviceError();
 }
 
 int ShahdMatMulNTF32Device(const float* a, const float* bt, float* out, int m, int k, int n, int acc, void* stream) {

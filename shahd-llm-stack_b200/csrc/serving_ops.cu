@@ -1,0 +1,267 @@
+// The second translation unit of libshahd_b200.so: the operators on caller-owned device buffers (section 3 of
+// shahd_b200.h). They share no device state with the session's kernels, so they compile beside them; their kernels record
+// a wait that gave up in a flag of their own, which ShahdDeviceErrorFlag reads too.
+#include <new>
+#include <type_traits>
+
+#include "ops_common.cuh"
+#include "rope.cuh"
+#include "tile_attention.cuh"
+#include "tree_verify.cuh"
+
+namespace shahd {
+
+int OpsDeviceError() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_ops_device_error, sizeof v) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return v;
+}
+
+namespace {
+
+typedef CUresult (*OpsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+OpsEncodeFn OpsEncode() {
+  static const OpsEncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<OpsEncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A map of 16-bit values (x, y, z) with 128-byte swizzle and boxes of 64 x by x bz. Made for every call: it is a
+// computation of the call's own pointers and strides, a fraction of a microsecond.
+bool MakeMap(int dtype, const void* p, uint64_t nx, uint64_t ny, uint64_t nz, int64_t sy, int64_t sz, int by, int bz, CUtensorMap* m) {
+  const OpsEncodeFn enc = OpsEncode();
+  if (!enc) return false;
+  if (ny == 1) sy = (int64_t)nx;  // the stride of a single row or head is free: TMA wants one that it could use
+  if (nz == 1) sz = (int64_t)nx;
+  const cuuint64_t dims[3] = {nx, ny, nz}, strides[2] = {(cuuint64_t)sy * 2, (cuuint64_t)sz * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)by, (cuuint32_t)bz}, step[3] = {1, 1, 1};
+  return enc(m, dtype == SHAHD_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims,
+             strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool CheckHeads(const char* op, int H, int Hk, int d) {
+  if (H >= 1 && Hk >= 1 && H % Hk == 0 && H / Hk <= 8 && H <= (1 << 16) && (d == 32 || d == 64 || d == 128)) return true;
+  SetError("%s: need kv_heads dividing num_heads with at most 8 query heads per kv head and head_dim 32, 64 or 128 (got "
+           "num_heads=%d kv_heads=%d head_dim=%d)", op, H, Hk, d);
+  return false;
+}
+
+bool ScaleOf(const char* op, double scale, int d, float* log2) {
+  if (scale == 0) scale = 1.0 / std::sqrt((double)d);
+  if (!(scale > 0) || !std::isfinite(scale)) {
+    SetError("%s: scale must be positive and finite, or 0 for 1/sqrt(head_dim)", op);
+    return false;
+  }
+  *log2 = (float)(scale * M_LOG2E);
+  return true;
+}
+
+template <int D, bool F16, bool TREE>
+void LaunchTiles(const TaArgs& a, unsigned blocks, cudaStream_t st) {
+  if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, TREE>, TaCfg<D>::kSmem)) return;
+  LaunchPdl(TileAttentionKernel<D, F16, TREE>, dim3(blocks), dim3(kTaThreads), TaCfg<D>::kSmem, st, a);
+  if constexpr (TREE)
+    if (a.nsplit > 1)
+      LaunchPdl(TreeJoinKernel<D, F16>, dim3((unsigned)(((long long)a.rows * a.H + 7) / 8)), dim3(256), 0, st, a);
+}
+
+template <bool TREE>
+void LaunchTiles(int d, int dtype, const TaArgs& a, unsigned blocks, cudaStream_t st) {
+  const bool f16 = dtype == SHAHD_F16;
+  if (d == 32) f16 ? LaunchTiles<32, true, TREE>(a, blocks, st) : LaunchTiles<32, false, TREE>(a, blocks, st);
+  else if (d == 64) f16 ? LaunchTiles<64, true, TREE>(a, blocks, st) : LaunchTiles<64, false, TREE>(a, blocks, st);
+  else f16 ? LaunchTiles<128, true, TREE>(a, blocks, st) : LaunchTiles<128, false, TREE>(a, blocks, st);
+}
+
+bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, const ShahdRows& q, const ShahdRows& k, const ShahdRows& v, TaArgs* a) {
+  if (MakeMap(dtype, q.data, d, H, rows, q.head_stride, q.row_stride, a->G, a->TB, &a->qmap) &&
+      MakeMap(dtype, k.data, d, Hk, rows, k.head_stride, k.row_stride, 1, kOpsPage, &a->kmap) &&
+      MakeMap(dtype, v.data, d, Hk, rows, v.head_stride, v.row_stride, 1, kOpsPage, &a->vmap))
+    return true;
+  SetError("%s: a tensor map of q, k or v could not be made", op);
+  return false;
+}
+
+// Parts that the key blocks of a sequence are cut into: one where the tiles fill the multiprocessors anyway, else as many
+// as fill them once, of two 128-key blocks at least.
+constexpr int kTaSms = 148;  // of a B200: the cut, and so the workspace, does not hang on a device being there
+int TreeParts(int n, int Hk, int pairs, int max_blocks) {
+  const long long tiles = (long long)n * Hk * pairs;
+  const int blocks = (max_blocks + 1) / 2 + 1;
+  return (int)std::max(1LL, std::min<long long>(kTaSms / tiles, blocks / 2));
+}
+
+int64_t TreeBytes(const char* op, const ShahdTreeCall* c, int* pairs, int* parts) {
+  const int H = c->num_heads, Hk = c->cache.kv_heads, d = c->cache.head_dim;
+  if (!CheckHeads(op, H, Hk, d) || !CheckCache(op, c->cache, Hk, d)) return SHAHD_EINVAL;
+  if (c->n < 0 || c->max_nodes < 1 || c->max_nodes > 64) {
+    SetError("%s: need n >= 0 and max_nodes in 1 .. 64 (got n=%d max_nodes=%d)", op, c->n, c->max_nodes);
+    return SHAHD_EINVAL;
+  }
+  const int G = H / Hk, TB = 128 / G;
+  *pairs = CeilDiv(c->max_nodes, 2 * TB);
+  *parts = TreeParts(std::max(c->n, 1), Hk, *pairs, c->cache.max_blocks);
+  if (*parts == 1) return 0;
+  return (int64_t)c->n * Hk * *parts * c->max_nodes * G * (d + 2) * (int64_t)sizeof(float);
+}
+
+}  // namespace
+}  // namespace shahd
+
+extern "C" {
+
+int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
+  using namespace shahd;
+  const char* op = "shahd_prompt_attention";
+  ClearError();
+  if (!c) {
+    SetError("%s: null argument", op);
+    return SHAHD_EINVAL;
+  }
+  const int H = c->num_heads, Hk = c->kv_heads, d = c->head_dim;
+  TaArgs a = {};
+  if (!CheckType(op, c->dtype, false) || !CheckHeads(op, H, Hk, d) || !ScaleOf(op, c->scale, d, &a.scale_log2)) return SHAHD_EINVAL;
+  if (c->n < 0 || c->rows < 0) {
+    SetError("%s: need n, rows >= 0 (got n=%d rows=%d)", op, c->n, c->rows);
+    return SHAHD_EINVAL;
+  }
+  if (!CheckRows(op, "q", c->q, c->rows, H, d, 8) || !CheckRows(op, "k", c->k, c->rows, Hk, d, 8) ||
+      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8))
+    return SHAHD_EINVAL;
+  if (c->n == 0 || c->rows == 0) return SHAHD_OK;
+  a.G = H / Hk;
+  a.TB = 128 / a.G;
+  const long long blocks = ((long long)c->rows / (2 * a.TB) + c->n) * Hk;
+  if (blocks > 0x7fffffffLL) {
+    SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
+    return SHAHD_EINVAL;
+  }
+  BufferCheck b(op);
+  b.Add("offsets", c->offsets, 4);
+  b.Add("q", c->q.data, 16);
+  b.Add("k", c->k.data, 16);
+  b.Add("v", c->v.data, 16);
+  b.Add("out", c->out.data, 16);
+  if (b.rc != SHAHD_OK) return b.rc;
+  const DeviceInfo info = InfoOf(b.device);
+  DeviceScope scope(b.device);
+  if (!info.usable || !scope.ok) {
+    SetError("%s: device %d is not a usable sm_100 device", op, b.device);
+    return SHAHD_ENODEV;
+  }
+  if (!MakeRowMaps(op, c->dtype, d, H, Hk, c->rows, c->q, c->k, c->v, &a)) return SHAHD_ECUDA;
+  a.out = static_cast<uint16_t*>(c->out.data);
+  a.out_row = c->out.row_stride;
+  a.out_head = c->out.head_stride;
+  a.offsets = c->offsets;
+  a.n = c->n;
+  a.rows = c->rows;
+  a.H = H;
+  a.Hk = Hk;
+  a.nsplit = 1;
+  TakeLaunchError(nullptr);
+  LaunchTiles<false>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
+  return LaunchStatus(op);
+}
+
+int64_t shahd_tree_attention_workspace(const ShahdTreeCall* c) {
+  using namespace shahd;
+  const char* op = "shahd_tree_attention_workspace";
+  ClearError();
+  if (!c) {
+    SetError("%s: null argument", op);
+    return SHAHD_EINVAL;
+  }
+  int pairs, parts;
+  return TreeBytes(op, c, &pairs, &parts);
+}
+
+int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
+  using namespace shahd;
+  const char* op = "shahd_tree_attention";
+  ClearError();
+  if (!c) {
+    SetError("%s: null argument", op);
+    return SHAHD_EINVAL;
+  }
+  TaArgs a = {};
+  const int H = c->num_heads, Hk = c->cache.kv_heads, d = c->cache.head_dim;
+  const int64_t bytes = TreeBytes(op, c, &a.pairs, &a.nsplit);
+  if (bytes < 0) return (int)bytes;
+  if (!CheckType(op, c->dtype, false) || !ScaleOf(op, c->scale, d, &a.scale_log2)) return SHAHD_EINVAL;
+  if (c->rows < 0) {
+    SetError("%s: need rows >= 0 (got %d)", op, c->rows);
+    return SHAHD_EINVAL;
+  }
+  if (!CheckRows(op, "q", c->q, c->rows, H, d, 8) || !CheckRows(op, "k", c->k, c->rows, Hk, d, 8) ||
+      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8))
+    return SHAHD_EINVAL;
+  if (c->n == 0 || c->rows == 0) return SHAHD_OK;
+  a.G = H / Hk;
+  a.TB = 128 / a.G;
+  const long long blocks = (long long)c->n * Hk * a.pairs * a.nsplit;
+  if (blocks > 0x7fffffffLL || ((long long)c->rows * H + 7) / 8 > 0x7fffffffLL) {
+    SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
+    return SHAHD_EINVAL;
+  }
+  if (c->workspace_bytes < bytes) {
+    SetError("%s: needs %lld bytes of workspace, got %lld", op, (long long)bytes, (long long)c->workspace_bytes);
+    return SHAHD_EINVAL;
+  }
+  BufferCheck b(op);
+  b.Add("offsets", c->offsets, 4);
+  b.Add("lengths", c->lengths, 4);
+  b.Add("masks", c->masks, 8);
+  b.Add("q", c->q.data, 16);
+  b.Add("k", c->k.data, 16);
+  b.Add("v", c->v.data, 16);
+  b.Add("out", c->out.data, 16);
+  b.Add("cache.pool", c->cache.pool, 16);
+  b.Add("cache.block_table", c->cache.block_table, 4);
+  if (bytes > 0) b.Add("workspace", c->workspace, 16);
+  if (b.rc != SHAHD_OK) return b.rc;
+  const DeviceInfo info = InfoOf(b.device);
+  DeviceScope scope(b.device);
+  if (!info.usable || !scope.ok) {
+    SetError("%s: device %d is not a usable sm_100 device", op, b.device);
+    return SHAHD_ENODEV;
+  }
+  if (!MakeRowMaps(op, c->dtype, d, H, Hk, c->rows, c->q, c->k, c->v, &a)) return SHAHD_ECUDA;
+  if (!MakeMap(c->dtype, c->cache.pool, d, (uint64_t)Hk * 2 * kOpsPage, c->cache.pages, d, c->cache.page_stride, kOpsPage, 1, &a.pool)) {
+    SetError("%s: a tensor map of the cache could not be made", op);
+    return SHAHD_ECUDA;
+  }
+  a.out = static_cast<uint16_t*>(c->out.data);
+  a.out_row = c->out.row_stride;
+  a.out_head = c->out.head_stride;
+  a.offsets = c->offsets;
+  a.n = c->n;
+  a.rows = c->rows;
+  a.H = H;
+  a.Hk = Hk;
+  a.masks = reinterpret_cast<const unsigned long long*>(c->masks);
+  a.lengths = c->lengths;
+  a.table = c->cache.block_table;
+  a.max_blocks = c->cache.max_blocks;
+  a.pages = c->cache.pages;
+  a.max_nodes = c->max_nodes;
+  a.part_o = static_cast<float*>(c->workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)c->n * Hk * a.nsplit * c->max_nodes * a.G * d);
+  TakeLaunchError(nullptr);
+  LaunchTiles<true>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
+  return LaunchStatus(op);
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import _lib
 from .decode import Session
 
 
@@ -236,3 +237,20 @@ def speculative_sample(target: Session, draft: Session, prompts, max_new: int, s
         target.truncate([slots[i] for i in active], keep_t)
         draft.truncate([slots[i] for i in active], keep_d)
     return SpeculativeResult([x[:len(p) + max_new] for x, p in zip(ids, prompts)], calls, proposed_n, accepted_n), rounds
+
+
+def verify_tree(dtype: int, target: int, draft: int, vocab: int, tokens: int, parents: int, uniforms: int, offsets: int, n: int,
+                rows: int, path: int, count: int, next_ids: int, lengths: int = 0, commit: int = 0, new_lengths: int = 0,
+                target_stride: int | None = None, draft_stride: int | None = None, stream: int = 0) -> None:
+    """SpeculativeSample's rule (SpeculativeSampling.ts:82-112) on trees of drafted tokens, decided on the device from
+    probabilities and random numbers that lie there (device addresses; asynchronous on `stream`, 0: the legacy stream).
+
+    Sequence s has nodes offsets[s] .. offsets[s+1]-1; node 0 is its root, the last token taken before. target and draft
+    [rows, vocab] (BF16, F16 or F32) hold each model's distribution after each node; a node's token (int32) was drawn from the
+    draft row of its parent (int32, index within the sequence). uniforms (float32): a node's decides on it, the root's draws the
+    next token. Results, int32: path [rows] the taken nodes, count [n], next_ids [n], and with lengths [n] given commit
+    [rows] (the cache position of each taken node, -1 for others: positions for Rope.apply) and new_lengths [n]."""
+    call = _lib.ShahdVerifyCall(dtype, rows, n, vocab, target, draft, vocab if target_stride is None else target_stride,
+                                vocab if draft_stride is None else draft_stride, offsets, parents, tokens, uniforms, lengths, path,
+                                count, next_ids, commit, new_lengths)
+    _lib.check(_lib.load().shahd_verify_tree(ctypes.byref(call), stream or None))
