@@ -71,7 +71,7 @@ bool ScaleOf(const char* op, double scale, int d, float* log2) {
 template <int D, bool F16, bool TREE>
 void LaunchTiles(const TaArgs& a, unsigned blocks, cudaStream_t st) {
   if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, TREE>, TaCfg<D>::kSmem)) return;
-  LaunchPdl(TileAttentionKernel<D, F16, TREE>, dim3(blocks), dim3(kTaThreads), TaCfg<D>::kSmem, st, a);
+  LaunchPdl(TileAttentionKernel<D, F16, TREE>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
   if constexpr (TREE)
     if (a.nsplit > 1)
       LaunchPdl(TreeJoinKernel<D, F16>, dim3((unsigned)(((long long)a.rows * a.H + 7) / 8)), dim3(256), 0, st, a);
@@ -95,7 +95,7 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
 }
 
 // Parts that the key blocks of a sequence are cut into: one where the tiles fill the multiprocessors anyway, else as many
-// as fill them once, of two 128-key blocks at least.
+// as fill them once, of two blocks of 128 keys at least.
 constexpr int kTaSms = 148;  // of a B200: the cut, and so the workspace, does not hang on a device being there
 int TreeParts(int n, int Hk, int pairs, int max_blocks) {
   const long long tiles = (long long)n * Hk * pairs;

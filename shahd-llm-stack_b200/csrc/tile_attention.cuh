@@ -9,39 +9,64 @@
 // sequence has only one tile of rows (decode steps, small trees), on that tile twice with the key blocks dealt out by turns
 // and one merge at the end, so there is always one tile's softmax under the other's products.
 //
-//   S = Q K^T   tcgen05 M 128, N up to 128 keys, into TMEM (128 columns per tile);
-//   softmax     one thread per row: the row's 128 scores in registers, running maximum and sum in 32 bits; the maximum
+//   S = Q K^T   tcgen05 M 128, N up to a block of 128 (head_dim 128) or 64 keys, into TMEM;
+//   softmax     one thread per row: the row's scores of a block in registers, running maximum and sum in 32 bits; the maximum
 //               moves only when a row's new one is over 8 (in log2) above it, since a probability of up to 2^8 costs
 //               nothing in floating point: then, rarely, the accumulator in TMEM is scaled;
 //   O += P V    P rounded to 16 bits (as every attention on these units) overwrites S in TMEM and is the A operand there; V
 //               is the MN-major B operand; O stays in TMEM until the end.
-// Keys and values come by TMA (128-byte swizzle) through a ring of 128-key units; the cache's pages are boxes of 64 positions.
+// Keys and values come by TMA (128-byte swizzle) through a ring of one block's K or V; the cache's pages are boxes of 64
+// positions.
 // A block that is cut short (a sequence's end, the diagonal) loads only the 64-row boxes and multiplies only the 16-key
 // steps that hold keys; rows of V behind a sequence's end are zeroed in shared memory, since 0 * inf would not be 0.
 //
-// Warps 0-3 and 4-7: the softmax of tile 0 and 1; warp 8: MMA issue; warp 9: loads.
+// Warps 0-3 and 4-7: the softmax of tile 0 and 1; warp 8: MMA issue; warp 9: loads; at head_dim 128, warps 10 and 11 only complete
+// the third warpgroup, which gives registers to the other two.
 #pragma once
+
+#ifndef TA_POLY128
+#define TA_POLY128 4
+#endif
+#ifndef TA_POLY64
+#define TA_POLY64 2
+#endif
 
 #include "ops_common.cuh"
 #include "rope.cuh"
 
 namespace shahd {
 
-constexpr int kTaThreads = 320;
-constexpr int kTaBox = 8192;   // 64 rows of 64 values
-constexpr int kTaHalf = 16384;  // 128 rows of 64 values
-constexpr float kTaLazy = 8.f;  // log2 of what a probability may grow to before the accumulator is scaled
+constexpr int kTaBox = 8192;    // 64 rows of 64 values
+constexpr int kTaQHalf = 16384;  // 128 rows of 64 values
+constexpr float kTaLazy = 8.f;   // log2 of what a probability may grow to before the accumulator is scaled
 
+// head_dim 128: blocks of 128 keys, and one block of threads per multiprocessor, whose TMEM it fills: S 2 x 128 columns (P over
+// S), O 2 x 128. Its products and its exponentials take about the same 2048 clocks per step of two tiles.
+// head_dim 64 and 32: products take half of that or less, so the steps are a chain of latencies around the exponentials.
+// Blocks of 64 keys (S 2 x 64 columns, O 2 x 64) let two blocks of threads share a multiprocessor, four softmax warps to a
+// scheduler instead of two (8192 tokens, 16 heads of 64: 218 us -> 196 us; 2048 tokens, 64 heads: 74 -> 60).
 template <int D>
 struct TaCfg {
-  static constexpr int kHalves = D == 128 ? 2 : 1;  // 64-value columns of a row (head_dim 32: half of one, the rest zero)
-  static constexpr int kUnit = kTaHalf * kHalves;   // 128 rows: a Q tile, or a block's K or V
-  static constexpr int kUnits = D == 128 ? 5 : 10;  // ring depth
-  static constexpr int kSmem = 1024 + (2 + kUnits) * kUnit + 512;
+  static constexpr bool kWide = D == 128;
+  static constexpr int kKeys = kWide ? 128 : 64;
+  static constexpr int kPerSm = kWide ? 1 : 2;
+  static constexpr int kThreads = kWide ? 384 : 320;
+  static constexpr int kHalves = kWide ? 2 : 1;        // 64-value columns of a row (head_dim 32: half of one, the rest zero)
+  static constexpr int kQTile = kTaQHalf * kHalves;
+  static constexpr int kHalf = kKeys * 128;            // a block's K or V: kHalves of these
+  static constexpr int kUnit = kHalf * kHalves;
+  static constexpr int kUnits = kWide ? 5 : 8;         // ring depth
+  static constexpr int kSmem = 1024 + 2 * kQTile + kUnits * kUnit + 512;
+  static constexpr uint32_t kCols = kWide ? 512 : 256, kO = 2 * kKeys, kOStep = kWide ? 128 : 64;
+  // of 16 pairs of probabilities, those that Exp2Poly takes
+  static constexpr int kPoly = kWide ? TA_POLY128 : TA_POLY64;
 };
+// Registers at head_dim 128: launched with 168 per thread (384 x 168 = 64512). The two softmax warpgroups take 216 each, the third
+// one, whose warps issue copies and products, keeps 72: 2 x 128 x 216 + 128 x 72 = 64512.
+constexpr int kTaRegsSoftmax = 216, kTaRegsIssue = 72;
 
 struct TaShared {
-  uint64_t full[10], empty[10], q_full, s_full[2], p_full[2], o_full[2], drained;
+  uint64_t full[8], empty[8], q_full, s_full[2], p_half[2], p_full[2], o_full[2], drained;
   uint32_t tmem;
   volatile int abort;
 };
@@ -72,16 +97,34 @@ __device__ __forceinline__ void TmaLoad3D(void* dst, const CUtensorMap* map, uin
       : "memory");
 }
 
-// D[tmem] (+)= A[tmem] B[smem], kind::f16, issued by one thread.
-__device__ __forceinline__ void UmmaTmemA(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Products and commits that a whole warp runs through and one elected lane issues. The warp's control flow and operands are
+// kept uniform (Uniform(), votes on waits), so that descriptors stay in uniform registers: from ordinary ones each
+// product took 67 cycles to issue in a loop, and 100 to 200 between the softmax warps' instructions.
+// D[tmem] (+)= A[smem] B[smem], kind::f16.
+__device__ __forceinline__ void UmmaIssueSS(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[tmem] B[smem], kind::f16.
+__device__ __forceinline__ void UmmaIssueTS(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void UmmaIssueCommit(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(SmemAddr(bar))
+      : "memory");
+}
+__device__ __forceinline__ int Uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// 16 / 32 consecutive columns per thread to TMEM.
+// 16 consecutive columns per thread to TMEM.
 __device__ __forceinline__ void TmemStore16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -89,22 +132,64 @@ __device__ __forceinline__ void TmemStore16(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void TmemStore32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void TmemWaitSt() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void RegsUp() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void RegsDown() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two floats in a register pair: one instruction for both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 Two(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void Split(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 Fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 Add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 __device__ __forceinline__ float Exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x of two values on the FMA units, for a part of the probabilities: the unit that Exp2 runs on gives 16 results a clock, and
+// a 128 x 128 block of scores wants 16384 of them next to products of 1024 (head_dim 128) or 512 clocks. x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 leaves n in the low bits), 2^f by the degree-4 polynomial of least greatest relative
+// error on [-1/2, 1/2] (Remez exchange; 2.7e-6 in 32 bits, a thousandth of a bf16 rounding), n added to the exponent.
+// x is cut at -126: what is smaller becomes 2^-126, nothing next to a sum that holds at least one 2^-8.
+__device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
+  const f32x2 magic = Two(12582912.f, 12582912.f), x = Two(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 r = Add2(x, magic);
+  const f32x2 f = Add2(x, Fma2(r, Two(-1.f, -1.f), magic));
+  f32x2 p = Fma2(Two(0.009570102207362652f, 0.009570102207362652f), f, Two(0.05591785907745361f, 0.05591785907745361f));
+  p = Fma2(p, f, Two(0.240247443318367f, 0.240247443318367f));
+  p = Fma2(p, f, Two(0.6931217908859253f, 0.6931217908859253f));
+  p = Fma2(p, f, Two(0.9999992847442627f, 0.9999992847442627f));
+  float p0, p1, r0, r1;
+  Split(p, p0, p1);
+  Split(r, r0, r1);
+  return Two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23)));
 }
 
 template <bool F16>
@@ -115,11 +200,24 @@ __device__ __forceinline__ uint32_t Pack2(float a, float b) {  // a in the low h
   return r;
 }
 
-// A wait that ends: false once it, or another warp's, has given up.
+// A wait that ends: false once it, or another warp's, has given up. (Not unrolled: copies of the loop at every wait made the
+// kernel larger than the instruction cache, and the warp that issues the products as slow as its fetches.)
 __device__ __forceinline__ bool TaWait(TaShared* sh, uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
   for (uint32_t i = 0; i < kOpsWaitLimit; i++) {
     if (MbarTryWait(bar, parity)) return true;
     if (sh->abort) return false;
+  }
+  atomicCAS(&g_ops_device_error, 0, kOpsErrTimeout);
+  sh->abort = 1;
+  return false;
+}
+// The same for a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool TaWaitWarp(TaShared* sh, uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kOpsWaitLimit; i++) {
+    if (__all_sync(0xffffffffu, MbarTryWait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, sh->abort)) return false;
   }
   atomicCAS(&g_ops_device_error, 0, kOpsErrTimeout);
   sh->abort = 1;
@@ -131,17 +229,20 @@ struct TaWork {
   int seq, start;       // sequence and its first row
   int head;             // kv head
   int q0;               // first token of tile 0 within the sequence
-  int tokens[2];        // of the tiles
-  int blocks[2];        // key blocks of the tiles
+  int tokens0, tokens1;  // of the tiles
+  int blocks0, blocks1;  // key blocks of the tiles
   bool turns;           // one tile of rows, its key blocks dealt out by turns
   int first;            // trees: first key block
   int cached;           // trees: cached positions
-  int cache_blocks;     // trees: 128-key blocks of the cache
+  int cache_blocks;     // trees: key blocks of the cache
   int nodes;            // trees: rows of the sequence; prompts: tokens of the sequence
+  __device__ __forceinline__ int Tokens(int i) const { return i ? tokens1 : tokens0; }
+  __device__ __forceinline__ int Blocks(int i) const { return i ? blocks1 : blocks0; }
 };
 
 // The prompt tile `tile` of all: sequence s owns tiles offsets[s] / (2 TB) + s .. offsets[s+1] / (2 TB) + s, at least as many
 // as it needs, so the mapping is a search in the offsets and needs no table. Each warp finds the same.
+template <int KEYS>
 __device__ __forceinline__ bool PromptWork(const TaArgs& A, int tile, TaWork& w) {
   const int lane = threadIdx.x & 31, span = 2 * A.TB;
   const auto off = [&](int s) { return min(max(A.offsets[s], 0), A.rows); };
@@ -161,15 +262,16 @@ __device__ __forceinline__ bool PromptWork(const TaArgs& A, int tile, TaWork& w)
   w.nodes = len;
   w.q0 = local * span;
   if (local < 0 || w.q0 >= len) return false;
-  for (int i = 0; i < 2; i++) {
-    w.tokens[i] = min(max(len - w.q0 - i * A.TB, 0), A.TB);
-    w.blocks[i] = w.tokens[i] > 0 ? (w.q0 + i * A.TB + w.tokens[i] + 127) / 128 : 0;
-  }
+  w.tokens0 = min(len - w.q0, A.TB);
+  w.tokens1 = min(max(len - w.q0 - A.TB, 0), A.TB);
+  w.blocks0 = (w.q0 + w.tokens0 + KEYS - 1) / KEYS;
+  w.blocks1 = w.tokens1 > 0 ? (w.q0 + A.TB + w.tokens1 + KEYS - 1) / KEYS : 0;
   w.turns = false;
   w.first = w.cached = w.cache_blocks = 0;
   return true;
 }
 
+template <int KEYS>
 __device__ __forceinline__ bool TreeWork(const TaArgs& A, int x, TaWork& w) {
   const int split = x % A.nsplit;
   x /= A.nsplit;
@@ -181,63 +283,76 @@ __device__ __forceinline__ bool TreeWork(const TaArgs& A, int x, TaWork& w) {
   const int end = min(max(A.offsets[w.seq + 1], w.start), A.rows);
   w.nodes = min(end - w.start, A.max_nodes);
   w.q0 = pair * 2 * A.TB;
-  for (int i = 0; i < 2; i++) w.tokens[i] = min(max(w.nodes - w.q0 - i * A.TB, 0), A.TB);
-  if (w.tokens[0] == 0) return false;
+  w.tokens0 = min(max(w.nodes - w.q0, 0), A.TB);
+  w.tokens1 = min(max(w.nodes - w.q0 - A.TB, 0), A.TB);
+  if (w.tokens0 == 0) return false;
   w.cached = (int)min((long long)max(A.lengths[w.seq], 0), (long long)A.max_blocks * kOpsPage);
-  w.cache_blocks = (w.cached + 127) / 128;
+  w.cache_blocks = (w.cached + KEYS - 1) / KEYS;
   const int all = w.cache_blocks + 1;
   w.first = (int)((long long)all * split / A.nsplit);
   const int count = (int)((long long)all * (split + 1) / A.nsplit) - w.first;
-  w.turns = w.tokens[1] == 0;
+  w.turns = w.tokens1 == 0;
   if (w.turns) {
-    w.tokens[1] = w.tokens[0];
-    w.blocks[0] = (count + 1) / 2;
-    w.blocks[1] = count / 2;
+    w.tokens1 = w.tokens0;
+    w.blocks0 = (count + 1) / 2;
+    w.blocks1 = count / 2;
   } else {
-    w.blocks[0] = w.blocks[1] = count;
+    w.blocks0 = w.blocks1 = count;
   }
   return true;
 }
 
-template <bool TREE>
+template <int KEYS, bool TREE>
 struct TaBlocks {
   const TaArgs& A;
   const TaWork& w;
   // The key block of step t of tile i.
   __device__ __forceinline__ int Index(int i, int t) const { return TREE ? (w.turns ? w.first + 2 * t + i : w.first + t) : t; }
-  // Keys of a block that belong to the sequence (1 .. 128).
+  // Keys of a block that belong to the sequence (1 .. KEYS).
   __device__ __forceinline__ int Keys(int b) const {
-    if constexpr (TREE) return b < w.cache_blocks ? min(128, w.cached - 128 * b) : w.nodes;
-    else return min(128, w.nodes - 128 * b);
+    if constexpr (TREE) return b < w.cache_blocks ? min(KEYS, w.cached - KEYS * b) : w.nodes;
+    else return min(KEYS, w.nodes - KEYS * b);
   }
   // Keys of a block that some row of tile i may see.
   __device__ __forceinline__ int Seen(int i, int b) const {
     if constexpr (TREE) return Keys(b);
-    else return min(128, w.q0 + i * A.TB + w.tokens[i] - 128 * b);
+    else return min(KEYS, w.q0 + i * A.TB + w.Tokens(i) - KEYS * b);
   }
 };
 
 template <int D, bool F16, bool TREE>
-__global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __grid_constant__ TaArgs A) {
+__global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAttentionKernel(const __grid_constant__ TaArgs A) {
   using Cfg = TaCfg<D>;
-  constexpr int U = Cfg::kUnits;
+  constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
   extern __shared__ uint8_t ta_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = base;
-  uint8_t* ring = base + 2 * Cfg::kUnit;
+  uint8_t* ring = base + 2 * Cfg::kQTile;
   TaShared* sh = reinterpret_cast<TaShared*>(ring + U * Cfg::kUnit);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   GridDepWait();
   TaWork w;
   if constexpr (TREE) {
-    if (!TreeWork(A, blockIdx.x, w)) return;
+    if (!TreeWork<KEYS>(A, blockIdx.x, w)) return;
   } else {
     // the last tiles of a sequence are the longest: they start first
     const int x = gridDim.x - 1 - blockIdx.x;
     w.head = x % A.Hk;
-    if (!PromptWork(A, x / A.Hk, w)) return;
+    if (!PromptWork<KEYS>(A, x / A.Hk, w)) return;
   }
-  const TaBlocks<TREE> blk{A, w};
+  w.seq = Uniform(w.seq);
+  w.start = Uniform(w.start);
+  w.q0 = Uniform(w.q0);
+  w.tokens0 = Uniform(w.tokens0);
+  w.tokens1 = Uniform(w.tokens1);
+  w.blocks0 = Uniform(w.blocks0);
+  w.blocks1 = Uniform(w.blocks1);
+  w.nodes = Uniform(w.nodes);
+  w.turns = TREE && Uniform(w.turns) != 0;
+  w.first = Uniform(w.first);
+  w.cached = Uniform(w.cached);
+  w.cache_blocks = Uniform(w.cache_blocks);
+  const TaBlocks<KEYS, TREE> blk{A, w};
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < U; s++) {
@@ -247,6 +362,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
     MbarInit(&sh->q_full, 1);
     for (int i = 0; i < 2; i++) {
       MbarInit(&sh->s_full[i], 1);
+      MbarInit(&sh->p_half[i], 128);
       MbarInit(&sh->p_full[i], 128);
       MbarInit(&sh->o_full[i], 1);
     }
@@ -255,233 +371,273 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
     FenceMbarInit();
   }
   if (warp == 8) {
-    TmemAlloc(&sh->tmem, 512);
+    TmemAlloc(&sh->tmem, Cfg::kCols);
     TmemRelinquish();
   }
   TcgenFenceBefore();
   __syncthreads();
   TcgenFenceAfter();
-  const uint32_t tmem = sh->tmem;
+  const uint32_t tmem = (uint32_t)Uniform((int)sh->tmem);
   GridDepLaunch();  // after this block holds its TMEM
-  const int steps = max(w.blocks[0], w.blocks[1]);
+  const int steps = max(w.blocks0, w.blocks1);
 
-  if (warp == 9) {
-    if (lane == 0) {
-      FenceProxyAsyncGlobal();
-      const int tiles = !w.turns && w.tokens[1] > 0 ? 2 : 1;
-      MbarArriveExpectTx(&sh->q_full, tiles * Cfg::kHalves * A.G * A.TB * 128);
-      for (int i = 0; i < tiles; i++)
-        for (int h = 0; h < Cfg::kHalves; h++)
-          TmaLoad3D(sQ + i * Cfg::kUnit + h * kTaHalf, &A.qmap, &sh->q_full, 64 * h, w.head * A.G, w.start + w.q0 + i * A.TB);
-      int u = 0;
-      // one block's K or V into the next unit of the ring
-      const auto load = [&](int b, int keys, bool value) -> bool {
-        const int st = u % U;
-        if (u >= U && !TaWait(sh, &sh->empty[st], (uint32_t)((u / U - 1) & 1))) return false;
-        uint8_t* dst = ring + st * Cfg::kUnit;
-        const int boxes = keys > 64 ? 2 : 1;
-        MbarArriveExpectTx(&sh->full[st], boxes * Cfg::kHalves * kTaBox);
-        for (int x = 0; x < boxes; x++) {
-          if (TREE && b < w.cache_blocks) {
-            const int p = 2 * b + x;
-            int page = p < A.max_blocks ? A.table[(long long)w.seq * A.max_blocks + p] : -1;
-            if (page < 0 || page >= A.pages) page = A.pages;  // behind the pool: TMA fills zeros, and the keys are masked
-            for (int h = 0; h < Cfg::kHalves; h++)
-              TmaLoad3D(dst + h * kTaHalf + x * kTaBox, &A.pool, &sh->full[st], 64 * h, (w.head * 2 + (value ? 1 : 0)) * kOpsPage, page);
-          } else {
-            const int row = w.start + (TREE ? 0 : 128 * b) + 64 * x;
-            for (int h = 0; h < Cfg::kHalves; h++)
-              TmaLoad3D(dst + h * kTaHalf + x * kTaBox, value ? &A.vmap : &A.kmap, &sh->full[st], 64 * h, w.head, row);
+  if (warp >= 8) {
+    if constexpr (Cfg::kWide) RegsDown<kTaRegsIssue>();
+    if (warp == 9) {
+      if (lane == 0) {
+        FenceProxyAsyncGlobal();
+        const int tiles = !w.turns && w.tokens1 > 0 ? 2 : 1;
+        MbarArriveExpectTx(&sh->q_full, tiles * Cfg::kHalves * A.G * A.TB * 128);
+        for (int i = 0; i < tiles; i++)
+          for (int h = 0; h < Cfg::kHalves; h++)
+            TmaLoad3D(sQ + i * Cfg::kQTile + h * kTaQHalf, &A.qmap, &sh->q_full, 64 * h, w.head * A.G, w.start + w.q0 + i * A.TB);
+        int st = 0, issued = 0;
+        uint32_t round = 0;  // times the ring has been gone through
+        // one block's K or V into the next unit of the ring
+        const auto load = [&](int b, int keys, bool value) -> bool {
+          if (round > 0 && !TaWait(sh, &sh->empty[st], (round - 1) & 1)) return false;
+          uint8_t* dst = ring + st * Cfg::kUnit;
+          const int boxes = keys > 64 ? 2 : 1;
+          MbarArriveExpectTx(&sh->full[st], boxes * Cfg::kHalves * kTaBox);
+#pragma unroll 1
+          for (int x = 0; x < boxes; x++) {
+            if (TREE && b < w.cache_blocks) {
+              const int p = b * (KEYS / 64) + x;
+              int page = p < A.max_blocks ? A.table[(long long)w.seq * A.max_blocks + p] : -1;
+              if (page < 0 || page >= A.pages) page = A.pages;  // behind the pool: TMA fills zeros, and the keys are masked
+              for (int h = 0; h < Cfg::kHalves; h++)
+                TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, &A.pool, &sh->full[st], 64 * h, (w.head * 2 + (value ? 1 : 0)) * kOpsPage, page);
+            } else {
+              const int row = w.start + (TREE ? 0 : KEYS * b) + 64 * x;
+              for (int h = 0; h < Cfg::kHalves; h++)
+                TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, value ? &A.vmap : &A.kmap, &sh->full[st], 64 * h, w.head, row);
+            }
+          }
+          issued++;
+          if (++st == U) {
+            st = 0;
+            round++;
+          }
+          return true;
+        };
+        // the order in which the MMA warp takes them: K of the first blocks, then by steps V of this and K of the next one
+        bool ok = true;
+        if (w.turns) {
+          const auto one = [&](int i, int t, bool value) {
+            if (ok && t < w.Blocks(i)) ok = load(blk.Index(i, t), blk.Keys(blk.Index(i, t)), value);
+          };
+          one(0, 0, false);
+          one(1, 0, false);
+#pragma unroll 1
+          for (int t = 0; t < steps && ok; t++) {
+            one(0, t, true);
+            one(0, t + 1, false);
+            one(1, t, true);
+            one(1, t + 1, false);
+          }
+        } else {
+          const int last = w.tokens1 > 0 ? 1 : 0;  // of the two tiles it sees most
+          const auto one = [&](int t, bool value) {
+            if (ok && t < steps) ok = load(blk.Index(0, t), blk.Seen(last, blk.Index(0, t)), value);
+          };
+          one(0, false);
+#pragma unroll 1
+          for (int t = 0; t < steps && ok; t++) {
+            one(t, true);
+            one(t + 1, false);
           }
         }
-        u++;
-        return true;
-      };
-      // the order in which the MMA warp comes to need them
+        // every copy lands before the block may leave: the last phase of each unit's barrier
+        MbarWaitBounded(&sh->q_full, 0, kOpsWaitLimit);
+        for (int v = max(0, issued - U); v < issued; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
+      }
+    } else if (warp == 8) {
+      // The whole warp follows the same path, one lane of it issues.
+      constexpr uint32_t kTypes = F16 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t idesc0 = (1u << 4) | kTypes | ((128u >> 4) << 24);
+      constexpr uint32_t idesc_pv = idesc0 | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // V is MN-major
+      constexpr int kFull16 = KEYS / 16;
+      int st = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      if (w.turns) {
-        for (int i = 0; i < 2 && ok; i++)
-          if (w.blocks[i] > 0) ok = load(blk.Index(i, 0), blk.Keys(blk.Index(i, 0)), false);
-        for (int t = 0; t < steps && ok; t++)
-          for (int i = 0; i < 2 && ok; i++) {
-            if (t < w.blocks[i]) ok = load(blk.Index(i, t), blk.Keys(blk.Index(i, t)), true);
-            if (ok && t + 1 < w.blocks[i]) ok = load(blk.Index(i, t + 1), blk.Keys(blk.Index(i, t + 1)), false);
-          }
-      } else {
-        const int last = w.tokens[1] > 0 ? 1 : 0;  // of the two tiles it sees most
-        const auto keys = [&](int t) { return blk.Seen(last, blk.Index(last, t)); };
-        if (steps > 0) ok = load(blk.Index(0, 0), keys(0), false);
-        for (int t = 0; t < steps && ok; t++) {
-          ok = load(blk.Index(0, t), keys(t), true);
-          if (ok && t + 1 < steps) ok = load(blk.Index(0, t + 1), keys(t + 1), false);
+      const auto acquire = [&]() -> int {
+        const int at = st;
+        ok = ok && TaWaitWarp(sh, &sh->full[at], phase);
+        if (++st == U) {
+          st = 0;
+          phase ^= 1;
         }
-      }
-      // every copy lands before the block may leave
-      MbarWaitBounded(&sh->q_full, 0, kOpsWaitLimit);
-      for (int v = max(0, u - U); v < u; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
-    }
-  } else if (warp == 8) {
-    // The whole warp follows the same path, lane 0 issues.
-    constexpr uint32_t kTypes = F16 ? 0u : (1u << 7) | (1u << 10);
-    const uint32_t idesc0 = (1u << 4) | kTypes | ((128u >> 4) << 24);
-    const uint32_t idesc_pv = idesc0 | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // V is MN-major
-    int u = 0;
-    bool ok = true;
-    const auto acquire = [&]() -> int {
-      const int st = u % U;
-      ok = ok && TaWait(sh, &sh->full[st], (uint32_t)((u / U) & 1));
-      u++;
-      return st;
-    };
-    const auto scores = [&](int i, int t, int st) {
-      const int kc = (blk.Seen(i, blk.Index(i, t)) + 15) & ~15;
-      if (lane == 0) {
-        TcgenFenceAfter();
+        return at;
+      };
+      const auto wait = [&](uint64_t* bar, int t) { ok = ok && TaWaitWarp(sh, bar, (uint32_t)(t & 1)); };
+      const uint64_t qdesc = SmemDescSw128(SmemAddr(sQ)), kdesc = SmemDescSw128(SmemAddr(ring));
+      // MN-major, 128-byte swizzle: 64-value columns kHalf apart, groups of 8 keys 1024 bytes apart
+      const uint64_t vdesc = (uint64_t)((SmemAddr(ring) & 0x3FFFF) >> 4) | (uint64_t)(Cfg::kHalf >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+                             (uint64_t)1 << 46 | (uint64_t)2 << 61;
+      const auto scores = [&](int i, int t, int unit) {
+        const int kc = (blk.Seen(i, blk.Index(i, t)) + 15) & ~15;
+        const uint64_t a = qdesc + (uint64_t)((w.turns ? 0 : i) * (Cfg::kQTile >> 4)), b = kdesc + (uint64_t)(unit * (Cfg::kUnit >> 4));
         const uint32_t idesc = idesc0 | ((uint32_t)(kc >> 3) << 17);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-          const uint64_t a = SmemDescSw128(SmemAddr(sQ + (w.turns ? 0 : i) * Cfg::kUnit + (kk / 4) * kTaHalf)) + (uint64_t)(2 * (kk % 4));
-          const uint64_t b = SmemDescSw128(SmemAddr(ring + st * Cfg::kUnit + (kk / 4) * kTaHalf)) + (uint64_t)(2 * (kk % 4));
-          UmmaBf16(tmem + 128u * i, a, b, idesc, kk > 0 ? 1u : 0u);
-        }
-        UmmaCommit(&sh->s_full[i]);
-      }
-    };
-    const auto values = [&](int i, int t, int st) {
-      const int steps16 = (blk.Seen(i, blk.Index(i, t)) + 15) / 16;
-      if (lane == 0) {
         TcgenFenceAfter();
-        // MN-major, 128-byte swizzle: 64-value columns kTaHalf apart, groups of 8 keys 1024 bytes apart
-        uint64_t b = (uint64_t)((SmemAddr(ring + st * Cfg::kUnit) & 0x3FFFF) >> 4) | (uint64_t)(kTaHalf >> 4) << 16 |
-                     (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-        for (int kk = 0; kk < steps16; kk++)
-          UmmaTmemA(tmem + 256u + 128u * i, tmem + 128u * i + 8u * kk, b + (uint64_t)(kk * (2048 >> 4)), idesc_pv, t > 0 || kk > 0 ? 1u : 0u);
-        if (t + 1 == w.blocks[i]) UmmaCommit(&sh->o_full[i]);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++)
+          UmmaIssueSS(tmem + (uint32_t)(KEYS * i), a + (uint64_t)((kk / 4) * (kTaQHalf >> 4) + 2 * (kk % 4)),
+                      b + (uint64_t)((kk / 4) * (Cfg::kHalf >> 4) + 2 * (kk % 4)), idesc, kk > 0 ? 1u : 0u);
+        UmmaIssueCommit(&sh->s_full[i]);
+      };
+      // O += P V; at 128 keys the first 64 as soon as their probabilities are there
+      const auto values = [&](int i, int t, int unit) {
+        const int steps16 = (blk.Seen(i, blk.Index(i, t)) + 15) / 16;
+        const uint64_t b = vdesc + (uint64_t)(unit * (Cfg::kUnit >> 4));
+        const uint32_t d = tmem + Cfg::kO + Cfg::kOStep * i, a = tmem + (uint32_t)(KEYS * i);
+        const uint32_t more = t > 0 ? 1u : 0u;
+        const auto some = [&](int from, int to) {
+#pragma unroll
+          for (int kk = from; kk < to; kk++) UmmaIssueTS(d, a + 8u * kk, b + (uint64_t)(kk * (2048 >> 4)), idesc_pv, kk > 0 ? 1u : more);
+        };
+        if (Cfg::kWide && steps16 == kFull16) {
+          wait(&sh->p_half[i], t);
+          if (!ok) return;
+          TcgenFenceAfter();
+          some(0, 4);
+        }
+        wait(&sh->p_full[i], t);
+        if (!ok) return;
+        TcgenFenceAfter();
+        if (steps16 == kFull16) {
+          some(Cfg::kWide ? 4 : 0, kFull16);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < steps16; kk++) UmmaIssueTS(d, a + 8u * kk, b + (uint64_t)(kk * (2048 >> 4)), idesc_pv, kk > 0 ? 1u : more);
+        }
+        if (t + 1 == w.Blocks(i)) UmmaIssueCommit(&sh->o_full[i]);
+      };
+      const auto release = [&](int unit) { UmmaIssueCommit(&sh->empty[unit]); };
+      // rows of V behind the sequence's end, as far as the last 16-key step reaches, become 0
+      const auto trim = [&](int b, int unit) {
+        const int keys = blk.Keys(b), upto = (keys + 15) & ~15;
+        if (keys == upto || !ok) return;
+        const int pieces = (upto - keys) * 8;
+        for (int h = 0; h < Cfg::kHalves; h++)
+#pragma unroll 1
+          for (int c = lane; c < pieces; c += 32)
+            *reinterpret_cast<uint4*>(ring + unit * Cfg::kUnit + h * Cfg::kHalf + (keys + (c >> 3)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        FenceProxyAsyncShared();
+        __syncwarp();
+      };
+      ok = TaWaitWarp(sh, &sh->q_full, 0);
+      if (w.turns) {
+        // each unit serves one tile
+        const auto next_scores = [&](int i, int t) {
+          if (!ok || t >= w.Blocks(i)) return;
+          const int unit = acquire();
+          if (!ok) return;
+          scores(i, t, unit);
+          release(unit);
+        };
+        const auto next_values = [&](int i, int t) {
+          if (!ok || t >= w.Blocks(i)) return;
+          const int unit = acquire();
+          trim(blk.Index(i, t), unit);
+          values(i, t, unit);
+          if (ok) release(unit);
+        };
+        next_scores(0, 0);
+        next_scores(1, 0);
+#pragma unroll 1
+        for (int t = 0; t < steps && ok; t++) {
+          next_values(0, t);
+          next_scores(0, t + 1);
+          next_values(1, t);
+          next_scores(1, t + 1);
+        }
+      } else if (steps > 0) {
+        // the tiles share the units, and the last tile of a step (tile 1, if there is one: blocks0 <= blocks1) releases them
+        const int last = w.blocks1 > 0 ? 1 : 0;
+        int unit = acquire();
+        if (ok) {
+          scores(0, 0, unit);
+          if (last) scores(1, 0, unit);
+          release(unit);
+        }
+#pragma unroll 1
+        for (int t = 0; t < steps && ok; t++) {
+          const int vunit = acquire();
+          trim(blk.Index(0, t), vunit);
+          if (t + 1 < steps) unit = acquire();
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            if (!ok || t >= w.Blocks(i)) continue;
+            values(i, t, vunit);
+            if (!ok) continue;
+            if (i == last) release(vunit);
+            if (t + 1 < w.Blocks(i)) {
+              scores(i, t + 1, unit);
+              if (i == last) release(unit);
+            }
+          }
+        }
       }
-    };
-    const auto release = [&](int st) {
-      if (lane == 0) UmmaCommit(&sh->empty[st]);
-    };
-    // rows of V behind the sequence's end, as far as the last 16-key step reaches, become 0
-    const auto trim = [&](int b, int st) {
-      const int keys = blk.Keys(b), upto = (keys + 15) & ~15;
-      if (keys == upto || !ok) return;
-      const int pieces = (upto - keys) * 8;
-      for (int h = 0; h < Cfg::kHalves; h++)
-        for (int c = lane; c < pieces; c += 32)
-          *reinterpret_cast<uint4*>(ring + st * Cfg::kUnit + h * kTaHalf + (keys + (c >> 3)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-      FenceProxyAsyncShared();
+      UmmaIssueCommit(&sh->drained);
       __syncwarp();
-    };
-    ok = TaWait(sh, &sh->q_full, 0);
-    if (w.turns) {
-      for (int i = 0; i < 2 && ok; i++)
-        if (w.blocks[i] > 0) {
-          const int st = acquire();
-          if (!ok) break;
-          scores(i, 0, st);
-          release(st);
-        }
-      for (int t = 0; t < steps && ok; t++)
-        for (int i = 0; i < 2 && ok; i++) {
-          if (t < w.blocks[i]) {
-            const int st = acquire();
-            trim(blk.Index(i, t), st);
-            ok = ok && TaWait(sh, &sh->p_full[i], (uint32_t)(t & 1));
-            if (!ok) break;
-            values(i, t, st);
-            release(st);
-          }
-          if (t + 1 < w.blocks[i]) {
-            const int st = acquire();
-            if (!ok) break;
-            scores(i, t + 1, st);
-            release(st);
-          }
-        }
-    } else if (steps > 0) {
-      // blocks[0] <= blocks[1], or there is no tile 1: the last tile of a step releases its units
-      const int last0 = w.blocks[1] > 0 ? 1 : 0;
-      int st = acquire();
-      for (int i = 0; i <= last0 && ok; i++) scores(i, 0, st);
-      if (ok) release(st);
-      for (int t = 0; t < steps && ok; t++) {
-        const int vst = acquire();
-        trim(blk.Index(0, t), vst);
-        int kst = -1;
-        for (int i = 0; i < 2 && ok; i++) {
-          if (t >= w.blocks[i]) continue;
-          ok = TaWait(sh, &sh->p_full[i], (uint32_t)(t & 1));
-          if (!ok) break;
-          values(i, t, vst);
-          if (i == last0) release(vst);
-          if (t + 1 < w.blocks[i]) {
-            if (kst < 0) kst = acquire();
-            if (!ok) break;
-            scores(i, t + 1, kst);
-            if (i == last0) release(kst);
-          }
-        }
-      }
+      MbarWaitBounded(&sh->drained, 0, kOpsWaitLimit);  // no product reads shared memory or TMEM after this
     }
-    if (lane == 0) UmmaCommit(&sh->drained);
-    __syncwarp();
-    MbarWaitBounded(&sh->drained, 0, kOpsWaitLimit);  // no product reads shared memory or TMEM after this
   } else {
+    if constexpr (Cfg::kWide) RegsUp<kTaRegsSoftmax>();
     // ---- softmax: thread = row of its tile = TMEM lane ----
     const int i = warp >> 2, r = threadIdx.x & 127;
     const int token = r / A.G, g = r - token * A.G;
     const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
-    const bool mine = token < w.tokens[i];
-    const bool busy = (r & ~31) < w.tokens[i] * A.G;  // some row of this warp is in use
+    const bool mine = token < w.Tokens(i);
+    const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t scol = lanes + 128u * i, ocol = lanes + 256u + 128u * i;
+    const uint32_t scol = lanes + (uint32_t)(KEYS * i), ocol = lanes + Cfg::kO + Cfg::kOStep * i;
     const float sc = A.scale_log2;
     constexpr float kBias = F16 ? 7.f : 0.f;  // probabilities up to 2^15 in fp16: 7 more bits above its smallest numbers
-    unsigned long long bits = 0;
-    if constexpr (TREE) {
-      if (mine) bits = A.masks[w.start + tok0 + token];
-      if (w.nodes < 64) bits &= (1ull << w.nodes) - 1;
-    }
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int t = 0; t < w.blocks[i]; t++) {
+#pragma unroll 1
+    for (int t = 0; t < w.Blocks(i); t++) {
       const int b = blk.Index(i, t), seen = blk.Seen(i, b);
-      // columns this row sees: 0 .. lim-1, or the bits of the mask
-      unsigned long long m0, m1;
-      bool cut;
-      if (TREE) {
+      bool cut;  // some row does not see all keys of a whole block
+      bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
+      if constexpr (TREE) {
+        cut = seen < KEYS || b >= w.cache_blocks;
         if (b < w.cache_blocks) {
-          m0 = seen >= 64 ? ~0ull : (1ull << seen) - 1;
-          m1 = seen >= 128 ? ~0ull : seen > 64 ? (1ull << (seen - 64)) - 1 : 0;
-          const int* tb = A.table + (long long)w.seq * A.max_blocks + 2 * b;
-          const int p0 = tb[0], p1 = 2 * b + 1 < A.max_blocks ? tb[1] : -1;
-          if (p0 < 0 || p0 >= A.pages) m0 = 0;
-          if (p1 < 0 || p1 >= A.pages) m1 = 0;
-          cut = (m0 & m1) != ~0ull;
-        } else {
-          m0 = bits;
-          m1 = 0;
-          cut = true;
+          const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
+          gone0 = (unsigned)tb[0] >= (unsigned)A.pages;
+          if (KEYS == 128 && seen > 64) gone1 = (unsigned)tb[1] >= (unsigned)A.pages;
+          cut = __any_sync(0xffffffffu, cut || gone0 || gone1);
         }
       } else {
-        const int lim = min(seen, tok0 + token - 128 * b + 1);
-        m0 = lim >= 64 ? ~0ull : lim > 0 ? (1ull << lim) - 1 : 0;
-        m1 = lim >= 128 ? ~0ull : lim > 64 ? (1ull << (lim - 64)) - 1 : 0;
-        cut = tok0 < 128 * b + 127 || seen < 128;
+        cut = tok0 < KEYS * b + KEYS - 1 || seen < KEYS;
       }
       ok = TaWait(sh, &sh->s_full[i], (uint32_t)(t & 1));
       if (!ok) break;
       TcgenFenceAfter();
-      if (busy) {
-        uint32_t s[128];
-        if (!cut) {
+      if (!busy) {
+        if (Cfg::kWide) MbarArrive(&sh->p_half[i]);
+      } else {
+        uint32_t s[KEYS];
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const auto most = [&](int from, int to) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
+          for (int c = from; c < to; c += 2)
+            x[(c >> 1) & 3] = Max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        };
+        if (!cut) {
+          // the maximum of one half runs under the load of the other
+#pragma unroll
+          for (int c = 0; c < KEYS / 64; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
           TmemWaitLd();
+#pragma unroll
+          for (int c = KEYS / 64; c < KEYS / 32; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
+          most(0, KEYS / 2);
+          TmemWaitLd();
+          most(KEYS / 2, KEYS);
         } else {
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
+          for (int c = 0; c < KEYS / 32; c++) {
             if (32 * c < seen) {
               TmemLoad32(scol + 32u * c, s + 32 * c);
             } else {
@@ -490,62 +646,91 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
             }
           }
           TmemWaitLd();
+          // columns this row sees: 0 .. lim-1, or the bits of its mask
+          unsigned long long m0, m1 = 0;
+          if (TREE && b >= w.cache_blocks) {
+            m0 = mine ? A.masks[w.start + tok0 + token] : 0;
+            if (w.nodes < 64) m0 &= (1ull << w.nodes) - 1;
+          } else {
+            const int lim = TREE ? seen : min(seen, tok0 + token - KEYS * b + 1);
+            m0 = lim >= 64 ? ~0ull : lim > 0 ? (1ull << lim) - 1 : 0;
+            if (KEYS == 128) m1 = lim >= 128 ? ~0ull : lim > 64 ? (1ull << (lim - 64)) - 1 : 0;
+            if (gone0) m0 = 0;
+            if (gone1) m1 = 0;
+          }
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
+          for (int c = 0; c < KEYS / 32; c++) {
             const uint32_t bm = (uint32_t)((c < 2 ? m0 : m1) >> (32 * (c & 1)));
 #pragma unroll
             for (int k = 0; k < 32; k++)
               if (!(bm >> k & 1)) s[32 * c + k] = 0xff800000u;
           }
+          most(0, KEYS);
         }
-        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 128; c++) x[c & 3] = fmaxf(x[c & 3], __uint_as_float(s[c]));
         const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         if (t == 0) {
           m = mx;
         } else if (__any_sync(0xffffffffu, (mx - m) * sc > kTaLazy)) {
-          // block t-1's products are complete: S of block t was issued behind them
+          // step t-1's products are complete: S of step t was issued behind them
           const float mn = fmaxf(m, mx);
           const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
           m = mn;
           l *= alpha;
-#pragma unroll
-          for (int c = 0; c < D / 32; c++) {
-            uint32_t o[32];
-            TmemLoad32(ocol + 32u * c, o);
+#pragma unroll 1
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t o[16];
+            TmemLoad16(ocol + 16u * c, o);
             TmemWaitLd();
 #pragma unroll
-            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            TmemStore32(ocol + 32u * c, o);
+            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            TmemStore16(ocol + 16u * c, o);
           }
         }
         const float neg = m == -INFINITY ? 0.f : kBias - m * sc;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const f32x2 sc2 = Two(sc, sc), neg2 = Two(neg, neg);
+        f32x2 sum[2] = {0, 0};
+        // 32 keys: the probabilities, their sum, and the 16-bit pairs into TMEM
+        const auto exps = [&](int c, auto poly) {
+          uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          if (c == 0 || 32 * c < seen) {
-            uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-              const float p0 = Exp2(fmaf(__uint_as_float(s[32 * c + 2 * k]), sc, neg));
-              const float p1 = Exp2(fmaf(__uint_as_float(s[32 * c + 2 * k + 1]), sc, neg));
-              sum[(2 * k) & 3] += p0;
-              sum[(2 * k + 1) & 3] += p1;
-              p[k] = Pack2<F16>(p0, p1);
-            }
-            TmemStore16(scol + 16u * c, p);
+          for (int k = 0; k < 16; k++) {
+            float p0, p1;
+            Split(Fma2(Two(__uint_as_float(s[32 * c + 2 * k]), __uint_as_float(s[32 * c + 2 * k + 1])), sc2, neg2), p0, p1);
+            f32x2 e;
+            // spread evenly: pair k where (k + 1) kPoly / 16 passes an integer
+            if (decltype(poly)::value && (k + 1) * Cfg::kPoly / 16 != k * Cfg::kPoly / 16) e = Exp2Poly(p0, p1);
+            else e = Two(Exp2(p0), Exp2(p1));
+            sum[k & 1] = Add2(sum[k & 1], e);
+            Split(e, p0, p1);
+            p[k] = Pack2<F16>(p0, p1);
           }
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          TmemStore16(scol + 16u * c, p);
+        };
+        const auto probabilities = [&](auto whole) {
+          constexpr bool kAll = decltype(whole)::value;  // nothing is cut: all keys
+          exps(0, whole);
+          if (kAll || seen > 32) exps(1, whole);
+          if constexpr (Cfg::kWide) {
+            TmemWaitSt();
+            TcgenFenceBefore();
+            MbarArrive(&sh->p_half[i]);
+            if (kAll || seen > 64) exps(2, whole);
+            if (kAll || seen > 96) exps(3, whole);
+          }
+        };
+        if (cut) probabilities(std::false_type());
+        else probabilities(std::true_type());
+        float l0, l1;
+        Split(Add2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
         TmemWaitSt();
       }
       TcgenFenceBefore();
       MbarArrive(&sh->p_full[i]);
     }
     // ---- the rows' results ----
-    const bool merge = TREE && w.turns && w.blocks[1] > 0;
-    bool have = w.blocks[i] > 0;
+    const bool merge = TREE && w.turns && w.blocks1 > 0;
+    bool have = w.Blocks(i) > 0;
     if (have) have = TaWait(sh, &sh->o_full[i], 0);
     float* shared_o = reinterpret_cast<float*>(ring);  // tile 1's accumulator: [value][row], then its maximum and sum
     if (merge) {
@@ -553,14 +738,14 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
         have = TaWait(sh, &sh->o_full[0], 0) && have;  // all loads and products are done: the ring is free
         TcgenFenceAfter();
         if (busy) {
-#pragma unroll
-          for (int c = 0; c < D / 32; c++) {
-            uint32_t o[32];
-            TmemLoad32(ocol + 32u * c, o);
+#pragma unroll 1
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t o[16];
+            TmemLoad16(ocol + 16u * c, o);
             TmemWaitLd();
             if (have) {
 #pragma unroll
-              for (int k = 0; k < 32; k++) shared_o[(32 * c + k) * 128 + r] = __uint_as_float(o[k]);
+              for (int k = 0; k < 16; k++) shared_o[(16 * c + k) * 128 + r] = __uint_as_float(o[k]);
             }
           }
           if (have) {
@@ -586,44 +771,37 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
       }
       const bool parts = TREE && A.nsplit > 1;
       if (!parts) {
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // nothing seen: 0; NaN stays
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
         a0 *= inv;
         a1 *= inv;
       }
+      const bool zero = !parts && l == 0.f;
       const int node = tok0 + token;
       uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)(w.head * A.G + g) * A.out_head;
       const long long slot =
           parts ? ((long long)(w.seq * A.Hk + w.head) * A.nsplit + blockIdx.x % A.nsplit) * (A.max_nodes * A.G) + node * A.G + g : 0;
-#pragma unroll
-      for (int c = 0; c < D / 32; c++) {
-        uint32_t o[32];
+#pragma unroll 1
+      for (int c = 0; c < D / 16; c++) {
+        uint32_t o[16];
         if (have) {
-          TmemLoad32(ocol + 32u * c, o);
+          TmemLoad16(ocol + 16u * c, o);
           TmemWaitLd();
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; k++) o[k] = 0;
         }
-        float v[32];
+        float v[16];
 #pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = __uint_as_float(o[k]) * a0;
-        if (merge) {
-#pragma unroll
-          for (int k = 0; k < 32; k++) v[k] = fmaf(shared_o[(32 * c + k) * 128 + r], a1, v[k]);
-        }
-        if (!parts && l == 0.f) {
-#pragma unroll
-          for (int k = 0; k < 32; k++) v[k] = 0.f;
+        for (int k = 0; k < 16; k++) {
+          v[k] = have && !zero ? __uint_as_float(o[k]) * a0 : 0.f;
+          if (merge && !zero) v[k] = fmaf(shared_o[(16 * c + k) * 128 + r], a1, v[k]);
         }
         if (mine && ok) {
           if (parts) {
-            float4* dst = reinterpret_cast<float4*>(A.part_o + slot * D + 32 * c);
+            float4* dst = reinterpret_cast<float4*>(A.part_o + slot * D + 16 * c);
 #pragma unroll
-            for (int k = 0; k < 8; k++) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            for (int k = 0; k < 4; k++) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
           } else {
-            uint4* dst = reinterpret_cast<uint4*>(out + 32 * c);
+            uint4* dst = reinterpret_cast<uint4*>(out + 16 * c);
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 2; k++)
               dst[k] = make_uint4(Pack2<F16>(v[8 * k], v[8 * k + 1]), Pack2<F16>(v[8 * k + 2], v[8 * k + 3]),
                                   Pack2<F16>(v[8 * k + 4], v[8 * k + 5]), Pack2<F16>(v[8 * k + 6], v[8 * k + 7]));
           }
@@ -635,7 +813,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) TileAttentionKernel(const __gri
   TcgenFenceBefore();
   __syncthreads();
   TcgenFenceAfter();
-  if (warp == 8) TmemDealloc(tmem, 512);
+  if (warp == 8) TmemDealloc(tmem, Cfg::kCols);
 }
 
 // Joins the parts of a tree call's rows: one warp per (row, query head), D / 32 values per lane.
