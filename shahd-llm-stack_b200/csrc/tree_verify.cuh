@@ -8,11 +8,16 @@
 //   p_k = max(0, p_{k-1} - q) / its sum;
 // a taken child becomes the current node, and when no candidate is left the next token is drawn from p_k.
 // Unrolled, p_k = max(0, p - a_k q) / Z_k with a_0 = 0, Z_0 = 1, a_{k+1} = a_k + Z_k and Z_k = sum max(0, p - a_k q):
-// a refusal costs one pass over the two rows and no row is written. Sums run in 64 bits in a fixed order, so a run
-// repeats bit for bit; the test u q(x) Z < max(0, p(x) - a q(x)) is formed in 64 bits from the rows' own values.
+// a refusal costs one pass over the two rows and no row is written. The test u q(x) Z < max(0, p(x) - a q(x)) is formed in 64
+// bits from the rows' own values. In a pass, max(0, p - a q) of one token is two fused 32-bit steps (a as the sum of two
+// floats; each rounds relative to its own result, so nothing cancels: off by 2^-23 of itself), a 16-byte piece's tokens are
+// added in 32 bits and the pieces in 64, in a fixed order: a running mass is good to about 2^-23 over the root of the
+// number of pieces, 10^-9 in a row of 32768, and a run repeats bit for bit. (Element by element in 64 bits the conversions
+// alone, 16 a clock, took twice as long as the rows from memory, and the registers left one block per multiprocessor: 64
+// trees over 32768 tokens 30 us, 128 over 50257 in bf16 61 us; now VERMEASURED.)
 //
 // Bound by latency: a walk is a chain of decisions. What the decisions read, p and q at each node's token in its parent's
-// rows, does not hang on the walk, so a block's threads fetch it for 512 nodes at once into shared memory, and the walk
+// rows, does not hang on the walk, so a block's threads fetch it for 256 nodes at once into shared memory, and the walk
 // itself reads memory only for refusals. A row is cut over the blocks of a cluster, which exchange 8 bytes per warp through
 // distributed shared memory: one cluster barrier per refusal.
 #pragma once
@@ -21,7 +26,8 @@
 
 namespace shahd {
 
-constexpr int kVerThreads = 512;
+constexpr int kVerThreads = 256;
+constexpr int kVerPerSm = 4;  // blocks that fit a multiprocessor
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerMaxCluster = 8;
 
@@ -50,44 +56,49 @@ __device__ __forceinline__ void StoreCluster(double* p, uint32_t rank, double v)
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(ra), "d"(v) : "memory");
 }
 
+// The same in 32 bits with a = hi + lo.
+__device__ __forceinline__ float Left32(float p, float q, float hi, float lo) {
+  p = fmaxf(p, 0.f);  // NaN and negative values are no mass
+  q = fmaxf(q, 0.f);
+  return fmaxf(fmaf(-lo, q, fmaf(-hi, q, p)), 0.f);
+}
+
 template <class T>
 struct VerifyRows {
   static constexpr int PER = 16 / sizeof(T);  // values of a 16-byte piece
   const T *p, *q;
-  int V, mis;   // mis: values between the piece that holds value 0 and value 0; -1: the rows lie unlike to each other
+  int V, mis;       // mis: values between the start of value 0's piece and value 0
   int first, last;  // this warp's pieces
-  __device__ __forceinline__ int Value(int piece, int i) const { return piece * PER + i - (mis < 0 ? 0 : mis); }
-  // The PER values of a piece; those outside the row are 0.
-  __device__ __forceinline__ void Get(int piece, bool need_q, double (&x)[PER], double (&y)[PER]) const {
-    const int v0 = Value(piece, 0);
-    if (mis >= 0 && v0 >= 0 && v0 + PER <= V) {
-      const uint4 u = LoadNc16(p + v0);
-      const T* h = reinterpret_cast<const T*>(&u);
+  int whole0, whole1;  // pieces that lie inside both rows and can be read as such (none where the rows lie unlike to each other)
+  __device__ __forceinline__ int Value(int piece, int i) const { return piece * PER + i - mis; }
+  // max(0, p - (hi + lo) q) of a whole piece from its 16-byte words, and of any piece value by value (0 outside the row).
+  __device__ __forceinline__ void Whole(const uint4& u, const uint4& w, float hi, float lo, float (&x)[PER]) const {
+    const T* h = reinterpret_cast<const T*>(&u);
+    const T* g = reinterpret_cast<const T*>(&w);
 #pragma unroll
-      for (int i = 0; i < PER; i++) x[i] = Prob(h[i]);
-      if (need_q) {
-        const uint4 w = LoadNc16(q + v0);
-        const T* g = reinterpret_cast<const T*>(&w);
+    for (int i = 0; i < PER; i++) x[i] = Left32(float(h[i]), float(g[i]), hi, lo);
+  }
+  __device__ __forceinline__ void Any(int piece, float hi, float lo, float (&x)[PER]) const {
 #pragma unroll
-        for (int i = 0; i < PER; i++) y[i] = Prob(g[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; i++) {
-        const bool in = v0 + i >= 0 && v0 + i < V;
-        x[i] = in ? Prob(p[v0 + i]) : 0.0;
-        if (need_q) y[i] = in ? Prob(q[v0 + i]) : 0.0;
-      }
+    for (int i = 0; i < PER; i++) {
+      const int v = Value(piece, i);
+      x[i] = v >= 0 && v < V ? Left32(float(p[v]), hi != 0.f ? float(q[v]) : 0.f, hi, lo) : 0.f;
     }
-    if (!need_q) {
+  }
+  static __device__ __forceinline__ double Sum(const float (&x)[PER]) {
+    float s[PER];
 #pragma unroll
-      for (int i = 0; i < PER; i++) y[i] = 0.0;
-    }
+    for (int i = 0; i < PER; i++) s[i] = x[i];
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < o; i++) s[i] += s[i + o];
+    return (double)s[0];
   }
 };
 
 template <class T>
-__global__ void __launch_bounds__(kVerThreads) VerifyTreeKernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const __grid_constant__ VerifyArgs a) {
   __shared__ double sums[2][kVerMaxCluster * kVerWarps];  // every warp's sum of the latest passes, by turns
   __shared__ double s_p[kVerThreads], s_q[kVerThreads];
   __shared__ float s_u[kVerThreads];
@@ -122,22 +133,45 @@ __global__ void __launch_bounds__(kVerThreads) VerifyTreeKernel(const __grid_con
     rows.p = target + (long long)(b + node) * a.target_row;
     rows.q = draft + (long long)(b + node) * a.draft_row;
     const int mp = (int)(reinterpret_cast<uintptr_t>(rows.p) % 16 / sizeof(T)), mq = (int)(reinterpret_cast<uintptr_t>(rows.q) % 16 / sizeof(T));
-    rows.mis = mp == mq ? mp : -1;
-    const int pieces = (rows.V + max(rows.mis, 0) + rows.PER - 1) / rows.PER;
+    rows.mis = mp == mq ? mp : 0;
+    const int pieces = (rows.V + rows.mis + rows.PER - 1) / rows.PER;
     const int share = CeilDiv(pieces, C * kVerWarps);
     rows.first = min(pieces, (rank * kVerWarps + warp) * share);
     rows.last = min(pieces, rows.first + share);
+    rows.whole0 = min(max(rows.first, rows.mis > 0 ? 1 : 0), rows.last);
+    rows.whole1 = mp == mq ? min(max(rows.whole0, (rows.V + rows.mis) / rows.PER), rows.last) : rows.whole0;
   };
   int buf = 0;
   // of the latest pass: the mass ahead of this warp's pieces, up to their end, in them, in the whole row
   double before = 0, after = 0, mine = 0, total = 0;
   const auto pass = [&](double w) {        // Z = sum of max(0, p - w q)
     double z = 0;
-    for (int c = rows.first + lane; c < rows.last; c += 32) {
-      double x[VerifyRows<T>::PER], y[VerifyRows<T>::PER];
-      rows.Get(c, w != 0, x, y);
+    const float hi = (float)w, lo = (float)(w - (double)hi);
+    float x[VerifyRows<T>::PER];
+    const uint4* vp = reinterpret_cast<const uint4*>(rows.p - rows.mis);
+    const uint4* vq = reinterpret_cast<const uint4*>(rows.q - rows.mis);
+    int c = rows.whole0 + lane;
+    for (; c + 96 < rows.whole1; c += 128) {  // four pieces of each row in flight
+      uint4 u[4], v[4];
 #pragma unroll
-      for (int i = 0; i < VerifyRows<T>::PER; i++) z += Left(x[i], y[i], w);
+      for (int k = 0; k < 4; k++) {
+        u[k] = LoadNc16(vp + c + 32 * k);
+        v[k] = w != 0 ? LoadNc16(vq + c + 32 * k) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        rows.Whole(u[k], v[k], hi, lo, x);
+        z += rows.Sum(x);
+      }
+    }
+    for (; c < rows.whole1; c += 32) {
+      rows.Whole(LoadNc16(vp + c), w != 0 ? LoadNc16(vq + c) : make_uint4(0, 0, 0, 0), hi, lo, x);
+      z += rows.Sum(x);
+    }
+    for (c = rows.first + lane; c < rows.last; c += 32) {
+      if (c >= rows.whole0 && c < rows.whole1) continue;
+      rows.Any(c, hi, lo, x);
+      z += rows.Sum(x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -240,14 +274,16 @@ __global__ void __launch_bounds__(kVerThreads) VerifyTreeKernel(const __grid_con
   if (mine > 0 && after >= goal && (before < goal || before == 0)) {
     int id = -1, seen = -1;
     double run = before;
+    const float hi = (float)w, lo = (float)(w - (double)hi);
     for (int c0 = rows.first; c0 < rows.last && id < 0; c0 += 32) {
       const int c = c0 + lane;
-      double x[VerifyRows<T>::PER], y[VerifyRows<T>::PER], own = 0;
+      float x[VerifyRows<T>::PER];
+      double own = 0;
 #pragma unroll
-      for (int i = 0; i < VerifyRows<T>::PER; i++) x[i] = y[i] = 0;
-      if (c < rows.last) rows.Get(c, w != 0, x, y);
+      for (int i = 0; i < VerifyRows<T>::PER; i++) x[i] = 0.f;
+      if (c < rows.last) rows.Any(c, hi, lo, x);
 #pragma unroll
-      for (int i = 0; i < VerifyRows<T>::PER; i++) own += x[i] = Left(x[i], y[i], w);
+      for (int i = 0; i < VerifyRows<T>::PER; i++) own += (double)x[i];
       double incl = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -258,9 +294,9 @@ __global__ void __launch_bounds__(kVerThreads) VerifyTreeKernel(const __grid_con
       double s = run + incl - own;
 #pragma unroll
       for (int i = 0; i < VerifyRows<T>::PER; i++) {
-        s += x[i];
-        if (x[i] > 0) last = rows.Value(c, i);
-        if (x[i] > 0 && s >= goal && found < 0) found = rows.Value(c, i);
+        s += (double)x[i];
+        if (x[i] > 0.f) last = rows.Value(c, i);
+        if (x[i] > 0.f && s >= goal && found < 0) found = rows.Value(c, i);
       }
       const unsigned hit = __ballot_sync(0xffffffffu, found >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
       if (any) seen = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
@@ -342,11 +378,11 @@ extern "C" int shahd_verify_tree(const ShahdVerifyCall* c, void* stream) {
   a.n = c->n;
   a.rows = c->rows;
   a.vocab = c->vocab;
-  // A row is cut over as many blocks as leave each thread a 16-byte piece of it, as long as all blocks run at once (four
-  // of them fit a multiprocessor): a pass is then one round of loads.
+  // A row is cut over as many blocks as leave each thread a 16-byte piece of it, as long as all blocks run at once: a pass is
+  // then a few rounds of loads.
   const long long pieces = ((long long)c->vocab * (long long)size + 15) / 16;
   a.cluster = 1;
-  while (a.cluster < kVerMaxCluster && pieces >= 2LL * a.cluster * kVerThreads && 2LL * a.cluster * c->n <= 4LL * info.sms) a.cluster *= 2;
+  while (a.cluster < kVerMaxCluster && pieces >= 2LL * a.cluster * kVerThreads && 2LL * a.cluster * c->n <= (long long)kVerPerSm * info.sms) a.cluster *= 2;
   if ((long long)c->n * a.cluster > 0x7fffffffLL) a.cluster = 1;
   TakeLaunchError(nullptr);
   const dim3 grid((unsigned)(c->n * a.cluster)), block(kVerThreads), cluster((unsigned)a.cluster);
