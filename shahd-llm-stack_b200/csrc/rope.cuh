@@ -7,10 +7,13 @@
 // with pairs (2i, 2i+1) or (i, i + r/2). Angles: the turn p * f_i / 2pi is formed in 64 bits and only its fraction is
 // rounded to 32, so a position of 10^6 loses nothing (in 32 bits the angle alone would be off by 0.03).
 //
-// Bound by memory: each value is read once and written once. A block takes a few rows: it first writes the rows'
-// (cos, sin) table to shared memory, one sincospi per (row, pair) for all heads together, then its threads go
-// over 8-value pieces of all heads of q, k and v with 16-byte accesses. Operands whose address, strides or pair count
-// do not allow 16-byte pieces go through one pair per thread.
+// Bound by memory: each value is read once and written once. A warp takes a row at a time and waits for no other: its lanes
+// form the row's (cos, sin), one sincospi per pair for all heads, in shared memory of the warp's own, and take their
+// piece's into registers; a lane's piece of a head (8 values; in the half layout two pieces, as far apart as pairs are) is the same
+// in all heads, so a lane goes over heads with up to eight 16-byte loads in flight. Operands whose address, strides or pair
+// count do not allow pieces go value by value. (Blocks of 256 threads over batches of rows, with a table per batch, lost a
+// fifth to a third of the time at the barriers: 56 K rows of 32 + 8 heads of 128 in f16, 1.15 GB, took 265 us; now 197, a plain
+// copy 182.)
 #pragma once
 
 #include "ops_common.cuh"
@@ -23,9 +26,12 @@ struct ShahdRope {
 
 namespace shahd {
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeMaxRows = 16;   // rows of a block
-constexpr int kRopeTable = 512;    // (row, pair) entries of a block's table
+constexpr int kRopeWarps = 8;   // of a block, at most
+enum RopeMode { kRopeValues = 0, kRopeInterleaved = 1, kRopeHalf = 2 };  // one pair per thread, or pieces of either layout
+// Blocks of a multiprocessor: in the half layout a lane holds two pieces and their eight (cos, sin), 16-bit ones twice, which spills
+// at 80 registers (265 us instead of 196 for 56 K rows of 32 + 8 heads of 128).
+template <class T, int MODE>
+constexpr int kRopePerSm = MODE == kRopeHalf && sizeof(T) == 2 ? 2 : 3;
 
 struct RopeOperand {
   const void* in;
@@ -38,7 +44,7 @@ struct RopeArgs {
   RopeOperand q, k, v;  // v.out is never set: values only go to the cache
   const int* positions;
   const int* offsets;  // null: every row counts
-  int n, rows, d, half, interleaved, rows_per_block, pieces, shift;
+  int n, rows, d, half, interleaved, pieces;
   float magnitude;
   uint16_t* pool;  // null: no cache
   long long page_stride;
@@ -58,18 +64,20 @@ __device__ __forceinline__ T FromFloat(float x) {
   else return __float2bfloat16_rn(x);
 }
 
+// Eight values as they lie in memory, and as floats.
 template <class T>
-__device__ __forceinline__ void Load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void Load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void Get(float (&v)[8]) const {
+    const T* h = reinterpret_cast<const T*>(u);
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = ToFloat(h[i]);
   }
-}
+};
 template <class T>
 __device__ __forceinline__ void Store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -95,141 +103,160 @@ __device__ __forceinline__ int SequenceOf(const int* offsets, int n, int row) {
   return lo;
 }
 
-// T: the operands' type, C: the cache's. VEC: 16-byte pieces.
-template <class T, class C, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) RopeKernel(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 turn[kRopeTable];
-  __shared__ int pos[kRopeMaxRows];
-  __shared__ long long at[kRopeMaxRows];  // the row's place in the cache (kv head 0, K), or -1
+// T: the operands' type, C: the cache's.
+template <class T, class C, int MODE>
+__global__ void __launch_bounds__(kRopeWarps * 32, kRopePerSm<T, MODE>) RopeKernel(const __grid_constant__ RopeArgs a) {
+  __shared__ __align__(16) float2 tables[kRopeWarps][128];
+  constexpr int kPer = MODE == kRopeHalf ? 8 : 4;  // pairs of a piece
   GridDepWait();
   GridDepLaunch();
-  const int r0 = blockIdx.x * a.rows_per_block, nr = min(a.rows_per_block, a.rows - r0);
-  if (threadIdx.x < nr) {
-    const int row = r0 + threadIdx.x;
-    int p = a.positions[row];
-    if (a.offsets && (row < a.offsets[0] || row >= a.offsets[a.n])) p = -1;
-    long long c = -1;
-    if (a.pool && p >= 0 && (p >> 6) < a.max_blocks) {
-      const int page = a.table[(long long)SequenceOf(a.offsets, a.n, row) * a.max_blocks + (p >> 6)];
-      if (page >= 0 && page < a.pages) c = page * a.page_stride + (long long)(p & 63) * a.d;
-    }
-    pos[threadIdx.x] = p;
-    at[threadIdx.x] = c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int d = a.d, half = a.half, heads = a.q.heads + a.k.heads + a.v.heads;
+  float2* turn = tables[warp];
+  // pieces: this lane's place in a head, and its first head (of every `lanes`-th)
+  const int piece = MODE == kRopeValues ? 0 : lane % a.pieces, lanes = MODE == kRopeValues ? 1 : 32 / a.pieces;
+  const int n0 = MODE == kRopeValues ? 0 : lane / a.pieces;
+  int j0 = piece * 8, apart = half;
+  bool rotary = MODE == kRopeInterleaved ? j0 < 2 * half : j0 < half;
+  if (MODE == kRopeHalf && !rotary) {  // behind the rotated part: this piece, and the one half of that part further on
+    j0 += half;
+    apart = d / 2 - half;
   }
-  for (int e = threadIdx.x; e < nr * a.half; e += kRopeThreads) {
-    const int r = e / a.half, i = e - r * a.half;
-    const double t = (double)max(a.positions[r0 + r], 0) * a.turns[i];
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    turn[e] = make_float2(c * a.magnitude, s * a.magnitude);
-  }
-  __syncthreads();
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
-  const int per_row = heads * a.pieces;
-  const int d = a.d, half = a.half;
-  for (int e = threadIdx.x; e < nr * per_row; e += kRopeThreads) {
-    const int r = e / per_row;
-    const int rest = e - r * per_row;
-    int h = a.shift >= 0 ? rest >> a.shift : rest / a.pieces;
-    const int piece = rest - h * a.pieces;
-    if (pos[r] < 0) continue;
-    const RopeOperand* o = &a.q;
-    int kv = -1;
-    if (h >= a.q.heads) {
-      h -= a.q.heads;
-      o = &a.k;
-      kv = 0;
-      if (h >= a.k.heads) {
-        h -= a.k.heads;
-        o = &a.v;
-        kv = 1;
-      }
+  const int first = a.offsets ? a.offsets[0] : 0, end = a.offsets ? a.offsets[a.n] : a.rows;
+  const long long step = (long long)gridDim.x * (blockDim.x >> 5);
+  long long row = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
+  int next = row < a.rows ? a.positions[row] : -1;
+  for (; row < a.rows; row += step) {
+    const int p = next;
+    next = row + step < a.rows ? a.positions[row + step] : -1;  // ahead of this row's values
+    if (p < 0 || row < first || row >= end) continue;
+    long long at = -1;  // the row's place in the cache (kv head 0, K)
+    if (a.pool && (p >> 6) < a.max_blocks) {
+      const int page = a.table[(long long)SequenceOf(a.offsets, a.n, (int)row) * a.max_blocks + (p >> 6)];
+      if (page >= 0 && page < a.pages) at = page * a.page_stride + (long long)(p & 63) * d;
     }
-    const int row = r0 + r;
-    const T* in = static_cast<const T*>(o->in) + row * o->in_row + h * o->in_head;
-    T* out = o->out ? static_cast<T*>(o->out) + row * o->out_row + h * o->out_head : nullptr;
-    C* cache = kv >= 0 && at[r] >= 0 ? reinterpret_cast<C*>(a.pool) + at[r] + (long long)(2 * h + kv) * kOpsPage * d : nullptr;
-    const float2* tr = turn + r * half;
-    if constexpr (VEC) {
-      float x[8], y[8];
-      const bool paired = !a.interleaved && piece * 8 < half;  // this piece stands for the one at + half as well
-      if (kv == 1 || !(paired || (a.interleaved && piece * 8 < 2 * half))) {  // values, or behind the rotated part
-        const int j = a.interleaved || paired ? piece * 8 : piece * 8 + half;
-        Load8(in + j, x);
-        if (paired) Load8(in + j + half, y);
-        if (out) Store8(out + j, x);
-        if (cache) {
-          Store8(cache + j, x);
-          if (paired) Store8(cache + j + half, y);
-        }
-        continue;
-      }
-      if (a.interleaved) {
-        const int j = piece * 8;
-        Load8(in + j, x);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 t = tr[j / 2 + i];
-          y[2 * i] = x[2 * i] * t.x - x[2 * i + 1] * t.y;
-          y[2 * i + 1] = x[2 * i] * t.y + x[2 * i + 1] * t.x;
-        }
-        if (out) Store8(out + j, y);
-        if (cache) Store8(cache + j, y);
-      } else {
-        const int j = piece * 8;
-        float b[8], z[8];
-        Load8(in + j, x);
-        Load8(in + j + half, b);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float2 t = tr[j + i];
-          y[i] = x[i] * t.x - b[i] * t.y;
-          z[i] = x[i] * t.y + b[i] * t.x;
-        }
-        if (out) {
-          Store8(out + j, y);
-          Store8(out + j + half, z);
-        }
-        if (cache) {
-          Store8(cache + j, y);
-          Store8(cache + j + half, z);
-        }
-      }
-    } else {  // piece: a pair, or one value behind the rotated part
-      int j0 = piece, j1 = -1;
-      float x, y = 0.f;
-      if (piece < half) {
-        j0 = a.interleaved ? 2 * piece : piece;
-        j1 = a.interleaved ? j0 + 1 : piece + half;
-      } else {
-        j0 = piece + half;
-      }
-      x = ToFloat(in[j0]);
-      if (j1 >= 0) {
-        y = ToFloat(in[j1]);
-        if (kv != 1) {
-          const float2 t = tr[piece];
-          const float u = x * t.x - y * t.y;
-          y = x * t.y + y * t.x;
+    __syncwarp();  // the last row's table has been read
+#pragma unroll 1
+    for (int i = lane; i < half; i += 32) {
+      // from the parameters by a generic load: as an indexed constant, 32 different frequencies take a warp 32 accesses
+      double f;
+      asm volatile("ld.f64 %0, [%1];" : "=d"(f) : "l"(a.turns + i));
+      const double t = (double)p * f;
+      float sn, cs;
+      sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+      // two pairs of every piece side by side, so that the lanes' 16-byte reads lie next to each other
+      const int place = MODE == kRopeValues ? i : (i % kPer / 2 * (half / kPer) + i / kPer) * 2 + i % 2;
+      turn[place] = make_float2(cs * a.magnitude, sn * a.magnitude);
+    }
+    __syncwarp();
+    if constexpr (MODE == kRopeValues) {
+      for (int item = lane; item < heads * a.pieces; item += 32) {
+        const int n = item / a.pieces, j = item - n * a.pieces;
+        const int kv = n < a.q.heads ? -1 : n < a.q.heads + a.k.heads ? 0 : 1;  // 0 for a key, 1 for a value, -1 for a query
+        const RopeOperand& o = kv < 0 ? a.q : kv == 0 ? a.k : a.v;
+        const int h = kv < 0 ? n : kv == 0 ? n - a.q.heads : n - a.q.heads - a.k.heads;
+        const bool two = j < half;  // a pair, or a value behind the rotated part
+        const int v0 = !two ? j + half : a.interleaved ? 2 * j : j, v1 = a.interleaved ? v0 + 1 : v0 + half;
+        const T* in = static_cast<const T*>(o.in) + row * o.in_row + h * o.in_head;
+        float x = ToFloat(in[v0]), y = two ? ToFloat(in[v1]) : 0.f;
+        if (two && kv != 1) {
+          const float2 cs = turn[j];
+          const float u = x * cs.x - y * cs.y;
+          y = x * cs.y + y * cs.x;
           x = u;
         }
+        if (o.out) {
+          T* out = static_cast<T*>(o.out) + row * o.out_row + h * o.out_head;
+          out[v0] = FromFloat<T>(x);
+          if (two) out[v1] = FromFloat<T>(y);
+        }
+        if (kv >= 0 && at >= 0) {
+          C* cache = reinterpret_cast<C*>(a.pool) + at + (long long)(2 * h + kv) * kOpsPage * d;
+          cache[v0] = FromFloat<C>(x);
+          if (two) cache[v1] = FromFloat<C>(y);
+        }
       }
-      if (out) {
-        out[j0] = FromFloat<T>(x);
-        if (j1 >= 0) out[j1] = FromFloat<T>(y);
+    } else if (n0 < lanes) {
+      float4 cs[kPer / 2];
+      if (rotary) {
+        const float4* from = reinterpret_cast<const float4*>(turn) + piece;
+#pragma unroll
+        for (int q = 0; q < kPer / 2; q++) cs[q] = from[q * (half / kPer)];
       }
-      if (cache) {
-        cache[j0] = FromFloat<C>(x);
-        if (j1 >= 0) cache[j1] = FromFloat<C>(y);
-      }
+      // one operand's heads; kv: 0 for keys, 1 for values, -1 for queries
+      const auto turn_heads = [&](const RopeOperand& o, int kv, int h0) {
+        constexpr int kDeep = (sizeof(T) == 4 ? 2 : 4) / (MODE == kRopeHalf ? 2 : 1);  // heads in flight
+        const T* in = static_cast<const T*>(o.in) + row * o.in_row + j0;
+        T* out = o.out ? static_cast<T*>(o.out) + row * o.out_row + j0 : nullptr;
+        C* cache = kv >= 0 && at >= 0 ? reinterpret_cast<C*>(a.pool) + at + (long long)kv * kOpsPage * d + j0 : nullptr;
+#pragma unroll 1
+        for (int h = h0; h < o.heads; h += kDeep * lanes) {
+          Raw8<T> ra[kDeep], rb[kDeep];
+#pragma unroll
+          for (int k = 0; k < kDeep; k++) {
+            const int hk = h + k * lanes;
+            if (hk < o.heads) {
+              ra[k].Load(in + hk * o.in_head);
+              if (MODE == kRopeHalf) rb[k].Load(in + hk * o.in_head + apart);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kDeep; k++) {
+            const int hk = h + k * lanes;
+            if (hk >= o.heads) break;
+            float x[8], y[8];
+            ra[k].Get(x);
+            if (MODE == kRopeHalf) rb[k].Get(y);
+            if (rotary && kv != 1) {
+#pragma unroll
+              for (int q = 0; q < kPer / 2; q++) {
+                if (MODE == kRopeInterleaved) {
+                  const float u = x[4 * q], v = x[4 * q + 1], s = x[4 * q + 2], w = x[4 * q + 3];
+                  x[4 * q] = u * cs[q].x - v * cs[q].y;
+                  x[4 * q + 1] = u * cs[q].y + v * cs[q].x;
+                  x[4 * q + 2] = s * cs[q].z - w * cs[q].w;
+                  x[4 * q + 3] = s * cs[q].w + w * cs[q].z;
+                } else {
+                  const float u = x[2 * q], v = y[2 * q], s = x[2 * q + 1], w = y[2 * q + 1];
+                  x[2 * q] = u * cs[q].x - v * cs[q].y;
+                  y[2 * q] = u * cs[q].y + v * cs[q].x;
+                  x[2 * q + 1] = s * cs[q].z - w * cs[q].w;
+                  y[2 * q + 1] = s * cs[q].w + w * cs[q].z;
+                }
+              }
+            }
+            if (out) {
+              Store8(out + hk * o.out_head, x);
+              if (MODE == kRopeHalf) Store8(out + hk * o.out_head + apart, y);
+            }
+            if (cache) {
+              C* to = cache + (long long)hk * 2 * kOpsPage * d;
+              Store8(to, x);
+              if (MODE == kRopeHalf) Store8(to + apart, y);
+            }
+          }
+        }
+      };
+      turn_heads(a.q, -1, n0);
+      turn_heads(a.k, 0, n0);
+      turn_heads(a.v, 1, n0);
     }
   }
 }
 
+template <class T, class C, int MODE>
+void LaunchRopeMode(const RopeArgs& a, int sms, cudaStream_t st) {
+  // a warp per row while they last, spread over the multiprocessors; then as many blocks as run at once
+  const int warps = std::max(1, std::min(kRopeWarps, a.rows / sms));
+  const int blocks = std::min(CeilDiv(a.rows, warps), kRopePerSm<T, MODE> * sms);
+  LaunchPdl(RopeKernel<T, C, MODE>, dim3(blocks), dim3(warps * 32), 0, st, a);
+}
+
 template <class T, class C>
-void LaunchRope(const RopeArgs& a, bool vec, int blocks, cudaStream_t st) {
-  if (vec) LaunchPdl(RopeKernel<T, C, true>, dim3(blocks), dim3(kRopeThreads), 0, st, a);
-  else LaunchPdl(RopeKernel<T, C, false>, dim3(blocks), dim3(kRopeThreads), 0, st, a);
+void LaunchRope(const RopeArgs& a, bool vec, int sms, cudaStream_t st) {
+  if (!vec) LaunchRopeMode<T, C, kRopeValues>(a, sms, st);
+  else if (a.interleaved) LaunchRopeMode<T, C, kRopeInterleaved>(a, sms, st);
+  else LaunchRopeMode<T, C, kRopeHalf>(a, sms, st);
 }
 
 }  // namespace shahd
@@ -379,7 +406,7 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
   RopeArgs a = {};
   // 16-byte pieces of 8 values: every address and stride in use a multiple of 16 bytes, whole pieces on both sides of
   // the rotated part's end and of the pairs' halves
-  bool vec = d % 8 == 0 && (rope->layout == SHAHD_ROPE_HALF ? rope->rotary % 16 == 0 : rope->rotary % 8 == 0);
+  bool vec = rope->layout == SHAHD_ROPE_HALF ? d % 16 == 0 && rope->rotary % 16 == 0 : d % 8 == 0 && rope->rotary % 8 == 0;
   const auto operand = [&](const ShahdRows& in, const ShahdRows& out, int heads) {
     for (const ShahdRows* r : {&in, &out})
       if (r->data)
@@ -405,18 +432,12 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
     a.pages = c->cache.pages;
   }
   std::copy(rope->turns, rope->turns + a.half, a.turns);
-  a.pieces = vec ? (a.interleaved ? d / 8 : (d - a.half) / 8) : d - a.half;
-  a.shift = -1;
-  for (int s = 0; s < 9; s++)
-    if (a.pieces == 1 << s) a.shift = s;
-  // as many rows as the block's table holds, fewer where that leaves multiprocessors without a block
-  a.rows_per_block = std::max(1, std::min({kRopeMaxRows, kRopeTable / a.half, c->rows / (4 * info.sms)}));
-  const int blocks = CeilDiv(c->rows, a.rows_per_block);
+  a.pieces = vec ? (a.interleaved ? d / 8 : d / 16) : d - a.half;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   TakeLaunchError(nullptr);
-  if (c->dtype == SHAHD_F32) LaunchRope<float, bf16>(a, vec, blocks, st);
-  else if (c->dtype == SHAHD_F16) LaunchRope<__half, __half>(a, vec, blocks, st);
-  else LaunchRope<bf16, bf16>(a, vec, blocks, st);
+  if (c->dtype == SHAHD_F32) LaunchRope<float, bf16>(a, vec, info.sms, st);
+  else if (c->dtype == SHAHD_F16) LaunchRope<__half, __half>(a, vec, info.sms, st);
+  else LaunchRope<bf16, bf16>(a, vec, info.sms, st);
   return LaunchStatus(op);
 }
 
