@@ -425,11 +425,11 @@ typedef struct ShahdTreeCall {
   const uint64_t* masks;   /* [rows] bit j: the row attends to row j of its sequence (itself included only by its bit) */
   ShahdRows q, k, v, out;  /* 16-byte aligned, strides multiples of 8; k and v are the nodes' own, not in the cache */
   ShahdKvCache cache;
-  void* workspace;         /* 16-byte aligned, shahd_tree_attention_workspace bytes; in use until the call has run */
+  void* workspace;         /* 32-byte aligned, shahd_tree_attention_workspace bytes; in use until the call has run */
   int64_t workspace_bytes;
 } ShahdTreeCall;
 /* Bytes of workspace for a call with these n, num_heads, max_nodes and cache sizes (0: none), or a negative status; dtype,
- * pointers, rows and scale are not looked at. The device is the current one. */
+ * pointers, rows and scale are not looked at, and no device is asked. */
 int64_t shahd_tree_attention_workspace(const ShahdTreeCall* call);
 /* out[i] = sum of softmax(scale q[i].k[j]) v[j] over the cached positions of the row's sequence and the rows of its mask;
  * a row that attends to nothing gives 0. Positions at or beyond the length are never used, whatever their pages

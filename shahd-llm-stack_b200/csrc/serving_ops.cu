@@ -73,7 +73,7 @@ void LaunchTiles(const TaArgs& a, unsigned blocks, cudaStream_t st) {
   if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, TREE>, TaCfg<D>::kSmem)) return;
   LaunchPdl(TileAttentionKernel<D, F16, TREE>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
   if constexpr (TREE)
-    if (a.nsplit > 1)
+    if (a.least > 0)
       LaunchPdl(TreeJoinKernel<D, F16>, dim3((unsigned)(((long long)a.rows * a.H + 7) / 8)), dim3(256), 0, st, a);
 }
 
@@ -94,27 +94,49 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
   return false;
 }
 
-// Parts that the key blocks of a sequence are cut into: one where the tiles fill the multiprocessors anyway, else as many
-// as fill them once, of two blocks of 128 keys at least.
-constexpr int kTaSms = 148;  // of a B200: the cut, and so the workspace, does not hang on a device being there
-int TreeParts(int n, int Hk, int pairs, int max_blocks) {
-  const long long tiles = (long long)n * Hk * pairs;
-  const int blocks = (max_blocks + 1) / 2 + 1;
-  return (int)std::max(1LL, std::min<long long>(kTaSms / tiles, blocks / 2));
-}
+// How a tree call's work is laid out. Where there are many tile pairs, or enough with short caches, each has a block of threads
+// of its own. Elsewhere as many blocks of threads as run at once take ranges of equal length out of all key blocks of all pairs,
+// 256 keys at least, and the pairs that a range cuts are joined by a second kernel: so long caches and short ones, one sequence and a
+// few hundred, end together (16 trees over 20 to 32 thousand positions, 8 kv heads of 128: a block of threads for each pair
+// 490 us, parts of 2048 keys 513 us, ranges 427 us; but 512 pairs of 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as
+// 256 pairs of heads).
+constexpr int kTaSms = 148;  // of a B200: the layout, and so the workspace, does not hang on a device being there
+struct TreeLayout {
+  int pairs, two_heads, least, part_rows;
+  long long grid;
+  int64_t plan_bytes, bytes;
+};
 
-int64_t TreeBytes(const char* op, const ShahdTreeCall* c, int* pairs, int* parts) {
+int LayTree(const char* op, const ShahdTreeCall* c, TreeLayout* out) {
   const int H = c->num_heads, Hk = c->cache.kv_heads, d = c->cache.head_dim;
   if (!CheckHeads(op, H, Hk, d) || !CheckCache(op, c->cache, Hk, d)) return SHAHD_EINVAL;
   if (c->n < 0 || c->max_nodes < 1 || c->max_nodes > 64) {
     SetError("%s: need n >= 0 and max_nodes in 1 .. 64 (got n=%d max_nodes=%d)", op, c->n, c->max_nodes);
     return SHAHD_EINVAL;
   }
-  const int G = H / Hk, TB = 128 / G;
-  *pairs = CeilDiv(c->max_nodes, 2 * TB);
-  *parts = TreeParts(std::max(c->n, 1), Hk, *pairs, c->cache.max_blocks);
-  if (*parts == 1) return 0;
-  return (int64_t)c->n * Hk * *parts * c->max_nodes * G * (d + 2) * (int64_t)sizeof(float);
+  const int G = H / Hk, TB = 128 / G, keys = d == 128 ? 128 : 64;
+  TreeLayout l = {};
+  l.pairs = CeilDiv(c->max_nodes, 2 * TB);
+  const long long slots = kTaSms * (d == 128 ? 1 : 2), tiles = (long long)c->n * Hk * l.pairs;
+  const long long most = tiles * (CeilDiv(c->cache.max_blocks, keys / 64) + 1);  // key blocks of all pairs, if all sequences were as long
+  if (most > 0x7fffffffLL) {
+    SetError("%s: too many key blocks: %lld tile pairs over %d pages each", op, tiles, c->cache.max_blocks);
+    return SHAHD_EINVAL;
+  }
+  if (tiles >= 8 * slots || (tiles >= slots && c->cache.max_blocks < 64)) {
+    // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge
+    l.two_heads = c->max_nodes <= TB && Hk % 2 == 0;
+    l.grid = l.two_heads ? tiles / 2 : tiles;
+  } else {
+    l.least = 256 / keys;
+    l.grid = std::max(1LL, std::min(slots, (most + l.least - 1) / l.least));
+    l.part_rows = std::min(c->max_nodes, 2 * TB) * G;
+    l.plan_bytes = ((int64_t)c->n + 1) * 4;
+    l.plan_bytes = (l.plan_bytes + 255) / 256 * 256;
+    l.bytes = l.plan_bytes + 2 * l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
+  }
+  *out = l;
+  return SHAHD_OK;
 }
 
 }  // namespace
@@ -170,7 +192,6 @@ int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
   a.rows = c->rows;
   a.H = H;
   a.Hk = Hk;
-  a.nsplit = 1;
   TakeLaunchError(nullptr);
   LaunchTiles<false>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);
@@ -184,8 +205,9 @@ int64_t shahd_tree_attention_workspace(const ShahdTreeCall* c) {
     SetError("%s: null argument", op);
     return SHAHD_EINVAL;
   }
-  int pairs, parts;
-  return TreeBytes(op, c, &pairs, &parts);
+  TreeLayout l;
+  const int rc = LayTree(op, c, &l);
+  return rc == SHAHD_OK ? l.bytes : rc;
 }
 
 int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
@@ -198,8 +220,9 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
   }
   TaArgs a = {};
   const int H = c->num_heads, Hk = c->cache.kv_heads, d = c->cache.head_dim;
-  const int64_t bytes = TreeBytes(op, c, &a.pairs, &a.nsplit);
-  if (bytes < 0) return (int)bytes;
+  TreeLayout lay;
+  const int rc = LayTree(op, c, &lay);
+  if (rc != SHAHD_OK) return rc;
   if (!CheckType(op, c->dtype, false) || !ScaleOf(op, c->scale, d, &a.scale_log2)) return SHAHD_EINVAL;
   if (c->rows < 0) {
     SetError("%s: need rows >= 0 (got %d)", op, c->rows);
@@ -211,13 +234,12 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
   if (c->n == 0 || c->rows == 0) return SHAHD_OK;
   a.G = H / Hk;
   a.TB = 128 / a.G;
-  const long long blocks = (long long)c->n * Hk * a.pairs * a.nsplit;
-  if (blocks > 0x7fffffffLL || ((long long)c->rows * H + 7) / 8 > 0x7fffffffLL) {
+  if (((long long)c->rows * H + 7) / 8 > 0x7fffffffLL) {
     SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
     return SHAHD_EINVAL;
   }
-  if (c->workspace_bytes < bytes) {
-    SetError("%s: needs %lld bytes of workspace, got %lld", op, (long long)bytes, (long long)c->workspace_bytes);
+  if (c->workspace_bytes < lay.bytes) {
+    SetError("%s: needs %lld bytes of workspace, got %lld", op, (long long)lay.bytes, (long long)c->workspace_bytes);
     return SHAHD_EINVAL;
   }
   BufferCheck b(op);
@@ -230,7 +252,7 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
   b.Add("out", c->out.data, 16);
   b.Add("cache.pool", c->cache.pool, 16);
   b.Add("cache.block_table", c->cache.block_table, 4);
-  if (bytes > 0) b.Add("workspace", c->workspace, 16);
+  if (lay.bytes > 0) b.Add("workspace", c->workspace, 32);
   if (b.rc != SHAHD_OK) return b.rc;
   const DeviceInfo info = InfoOf(b.device);
   DeviceScope scope(b.device);
@@ -257,10 +279,17 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
   a.max_blocks = c->cache.max_blocks;
   a.pages = c->cache.pages;
   a.max_nodes = c->max_nodes;
-  a.part_o = static_cast<float*>(c->workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)c->n * Hk * a.nsplit * c->max_nodes * a.G * d);
+  a.pairs = lay.pairs;
+  a.least = lay.least;
+  a.two_heads = lay.two_heads;
+  if (lay.bytes > 0) {
+    a.part_rows = lay.part_rows;
+    a.plan = static_cast<int*>(c->workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(c->workspace) + lay.plan_bytes);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * lay.grid * lay.part_rows * d);
+  }
   TakeLaunchError(nullptr);
-  LaunchTiles<true>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
+  LaunchTiles<true>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);
 }
 

@@ -6,8 +6,8 @@
 // A tile's rows are (token, query head of one kv head) pairs, tokens outside: 128/G tokens times G heads, so the G heads
 // that share keys sit in one tile, a decode step of few rows fills what it can, and a tile's last key block is cut close to
 // the diagonal. A block of threads works on two tiles at a time: on two neighbours that read the same keys, or, when a
-// sequence has only one tile of rows (decode steps, small trees), on that tile twice with the key blocks dealt out by turns
-// and one merge at the end, so there is always one tile's softmax under the other's products.
+// sequence has only one tile of rows (decode steps, small trees), on those of two kv heads or on one tile twice, with the key
+// blocks dealt out by turns and one merge at the end: so there is always one tile's softmax under the other's products.
 //
 //   S = Q K^T   tcgen05 M 128, N up to a block of 128 (head_dim 128) or 64 keys, into TMEM;
 //   softmax     one thread per row: the row's scores of a block in registers, running maximum and sum in 32 bits; the maximum
@@ -56,7 +56,7 @@ struct TaCfg {
   static constexpr int kHalf = kKeys * 128;            // a block's K or V: kHalves of these
   static constexpr int kUnit = kHalf * kHalves;
   static constexpr int kUnits = kWide ? 5 : 8;         // ring depth
-  static constexpr int kSmem = 1024 + 2 * kQTile + kUnits * kUnit + 512;
+  static constexpr int kSmem = 1024 + 2 * kQTile + kUnits * kUnit + 768 + 1024;
   static constexpr uint32_t kCols = kWide ? 512 : 256, kO = 2 * kKeys, kOStep = kWide ? 128 : 64;
   // of 16 pairs of probabilities, those that Exp2Poly takes
   static constexpr int kPoly = kWide ? TA_POLY128 : TA_POLY64;
@@ -66,11 +66,14 @@ struct TaCfg {
 constexpr int kTaRegsSoftmax = 216, kTaRegsIssue = 72;
 
 struct TaShared {
-  uint64_t full[8], empty[8], q_full, s_full[2], p_half[2], p_full[2], o_full[2], drained;
+  uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], ml_full, ml_free, drained;
+  uint64_t work_full[4];
+  int4 work[4][4];  // trees: what the block works on, by turns; the loading warp writes it
   uint32_t tmem;
   volatile int abort;
+  int found_seq, found_at, sums[12];  // trees: where the block's range begins
 };
-static_assert(sizeof(TaShared) <= 512, "TaShared");
+static_assert(sizeof(TaShared) <= 768, "TaShared");
 
 struct TaArgs {
   CUtensorMap qmap, kmap, vmap;  // rows: (value, head, row), boxes 64 x G x 128/G for q, 64 x 1 x 64 for k and v
@@ -84,9 +87,14 @@ struct TaArgs {
   const unsigned long long* masks;
   const int* lengths;
   const int* table;
-  int max_blocks, pages, max_nodes, pairs, nsplit;
-  float* part_o;    // [n, Hk, nsplit, max_nodes * G, D]
-  float2* part_ml;  // [n, Hk, nsplit, max_nodes * G]: running maximum (of scaled log2 scores) and sum
+  int max_blocks, pages, max_nodes, pairs, two_heads;  // two_heads: the pair's tiles are those of two kv heads
+  // All key blocks of all tile pairs in one line, dealt out to the blocks of threads in ranges of equal length, at least
+  // `least`: 0 where every pair has a block of threads of its own instead. A pair that a range cuts leaves parts: block of threads c
+  // has room for two, [2 c] for a pair that it does not begin and [2 c + 1] for one that it does not end.
+  int least, part_rows;
+  float* part_o;    // [2 grid, part_rows, D]
+  float2* part_ml;  // [2 grid, part_rows]: running maximum (of scaled log2 scores) and sum
+  int* plan;        // the ranges' length, then for every sequence the blocks of all before it, and their total
 };
 
 __device__ __forceinline__ void TmaLoad3D(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -192,6 +200,13 @@ __device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
   return Two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23)));
 }
 
+// 32 bytes at once: a whole sector, where 16-byte stores of lanes that lie a row apart write halves.
+__device__ __forceinline__ void Store32B(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 template <bool F16>
 __device__ __forceinline__ uint32_t Pack2(float a, float b) {  // a in the low half
   uint32_t r;
@@ -224,18 +239,24 @@ __device__ __forceinline__ bool TaWaitWarp(TaShared* sh, uint64_t* bar, uint32_t
   return false;
 }
 
-// What a block of threads works on.
+// What the two tiles are: neighbours of one kv head that read the same key blocks; one tile of rows, its key blocks dealt out by
+// turns and the results merged; or the one tile of rows of two kv heads, `head` and the next.
+enum TaMode { kShared = 0, kTurns = 1, kHeads = 2 };
+
+// What a block of threads works on at a time: key blocks of two tiles of rows.
 struct TaWork {
   int seq, start;       // sequence and its first row
   int head;             // kv head
   int q0;               // first token of tile 0 within the sequence
   int tokens0, tokens1;  // of the tiles
   int blocks0, blocks1;  // key blocks of the tiles
-  bool turns;           // one tile of rows, its key blocks dealt out by turns
+  int turns;            // kShared, kTurns or kHeads
   int first;            // trees: first key block
   int cached;           // trees: cached positions
   int cache_blocks;     // trees: key blocks of the cache
   int nodes;            // trees: rows of the sequence; prompts: tokens of the sequence
+  int part;             // trees: the place of the results among the block's parts, or -1: these are all key blocks
+  int more;             // trees: there is another pair behind this one
   __device__ __forceinline__ int Tokens(int i) const { return i ? tokens1 : tokens0; }
   __device__ __forceinline__ int Blocks(int i) const { return i ? blocks1 : blocks0; }
 };
@@ -266,40 +287,163 @@ __device__ __forceinline__ bool PromptWork(const TaArgs& A, int tile, TaWork& w)
   w.tokens1 = min(max(len - w.q0 - A.TB, 0), A.TB);
   w.blocks0 = (w.q0 + w.tokens0 + KEYS - 1) / KEYS;
   w.blocks1 = w.tokens1 > 0 ? (w.q0 + A.TB + w.tokens1 + KEYS - 1) / KEYS : 0;
-  w.turns = false;
+  w.turns = 0;
   w.first = w.cached = w.cache_blocks = 0;
+  w.part = -1;
   return true;
 }
 
+// A sequence of a tree call: its rows, cached positions, tile pairs and key blocks (its own rows are the last block).
 template <int KEYS>
-__device__ __forceinline__ bool TreeWork(const TaArgs& A, int x, TaWork& w) {
-  const int split = x % A.nsplit;
-  x /= A.nsplit;
-  const int pair = x % A.pairs;
-  x /= A.pairs;
-  w.head = x % A.Hk;
-  w.seq = x / A.Hk;
-  w.start = min(max(A.offsets[w.seq], 0), A.rows);
-  const int end = min(max(A.offsets[w.seq + 1], w.start), A.rows);
-  w.nodes = min(end - w.start, A.max_nodes);
-  w.q0 = pair * 2 * A.TB;
-  w.tokens0 = min(max(w.nodes - w.q0, 0), A.TB);
-  w.tokens1 = min(max(w.nodes - w.q0 - A.TB, 0), A.TB);
-  if (w.tokens0 == 0) return false;
-  w.cached = (int)min((long long)max(A.lengths[w.seq], 0), (long long)A.max_blocks * kOpsPage);
-  w.cache_blocks = (w.cached + KEYS - 1) / KEYS;
-  const int all = w.cache_blocks + 1;
-  w.first = (int)((long long)all * split / A.nsplit);
-  const int count = (int)((long long)all * (split + 1) / A.nsplit) - w.first;
-  w.turns = w.tokens1 == 0;
-  if (w.turns) {
-    w.tokens1 = w.tokens0;
-    w.blocks0 = (count + 1) / 2;
-    w.blocks1 = count / 2;
-  } else {
-    w.blocks0 = w.blocks1 = count;
+struct TreeSeq {
+  int start, nodes, cached, pairs, blocks;
+  __device__ __forceinline__ TreeSeq(const TaArgs& A, int s) {
+    start = min(max(A.offsets[s], 0), A.rows);
+    nodes = min(min(max(A.offsets[s + 1], start), A.rows) - start, A.max_nodes);
+    cached = (int)min((long long)max(A.lengths[s], 0), (long long)A.max_blocks * kOpsPage);
+    pairs = (nodes + 2 * A.TB - 1) / (2 * A.TB);
+    blocks = (cached + KEYS - 1) / KEYS + 1;
   }
+};
+
+// The key blocks of a tree call that this block of threads takes, pair by pair.
+template <int KEYS>
+struct TreeWalk {
+  const TaArgs& A;
+  TreeSeq<KEYS> q;         // of `seq`
+  int seq, item, at, pos, end;  // the pair's sequence, number in it and first block; the range that is left
+  // From block `at_` of sequence seq_'s on, pos_ in the line, to end_.
+  __device__ __forceinline__ TreeWalk(const TaArgs& a, int seq_, int at_, int pos_, int end_)
+      : A(a), q(a, seq_), seq(seq_), item(at_ / q.blocks), at(at_ - item * q.blocks), pos(pos_), end(end_) {}
+  // Tile pairs of a sequence.
+  static __device__ __forceinline__ int Items(const TaArgs& A, const TreeSeq<KEYS>& q) {
+    return A.two_heads ? (q.pairs > 0 ? A.Hk / 2 : 0) : A.Hk * q.pairs;
+  }
+  // The next pair's work; there is one (pos < end).
+  __device__ __forceinline__ TaWork Take() {
+    TaWork w;
+    const int count = min(q.blocks - at, end - pos);
+    w.seq = seq;
+    w.start = q.start;
+    w.nodes = q.nodes;
+    w.cached = q.cached;
+    w.cache_blocks = q.blocks - 1;
+    w.head = A.two_heads ? 2 * item : item / q.pairs;
+    w.q0 = A.two_heads ? 0 : (item - w.head * q.pairs) * 2 * A.TB;
+    w.tokens0 = min(w.nodes - w.q0, A.TB);
+    w.tokens1 = min(max(w.nodes - w.q0 - A.TB, 0), A.TB);
+    w.first = at;
+    w.part = count == q.blocks ? -1 : 2 * (int)blockIdx.x + (at > 0 ? 0 : 1);
+    w.turns = A.two_heads ? kHeads : w.tokens1 == 0 ? kTurns : kShared;
+    if (w.turns != kShared) w.tokens1 = w.tokens0;
+    if (w.turns == kTurns) {
+      w.blocks0 = (count + 1) / 2;
+      w.blocks1 = count / 2;
+    } else {
+      w.blocks0 = w.blocks1 = count;
+    }
+    pos += count;
+    w.more = pos < end;
+    if (w.more) {
+      item++;
+      at = 0;
+      while (item >= Items(A, q) && seq + 1 < A.n) {  // also past sequences without rows
+        item = 0;
+        q = TreeSeq<KEYS>(A, ++seq);
+      }
+    }
+    return w;
+  }
+};
+
+// Where this block of threads begins: the sequence, its key block in the line of the sequence's pairs, the range. All of its
+// threads take part; false: there is nothing for it.
+template <int KEYS>
+__device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& seq, int& at, int& pos, int& end) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto work = [&](int s) {
+    if (s >= A.n) return 0;
+    const TreeSeq<KEYS> q(A, s);
+    return TreeWalk<KEYS>::Items(A, q) * q.blocks;
+  };
+  if (A.least == 0) {
+    const int items = A.two_heads ? A.Hk / 2 : A.Hk * A.pairs;
+    seq = blockIdx.x / items;
+    const int item = blockIdx.x - seq * items;
+    const TreeSeq<KEYS> q(A, seq);
+    at = item * q.blocks;
+    pos = 0;
+    end = q.blocks;
+    return item < TreeWalk<KEYS>::Items(A, q);
+  }
+  const int first = work(threadIdx.x);
+  int sum = first;
+  for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sh->sums[warp] = sum;
+  __syncthreads();
+  int total = 0;
+  for (int k = 0; k < warps; k++) total += sh->sums[k];
+  const int per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  pos = (int)min((long long)blockIdx.x * per, (long long)total);
+  end = min(pos + per, total);
+  if (blockIdx.x == 0 && threadIdx.x == 0) A.plan[0] = per;
+  if (pos >= end && blockIdx.x != 0) return false;
+  int before = 0;
+  for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) sh->sums[warp] = incl;
+    __syncthreads();
+    int ahead = before;
+    for (int k = 0; k < warps; k++) {
+      if (k < warp) ahead += sh->sums[k];
+      before += sh->sums[k];
+    }
+    ahead += incl - mine;
+    if (blockIdx.x == 0 && s < A.n) A.plan[1 + s] = ahead;
+    if (pos < end && ahead <= pos && pos < ahead + mine) {
+      sh->found_seq = s;
+      sh->found_at = pos - ahead;
+    }
+  }
+  __syncthreads();
+  if (pos >= end) return false;
+  seq = sh->found_seq;
+  at = sh->found_at;
   return true;
+}
+
+__device__ __forceinline__ void PutWork(TaShared* sh, int slot, const TaWork& w) {
+  sh->work[slot][0] = make_int4(w.seq, w.start, w.head, w.q0);
+  sh->work[slot][1] = make_int4(w.tokens0, w.tokens1, w.blocks0, w.blocks1);
+  sh->work[slot][2] = make_int4(w.turns, w.first, w.cached, w.cache_blocks);
+  sh->work[slot][3] = make_int4(w.nodes, w.part, w.more, 0);
+}
+__device__ __forceinline__ void GetWork(const TaShared* sh, int slot, TaWork& w) {
+  const int4 a = sh->work[slot][0], b = sh->work[slot][1], c = sh->work[slot][2], d = sh->work[slot][3];
+  w.seq = Uniform(a.x);
+  w.start = Uniform(a.y);
+  w.head = Uniform(a.z);
+  w.q0 = Uniform(a.w);
+  w.tokens0 = Uniform(b.x);
+  w.tokens1 = Uniform(b.y);
+  w.blocks0 = Uniform(b.z);
+  w.blocks1 = Uniform(b.w);
+  w.turns = Uniform(c.x);
+  w.first = Uniform(c.y);
+  w.cached = Uniform(c.z);
+  w.cache_blocks = Uniform(c.w);
+  w.nodes = Uniform(d.x);
+  w.part = Uniform(d.y);
+  w.more = Uniform(d.z);
 }
 
 template <int KEYS, bool TREE>
@@ -307,7 +451,7 @@ struct TaBlocks {
   const TaArgs& A;
   const TaWork& w;
   // The key block of step t of tile i.
-  __device__ __forceinline__ int Index(int i, int t) const { return TREE ? (w.turns ? w.first + 2 * t + i : w.first + t) : t; }
+  __device__ __forceinline__ int Index(int i, int t) const { return TREE ? (w.turns == kTurns ? w.first + 2 * t + i : w.first + t) : t; }
   // Keys of a block that belong to the sequence (1 .. KEYS).
   __device__ __forceinline__ int Keys(int b) const {
     if constexpr (TREE) return b < w.cache_blocks ? min(KEYS, w.cached - KEYS * b) : w.nodes;
@@ -330,44 +474,49 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   uint8_t* ring = base + 2 * Cfg::kQTile;
   TaShared* sh = reinterpret_cast<TaShared*>(ring + U * Cfg::kUnit);
   const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (warp == 9 && lane < (TREE ? 4 : 3)) PrefetchTmaDesc(lane == 0 ? &A.qmap : lane == 1 ? &A.kmap : lane == 2 ? &A.vmap : &A.pool);
   GridDepWait();
   TaWork w;
+  int begin_seq = 0, begin_at = 0, begin_pos = 0, begin_end = 0;
   if constexpr (TREE) {
-    if (!TreeWork<KEYS>(A, blockIdx.x, w)) return;
+    if (!TreeBegin<KEYS>(A, sh, begin_seq, begin_at, begin_pos, begin_end)) return;
   } else {
     // the last tiles of a sequence are the longest: they start first
     const int x = gridDim.x - 1 - blockIdx.x;
     w.head = x % A.Hk;
     if (!PromptWork<KEYS>(A, x / A.Hk, w)) return;
+    w.seq = Uniform(w.seq);
+    w.start = Uniform(w.start);
+    w.q0 = Uniform(w.q0);
+    w.tokens0 = Uniform(w.tokens0);
+    w.tokens1 = Uniform(w.tokens1);
+    w.blocks0 = Uniform(w.blocks0);
+    w.blocks1 = Uniform(w.blocks1);
+    w.nodes = Uniform(w.nodes);
+    w.more = 0;
   }
-  w.seq = Uniform(w.seq);
-  w.start = Uniform(w.start);
-  w.q0 = Uniform(w.q0);
-  w.tokens0 = Uniform(w.tokens0);
-  w.tokens1 = Uniform(w.tokens1);
-  w.blocks0 = Uniform(w.blocks0);
-  w.blocks1 = Uniform(w.blocks1);
-  w.nodes = Uniform(w.nodes);
-  w.turns = TREE && Uniform(w.turns) != 0;
-  w.first = Uniform(w.first);
-  w.cached = Uniform(w.cached);
-  w.cache_blocks = Uniform(w.cache_blocks);
   const TaBlocks<KEYS, TREE> blk{A, w};
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < U; s++) {
-      MbarInit(&sh->full[s], 1);
-      MbarInit(&sh->empty[s], 1);
-    }
-    MbarInit(&sh->q_full, 1);
-    for (int i = 0; i < 2; i++) {
+  if (warp == 0) {
+    if (lane < U) {
+      MbarInit(&sh->full[lane], 1);
+      MbarInit(&sh->empty[lane], 1);
+    } else if (lane < U + 2) {
+      const int i = lane - U;
       MbarInit(&sh->s_full[i], 1);
       MbarInit(&sh->p_half[i], 128);
       MbarInit(&sh->p_full[i], 128);
       MbarInit(&sh->o_full[i], 1);
+    } else if (lane < U + 6) {
+      MbarInit(&sh->work_full[lane - U - 2], 1);
+    } else if (lane == U + 6) {
+      MbarInit(&sh->q_full, 1);
+      MbarInit(&sh->q_empty, 1);
+      MbarInit(&sh->ml_full, 128);
+      MbarInit(&sh->ml_free, 128);
+      MbarInit(&sh->drained, 1);
+      sh->abort = 0;
     }
-    MbarInit(&sh->drained, 1);
-    sh->abort = 0;
     FenceMbarInit();
   }
   if (warp == 8) {
@@ -378,79 +527,104 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   __syncthreads();
   TcgenFenceAfter();
   const uint32_t tmem = (uint32_t)Uniform((int)sh->tmem);
+  // The work behind this one, number `segment` (trees: the loading warp is ahead of the others by one at most, so four places
+  // are enough and none is waited for).
+  const auto next = [&](uint32_t segment, bool& ok) -> bool {
+    if (!TREE || !ok || !w.more) return false;
+    ok = TaWaitWarp(sh, &sh->work_full[segment & 3], (segment >> 2) & 1);
+    if (ok) GetWork(sh, segment & 3, w);
+    return ok;
+  };
   GridDepLaunch();  // after this block holds its TMEM
-  const int steps = max(w.blocks0, w.blocks1);
+  float* const sml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 768);  // tile 1's maxima and sums, for a merge
 
   if (warp >= 8) {
     if constexpr (Cfg::kWide) RegsDown<kTaRegsIssue>();
     if (warp == 9) {
-      if (lane == 0) {
-        FenceProxyAsyncGlobal();
-        const int tiles = !w.turns && w.tokens1 > 0 ? 2 : 1;
-        MbarArriveExpectTx(&sh->q_full, tiles * Cfg::kHalves * A.G * A.TB * 128);
-        for (int i = 0; i < tiles; i++)
-          for (int h = 0; h < Cfg::kHalves; h++)
-            TmaLoad3D(sQ + i * Cfg::kQTile + h * kTaQHalf, &A.qmap, &sh->q_full, 64 * h, w.head * A.G, w.start + w.q0 + i * A.TB);
-        int st = 0, issued = 0;
-        uint32_t round = 0;  // times the ring has been gone through
-        // one block's K or V into the next unit of the ring
-        const auto load = [&](int b, int keys, bool value) -> bool {
-          if (round > 0 && !TaWait(sh, &sh->empty[st], (round - 1) & 1)) return false;
-          uint8_t* dst = ring + st * Cfg::kUnit;
-          const int boxes = keys > 64 ? 2 : 1;
-          MbarArriveExpectTx(&sh->full[st], boxes * Cfg::kHalves * kTaBox);
+      // The whole warp follows the same path, lane 0 issues. Lane l holds the l-th page of the 32 that come next.
+      FenceProxyAsyncGlobal();
+      constexpr int kPages = KEYS / 64;  // of a block
+      int held = 0, ids = 0;             // the first of the 32 pages whose numbers the lanes hold
+      const auto hold = [&](int from) {
+        held = from;
+        const int p = from + lane;
+        ids = TREE && p < A.max_blocks ? A.table[(long long)w.seq * A.max_blocks + p] : -1;
+        if (ids < 0 || ids >= A.pages) ids = A.pages;  // behind the pool: TMA fills zeros, and the keys are masked
+      };
+      int st = 0, issued = 0;
+      uint32_t round = 0;  // times the ring has been gone through
+      // one block's K or V into the next unit of the ring
+      const auto load = [&](int b, int keys, bool value, int head) -> bool {
+        if (round > 0 && !TaWaitWarp(sh, &sh->empty[st], (round - 1) & 1)) return false;
+        uint8_t* dst = ring + st * Cfg::kUnit;
+        const int boxes = keys > 64 ? 2 : 1;
+        if (lane == 0) MbarArriveExpectTx(&sh->full[st], boxes * Cfg::kHalves * kTaBox);
+        if (TREE && b < w.cache_blocks && b * kPages + boxes > held + 32) hold((b - 2) * kPages);  // by turns, a block before the last one can follow it
 #pragma unroll 1
-          for (int x = 0; x < boxes; x++) {
-            if (TREE && b < w.cache_blocks) {
-              const int p = b * (KEYS / 64) + x;
-              int page = p < A.max_blocks ? A.table[(long long)w.seq * A.max_blocks + p] : -1;
-              if (page < 0 || page >= A.pages) page = A.pages;  // behind the pool: TMA fills zeros, and the keys are masked
+        for (int x = 0; x < boxes; x++) {
+          if (TREE && b < w.cache_blocks) {
+            const int page = __shfl_sync(0xffffffffu, ids, b * kPages + x - held);
+            if (lane == 0)
               for (int h = 0; h < Cfg::kHalves; h++)
-                TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, &A.pool, &sh->full[st], 64 * h, (w.head * 2 + (value ? 1 : 0)) * kOpsPage, page);
-            } else {
-              const int row = w.start + (TREE ? 0 : KEYS * b) + 64 * x;
-              for (int h = 0; h < Cfg::kHalves; h++)
-                TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, value ? &A.vmap : &A.kmap, &sh->full[st], 64 * h, w.head, row);
-            }
-          }
-          issued++;
-          if (++st == U) {
-            st = 0;
-            round++;
-          }
-          return true;
-        };
-        // the order in which the MMA warp takes them: K of the first blocks, then by steps V of this and K of the next one
-        bool ok = true;
-        if (w.turns) {
-          const auto one = [&](int i, int t, bool value) {
-            if (ok && t < w.Blocks(i)) ok = load(blk.Index(i, t), blk.Keys(blk.Index(i, t)), value);
-          };
-          one(0, 0, false);
-          one(1, 0, false);
-#pragma unroll 1
-          for (int t = 0; t < steps && ok; t++) {
-            one(0, t, true);
-            one(0, t + 1, false);
-            one(1, t, true);
-            one(1, t + 1, false);
-          }
-        } else {
-          const int last = w.tokens1 > 0 ? 1 : 0;  // of the two tiles it sees most
-          const auto one = [&](int t, bool value) {
-            if (ok && t < steps) ok = load(blk.Index(0, t), blk.Seen(last, blk.Index(0, t)), value);
-          };
-          one(0, false);
-#pragma unroll 1
-          for (int t = 0; t < steps && ok; t++) {
-            one(t, true);
-            one(t + 1, false);
+                TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, &A.pool, &sh->full[st], 64 * h, (head * 2 + (value ? 1 : 0)) * kOpsPage, page);
+          } else if (lane == 0) {
+            const int row = w.start + (TREE ? 0 : KEYS * b) + 64 * x;
+            for (int h = 0; h < Cfg::kHalves; h++)
+              TmaLoad3D(dst + h * Cfg::kHalf + x * kTaBox, value ? &A.vmap : &A.kmap, &sh->full[st], 64 * h, head, row);
           }
         }
-        // every copy lands before the block may leave: the last phase of each unit's barrier
-        MbarWaitBounded(&sh->q_full, 0, kOpsWaitLimit);
-        for (int v = max(0, issued - U); v < issued; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
-      }
+        issued++;
+        if (++st == U) {
+          st = 0;
+          round++;
+        }
+        return true;
+      };
+      // the order in which the MMA warp takes them: K of the first blocks, then by steps V of this and K of the next one, for
+      // both tiles at once or, by turns, for each
+      bool ok = true;
+      uint32_t segment = 0;
+      TreeWalk<KEYS> walk(A, begin_seq, begin_at, begin_pos, begin_end);
+      do {
+        if (segment > 0) ok = TaWaitWarp(sh, &sh->q_empty, (segment - 1) & 1);
+        if (!ok) break;
+        if constexpr (TREE) {
+          w = walk.Take();
+          if (lane == 0) {
+            PutWork(sh, segment & 3, w);
+            MbarArrive(&sh->work_full[segment & 3]);
+          }
+          __syncwarp();
+          GetWork(sh, segment & 3, w);
+        }
+        const int steps = max(w.blocks0, w.blocks1), last = w.tokens1 > 0 ? 1 : 0, units = w.turns ? 2 : 1;  // last: it sees most
+        const int tiles = w.turns != kTurns && w.tokens1 > 0 ? 2 : 1;
+        if (lane == 0) {
+          MbarArriveExpectTx(&sh->q_full, tiles * Cfg::kHalves * A.G * A.TB * 128);
+          for (int i = 0; i < tiles; i++)
+            for (int h = 0; h < Cfg::kHalves; h++)
+              TmaLoad3D(sQ + i * Cfg::kQTile + h * kTaQHalf, &A.qmap, &sh->q_full, 64 * h,
+                        (w.head + (w.turns == kHeads ? i : 0)) * A.G, w.start + w.q0 + (w.turns == kShared ? i * A.TB : 0));
+        }
+        segment++;
+        if (TREE) hold(w.first * kPages);
+        const auto one = [&](int i, int t, bool value) {
+          if (!ok || t >= (w.turns ? w.Blocks(i) : steps)) return;
+          const int b = blk.Index(i, t);
+          ok = load(b, w.turns ? blk.Keys(b) : blk.Seen(last, b), value, w.head + (w.turns == kHeads ? i : 0));
+        };
+        for (int i = 0; i < units; i++) one(i, 0, false);
+#pragma unroll 1
+        for (int t = 0; t < steps && ok; t++)
+#pragma unroll 1
+          for (int i = 0; i < units; i++) {
+            one(i, t, true);
+            one(i, t + 1, false);
+          }
+      } while (ok && w.more);
+      // every copy lands before the block may leave: the last phase of each unit's barrier
+      if (segment > 0) MbarWaitBounded(&sh->q_full, (segment - 1) & 1, kOpsWaitLimit);
+      for (int v = max(0, issued - U); v < issued; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
     } else if (warp == 8) {
       // The whole warp follows the same path, one lane of it issues.
       constexpr uint32_t kTypes = F16 ? 0u : (1u << 7) | (1u << 10);
@@ -469,14 +643,15 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         }
         return at;
       };
-      const auto wait = [&](uint64_t* bar, int t) { ok = ok && TaWaitWarp(sh, bar, (uint32_t)(t & 1)); };
+      int done0 = 0, done1 = 0;  // steps of the tiles in the segments before this one: barriers count on
+      const auto wait = [&](uint64_t* bar, int i, int t) { ok = ok && TaWaitWarp(sh, bar, (uint32_t)((t + (i ? done1 : done0)) & 1)); };
       const uint64_t qdesc = SmemDescSw128(SmemAddr(sQ)), kdesc = SmemDescSw128(SmemAddr(ring));
       // MN-major, 128-byte swizzle: 64-value columns kHalf apart, groups of 8 keys 1024 bytes apart
       const uint64_t vdesc = (uint64_t)((SmemAddr(ring) & 0x3FFFF) >> 4) | (uint64_t)(Cfg::kHalf >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
                              (uint64_t)1 << 46 | (uint64_t)2 << 61;
       const auto scores = [&](int i, int t, int unit) {
         const int kc = (blk.Seen(i, blk.Index(i, t)) + 15) & ~15;
-        const uint64_t a = qdesc + (uint64_t)((w.turns ? 0 : i) * (Cfg::kQTile >> 4)), b = kdesc + (uint64_t)(unit * (Cfg::kUnit >> 4));
+        const uint64_t a = qdesc + (uint64_t)((w.turns == kTurns ? 0 : i) * (Cfg::kQTile >> 4)), b = kdesc + (uint64_t)(unit * (Cfg::kUnit >> 4));
         const uint32_t idesc = idesc0 | ((uint32_t)(kc >> 3) << 17);
         TcgenFenceAfter();
 #pragma unroll
@@ -496,12 +671,12 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           for (int kk = from; kk < to; kk++) UmmaIssueTS(d, a + 8u * kk, b + (uint64_t)(kk * (2048 >> 4)), idesc_pv, kk > 0 ? 1u : more);
         };
         if (Cfg::kWide && steps16 == kFull16) {
-          wait(&sh->p_half[i], t);
+          wait(&sh->p_half[i], i, t);
           if (!ok) return;
           TcgenFenceAfter();
           some(0, 4);
         }
-        wait(&sh->p_full[i], t);
+        wait(&sh->p_full[i], i, t);
         if (!ok) return;
         TcgenFenceAfter();
         if (steps16 == kFull16) {
@@ -525,58 +700,51 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         FenceProxyAsyncShared();
         __syncwarp();
       };
-      ok = TaWaitWarp(sh, &sh->q_full, 0);
-      if (w.turns) {
-        // each unit serves one tile
+      uint32_t segment = 0;
+      if constexpr (TREE) w.more = 1;
+      while (segment == 0 && !TREE ? true : next(segment, ok)) {
+        const int steps = max(w.blocks0, w.blocks1);
+        // A unit serves one tile, or both that share their keys: then the last tile of a step (tile 1, if there is one: blocks0 <= blocks1)
+        // releases it.
+        const int last = w.blocks1 > 0 ? 1 : 0;
+        ok = TaWaitWarp(sh, &sh->q_full, segment & 1);
+        segment++;
+        int kunit = 0, vunit = 0;
         const auto next_scores = [&](int i, int t) {
           if (!ok || t >= w.Blocks(i)) return;
-          const int unit = acquire();
+          if (w.turns) kunit = acquire();
           if (!ok) return;
-          scores(i, t, unit);
-          release(unit);
+          scores(i, t, kunit);
+          if (w.turns || i == last) release(kunit);
         };
         const auto next_values = [&](int i, int t) {
           if (!ok || t >= w.Blocks(i)) return;
-          const int unit = acquire();
-          trim(blk.Index(i, t), unit);
-          values(i, t, unit);
-          if (ok) release(unit);
+          if (w.turns) {
+            vunit = acquire();
+            trim(blk.Index(i, t), vunit);
+          }
+          values(i, t, vunit);
+          if (ok && (w.turns || i == last)) release(vunit);
         };
+        if (!w.turns) kunit = acquire();
         next_scores(0, 0);
         next_scores(1, 0);
+        if (steps == 1 && ok) UmmaIssueCommit(&sh->q_empty);
 #pragma unroll 1
         for (int t = 0; t < steps && ok; t++) {
+          if (!w.turns) {  // both units of the step ahead of the first wait for probabilities
+            vunit = acquire();
+            trim(blk.Index(0, t), vunit);
+            if (t + 1 < steps) kunit = acquire();
+          }
           next_values(0, t);
           next_scores(0, t + 1);
           next_values(1, t);
           next_scores(1, t + 1);
+          if (t + 2 == steps && ok) UmmaIssueCommit(&sh->q_empty);  // the last scores: Q may be replaced behind them
         }
-      } else if (steps > 0) {
-        // the tiles share the units, and the last tile of a step (tile 1, if there is one: blocks0 <= blocks1) releases them
-        const int last = w.blocks1 > 0 ? 1 : 0;
-        int unit = acquire();
-        if (ok) {
-          scores(0, 0, unit);
-          if (last) scores(1, 0, unit);
-          release(unit);
-        }
-#pragma unroll 1
-        for (int t = 0; t < steps && ok; t++) {
-          const int vunit = acquire();
-          trim(blk.Index(0, t), vunit);
-          if (t + 1 < steps) unit = acquire();
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            if (!ok || t >= w.Blocks(i)) continue;
-            values(i, t, vunit);
-            if (!ok) continue;
-            if (i == last) release(vunit);
-            if (t + 1 < w.Blocks(i)) {
-              scores(i, t + 1, unit);
-              if (i == last) release(unit);
-            }
-          }
-        }
+        done0 += w.blocks0;
+        done1 += w.blocks1;
       }
       UmmaIssueCommit(&sh->drained);
       __syncwarp();
@@ -587,34 +755,43 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     // ---- softmax: thread = row of its tile = TMEM lane ----
     const int i = warp >> 2, r = threadIdx.x & 127;
     const int token = r / A.G, g = r - token * A.G;
-    const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
-    const bool mine = token < w.Tokens(i);
-    const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t scol = lanes + (uint32_t)(KEYS * i), ocol = lanes + Cfg::kO + Cfg::kOStep * i;
     const float sc = A.scale_log2;
     constexpr float kBias = F16 ? 7.f : 0.f;  // probabilities up to 2^15 in fp16: 7 more bits above its smallest numbers
-    float m = -INFINITY, l = 0.f;
     bool ok = true;
+    uint32_t done = 0, outs0 = 0, outs1 = 0, merges = 0;  // of the segments so far: this tile's steps, the tiles' results, merges
+    uint32_t segment = 0;
+    if constexpr (TREE) w.more = 1;
+    while (segment == 0 && !TREE ? true : next(segment, ok)) {
+    segment++;
+    const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
+    const bool mine = token < w.Tokens(i);
+    const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
+    float m = -INFINITY, l = 0.f;
 #pragma unroll 1
     for (int t = 0; t < w.Blocks(i); t++) {
       const int b = blk.Index(i, t), seen = blk.Seen(i, b);
       bool cut;  // some row does not see all keys of a whole block
       bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
+      int page0 = 0, page1 = 0;           // read ahead of the wait, looked at behind it
       if constexpr (TREE) {
-        cut = seen < KEYS || b >= w.cache_blocks;
         if (b < w.cache_blocks) {
           const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
-          gone0 = (unsigned)tb[0] >= (unsigned)A.pages;
-          if (KEYS == 128 && seen > 64) gone1 = (unsigned)tb[1] >= (unsigned)A.pages;
-          cut = __any_sync(0xffffffffu, cut || gone0 || gone1);
+          page0 = tb[0];
+          if (KEYS == 128 && seen > 64) page1 = tb[1];
         }
+      }
+      ok = TaWait(sh, &sh->s_full[i], (done + t) & 1);
+      if (!ok) break;
+      TcgenFenceAfter();
+      if constexpr (TREE) {
+        gone0 = (unsigned)page0 >= (unsigned)A.pages;
+        gone1 = (unsigned)page1 >= (unsigned)A.pages;
+        cut = seen < KEYS || b >= w.cache_blocks || __any_sync(0xffffffffu, gone0 || gone1);
       } else {
         cut = tok0 < KEYS * b + KEYS - 1 || seen < KEYS;
       }
-      ok = TaWait(sh, &sh->s_full[i], (uint32_t)(t & 1));
-      if (!ok) break;
-      TcgenFenceAfter();
       if (!busy) {
         if (Cfg::kWide) MbarArrive(&sh->p_half[i]);
       } else {
@@ -670,7 +847,9 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         if (t == 0) {
           m = mx;
-        } else if (__any_sync(0xffffffffu, (mx - m) * sc > kTaLazy)) {
+        } else if (__any_sync(0xffffffffu, mine && (mx - m) * sc > kTaLazy)) {
+          // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
+          // or a result's last bits would hang on them)
           // step t-1's products are complete: S of step t was issued behind them
           const float mn = fmaxf(m, mx);
           const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
@@ -729,39 +908,20 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       MbarArrive(&sh->p_full[i]);
     }
     // ---- the rows' results ----
-    const bool merge = TREE && w.turns && w.blocks1 > 0;
-    bool have = w.Blocks(i) > 0;
-    if (have) have = TaWait(sh, &sh->o_full[i], 0);
-    float* shared_o = reinterpret_cast<float*>(ring);  // tile 1's accumulator: [value][row], then its maximum and sum
-    if (merge) {
-      if (i == 1) {
-        have = TaWait(sh, &sh->o_full[0], 0) && have;  // all loads and products are done: the ring is free
-        TcgenFenceAfter();
-        if (busy) {
-#pragma unroll 1
-          for (int c = 0; c < D / 16; c++) {
-            uint32_t o[16];
-            TmemLoad16(ocol + 16u * c, o);
-            TmemWaitLd();
-            if (have) {
-#pragma unroll
-              for (int k = 0; k < 16; k++) shared_o[(16 * c + k) * 128 + r] = __uint_as_float(o[k]);
-            }
-          }
-          if (have) {
-            shared_o[D * 128 + r] = m;
-            shared_o[D * 128 + 128 + r] = l;
-          }
-        }
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
-    if (busy && !(w.turns && i == 1)) {
-      TcgenFenceAfter();
+    done += w.Blocks(i);
+    const bool merge = TREE && w.turns == kTurns && w.blocks1 > 0;
+    if (w.Blocks(i) > 0) ok = ok && TaWait(sh, &sh->o_full[i], (i ? outs1 : outs0) & 1);
+    if (merge && i == 1) {
+      // the same rows' other key blocks: tile 0's threads read this accumulator, in the same lanes, too
+      sml[r] = m;
+      sml[128 + r] = l;
+      MbarArrive(&sh->ml_full);
+      ok = TaWait(sh, &sh->ml_free, merges & 1) && ok;  // before the next segment's products may write over it
+    } else if (!(w.turns == kTurns && i == 1)) {
       float a0 = 1.f, a1 = 0.f;
       if (merge) {
-        const float m2 = shared_o[D * 128 + r], l2 = shared_o[D * 128 + 128 + r];
-        const float mn = fmaxf(m, m2);
+        ok = ok && TaWait(sh, &sh->ml_full, merges & 1) && TaWait(sh, &sh->o_full[1], outs1 & 1);
+        const float m2 = sml[r], l2 = sml[128 + r], mn = fmaxf(m, m2);
         if (mn != -INFINITY) {
           a0 = Exp2((m - mn) * sc);
           a1 = Exp2((m2 - mn) * sc);
@@ -769,45 +929,55 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         m = mn;
         l = l * a0 + l2 * a1;
       }
-      const bool parts = TREE && A.nsplit > 1;
-      if (!parts) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
-        a0 *= inv;
-        a1 *= inv;
-      }
-      const bool zero = !parts && l == 0.f;
-      const int node = tok0 + token;
-      uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)(w.head * A.G + g) * A.out_head;
-      const long long slot =
-          parts ? ((long long)(w.seq * A.Hk + w.head) * A.nsplit + blockIdx.x % A.nsplit) * (A.max_nodes * A.G) + node * A.G + g : 0;
+      if (busy && ok) {
+        TcgenFenceAfter();
+        const bool parts = TREE && w.part >= 0;
+        if (!parts) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
+          a0 *= inv;
+          a1 *= inv;
+        }
+        const bool zero = !parts && l == 0.f;
+        const int node = tok0 + token;
+        uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
+        const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; c++) {
-        uint32_t o[16];
-        if (have) {
+        for (int c = 0; c < D / 16; c++) {
+          uint32_t o[16], o1[16];
           TmemLoad16(ocol + 16u * c, o);
+          if (merge) TmemLoad16(ocol + Cfg::kOStep + 16u * c, o1);
           TmemWaitLd();
-        }
-        float v[16];
+          float v[16];
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
-          v[k] = have && !zero ? __uint_as_float(o[k]) * a0 : 0.f;
-          if (merge && !zero) v[k] = fmaf(shared_o[(16 * c + k) * 128 + r], a1, v[k]);
-        }
-        if (mine && ok) {
-          if (parts) {
-            float4* dst = reinterpret_cast<float4*>(A.part_o + slot * D + 16 * c);
+          for (int k = 0; k < 16; k++) {
+            v[k] = __uint_as_float(o[k]) * a0;
+            if (merge) v[k] = fmaf(__uint_as_float(o1[k]), a1, v[k]);
+            if (zero) v[k] = 0.f;
+          }
+          if (mine) {
+            if (parts) {
+              float* dst = A.part_o + slot * D + 16 * c;
 #pragma unroll
-            for (int k = 0; k < 4; k++) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(out + 16 * c);
+              for (int k = 0; k < 16; k += 8) Store32B(dst + k, v + k);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(out + 16 * c);
 #pragma unroll
-            for (int k = 0; k < 2; k++)
-              dst[k] = make_uint4(Pack2<F16>(v[8 * k], v[8 * k + 1]), Pack2<F16>(v[8 * k + 2], v[8 * k + 3]),
-                                  Pack2<F16>(v[8 * k + 4], v[8 * k + 5]), Pack2<F16>(v[8 * k + 6], v[8 * k + 7]));
+              for (int k = 0; k < 2; k++)
+                dst[k] = make_uint4(Pack2<F16>(v[8 * k], v[8 * k + 1]), Pack2<F16>(v[8 * k + 2], v[8 * k + 3]),
+                                    Pack2<F16>(v[8 * k + 4], v[8 * k + 5]), Pack2<F16>(v[8 * k + 6], v[8 * k + 7]));
+            }
           }
         }
+        if (parts && mine) A.part_ml[slot] = make_float2(m * sc, l);
       }
-      if (parts && mine && ok) A.part_ml[slot] = make_float2(m * sc, l);
+      if (merge) {
+        TcgenFenceBefore();
+        MbarArrive(&sh->ml_free);
+      }
+    }
+    outs0 += w.blocks0 > 0;
+    outs1 += w.blocks1 > 0;
+    merges += merge;
     }
   }
   TcgenFenceBefore();
@@ -816,7 +986,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   if (warp == 8) TmemDealloc(tmem, Cfg::kCols);
 }
 
-// Joins the parts of a tree call's rows: one warp per (row, query head), D / 32 values per lane.
+// Joins the parts of a tree call's rows: one warp per (row, query head), D / 32 values per lane. Rows whose tile pair was not
+// cut have their results already.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) TreeJoinKernel(const __grid_constant__ TaArgs A) {
   GridDepWait();
@@ -825,18 +996,25 @@ __global__ void __launch_bounds__(256) TreeJoinKernel(const __grid_constant__ Ta
   if (item >= (long long)A.rows * A.H) return;
   const int row = (int)(item / A.H), h = (int)(item - (long long)row * A.H);
   if (row < A.offsets[0] || row >= A.offsets[A.n]) return;
-  const int s = SequenceOf(A.offsets, A.n, row), node = row - A.offsets[s];
-  if (node >= A.max_nodes) return;
-  const int kv = h / A.G, stride = A.max_nodes * A.G;
-  const long long slot = ((long long)s * A.Hk + kv) * A.nsplit * stride + node * A.G + (h - kv * A.G);
+  const int s = SequenceOf(A.offsets, A.n, row);
+  const TreeSeq<TaCfg<D>::kKeys> q(A, s);
+  const int node = row - q.start;
+  if (node >= q.nodes) return;
+  const int pair = node / (2 * A.TB), kv = h / A.G, per = A.plan[0];
+  const int from = A.plan[1 + s] + (kv * q.pairs + pair) * q.blocks, c0 = from / per, c1 = (from + q.blocks - 1) / per;
+  if (c0 == c1) return;
+  const int local = (node - pair * 2 * A.TB) * A.G + h - kv * A.G;
+  // the block of threads that begins the pair holds its part in its second place, the others in their first
+  const auto slot = [&](int c) { return (long long)(2 * c + (c == c0 ? 1 : 0)) * A.part_rows + local; };
   float m = -INFINITY;
-  for (int k = 0; k < A.nsplit; k++) m = fmaxf(m, A.part_ml[slot + (long long)k * stride].x);
+  for (int c = c0; c <= c1; c++) m = fmaxf(m, A.part_ml[slot(c)].x);
   float l = 0.f, v[D / 32] = {};
-  for (int k = 0; k < A.nsplit; k++) {
-    const float2 ml = A.part_ml[slot + (long long)k * stride];
+#pragma unroll 2
+  for (int c = c0; c <= c1; c++) {
+    const float2 ml = A.part_ml[slot(c)];
     const float a = m == -INFINITY ? 0.f : Exp2(ml.x - m);
     l = fmaf(ml.y, a, l);
-    const float* o = A.part_o + (slot + (long long)k * stride) * D + lane * (D / 32);
+    const float* o = A.part_o + slot(c) * D + lane * (D / 32);
 #pragma unroll
     for (int j = 0; j < D / 32; j++) v[j] = fmaf(o[j], a, v[j]);
   }

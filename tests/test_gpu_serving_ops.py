@@ -355,6 +355,24 @@ def test_tree_attention_many_sequences(nodes):
     assert torch.equal(out, _tree(q, k, v, cache, lengths, masks, counts, BF16, max_nodes=nodes))
 
 
+@pytest.mark.parametrize("n,heads,nodes,most", [(90, (8, 4, 128), 5, 700), (330, (4, 1, 64), 3, 500), (80, (6, 2, 32), 64, 900), (20, (32, 8, 128), 64, 6000),
+                                                (1300, (2, 1, 64), 2, 300), (5, (16, 2, 64), 33, 9000)], ids=str)
+def test_tree_attention_layouts_of_the_work(n, heads, nodes, most):
+    """Pairs of heads, pairs of row tiles and ranges cut across sequences, empty ones among them, more sequences than threads."""
+    H, Hk, d = heads
+    rng = np.random.default_rng(n)
+    lengths, counts = rng.integers(0, most, n).tolist(), rng.integers(0, nodes + 1, n).tolist()
+    lengths[0], counts[n // 2], counts[-1] = most, nodes, 0
+    g = _gen(16)
+    q, k, v = (_normal(g, max(sum(counts), 1), h, d, dtype=F16) for h in (H, Hk, Hk))
+    pool, table, cache = _cache_of(lengths, Hk, d, F16, g)
+    pool.normal_(generator=g)
+    masks = _random_masks(counts, 8)
+    out = _tree(q, k, v, cache, lengths, masks, counts, F16, max_nodes=nodes)
+    _check_tree(q, k, v, pool, table, lengths, masks, counts, out, F16, seqs=set(rng.integers(0, n, 16).tolist()) | {0, n // 2})
+    assert torch.equal(out, _tree(q, k, v, cache, lengths, masks, counts, F16, max_nodes=nodes))
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("n", [1, 40])
 def test_tree_attention_reads_nothing_behind_the_lengths(bad, n):
