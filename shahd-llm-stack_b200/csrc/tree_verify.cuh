@@ -150,13 +150,13 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
     float x[VerifyRows<T>::PER];
     const uint4* vp = reinterpret_cast<const uint4*>(rows.p - rows.mis);
     const uint4* vq = reinterpret_cast<const uint4*>(rows.q - rows.mis);
-    int c = rows.whole0 + lane;
-    for (; c + 96 < rows.whole1; c += 128) {  // four pieces of each row in flight
+    for (int c = rows.whole0 + lane; c < rows.whole1; c += 128) {  // four pieces of each row in flight
       uint4 u[4], v[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        u[k] = LoadNc16(vp + c + 32 * k);
-        v[k] = w != 0 ? LoadNc16(vq + c + 32 * k) : make_uint4(0, 0, 0, 0);
+        const bool in = c + 32 * k < rows.whole1;
+        u[k] = in ? LoadNc16(vp + c + 32 * k) : make_uint4(0, 0, 0, 0);
+        v[k] = in && w != 0 ? LoadNc16(vq + c + 32 * k) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -164,11 +164,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
         z += rows.Sum(x);
       }
     }
-    for (; c < rows.whole1; c += 32) {
-      rows.Whole(LoadNc16(vp + c), w != 0 ? LoadNc16(vq + c) : make_uint4(0, 0, 0, 0), hi, lo, x);
-      z += rows.Sum(x);
-    }
-    for (c = rows.first + lane; c < rows.last; c += 32) {
+    for (int c = rows.first + lane; c < rows.last; c += 32) {
       if (c >= rows.whole0 && c < rows.whole1) continue;
       rows.Any(c, hi, lo, x);
       z += rows.Sum(x);
