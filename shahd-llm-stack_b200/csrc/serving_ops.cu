@@ -68,21 +68,20 @@ bool ScaleOf(const char* op, double scale, int d, float* log2) {
   return true;
 }
 
-template <int D, bool F16, bool TREE>
+template <int D, bool F16, int KIND>
 void LaunchTiles(const TaArgs& a, unsigned blocks, cudaStream_t st) {
-  if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, TREE>, TaCfg<D>::kSmem)) return;
-  LaunchPdl(TileAttentionKernel<D, F16, TREE>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
-  if constexpr (TREE)
-    if (a.least > 0)
-      LaunchPdl(TreeJoinKernel<D, F16>, dim3((unsigned)(((long long)a.rows * a.H + 7) / 8)), dim3(256), 0, st, a);
+  if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, KIND>, TaCfg<D>::kSmem)) return;
+  LaunchPdl(TileAttentionKernel<D, F16, KIND>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
+  if constexpr (KIND == kTreeRanges)
+    LaunchPdl(TreeJoinKernel<D, F16>, dim3((unsigned)(((long long)a.rows * a.H + 7) / 8)), dim3(256), 0, st, a);
 }
 
-template <bool TREE>
+template <int KIND>
 void LaunchTiles(int d, int dtype, const TaArgs& a, unsigned blocks, cudaStream_t st) {
   const bool f16 = dtype == SHAHD_F16;
-  if (d == 32) f16 ? LaunchTiles<32, true, TREE>(a, blocks, st) : LaunchTiles<32, false, TREE>(a, blocks, st);
-  else if (d == 64) f16 ? LaunchTiles<64, true, TREE>(a, blocks, st) : LaunchTiles<64, false, TREE>(a, blocks, st);
-  else f16 ? LaunchTiles<128, true, TREE>(a, blocks, st) : LaunchTiles<128, false, TREE>(a, blocks, st);
+  if (d == 32) f16 ? LaunchTiles<32, true, KIND>(a, blocks, st) : LaunchTiles<32, false, KIND>(a, blocks, st);
+  else if (d == 64) f16 ? LaunchTiles<64, true, KIND>(a, blocks, st) : LaunchTiles<64, false, KIND>(a, blocks, st);
+  else f16 ? LaunchTiles<128, true, KIND>(a, blocks, st) : LaunchTiles<128, false, KIND>(a, blocks, st);
 }
 
 bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, const ShahdRows& q, const ShahdRows& k, const ShahdRows& v, TaArgs* a) {
@@ -193,7 +192,7 @@ int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
   a.H = H;
   a.Hk = Hk;
   TakeLaunchError(nullptr);
-  LaunchTiles<false>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
+  LaunchTiles<kPrompt>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);
 }
 
@@ -289,7 +288,8 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * lay.grid * lay.part_rows * d);
   }
   TakeLaunchError(nullptr);
-  LaunchTiles<true>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
+  if (lay.least > 0) LaunchTiles<kTreeRanges>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
+  else LaunchTiles<kTreePairs>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);
 }
 

@@ -24,12 +24,6 @@
 // the third warpgroup, which gives registers to the other two.
 #pragma once
 
-#ifndef TA_POLY128
-#define TA_POLY128 4
-#endif
-#ifndef TA_POLY64
-#define TA_POLY64 2
-#endif
 
 #include "ops_common.cuh"
 #include "rope.cuh"
@@ -59,7 +53,7 @@ struct TaCfg {
   static constexpr int kSmem = 1024 + 2 * kQTile + kUnits * kUnit + 768 + 1024;
   static constexpr uint32_t kCols = kWide ? 512 : 256, kO = 2 * kKeys, kOStep = kWide ? 128 : 64;
   // of 16 pairs of probabilities, those that Exp2Poly takes
-  static constexpr int kPoly = kWide ? TA_POLY128 : TA_POLY64;
+  static constexpr int kPoly = kWide ? 3 : 2;
 };
 // Registers at head_dim 128: launched with 168 per thread (384 x 168 = 64512). The two softmax warpgroups take 216 each, the third
 // one, whose warps issue copies and products, keeps 72: 2 x 128 x 216 + 128 x 72 = 64512.
@@ -67,7 +61,7 @@ constexpr int kTaRegsSoftmax = 216, kTaRegsIssue = 72;
 
 struct TaShared {
   uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], ml_full, ml_free, drained;
-  uint64_t work_full[4];
+  uint64_t work_full[4], work_read[4];
   int4 work[4][4];  // trees: what the block works on, by turns; the loading warp writes it
   uint32_t tmem;
   volatile int abort;
@@ -239,6 +233,13 @@ __device__ __forceinline__ bool TaWaitWarp(TaShared* sh, uint64_t* bar, uint32_t
   return false;
 }
 
+// Two barriers under one vote.
+__device__ __forceinline__ bool TaWaitWarp2(TaShared* sh, uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+  const bool ra = MbarTryWait(a, pa), rb = MbarTryWait(b, pb);
+  if (__all_sync(0xffffffffu, ra && rb)) return true;
+  return TaWaitWarp(sh, a, pa) && TaWaitWarp(sh, b, pb);
+}
+
 // What the two tiles are: neighbours of one kv head that read the same key blocks; one tile of rows, its key blocks dealt out by
 // turns and the results merged; or the one tile of rows of two kv heads, `head` and the next.
 enum TaMode { kShared = 0, kTurns = 1, kHeads = 2 };
@@ -356,9 +357,13 @@ struct TreeWalk {
   }
 };
 
+struct NoWalk {  // where there are no ranges
+  __device__ __forceinline__ NoWalk(const TaArgs&, int, int, int, int) {}
+};
+
 // Where this block of threads begins: the sequence, its key block in the line of the sequence's pairs, the range. All of its
 // threads take part; false: there is nothing for it.
-template <int KEYS>
+template <int KEYS, bool RANGES>
 __device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& seq, int& at, int& pos, int& end) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto work = [&](int s) {
@@ -366,7 +371,7 @@ __device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& se
     const TreeSeq<KEYS> q(A, s);
     return TreeWalk<KEYS>::Items(A, q) * q.blocks;
   };
-  if (A.least == 0) {
+  if constexpr (!RANGES) {
     const int items = A.two_heads ? A.Hk / 2 : A.Hk * A.pairs;
     seq = blockIdx.x / items;
     const int item = blockIdx.x - seq * items;
@@ -375,50 +380,51 @@ __device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& se
     pos = 0;
     end = q.blocks;
     return item < TreeWalk<KEYS>::Items(A, q);
-  }
-  const int first = work(threadIdx.x);
-  int sum = first;
-  for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
+  } else {
+    const int first = work(threadIdx.x);
+    int sum = first;
+    for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) sh->sums[warp] = sum;
-  __syncthreads();
-  int total = 0;
-  for (int k = 0; k < warps; k++) total += sh->sums[k];
-  const int per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-  pos = (int)min((long long)blockIdx.x * per, (long long)total);
-  end = min(pos + per, total);
-  if (blockIdx.x == 0 && threadIdx.x == 0) A.plan[0] = per;
-  if (pos >= end && blockIdx.x != 0) return false;
-  int before = 0;
-  for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
-    int incl = mine;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sh->sums[warp] = sum;
+    __syncthreads();
+    int total = 0;
+    for (int k = 0; k < warps; k++) total += sh->sums[k];
+    const int per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    pos = (int)min((long long)blockIdx.x * per, (long long)total);
+    end = min(pos + per, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) A.plan[0] = per;
+    if (pos >= end && blockIdx.x != 0) return false;
+    int before = 0;
+    for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
+      const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
+      int incl = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      __syncthreads();
+      if (lane == 31) sh->sums[warp] = incl;
+      __syncthreads();
+      int ahead = before;
+      for (int k = 0; k < warps; k++) {
+        if (k < warp) ahead += sh->sums[k];
+        before += sh->sums[k];
+      }
+      ahead += incl - mine;
+      if (blockIdx.x == 0 && s < A.n) A.plan[1 + s] = ahead;
+      if (pos < end && ahead <= pos && pos < ahead + mine) {
+        sh->found_seq = s;
+        sh->found_at = pos - ahead;
+      }
     }
     __syncthreads();
-    if (lane == 31) sh->sums[warp] = incl;
-    __syncthreads();
-    int ahead = before;
-    for (int k = 0; k < warps; k++) {
-      if (k < warp) ahead += sh->sums[k];
-      before += sh->sums[k];
-    }
-    ahead += incl - mine;
-    if (blockIdx.x == 0 && s < A.n) A.plan[1 + s] = ahead;
-    if (pos < end && ahead <= pos && pos < ahead + mine) {
-      sh->found_seq = s;
-      sh->found_at = pos - ahead;
-    }
+    if (pos >= end) return false;
+    seq = sh->found_seq;
+    at = sh->found_at;
+    return true;
   }
-  __syncthreads();
-  if (pos >= end) return false;
-  seq = sh->found_seq;
-  at = sh->found_at;
-  return true;
 }
 
 __device__ __forceinline__ void PutWork(TaShared* sh, int slot, const TaWork& w) {
@@ -464,8 +470,14 @@ struct TaBlocks {
   }
 };
 
-template <int D, bool F16, bool TREE>
+// Prompts; trees with a block of threads for every tile pair; trees with a range of key blocks for every block of threads, pair after
+// pair. (Pairs on their own are worth a kernel: what goes on from one pair to the next takes registers that head_dim 64
+// does not have, and 256 single tokens over 512 positions took 27 us instead of TREEONE.)
+enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2 };
+
+template <int D, bool F16, int KIND>
 __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAttentionKernel(const __grid_constant__ TaArgs A) {
+  constexpr bool TREE = KIND != kPrompt, RANGES = KIND == kTreeRanges;
   using Cfg = TaCfg<D>;
   constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
   extern __shared__ uint8_t ta_raw[];
@@ -479,21 +491,31 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   TaWork w;
   int begin_seq = 0, begin_at = 0, begin_pos = 0, begin_end = 0;
   if constexpr (TREE) {
-    if (!TreeBegin<KEYS>(A, sh, begin_seq, begin_at, begin_pos, begin_end)) return;
+    if (!TreeBegin<KEYS, RANGES>(A, sh, begin_seq, begin_at, begin_pos, begin_end)) return;
+    if constexpr (!RANGES) {
+      w = TreeWalk<KEYS>(A, begin_seq, begin_at, begin_pos, begin_end).Take();
+      w.part = -1;
+    }
   } else {
     // the last tiles of a sequence are the longest: they start first
     const int x = gridDim.x - 1 - blockIdx.x;
     w.head = x % A.Hk;
     if (!PromptWork<KEYS>(A, x / A.Hk, w)) return;
+  }
+  if constexpr (!RANGES) {
     w.seq = Uniform(w.seq);
     w.start = Uniform(w.start);
+    w.head = Uniform(w.head);
     w.q0 = Uniform(w.q0);
     w.tokens0 = Uniform(w.tokens0);
     w.tokens1 = Uniform(w.tokens1);
     w.blocks0 = Uniform(w.blocks0);
     w.blocks1 = Uniform(w.blocks1);
+    w.turns = TREE ? Uniform(w.turns) : 0;
+    w.first = TREE ? Uniform(w.first) : 0;
+    w.cached = Uniform(w.cached);
+    w.cache_blocks = Uniform(w.cache_blocks);
     w.nodes = Uniform(w.nodes);
-    w.more = 0;
   }
   const TaBlocks<KEYS, TREE> blk{A, w};
 
@@ -509,6 +531,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       MbarInit(&sh->o_full[i], 1);
     } else if (lane < U + 6) {
       MbarInit(&sh->work_full[lane - U - 2], 1);
+      MbarInit(&sh->work_read[lane - U - 2], 9);  // by the MMA warp and the eight softmax warps
     } else if (lane == U + 6) {
       MbarInit(&sh->q_full, 1);
       MbarInit(&sh->q_empty, 1);
@@ -527,13 +550,17 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   __syncthreads();
   TcgenFenceAfter();
   const uint32_t tmem = (uint32_t)Uniform((int)sh->tmem);
-  // The work behind this one, number `segment` (trees: the loading warp is ahead of the others by one at most, so four places
-  // are enough and none is waited for).
+  // Ranges: work number `segment`, if there is any. The loading warp writes it down, in four places by turns; a warp that has no
+  // rows for some time may be that far behind, so a place is written again only when all have read it (lane 0's values count).
   const auto next = [&](uint32_t segment, bool& ok) -> bool {
-    if (!TREE || !ok || !w.more) return false;
-    ok = TaWaitWarp(sh, &sh->work_full[segment & 3], (segment >> 2) & 1);
-    if (ok) GetWork(sh, segment & 3, w);
-    return ok;
+    if (!RANGES || !w.more) return false;
+    const bool got = TaWaitWarp(sh, &sh->work_full[segment & 3], (segment >> 2) & 1);
+    ok = ok && got;
+    if (got) {
+      GetWork(sh, segment & 3, w);
+      if (lane == 0) MbarArrive(&sh->work_read[segment & 3]);
+    }
+    return got;
   };
   GridDepLaunch();  // after this block holds its TMEM
   float* const sml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 768);  // tile 1's maxima and sums, for a merge
@@ -584,12 +611,14 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       // both tiles at once or, by turns, for each
       bool ok = true;
       uint32_t segment = 0;
-      TreeWalk<KEYS> walk(A, begin_seq, begin_at, begin_pos, begin_end);
+      typename std::conditional<RANGES, TreeWalk<KEYS>, NoWalk>::type walk(A, begin_seq, begin_at, begin_pos, begin_end);
       do {
         if (segment > 0) ok = TaWaitWarp(sh, &sh->q_empty, (segment - 1) & 1);
         if (!ok) break;
-        if constexpr (TREE) {
+        if constexpr (RANGES) {
           w = walk.Take();
+          if (segment >= 4) ok = TaWaitWarp(sh, &sh->work_read[segment & 3], ((segment >> 2) - 1) & 1);
+          if (!ok) break;
           if (lane == 0) {
             PutWork(sh, segment & 3, w);
             MbarArrive(&sh->work_full[segment & 3]);
@@ -621,7 +650,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             one(i, t, true);
             one(i, t + 1, false);
           }
-      } while (ok && w.more);
+      } while (RANGES && ok && w.more);
       // every copy lands before the block may leave: the last phase of each unit's barrier
       if (segment > 0) MbarWaitBounded(&sh->q_full, (segment - 1) & 1, kOpsWaitLimit);
       for (int v = max(0, issued - U); v < issued; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
@@ -701,8 +730,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         __syncwarp();
       };
       uint32_t segment = 0;
-      if constexpr (TREE) w.more = 1;
-      while (segment == 0 && !TREE ? true : next(segment, ok)) {
+      if constexpr (RANGES) w.more = 1;
+      while ((segment == 0 && !RANGES) || next(segment, ok)) {
         const int steps = max(w.blocks0, w.blocks1);
         // A unit serves one tile, or both that share their keys: then the last tile of a step (tile 1, if there is one: blocks0 <= blocks1)
         // releases it.
@@ -726,19 +755,49 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           values(i, t, vunit);
           if (ok && (w.turns || i == last)) release(vunit);
         };
+        // prompts: V of step t and K of step t + 1, under one wait
+        int vnext = 0, knext = 0;
+        const auto acquire_step = [&](int t) {
+          if (t >= steps) return;
+          if (t + 1 == steps) {
+            vnext = acquire();
+            return;
+          }
+          const int v = st;
+          const uint32_t pv = phase;
+          if (++st == U) {
+            st = 0;
+            phase ^= 1;
+          }
+          const int k = st;
+          const uint32_t pk = phase;
+          if (++st == U) {
+            st = 0;
+            phase ^= 1;
+          }
+          ok = ok && TaWaitWarp2(sh, &sh->full[v], pv, &sh->full[k], pk);
+          vnext = v;
+          knext = k;
+        };
         if (!w.turns) kunit = acquire();
         next_scores(0, 0);
         next_scores(1, 0);
         if (steps == 1 && ok) UmmaIssueCommit(&sh->q_empty);
+        if (!TREE) acquire_step(0);
 #pragma unroll 1
         for (int t = 0; t < steps && ok; t++) {
-          if (!w.turns) {  // both units of the step ahead of the first wait for probabilities
+          if (!TREE) {
+            vunit = vnext;
+            kunit = knext;
+            trim(blk.Index(0, t), vunit);
+          } else if (!w.turns) {  // (trees, as above, lose a tenth: their units come from memory, not from the cache)
             vunit = acquire();
             trim(blk.Index(0, t), vunit);
             if (t + 1 < steps) kunit = acquire();
           }
           next_values(0, t);
           next_scores(0, t + 1);
+          if (!TREE) acquire_step(t + 1);  // under the products just issued
           next_values(1, t);
           next_scores(1, t + 1);
           if (t + 2 == steps && ok) UmmaIssueCommit(&sh->q_empty);  // the last scores: Q may be replaced behind them
@@ -762,222 +821,226 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     bool ok = true;
     uint32_t done = 0, outs0 = 0, outs1 = 0, merges = 0;  // of the segments so far: this tile's steps, the tiles' results, merges
     uint32_t segment = 0;
-    if constexpr (TREE) w.more = 1;
-    while (segment == 0 && !TREE ? true : next(segment, ok)) {
-    segment++;
-    const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
-    const bool mine = token < w.Tokens(i);
-    const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
-    float m = -INFINITY, l = 0.f;
+    if constexpr (RANGES) w.more = 1;
+    while ((segment == 0 && !RANGES) || next(segment, ok)) {
+      segment++;
+      const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
+      const bool mine = token < w.Tokens(i);
+      const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
+      float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-    for (int t = 0; t < w.Blocks(i); t++) {
-      const int b = blk.Index(i, t), seen = blk.Seen(i, b);
-      bool cut;  // some row does not see all keys of a whole block
-      bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
-      int page0 = 0, page1 = 0;           // read ahead of the wait, looked at behind it
-      if constexpr (TREE) {
-        if (b < w.cache_blocks) {
-          const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
-          page0 = tb[0];
-          if (KEYS == 128 && seen > 64) page1 = tb[1];
+      for (int t = 0; t < w.Blocks(i); t++) {
+        const int b = blk.Index(i, t), seen = blk.Seen(i, b);
+        bool cut;  // some row does not see all keys of a whole block
+        bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
+        int page0 = 0, page1 = 0;           // read ahead of the wait, looked at behind it
+        if constexpr (TREE) {
+          if (b < w.cache_blocks) {
+            const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
+            page0 = tb[0];
+            if (KEYS == 128 && seen > 64) page1 = tb[1];
+          }
         }
-      }
-      ok = TaWait(sh, &sh->s_full[i], (done + t) & 1);
-      if (!ok) break;
-      TcgenFenceAfter();
-      if constexpr (TREE) {
-        gone0 = (unsigned)page0 >= (unsigned)A.pages;
-        gone1 = (unsigned)page1 >= (unsigned)A.pages;
-        cut = seen < KEYS || b >= w.cache_blocks || __any_sync(0xffffffffu, gone0 || gone1);
-      } else {
-        cut = tok0 < KEYS * b + KEYS - 1 || seen < KEYS;
-      }
-      if (!busy) {
-        if (Cfg::kWide) MbarArrive(&sh->p_half[i]);
-      } else {
-        uint32_t s[KEYS];
-        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const auto most = [&](int from, int to) {
-#pragma unroll
-          for (int c = from; c < to; c += 2)
-            x[(c >> 1) & 3] = Max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-        };
-        if (!cut) {
-          // the maximum of one half runs under the load of the other
-#pragma unroll
-          for (int c = 0; c < KEYS / 64; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
-          TmemWaitLd();
-#pragma unroll
-          for (int c = KEYS / 64; c < KEYS / 32; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
-          most(0, KEYS / 2);
-          TmemWaitLd();
-          most(KEYS / 2, KEYS);
+        // A wait that gave up stops no lane here, since loads from TMEM take the whole warp: the steps run out (no wait holds any
+        // more) and nothing is stored.
+        ok = TaWait(sh, &sh->s_full[i], (done + t) & 1) && ok;
+        TcgenFenceAfter();
+        if constexpr (TREE) {
+          gone0 = (unsigned)page0 >= (unsigned)A.pages;
+          gone1 = (unsigned)page1 >= (unsigned)A.pages;
+          cut = seen < KEYS || b >= w.cache_blocks || __any_sync(0xffffffffu, gone0 || gone1);
         } else {
-#pragma unroll
-          for (int c = 0; c < KEYS / 32; c++) {
-            if (32 * c < seen) {
-              TmemLoad32(scol + 32u * c, s + 32 * c);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; k++) s[32 * c + k] = 0;
-            }
-          }
-          TmemWaitLd();
-          // columns this row sees: 0 .. lim-1, or the bits of its mask
-          unsigned long long m0, m1 = 0;
-          if (TREE && b >= w.cache_blocks) {
-            m0 = mine ? A.masks[w.start + tok0 + token] : 0;
-            if (w.nodes < 64) m0 &= (1ull << w.nodes) - 1;
-          } else {
-            const int lim = TREE ? seen : min(seen, tok0 + token - KEYS * b + 1);
-            m0 = lim >= 64 ? ~0ull : lim > 0 ? (1ull << lim) - 1 : 0;
-            if (KEYS == 128) m1 = lim >= 128 ? ~0ull : lim > 64 ? (1ull << (lim - 64)) - 1 : 0;
-            if (gone0) m0 = 0;
-            if (gone1) m1 = 0;
-          }
-#pragma unroll
-          for (int c = 0; c < KEYS / 32; c++) {
-            const uint32_t bm = (uint32_t)((c < 2 ? m0 : m1) >> (32 * (c & 1)));
-#pragma unroll
-            for (int k = 0; k < 32; k++)
-              if (!(bm >> k & 1)) s[32 * c + k] = 0xff800000u;
-          }
-          most(0, KEYS);
+          cut = tok0 < KEYS * b + KEYS - 1 || seen < KEYS;
         }
-        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        if (t == 0) {
-          m = mx;
-        } else if (__any_sync(0xffffffffu, mine && (mx - m) * sc > kTaLazy)) {
-          // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
-          // or a result's last bits would hang on them)
-          // step t-1's products are complete: S of step t was issued behind them
-          const float mn = fmaxf(m, mx);
-          const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
-          m = mn;
-          l *= alpha;
-#pragma unroll 1
-          for (int c = 0; c < D / 16; c++) {
-            uint32_t o[16];
-            TmemLoad16(ocol + 16u * c, o);
+        if (!busy) {
+          if (Cfg::kWide) MbarArrive(&sh->p_half[i]);
+        } else {
+          uint32_t s[KEYS];
+          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const auto most = [&](int from, int to) {
+#pragma unroll
+            for (int c = from; c < to; c += 2)
+              x[(c >> 1) & 3] = Max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          };
+          if (!cut) {
+            // the maximum of one half runs under the load of the other
+#pragma unroll
+            for (int c = 0; c < KEYS / 64; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
             TmemWaitLd();
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            TmemStore16(ocol + 16u * c, o);
-          }
-        }
-        const float neg = m == -INFINITY ? 0.f : kBias - m * sc;
-        const f32x2 sc2 = Two(sc, sc), neg2 = Two(neg, neg);
-        f32x2 sum[2] = {0, 0};
-        // 32 keys: the probabilities, their sum, and the 16-bit pairs into TMEM
-        const auto exps = [&](int c, auto poly) {
-          uint32_t p[16];
+            for (int c = KEYS / 64; c < KEYS / 32; c++) TmemLoad32(scol + 32u * c, s + 32 * c);
+            most(0, KEYS / 2);
+            TmemWaitLd();
+            most(KEYS / 2, KEYS);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 16; k++) {
-            float p0, p1;
-            Split(Fma2(Two(__uint_as_float(s[32 * c + 2 * k]), __uint_as_float(s[32 * c + 2 * k + 1])), sc2, neg2), p0, p1);
-            f32x2 e;
-            // spread evenly: pair k where (k + 1) kPoly / 16 passes an integer
-            if (decltype(poly)::value && (k + 1) * Cfg::kPoly / 16 != k * Cfg::kPoly / 16) e = Exp2Poly(p0, p1);
-            else e = Two(Exp2(p0), Exp2(p1));
-            sum[k & 1] = Add2(sum[k & 1], e);
-            Split(e, p0, p1);
-            p[k] = Pack2<F16>(p0, p1);
-          }
-          TmemStore16(scol + 16u * c, p);
-        };
-        const auto probabilities = [&](auto whole) {
-          constexpr bool kAll = decltype(whole)::value;  // nothing is cut: all keys
-          exps(0, whole);
-          if (kAll || seen > 32) exps(1, whole);
-          if constexpr (Cfg::kWide) {
-            TmemWaitSt();
-            TcgenFenceBefore();
-            MbarArrive(&sh->p_half[i]);
-            if (kAll || seen > 64) exps(2, whole);
-            if (kAll || seen > 96) exps(3, whole);
-          }
-        };
-        if (cut) probabilities(std::false_type());
-        else probabilities(std::true_type());
-        float l0, l1;
-        Split(Add2(sum[0], sum[1]), l0, l1);
-        l += l0 + l1;
-        TmemWaitSt();
-      }
-      TcgenFenceBefore();
-      MbarArrive(&sh->p_full[i]);
-    }
-    // ---- the rows' results ----
-    done += w.Blocks(i);
-    const bool merge = TREE && w.turns == kTurns && w.blocks1 > 0;
-    if (w.Blocks(i) > 0) ok = ok && TaWait(sh, &sh->o_full[i], (i ? outs1 : outs0) & 1);
-    if (merge && i == 1) {
-      // the same rows' other key blocks: tile 0's threads read this accumulator, in the same lanes, too
-      sml[r] = m;
-      sml[128 + r] = l;
-      MbarArrive(&sh->ml_full);
-      ok = TaWait(sh, &sh->ml_free, merges & 1) && ok;  // before the next segment's products may write over it
-    } else if (!(w.turns == kTurns && i == 1)) {
-      float a0 = 1.f, a1 = 0.f;
-      if (merge) {
-        ok = ok && TaWait(sh, &sh->ml_full, merges & 1) && TaWait(sh, &sh->o_full[1], outs1 & 1);
-        const float m2 = sml[r], l2 = sml[128 + r], mn = fmaxf(m, m2);
-        if (mn != -INFINITY) {
-          a0 = Exp2((m - mn) * sc);
-          a1 = Exp2((m2 - mn) * sc);
-        }
-        m = mn;
-        l = l * a0 + l2 * a1;
-      }
-      if (busy && ok) {
-        TcgenFenceAfter();
-        const bool parts = TREE && w.part >= 0;
-        if (!parts) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
-          a0 *= inv;
-          a1 *= inv;
-        }
-        const bool zero = !parts && l == 0.f;
-        const int node = tok0 + token;
-        uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
-        const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
-#pragma unroll 1
-        for (int c = 0; c < D / 16; c++) {
-          uint32_t o[16], o1[16];
-          TmemLoad16(ocol + 16u * c, o);
-          if (merge) TmemLoad16(ocol + Cfg::kOStep + 16u * c, o1);
-          TmemWaitLd();
-          float v[16];
+            for (int c = 0; c < KEYS / 32; c++) {
+              if (32 * c < seen) {
+                TmemLoad32(scol + 32u * c, s + 32 * c);
+              } else {
 #pragma unroll
-          for (int k = 0; k < 16; k++) {
-            v[k] = __uint_as_float(o[k]) * a0;
-            if (merge) v[k] = fmaf(__uint_as_float(o1[k]), a1, v[k]);
-            if (zero) v[k] = 0.f;
-          }
-          if (mine) {
-            if (parts) {
-              float* dst = A.part_o + slot * D + 16 * c;
-#pragma unroll
-              for (int k = 0; k < 16; k += 8) Store32B(dst + k, v + k);
+                for (int k = 0; k < 32; k++) s[32 * c + k] = 0;
+              }
+            }
+            TmemWaitLd();
+            // columns this row sees: 0 .. lim-1, or the bits of its mask
+            unsigned long long m0, m1 = 0;
+            if (TREE && b >= w.cache_blocks) {
+              m0 = mine ? A.masks[w.start + tok0 + token] : 0;
+              if (w.nodes < 64) m0 &= (1ull << w.nodes) - 1;
             } else {
-              uint4* dst = reinterpret_cast<uint4*>(out + 16 * c);
+              const int lim = TREE ? seen : min(seen, tok0 + token - KEYS * b + 1);
+              m0 = lim >= 64 ? ~0ull : lim > 0 ? (1ull << lim) - 1 : 0;
+              if (KEYS == 128) m1 = lim >= 128 ? ~0ull : lim > 64 ? (1ull << (lim - 64)) - 1 : 0;
+              if (gone0) m0 = 0;
+              if (gone1) m1 = 0;
+            }
 #pragma unroll
-              for (int k = 0; k < 2; k++)
-                dst[k] = make_uint4(Pack2<F16>(v[8 * k], v[8 * k + 1]), Pack2<F16>(v[8 * k + 2], v[8 * k + 3]),
-                                    Pack2<F16>(v[8 * k + 4], v[8 * k + 5]), Pack2<F16>(v[8 * k + 6], v[8 * k + 7]));
+            for (int c = 0; c < KEYS / 32; c++) {
+              const uint32_t bm = (uint32_t)((c < 2 ? m0 : m1) >> (32 * (c & 1)));
+#pragma unroll
+              for (int k = 0; k < 32; k++)
+                if (!(bm >> k & 1)) s[32 * c + k] = 0xff800000u;
+            }
+            most(0, KEYS);
+          }
+          const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          if (t == 0) {
+            m = mx;
+          } else if (__any_sync(0xffffffffu, mine && (mx - m) * sc > kTaLazy)) {
+            // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
+            // or a result's last bits would hang on them)
+            // step t-1's products are complete: S of step t was issued behind them
+            const float mn = fmaxf(m, mx);
+            const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
+            m = mn;
+            l *= alpha;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; c++) {
+              uint32_t o[16];
+              TmemLoad16(ocol + 16u * c, o);
+              TmemWaitLd();
+#pragma unroll
+              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              TmemStore16(ocol + 16u * c, o);
             }
           }
+          const float neg = m == -INFINITY ? 0.f : kBias - m * sc;
+          const f32x2 sc2 = Two(sc, sc), neg2 = Two(neg, neg);
+          f32x2 sum[2] = {0, 0};
+          // 32 keys: the probabilities, their sum, and the 16-bit pairs into TMEM
+          const auto exps = [&](int c, auto poly) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+              float p0, p1;
+              Split(Fma2(Two(__uint_as_float(s[32 * c + 2 * k]), __uint_as_float(s[32 * c + 2 * k + 1])), sc2, neg2), p0, p1);
+              f32x2 e;
+              // spread evenly: pair k where (k + 1) kPoly / 16 passes an integer
+              if (decltype(poly)::value && (k + 1) * Cfg::kPoly / 16 != k * Cfg::kPoly / 16) e = Exp2Poly(p0, p1);
+              else e = Two(Exp2(p0), Exp2(p1));
+              sum[k & 1] = Add2(sum[k & 1], e);
+              Split(e, p0, p1);
+              p[k] = Pack2<F16>(p0, p1);
+            }
+            TmemStore16(scol + 16u * c, p);
+          };
+          const auto probabilities = [&](auto whole) {
+            constexpr bool kAll = decltype(whole)::value;  // nothing is cut: all keys
+            exps(0, whole);
+            if (kAll || seen > 32) exps(1, whole);
+            if constexpr (Cfg::kWide) {
+              TmemWaitSt();
+              TcgenFenceBefore();
+              MbarArrive(&sh->p_half[i]);
+              if (kAll || seen > 64) exps(2, whole);
+              if (kAll || seen > 96) exps(3, whole);
+            }
+          };
+          if (cut) probabilities(std::false_type());
+          else probabilities(std::true_type());
+          float l0, l1;
+          Split(Add2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
+          TmemWaitSt();
         }
-        if (parts && mine) A.part_ml[slot] = make_float2(m * sc, l);
-      }
-      if (merge) {
         TcgenFenceBefore();
-        MbarArrive(&sh->ml_free);
+        MbarArrive(&sh->p_full[i]);
       }
-    }
-    outs0 += w.blocks0 > 0;
-    outs1 += w.blocks1 > 0;
-    merges += merge;
+      // ---- the rows' results ----
+      done += w.Blocks(i);
+      const bool merge = TREE && w.turns == kTurns && w.blocks1 > 0;
+      if (w.Blocks(i) > 0) ok = TaWait(sh, &sh->o_full[i], (i ? outs1 : outs0) & 1) && ok;
+      if (merge && i == 1) {
+        // the same rows' other key blocks: tile 0's threads read this accumulator, in the same lanes, too
+        sml[r] = m;
+        sml[128 + r] = l;
+        MbarArrive(&sh->ml_full);
+        ok = TaWait(sh, &sh->ml_free, merges & 1) && ok;  // before the next segment's products may write over it
+      } else if (!(w.turns == kTurns && i == 1)) {
+        float a0 = 1.f, a1 = 0.f;
+        if (merge) {
+          ok = TaWait(sh, &sh->ml_full, merges & 1) && ok;
+          ok = TaWait(sh, &sh->o_full[1], outs1 & 1) && ok;
+          const float m2 = sml[r], l2 = sml[128 + r], mn = fmaxf(m, m2);
+          if (mn != -INFINITY) {
+            a0 = Exp2((m - mn) * sc);
+            a1 = Exp2((m2 - mn) * sc);
+          }
+          m = mn;
+          l = l * a0 + l2 * a1;
+        }
+        if (busy) {
+          TcgenFenceAfter();
+          const bool parts = RANGES && w.part >= 0;
+          if (!parts) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
+            a0 *= inv;
+            a1 *= inv;
+          }
+          const bool zero = !parts && l == 0.f;
+          const int node = tok0 + token;
+          uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
+          const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
+          // 16 columns at a time, 8 where registers are few
+          constexpr int kCols = Cfg::kWide || !TREE ? 16 : 8;
+          const auto columns = [](uint32_t addr, uint32_t* v) {
+            if constexpr (kCols == 16) TmemLoad16(addr, v);
+            else TmemLoad8(addr, v);
+          };
+#pragma unroll 1
+          for (int c = 0; c < D; c += kCols) {
+            uint32_t o[kCols], o1[kCols];
+            columns(ocol + (uint32_t)c, o);
+            if (merge) columns(ocol + Cfg::kOStep + (uint32_t)c, o1);
+            TmemWaitLd();
+            float v[kCols];
+#pragma unroll
+            for (int k = 0; k < kCols; k++) {
+              v[k] = __uint_as_float(o[k]) * a0;
+              if (merge) v[k] = fmaf(__uint_as_float(o1[k]), a1, v[k]);
+              if (zero) v[k] = 0.f;
+            }
+            if (mine && ok) {
+#pragma unroll
+              for (int k = 0; k < kCols; k += 8) {
+                if (parts) Store32B(A.part_o + slot * D + c + k, v + k);
+                else
+                  *reinterpret_cast<uint4*>(out + c + k) = make_uint4(Pack2<F16>(v[k], v[k + 1]), Pack2<F16>(v[k + 2], v[k + 3]),
+                                                                      Pack2<F16>(v[k + 4], v[k + 5]), Pack2<F16>(v[k + 6], v[k + 7]));
+              }
+            }
+          }
+          if (parts && mine && ok) A.part_ml[slot] = make_float2(m * sc, l);
+        }
+        if (merge) {
+          TcgenFenceBefore();
+          MbarArrive(&sh->ml_free);
+        }
+      }
+      outs0 += w.blocks0 > 0;
+      outs1 += w.blocks1 > 0;
+      merges += merge;
     }
   }
   TcgenFenceBefore();
