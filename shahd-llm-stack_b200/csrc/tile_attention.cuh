@@ -262,25 +262,77 @@ struct TaWork {
   __device__ __forceinline__ int Blocks(int i) const { return i ? blocks1 : blocks0; }
 };
 
-// The prompt tile `tile` of all: sequence s owns tiles offsets[s] / (2 TB) + s .. offsets[s+1] / (2 TB) + s, at least as many
-// as it needs, so the mapping is a search in the offsets and needs no table. Each warp finds the same.
+// The pair of tiles that a block of threads takes: number `rank` of `all` places, of which some are empty. Each warp finds the same.
+// The later a pair lies in its sequence, the more keys it has, and the longest should start first. 2 to 128 sequences, whose
+// lengths fit a warp's registers: pairs go by their place in the sequence, last places first, over all sequences together, by a
+// search for the place that number `rank` falls on (16 prompts of 300 to 2048 tokens, 16/4 heads of 64: 112 us, by sequences
+// 118; 2 prompts of 7000 to 8192, 16/2 heads of 128, whose blocks all take long: 530 and 525). One sequence, where the
+// order is the same without the search (64/16 heads of 64 over 2048 tokens: 60 us, with it 62), and more than 128 go by
+// sequences: s owns places offsets[s] / span + s .. offsets[s+1] / span + s, at least as many as it needs, which a search in
+// the offsets finds.
 template <int KEYS>
-__device__ __forceinline__ bool PromptWork(const TaArgs& A, int tile, TaWork& w) {
+__device__ __forceinline__ bool PromptWork(const TaArgs& A, int rank, int all, TaWork& w) {
   const int lane = threadIdx.x & 31, span = 2 * A.TB;
   const auto off = [&](int s) { return min(max(A.offsets[s], 0), A.rows); };
-  int lo = 0, cnt = A.n;
-  while (cnt > 1) {
-    const int step = (cnt + 31) / 32;
-    const bool le = lane * step < cnt && off(lo + lane * step) / span + lo + lane * step <= tile;
-    const unsigned hit = __ballot_sync(0xffffffffu, le);
-    if (!hit) return false;
-    const int k = 31 - __clz(hit);
-    lo += k * step;
-    cnt = min(step, cnt - k * step);
+  int seq, local;
+  if (A.n > 1 && A.n <= 128) {
+    int count[4], most = 0, total = 0;
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+      const int s = lane + 32 * m;
+      count[m] = s < A.n ? (max(off(s + 1) - off(s), 0) + span - 1) / span : 0;
+      most = max(most, count[m]);
+      total += count[m];
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (rank >= total) return false;
+    const auto from = [&](int j) {  // pairs at place j or behind it
+      int v = 0;
+#pragma unroll
+      for (int m = 0; m < 4; m++)
+        if (32 * m < A.n) v += max(count[m] - j, 0);
+      return (int)__reduce_add_sync(0xffffffffu, v);
+    };
+    int lo = 0, hi = most, behind = 0;  // from(lo) > rank >= from(hi) = behind
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, f = from(mid);
+      if (f > rank) lo = mid;
+      else {
+        hi = mid;
+        behind = f;
+      }
+    }
+    local = lo;
+    seq = 0;
+    int nth = rank - behind;  // the sequence: the nth of those with a pair at that place
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+      if (32 * m >= A.n) break;
+      const bool mine = count[m] > local;
+      const unsigned have = __ballot_sync(0xffffffffu, mine);
+      const unsigned hit = __ballot_sync(0xffffffffu, mine && __popc(have & ((1u << lane) - 1)) == nth);
+      if (hit) seq = 32 * m + __ffs(hit) - 1;
+      nth -= __popc(have);
+    }
+  } else {
+    const int tile = all - 1 - rank;
+    int lo = 0, cnt = A.n;
+    while (cnt > 1) {
+      const int step = (cnt + 31) / 32;
+      const bool le = lane * step < cnt && off(lo + lane * step) / span + lo + lane * step <= tile;
+      const unsigned hit = __ballot_sync(0xffffffffu, le);
+      if (!hit) return false;
+      const int k = 31 - __clz(hit);
+      lo += k * step;
+      cnt = min(step, cnt - k * step);
+    }
+    seq = lo;
+    local = tile - (off(lo) / span + lo);
   }
-  w.seq = lo;
-  w.start = off(lo);
-  const int len = max(off(lo + 1) - w.start, 0), local = tile - (w.start / span + lo);
+  w.seq = seq;
+  w.start = off(seq);
+  const int len = max(off(seq + 1) - w.start, 0);
   w.nodes = len;
   w.q0 = local * span;
   if (local < 0 || w.q0 >= len) return false;
@@ -472,7 +524,7 @@ struct TaBlocks {
 
 // Prompts; trees with a block of threads for every tile pair; trees with a range of key blocks for every block of threads, pair after
 // pair. (Pairs on their own are worth a kernel: what goes on from one pair to the next takes registers that head_dim 64
-// does not have, and 256 single tokens over 512 positions took 27 us instead of TREEONE.)
+// does not have, and 256 single tokens over 512 positions took 27 us instead of 21.)
 enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2 };
 
 template <int D, bool F16, int KIND>
@@ -496,13 +548,12 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       w = TreeWalk<KEYS>(A, begin_seq, begin_at, begin_pos, begin_end).Take();
       w.part = -1;
     }
-  } else {
-    // the last tiles of a sequence are the longest: they start first
-    const int x = gridDim.x - 1 - blockIdx.x;
-    w.head = x % A.Hk;
-    if (!PromptWork<KEYS>(A, x / A.Hk, w)) return;
+  } else if (warp == 9) {  // one warp looks, the others prepare meanwhile
+    w.head = blockIdx.x % A.Hk;
+    if (!PromptWork<KEYS>(A, blockIdx.x / A.Hk, gridDim.x / A.Hk, w)) w.nodes = 0;
+    if (lane == 0) PutWork(sh, 0, w);
   }
-  if constexpr (!RANGES) {
+  if constexpr (KIND == kTreePairs) {
     w.seq = Uniform(w.seq);
     w.start = Uniform(w.start);
     w.head = Uniform(w.head);
@@ -511,8 +562,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     w.tokens1 = Uniform(w.tokens1);
     w.blocks0 = Uniform(w.blocks0);
     w.blocks1 = Uniform(w.blocks1);
-    w.turns = TREE ? Uniform(w.turns) : 0;
-    w.first = TREE ? Uniform(w.first) : 0;
+    w.turns = Uniform(w.turns);
+    w.first = Uniform(w.first);
     w.cached = Uniform(w.cached);
     w.cache_blocks = Uniform(w.cache_blocks);
     w.nodes = Uniform(w.nodes);
@@ -550,6 +601,15 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   __syncthreads();
   TcgenFenceAfter();
   const uint32_t tmem = (uint32_t)Uniform((int)sh->tmem);
+  if constexpr (KIND == kPrompt) {
+    GetWork(sh, 0, w);
+    w.turns = w.first = w.cached = w.cache_blocks = 0;
+    w.part = -1;
+    if (w.nodes == 0) {
+      if (warp == 8) TmemDealloc(tmem, Cfg::kCols);
+      return;
+    }
+  }
   // Ranges: work number `segment`, if there is any. The loading warp writes it down, in four places by turns; a warp that has no
   // rows for some time may be that far behind, so a place is written again only when all have read it (lane 0's values count).
   const auto next = [&](uint32_t segment, bool& ok) -> bool {

@@ -77,9 +77,12 @@ def test_tree_calls():
     _refused("v needs strides", call, **{**ok, "v": pkg.Rows(1 << 20, 132, 64)})
     big = pkg.KvCache(1 << 20, 2 * 2 * 64 * 64, 1 << 20, 512, 9, 2, 64)
     size = pkg.tree_attention_workspace(1, 4, 8, big)
-    assert size > 0 and size % (66 * 4) == 0
+    assert size > 0 and size % 32 == 0
     _refused("bytes of workspace", call, **{**ok, "cache": big, "num_heads": 8, "q": pkg.Rows(1 << 20, 512, 64), "out": pkg.Rows(1 << 20, 512, 64)})
-    assert pkg.tree_attention_workspace(1000, 4, 8, big) == 0  # the tiles fill the device: one part
+    assert pkg.tree_attention_workspace(1000, 4, 8, big) > size  # long caches of 2000 tile pairs are still cut into ranges
+    assert pkg.tree_attention_workspace(2000, 4, 8, big) == 0  # the pairs fill the device many times over: a block of threads each
+    short = pkg.KvCache(1 << 20, 2 * 2 * 64 * 64, 1 << 20, 16, 9, 2, 64)
+    assert pkg.tree_attention_workspace(1000, 4, 8, short) == 0
     _refused("at most 8", pkg.tree_attention_workspace, 1, 4, 64, big)
 
 
