@@ -313,7 +313,8 @@ const char* shahd_last_error(void);
  *    asynchronous on `stream` (0 = the legacy stream), allocate nothing, keep nothing between calls and can be captured
  *    into CUDA graphs. Sequences are packed: rows offsets[s] .. offsets[s+1]-1 are sequence s (offsets int32 [n+1] on the
  *    device, ascending, offsets[n] <= rows; empty sequences are allowed). Rows behind the last sequence are neither
- *    read nor written. Operands and results must not overlap unless a function says so.
+ *    read nor written. Operands and results must not overlap unless a function says so. At most 2^30 rows; a result's rows
+ *    lie apart by all its heads, or its heads by all its rows.
  * ============================================================================================== */
 
 #define SHAHD_BF16 0
@@ -433,7 +434,8 @@ typedef struct ShahdTreeCall {
 int64_t shahd_tree_attention_workspace(const ShahdTreeCall* call);
 /* out[i] = sum of softmax(scale q[i].k[j]) v[j] over the cached positions of the row's sequence and the rows of its mask;
  * a row that attends to nothing gives 0. Positions at or beyond the length are never used, whatever their pages
- * hold. */
+ * hold. A value of the nodes' or the cached k or v that is not finite can reach every row of its own sequence, masked rows
+ * too, but no other sequence. */
 int shahd_tree_attention(const ShahdTreeCall* call, void* stream);
 
 /* ---- verification of drafted trees (SpeculativeSample, SpeculativeSampling.ts:82-112, for trees and device rows) ---- */
@@ -458,8 +460,8 @@ typedef struct ShahdVerifyCall {
 } ShahdVerifyCall;
 /* Each child x of the current node, in index order, is taken with probability min(1, p(x)/q(x)); a refusal replaces p by
  * max(0, p - q) over its sum. The next token is drawn from what p is at the end (the target's row itself when nothing is
- * left), in index order against the root's number. Values that are not positive numbers count as 0; nodes whose token is
- * outside the vocabulary or whose parent is not below them are passed over. */
+ * left), in index order against the root's number. Values that are not positive numbers count as 0; a row without mass, or
+ * with an infinite value, draws token 0; nodes whose token is outside the vocabulary or whose parent is not below them are passed over. */
 int shahd_verify_tree(const ShahdVerifyCall* call, void* stream);
 
 #ifdef __cplusplus

@@ -124,8 +124,14 @@ inline bool CheckType(const char* op, int dtype, bool f32) {
 }
 
 // Rows and heads of an operand may lie in any order and distance; both strides are at least the head's extent
-// where there is more than one of them (rows or heads that share memory are refused).
-inline bool CheckRows(const char* op, const char* name, const ShahdRows& r, int64_t rows, int heads, int d, int multiple) {
+// where there is more than one of them. Rows of a result share no memory: either all heads of a row lie between it and the
+// next, or all rows of a head. Row counts up to 2^30 leave 32-bit sums of a row and a step in range.
+constexpr int64_t kOpsMaxRows = 1LL << 30;
+inline bool CheckRows(const char* op, const char* name, const ShahdRows& r, int64_t rows, int heads, int d, int multiple, bool result = false) {
+  if (rows > kOpsMaxRows) {
+    SetError("%s: too many rows: %lld, at most 2^30", op, (long long)rows);
+    return false;
+  }
   if ((rows > 1 && r.row_stride < d) || (heads > 1 && r.head_stride < d) || r.row_stride < 0 || r.head_stride < 0) {
     SetError("%s: %s needs row and head strides of at least head_dim %d elements (got %lld and %lld)", op, name, d,
              (long long)r.row_stride, (long long)r.head_stride);
@@ -133,6 +139,11 @@ inline bool CheckRows(const char* op, const char* name, const ShahdRows& r, int6
   }
   if (r.row_stride > (1LL << 36) || r.head_stride > (1LL << 36)) {
     SetError("%s: %s has a stride beyond 2^36 elements", op, name);
+    return false;
+  }
+  if (result && rows > 1 && heads > 1 && (double)r.row_stride < (heads - 1) * (double)r.head_stride + d &&
+      (double)r.head_stride < (rows - 1) * (double)r.row_stride + d) {
+    SetError("%s: rows and heads of %s share memory (strides %lld and %lld)", op, name, (long long)r.row_stride, (long long)r.head_stride);
     return false;
   }
   if ((rows > 1 && r.row_stride % multiple != 0) || (heads > 1 && r.head_stride % multiple != 0)) {

@@ -375,9 +375,9 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
     SetError("%s: keys need k_out or a cache", op);
     return SHAHD_EINVAL;
   }
-  if ((q && (!CheckRows(op, "q", c->q, c->rows, c->num_heads, d, 1) || !CheckRows(op, "q_out", c->q_out, c->rows, c->num_heads, d, 1))) ||
+  if ((q && (!CheckRows(op, "q", c->q, c->rows, c->num_heads, d, 1) || !CheckRows(op, "q_out", c->q_out, c->rows, c->num_heads, d, 1, true))) ||
       (k && !CheckRows(op, "k", c->k, c->rows, c->kv_heads, d, 1)) ||
-      (k && c->k_out.data && !CheckRows(op, "k_out", c->k_out, c->rows, c->kv_heads, d, 1)) ||
+      (k && c->k_out.data && !CheckRows(op, "k_out", c->k_out, c->rows, c->kv_heads, d, 1, true)) ||
       (cache && !CheckRows(op, "v", c->v, c->rows, c->kv_heads, d, 1)))
     return SHAHD_EINVAL;
   if (c->rows == 0) return SHAHD_OK;

@@ -159,7 +159,7 @@ int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
     return SHAHD_EINVAL;
   }
   if (!CheckRows(op, "q", c->q, c->rows, H, d, 8) || !CheckRows(op, "k", c->k, c->rows, Hk, d, 8) ||
-      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8))
+      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8, true))
     return SHAHD_EINVAL;
   if (c->n == 0 || c->rows == 0) return SHAHD_OK;
   a.G = H / Hk;
@@ -228,7 +228,7 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
     return SHAHD_EINVAL;
   }
   if (!CheckRows(op, "q", c->q, c->rows, H, d, 8) || !CheckRows(op, "k", c->k, c->rows, Hk, d, 8) ||
-      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8))
+      !CheckRows(op, "v", c->v, c->rows, Hk, d, 8) || !CheckRows(op, "out", c->out, c->rows, H, d, 8, true))
     return SHAHD_EINVAL;
   if (c->n == 0 || c->rows == 0) return SHAHD_OK;
   a.G = H / Hk;

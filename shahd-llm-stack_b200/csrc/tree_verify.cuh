@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
   if (rank == 0 && threadIdx.x == 0) a.path[b] = 0;  // thread 0 filled this place itself
   int at = 1;  // first node not asked yet
   for (int loaded = -1; at < N;) {
-    if (window != loaded) {  // what the decisions on nodes window .. window + 511 read
+    if (window != loaded) {  // what the decisions on nodes window .. window + 255 read
       __syncthreads();
       const int j = window + threadIdx.x;
       int parent = -1;
@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
   // the first token whose running mass reaches u * total; the root's number is the draw's
   const float uf = a.uniforms[b];
   const double goal = (uf > 0.f ? fmin((double)uf, 1.0) : 0.0) * total;
-  if (mine > 0 && after >= goal && (before < goal || before == 0)) {
+  const bool mass = total > 0 && isfinite(total);
+  if (mass && mine > 0 && after >= goal && (before < goal || before == 0)) {
     int id = -1, seen = -1;
     double run = before;
     const float hi = (float)w, lo = (float)(w - (double)hi);
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
     if (lane == 0) a.next[sq] = id >= 0 ? id : seen;  // the scan's own rounding can end just below the goal
   }
   if (rank == 0 && threadIdx.x == 0) {
-    if (!(total > 0)) a.next[sq] = 0;  // a row without mass, as SampleFromDistribution answers
+    if (!mass) a.next[sq] = 0;  // a row without mass, as SampleFromDistribution answers, or with an endless one
     a.count[sq] = depth;
     if (a.commit) a.commit[b] = len;
     if (a.new_lengths) a.new_lengths[sq] = len + depth + 1;
@@ -326,6 +327,10 @@ extern "C" int shahd_verify_tree(const ShahdVerifyCall* c, void* stream) {
     SetError("%s: need n, rows >= 0, 1 <= vocab <= 2^30 and row strides of at least vocab (got n=%d rows=%d vocab=%d "
              "target_stride=%lld draft_stride=%lld)",
              op, c->n, c->rows, c->vocab, (long long)c->target_stride, (long long)c->draft_stride);
+    return SHAHD_EINVAL;
+  }
+  if (c->rows > kOpsMaxRows) {
+    SetError("%s: too many rows: %d, at most 2^30", op, c->rows);
     return SHAHD_EINVAL;
   }
   if (c->n == 0) return SHAHD_OK;

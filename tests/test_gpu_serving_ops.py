@@ -547,6 +547,18 @@ def test_verify_tree_edges():
     walk([flat] * 4, [flat] * 4, [0.3] * 4, tokens, np.array([0, 1, 3, -7], np.int32))
 
 
+@pytest.mark.parametrize("V", [64, 50257])
+@pytest.mark.parametrize("refused", [0, 1, 2])
+def test_verify_tree_rows_with_an_infinite_value_draw_token_0(V, refused):
+    target = torch.full((1 + refused, V), 1.0 / V)
+    target[0, 33], target[0, 5], target[0, 6] = math.inf, 0.0, 0.0
+    draft = torch.full((1 + refused, V), 1.0 / V)
+    for u in (0.0, 0.5):
+        got = _verify(target.cuda(), draft.cuda(), np.array([0, 5, 6][: 1 + refused], np.int32), np.array([-1, 0, 0][: 1 + refused], np.int32),
+                      np.full(1 + refused, u, np.float32), [1 + refused])
+        assert got[1][0] == 0 and got[2][0] == 0
+
+
 def test_verify_tree_follows_the_distribution():
     """Over many independent sequences, the first token after the root is distributed as the target's row, whatever the draft."""
     V, n = 8, 40000

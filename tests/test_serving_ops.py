@@ -44,6 +44,8 @@ def test_rope_calls():
         _refused("page_stride", rope.apply, **ok, k=ROWS, v=ROWS, kv_heads=2, cache=pkg.KvCache(1 << 20, 100, 1 << 20, 4, 9, 2, 64), offsets=1 << 20, n=1)
         _refused("q needs row and head strides", rope.apply, **{**ok, "q": pkg.Rows(1 << 20, 128, 32)})
         _refused("q_out needs row and head strides", rope.apply, **{**ok, "q_out": pkg.Rows(1 << 20, -128, 64)})
+        _refused("rows and heads of q_out share memory", rope.apply, **{**ok, "q_out": pkg.Rows(1 << 20, 64, 64)})
+        _refused("too many rows", rope.apply, **{**ok, "rows": 2**30 + 1})
 
 
 def test_prompt_calls():
@@ -58,7 +60,10 @@ def test_prompt_calls():
     _refused("scale", call, **{**ok, "scale": float("nan")})
     _refused("k needs strides that are multiples of 8", call, **{**ok, "k": pkg.Rows(1 << 20, 132, 64)})
     _refused("out needs row and head strides", call, **{**ok, "out": pkg.Rows(1 << 20, 128, 0)})
-    _refused("too many rows", call, **{**ok, "n": 2**31 - 1, "rows": 2**31 - 1})
+    _refused("too many rows", call, **{**ok, "n": 2**31 - 1, "rows": 2**30})
+    _refused("too many rows", call, **{**ok, "rows": 2**30 + 1})
+    _refused("share memory", call, **{**ok, "out": pkg.Rows(1 << 20, 64, 64)})
+    _refused("share memory", call, **{**ok, "out": pkg.Rows(1 << 20, 64, 3 * 64)})
     if not has_gpu():
         with pytest.raises(pkg._lib.ShahdError) as e:
             call(**ok)
@@ -74,6 +79,8 @@ def test_tree_calls():
     _refused("pages and max_blocks", call, **{**ok, "cache": pkg.KvCache(1 << 20, 2 * 2 * 64 * 64 + 4, 1 << 20, 4, 9, 2, 64)})
     _refused("dtype", call, **{**ok, "dtype": pkg.F32})
     _refused("rows >= 0", call, **{**ok, "rows": -4})
+    _refused("too many rows", call, **{**ok, "rows": 2**30 + 1})
+    _refused("share memory", call, **{**ok, "out": pkg.Rows(1 << 20, 64, 64)})
     _refused("v needs strides", call, **{**ok, "v": pkg.Rows(1 << 20, 132, 64)})
     big = pkg.KvCache(1 << 20, 2 * 2 * 64 * 64, 1 << 20, 512, 9, 2, 64)
     size = pkg.tree_attention_workspace(1, 4, 8, big)
@@ -93,6 +100,7 @@ def test_verify_calls():
     _refused("dtype", call, **{**ok, "dtype": 3})
     _refused("1 <= vocab", call, **{**ok, "vocab": 0})
     _refused("strides of at least vocab", call, **{**ok, "target_stride": 9})
+    _refused("too many rows", call, **{**ok, "rows": 2**30 + 1})
     _refused("need lengths", call, **{**ok, "commit": at})
     _refused("need lengths", call, **{**ok, "new_lengths": at})
     call(**{**ok, "n": 0})
