@@ -10,8 +10,9 @@
 // Bound by memory: each value is read once and written once. A warp takes a row at a time and waits for no other: its lanes
 // form the row's (cos, sin), one sincospi per pair for all heads, in shared memory of the warp's own, and take their
 // piece's into registers; a lane's piece of a head (8 values; in the half layout two pieces, as far apart as pairs are) is the same
-// in all heads, so a lane goes over heads with up to eight 16-byte loads in flight. Operands whose address, strides or pair
-// count do not allow pieces go value by value. (Blocks of 256 threads over batches of rows, with a table per batch, lost a
+// in all heads, so a lane goes over heads with up to eight 16-byte loads in flight. Where pairs do not
+// fill whole pieces, a lane's eight values find their partners in shared memory, where the warp puts the heads it has loaded.
+// Operands whose address or strides do not allow pieces go value by value. (Blocks of 256 threads over batches of rows, with a table per batch, lost a
 // fifth to a third of the time at the barriers: 56 K rows of 32 + 8 heads of 128 in f16, 1.15 GB, took 265 us; now 197, a plain
 // copy 182.)
 #pragma once
@@ -27,11 +28,13 @@ struct ShahdRope {
 namespace shahd {
 
 constexpr int kRopeWarps = 8;   // of a block, at most
-enum RopeMode { kRopeValues = 0, kRopeInterleaved = 1, kRopeHalf = 2 };  // one pair per thread, or pieces of either layout
+// One pair per thread; pieces of either layout; pieces whose values find their partners in shared memory.
+enum RopeMode { kRopeValues = 0, kRopeInterleaved = 1, kRopeHalf = 2, kRopeStaged = 3 };
 // Blocks of a multiprocessor: in the half layout a lane holds two pieces and their eight (cos, sin), 16-bit ones twice, which spills
-// at 80 registers (265 us instead of 196 for 56 K rows of 32 + 8 heads of 128).
+// at 80 registers (265 us instead of 196 for 56 K rows of 32 + 8 heads of 128), and so do staged pieces (296 us instead of 254,
+// 126 of the 128 values turned).
 template <class T, int MODE>
-constexpr int kRopePerSm = MODE == kRopeHalf && sizeof(T) == 2 ? 2 : 3;
+constexpr int kRopePerSm = (MODE == kRopeHalf && sizeof(T) == 2) || MODE == kRopeStaged ? 2 : 3;
 
 struct RopeOperand {
   const void* in;
@@ -107,6 +110,8 @@ __device__ __forceinline__ int SequenceOf(const int* offsets, int n, int row) {
 template <class T, class C, int MODE>
 __global__ void __launch_bounds__(kRopeWarps * 32, kRopePerSm<T, MODE>) RopeKernel(const __grid_constant__ RopeArgs a) {
   __shared__ __align__(16) float2 tables[kRopeWarps][128];
+  constexpr int kStage = sizeof(T) == 4 ? 2 : 4;  // staged: heads of a lane in flight
+  __shared__ __align__(16) T stages[MODE == kRopeStaged ? kRopeWarps : 1][MODE == kRopeStaged ? kStage : 1][32 * 8];
   constexpr int kPer = MODE == kRopeHalf ? 8 : 4;  // pairs of a piece
   GridDepWait();
   GridDepLaunch();
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopePerSm<T, MODE>) RopeKern
       float sn, cs;
       sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
       // two pairs of every piece side by side, so that the lanes' 16-byte reads lie next to each other
-      const int place = MODE == kRopeValues ? i : (i % kPer / 2 * (half / kPer) + i / kPer) * 2 + i % 2;
+      const int place = MODE == kRopeValues || MODE == kRopeStaged ? i : (i % kPer / 2 * (half / kPer) + i / kPer) * 2 + i % 2;
       turn[place] = make_float2(cs * a.magnitude, sn * a.magnitude);
     }
     __syncwarp();
@@ -176,6 +181,60 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopePerSm<T, MODE>) RopeKern
           if (two) cache[v1] = FromFloat<C>(y);
         }
       }
+    } else if constexpr (MODE == kRopeStaged) {
+      // of this lane's eight values: cos, sin with its sign, and how far away the partner lies (0: not turned)
+      float cv[8], sv[8];
+      int apart_v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int v = j0 + i, first_of = a.interleaved ? !(v & 1) : v < half;
+        apart_v[i] = v >= 2 * half ? 0 : a.interleaved ? (first_of ? 1 : -1) : first_of ? half : -half;
+        const float2 cs = turn[apart_v[i] == 0 ? 0 : a.interleaved ? v >> 1 : first_of ? v : v - half];
+        cv[i] = cs.x;
+        sv[i] = first_of ? -cs.y : cs.y;
+      }
+      const auto turn_heads = [&](const RopeOperand& o, int kv) {
+        const T* in = static_cast<const T*>(o.in) + row * o.in_row + j0;
+        T* out = o.out ? static_cast<T*>(o.out) + row * o.out_row + j0 : nullptr;
+        C* cache = kv >= 0 && at >= 0 ? reinterpret_cast<C*>(a.pool) + at + (long long)kv * kOpsPage * d + j0 : nullptr;
+#pragma unroll 1
+        for (int h = 0; h < o.heads; h += kStage * lanes) {
+          Raw8<T> raw[kStage];
+#pragma unroll
+          for (int k = 0; k < kStage; k++) {
+            const int hk = h + n0 + k * lanes;
+            if (n0 < lanes && hk < o.heads) raw[k].Load(in + hk * o.in_head);
+          }
+          if (kv != 1) {
+            __syncwarp();  // the last heads have been read
+#pragma unroll
+            for (int k = 0; k < kStage; k++)
+#pragma unroll
+              for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(&stages[warp][k][lane * 8])[i] = raw[k].u[i];
+            __syncwarp();
+          }
+#pragma unroll
+          for (int k = 0; k < kStage; k++) {
+            const int hk = h + n0 + k * lanes;
+            if (n0 >= lanes || hk >= o.heads) break;
+            float x[8];
+            raw[k].Get(x);
+            if (kv != 1) {
+              const T* own = &stages[warp][k][lane * 8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const float y = ToFloat(own[i + apart_v[i]]);
+                if (apart_v[i] != 0) x[i] = x[i] * cv[i] + y * sv[i];
+              }
+            }
+            if (out) Store8(out + hk * o.out_head, x);
+            if (cache) Store8(cache + (long long)hk * 2 * kOpsPage * d, x);
+          }
+        }
+      };
+      turn_heads(a.q, -1);
+      turn_heads(a.k, 0);
+      turn_heads(a.v, 1);
     } else if (n0 < lanes) {
       float4 cs[kPer / 2];
       if (rotary) {
@@ -253,10 +312,11 @@ void LaunchRopeMode(const RopeArgs& a, int sms, cudaStream_t st) {
 }
 
 template <class T, class C>
-void LaunchRope(const RopeArgs& a, bool vec, int sms, cudaStream_t st) {
-  if (!vec) LaunchRopeMode<T, C, kRopeValues>(a, sms, st);
-  else if (a.interleaved) LaunchRopeMode<T, C, kRopeInterleaved>(a, sms, st);
-  else LaunchRopeMode<T, C, kRopeHalf>(a, sms, st);
+void LaunchRope(const RopeArgs& a, int mode, int sms, cudaStream_t st) {
+  if (mode == kRopeValues) LaunchRopeMode<T, C, kRopeValues>(a, sms, st);
+  else if (mode == kRopeInterleaved) LaunchRopeMode<T, C, kRopeInterleaved>(a, sms, st);
+  else if (mode == kRopeHalf) LaunchRopeMode<T, C, kRopeHalf>(a, sms, st);
+  else LaunchRopeMode<T, C, kRopeStaged>(a, sms, st);
 }
 
 }  // namespace shahd
@@ -404,9 +464,12 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
     return SHAHD_ENODEV;
   }
   RopeArgs a = {};
-  // 16-byte pieces of 8 values: every address and stride in use a multiple of 16 bytes, whole pieces on both sides of
-  // the rotated part's end and of the pairs' halves
-  bool vec = rope->layout == SHAHD_ROPE_HALF ? d % 16 == 0 && rope->rotary % 16 == 0 : d % 8 == 0 && rope->rotary % 8 == 0;
+  // 16-byte pieces of 8 values need every address and stride in use a multiple of 16 bytes. With whole pieces on both sides of
+  // the rotated part's end and of the pairs' halves a lane holds both values of its pairs; otherwise shared memory brings
+  // them together (56 K f16 rows of 32 + 8 heads of 128 with 126 values turned: 254 us, value by value 866;
+  // with 54 272 and 1377).
+  bool vec = d % 8 == 0;
+  const bool whole = rope->layout == SHAHD_ROPE_HALF ? d % 16 == 0 && rope->rotary % 16 == 0 : rope->rotary % 8 == 0;
   const auto operand = [&](const ShahdRows& in, const ShahdRows& out, int heads) {
     for (const ShahdRows* r : {&in, &out})
       if (r->data)
@@ -432,12 +495,13 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
     a.pages = c->cache.pages;
   }
   std::copy(rope->turns, rope->turns + a.half, a.turns);
-  a.pieces = vec ? (a.interleaved ? d / 8 : d / 16) : d - a.half;
+  const int mode = !vec ? kRopeValues : !whole ? kRopeStaged : a.interleaved ? kRopeInterleaved : kRopeHalf;
+  a.pieces = mode == kRopeValues ? d - a.half : mode == kRopeHalf ? d / 16 : d / 8;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   TakeLaunchError(nullptr);
-  if (c->dtype == SHAHD_F32) LaunchRope<float, bf16>(a, vec, info.sms, st);
-  else if (c->dtype == SHAHD_F16) LaunchRope<__half, __half>(a, vec, info.sms, st);
-  else LaunchRope<bf16, bf16>(a, vec, info.sms, st);
+  if (c->dtype == SHAHD_F32) LaunchRope<float, bf16>(a, mode, info.sms, st);
+  else if (c->dtype == SHAHD_F16) LaunchRope<__half, __half>(a, mode, info.sms, st);
+  else LaunchRope<bf16, bf16>(a, mode, info.sms, st);
   return LaunchStatus(op);
 }
 

@@ -118,7 +118,7 @@ int LayTree(const char* op, const ShahdTreeCall* c, TreeLayout* out) {
   l.pairs = CeilDiv(c->max_nodes, 2 * TB);
   const long long slots = kTaSms * (d == 128 ? 1 : 2), tiles = (long long)c->n * Hk * l.pairs;
   const long long most = tiles * (CeilDiv(c->cache.max_blocks, keys / 64) + 1);  // key blocks of all pairs, if all sequences were as long
-  if (most > 0x7fffffffLL) {
+  if (most > 0x3fffffffLL) {
     SetError("%s: too many key blocks: %lld tile pairs over %d pages each", op, tiles, c->cache.max_blocks);
     return SHAHD_EINVAL;
   }

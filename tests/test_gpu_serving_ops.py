@@ -79,6 +79,39 @@ def test_rope_turns_queries_and_keys(dtype, layout, heads, kv, d, r):
         assert bool((y[2] == 7.0).all())  # a negative position leaves its row
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("heads,kv,d,r", [(4, 2, 128, 54), (33, 9, 64, 6), (5, 5, 32, 30), (2, 1, 128, 126), (41, 3, 24, 10), (3, 1, 256, 250),
+                                          (7, 2, 8, 2), (6, 2, 64, 40)])
+def test_rope_rotary_parts_of_any_even_size(dtype, layout, heads, kv, d, r):
+    """In place and into the cache; what lies behind the rotated part passes as it is, whatever it holds."""
+    g, N = _gen(11), 67
+    cdt = BF16 if dtype == F32 else dtype
+    pool, table, cache = _cache_of([N], kv, d, cdt, g)
+    q, k, v = (_normal(g, N, h, d, dtype=dtype) for h in (heads, kv, kv))
+    if r < d:
+        q[5, :, r:], k[6, :, d - 1], v[7, :, 0] = math.inf, math.nan, -math.inf
+    old_q, old_k = q.clone(), k.clone()
+    pos = torch.randperm(N, generator=g, device="cuda").int()
+    with pkg.Rope(d, r, layout) as rope:
+        rope.apply(CODE[dtype], N, pos.data_ptr(), q=_rows(q), q_out=_rows(q), num_heads=heads, k=_rows(k), k_out=_rows(k), kv_heads=kv, v=_rows(v),
+                   cache=cache, offsets=_ints([0, N]).data_ptr(), n=1, stream=_stream())
+    freq = R.frequencies(r)
+    for old, new in ((old_q, q), (old_k, k)):
+        want, off = R.rotate(old, pos, freq, layout)
+        _within(new[..., :r], want[..., :r], (off + R.HALF_STEP[dtype] * want.abs() + 1e-7)[..., :r])
+        assert torch.equal(new[..., r:].nan_to_num(9.0), old[..., r:].nan_to_num(9.0))
+    for h in range(kv):
+        held_k, held_v = _held(pool, table, 0, N, h)
+        at = pos.long()
+        assert torch.equal(held_v[at].nan_to_num(9.0), v[:, h].to(cdt).nan_to_num(9.0))
+        if dtype != F32:  # one rounding for both
+            assert torch.equal(held_k[at].nan_to_num(9.0), k[:, h].nan_to_num(9.0))
+        else:
+            want, off = R.rotate(old_k, pos, freq, layout)
+            _within(held_k[at][:, :r], want[:, h, :r], (off + R.HALF_STEP[cdt] * want.abs() * 1.01 + 1e-7)[:, h, :r])
+
+
 @pytest.mark.parametrize("scaling,factor", [("linear", 4.0), ("stretched", 8.0), ("by_parts", 16.0)])
 def test_rope_scalings_far_positions_and_single_operands(scaling, factor):
     g, N, d, r = _gen(2), 9, 128, 96
