@@ -96,7 +96,10 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
 // How a tree call's work is laid out. Where there are many tile pairs, or enough with short caches, each has a block of threads
 // of its own. Elsewhere as many blocks of threads as run at once take ranges of equal length out of all key blocks of all pairs,
 // 256 keys at least, and the pairs that a range cuts are joined by a second kernel: so long caches and short ones, one sequence and a
-// few hundred, end together (16 trees over 20 to 32 thousand positions, 8 kv heads of 128: a block of threads for each pair
+// few hundred, end together. A range costs the second kernel, about as long as eight steps, and both parts' rows written and
+// read in 32 bits; so where there is a place for every pair and its steps are few, pairs it is (72 trees of 13 to 26 nodes,
+// 12/4 heads of 64, up to 254 positions: ranges 29 us, pairs 10.9; 8 single tokens, 32/8 heads of 128, up to 2000 positions: 25.9
+// and 21.6; one tree of 24 over 2047 positions, 16/4 heads of 64: 13.5 and 23.3). Long caches in ranges (16 trees over 20 to 32 thousand positions, 8 kv heads of 128: a block of threads for each pair
 // 490 us, parts of 2048 keys 513 us, ranges 427 us; but 512 pairs of 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as
 // 256 pairs of heads).
 constexpr int kTaSms = 148;  // of a B200: the layout, and so the workspace, does not hang on a device being there
@@ -122,9 +125,14 @@ int LayTree(const char* op, const ShahdTreeCall* c, TreeLayout* out) {
     SetError("%s: too many key blocks: %lld tile pairs over %d pages each", op, tiles, c->cache.max_blocks);
     return SHAHD_EINVAL;
   }
-  if (tiles >= 8 * slots || (tiles >= slots && c->cache.max_blocks < 64)) {
-    // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge
-    l.two_heads = c->max_nodes <= TB && Hk % 2 == 0;
+  // steps of a pair's two tiles, the whole call's in ranges (by turns a step takes two blocks of keys, and costs a merge of about two)
+  const bool turns = c->max_nodes <= TB;
+  const long long blocks = CeilDiv(c->cache.max_blocks, keys / 64) + 1, alone = turns ? blocks / 2 + 2 : blocks;
+  const long long dealt = std::max(most / slots, 256LL / keys) / (turns ? 2 : 1) + 8 + 4LL * std::min(c->max_nodes, 2 * TB) * G / keys;
+  if (tiles >= 8 * slots || (tiles >= slots && c->cache.max_blocks < 64) || (tiles < slots && alone <= dealt)) {
+    // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge; where
+    // there are places for all, by turns half the steps (72 trees of 13 to 26, 12/4 heads, up to 254 positions: 10.9 and 11.7 us)
+    l.two_heads = turns && Hk % 2 == 0 && tiles >= slots;
     l.grid = l.two_heads ? tiles / 2 : tiles;
   } else {
     l.least = 256 / keys;

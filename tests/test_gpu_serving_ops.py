@@ -372,6 +372,30 @@ def test_tree_attention(dtype, heads, lengths, nodes):
     assert bool((out[sum(nodes):] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("lengths,nodes", [
+    ([0, 1, 63, 64, 65, 127, 128, 129], [1, 1, 1, 1, 1, 1, 1, 1]),
+    ([0, 0, 700, 5, 130], [3, 1, 17, 0, 64]), ([0, 300, 0], [0, 2, 0]), ([0], [1]), ([0], [64]),
+], ids=str)
+def test_tree_attention_short_lengths_in_a_long_cache(dtype, heads, lengths, nodes):
+    """Room for 600 pages a sequence: the work goes in ranges. Unused pages and table entries hold what must not be read."""
+    H, Hk, d = heads
+    g, N = _gen(17), sum(nodes) + 2
+    q, k, v = (_normal(g, N, h, d, dtype=dtype) for h in (H, Hk, Hk))
+    pool, table, cache = _cache_of(lengths, Hk, d, dtype, g, fill=math.nan)
+    for s, L in enumerate(lengths):
+        for b in range(-(-L // 64)):
+            pool[table[s, b], -1, :, :, : min(64, L - 64 * b)] = torch.randn(Hk, 2, min(64, L - 64 * b), d, generator=g, device="cuda").to(dtype)
+    wide = torch.cat([table, torch.full((len(nodes), 600 - table.shape[1]), 2**31 - 1, dtype=torch.int32, device="cuda")], 1)
+    cache = pkg.KvCache(cache.pool, cache.page_stride, wide.data_ptr(), 600, cache.pages, Hk, d)
+    assert pkg.tree_attention_workspace(len(nodes), max(nodes), H, cache) > 0
+    masks = _random_masks(nodes, 9)
+    out = _tree(q, k, v, cache, lengths, masks, nodes, dtype)
+    _check_tree(q, k, v, pool, table, lengths, masks, nodes, out, dtype)
+    assert bool((out[sum(nodes):] == 7.0).all())
+
+
 @pytest.mark.parametrize("nodes", [1, 7, 40])
 def test_tree_attention_many_sequences(nodes):
     """Grids of several waves, ragged lengths, nodes fewer than max_nodes."""
@@ -706,6 +730,8 @@ def test_captured_step_follows_its_inputs():
     lengths = [500, 20]
     pool, table, cache = _cache_of([640, 640], Hk, d, BF16, g)
     pool.normal_(generator=g)
+    wide = torch.cat([table, torch.full((2, 90), -1, dtype=torch.int32, device="cuda")], 1)  # room for long caches: the work goes in parts
+    cache = pkg.KvCache(cache.pool, cache.page_stride, wide.data_ptr(), 100, cache.pages, Hk, d)
     n, M = 2, 2 * T
     off = _ints([0, T, 2 * T])
     size = pkg.tree_attention_workspace(n, T, H, cache)
