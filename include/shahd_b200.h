@@ -313,7 +313,7 @@ const char* shahd_last_error(void);
  *    asynchronous on `stream` (0 = the legacy stream), allocate nothing, keep nothing between calls and can be captured
  *    into CUDA graphs. Sequences are packed: rows offsets[s] .. offsets[s+1]-1 are sequence s (offsets int32 [n+1] on the
  *    device, ascending, offsets[n] <= rows; empty sequences are allowed). Rows behind the last sequence are neither
- *    read nor written. Operands and results must not overlap unless a function says so. At most 2^30 rows; a result's rows
+ *    read nor written. Operands and results must not overlap unless a function says so. At most 2^30 rows and sequences; a result's rows
  *    lie apart by all its heads, or its heads by all its rows.
  * ============================================================================================== */
 

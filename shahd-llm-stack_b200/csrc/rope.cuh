@@ -423,6 +423,10 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
              c->kv_heads);
     return SHAHD_EINVAL;
   }
+  if (c->n > kOpsMaxRows) {
+    SetError("%s: too many sequences: %d, at most 2^30", op, c->n);
+    return SHAHD_EINVAL;
+  }
   if (c->n < 0 || (cache && (c->n < 1 || !c->offsets)) || (c->offsets && c->n < 1)) {
     SetError("%s: offsets, and so a cache, need n >= 1 sequences (got n=%d)", op, c->n);
     return SHAHD_EINVAL;

@@ -99,9 +99,9 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
 // few hundred, end together. A range costs the second kernel, about as long as eight steps, and both parts' rows written and
 // read in 32 bits; so where there is a place for every pair and its steps are few, pairs it is (72 trees of 13 to 26 nodes,
 // 12/4 heads of 64, up to 254 positions: ranges 29 us, pairs 10.9; 8 single tokens, 32/8 heads of 128, up to 2000 positions: 25.9
-// and 21.6; one tree of 24 over 2047 positions, 16/4 heads of 64: 13.5 and 23.3). Long caches in ranges (16 trees over 20 to 32 thousand positions, 8 kv heads of 128: a block of threads for each pair
-// 490 us, parts of 2048 keys 513 us, ranges 427 us; but 512 pairs of 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as
-// 256 pairs of heads).
+// and 21.6; one tree of 24 over 2047 positions, 16/4 heads of 64: 13.5 and 23.3). 16 trees over 20 to 32 thousand positions, 8
+// kv heads of 128, kernel alone: a block of threads for each pair 490 us, parts of 2048 keys 513, ranges 427; but 512 pairs of
+// 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as 256 pairs of heads.
 constexpr int kTaSms = 148;  // of a B200: the layout, and so the workspace, does not hang on a device being there
 struct TreeLayout {
   int pairs, two_heads, least, part_rows;
@@ -173,7 +173,7 @@ int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
   a.G = H / Hk;
   a.TB = 128 / a.G;
   const long long blocks = ((long long)c->rows / (2 * a.TB) + c->n) * Hk;
-  if (blocks > 0x7fffffffLL) {
+  if (blocks > kOpsMaxRows) {
     SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
     return SHAHD_EINVAL;
   }

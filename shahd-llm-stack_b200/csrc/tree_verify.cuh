@@ -329,8 +329,8 @@ extern "C" int shahd_verify_tree(const ShahdVerifyCall* c, void* stream) {
              op, c->n, c->rows, c->vocab, (long long)c->target_stride, (long long)c->draft_stride);
     return SHAHD_EINVAL;
   }
-  if (c->rows > kOpsMaxRows) {
-    SetError("%s: too many rows: %d, at most 2^30", op, c->rows);
+  if (c->rows > kOpsMaxRows || c->n > kOpsMaxRows) {
+    SetError("%s: too many rows or sequences: %d and %d, at most 2^30", op, c->rows, c->n);
     return SHAHD_EINVAL;
   }
   if (c->n == 0) return SHAHD_OK;

@@ -46,6 +46,7 @@ def test_rope_calls():
         _refused("q_out needs row and head strides", rope.apply, **{**ok, "q_out": pkg.Rows(1 << 20, -128, 64)})
         _refused("rows and heads of q_out share memory", rope.apply, **{**ok, "q_out": pkg.Rows(1 << 20, 64, 64)})
         _refused("too many rows", rope.apply, **{**ok, "rows": 2**30 + 1})
+        _refused("too many sequences", rope.apply, **{**ok, "offsets": 1 << 20, "n": 2**30 + 1})
 
 
 def test_prompt_calls():
@@ -62,6 +63,7 @@ def test_prompt_calls():
     _refused("out needs row and head strides", call, **{**ok, "out": pkg.Rows(1 << 20, 128, 0)})
     _refused("too many rows", call, **{**ok, "n": 2**31 - 1, "rows": 2**30})
     _refused("too many rows", call, **{**ok, "rows": 2**30 + 1})
+    _refused("too many rows and sequences", call, **{**ok, "n": 2**30 + 1, "num_heads": 1, "kv_heads": 1})
     _refused("share memory", call, **{**ok, "out": pkg.Rows(1 << 20, 64, 64)})
     _refused("share memory", call, **{**ok, "out": pkg.Rows(1 << 20, 64, 3 * 64)})
     if not has_gpu():
@@ -101,6 +103,7 @@ def test_verify_calls():
     _refused("1 <= vocab", call, **{**ok, "vocab": 0})
     _refused("strides of at least vocab", call, **{**ok, "target_stride": 9})
     _refused("too many rows", call, **{**ok, "rows": 2**30 + 1})
+    _refused("or sequences", call, **{**ok, "n": 2**30 + 1})
     _refused("need lengths", call, **{**ok, "commit": at})
     _refused("need lengths", call, **{**ok, "new_lengths": at})
     call(**{**ok, "n": 0})
