@@ -408,8 +408,9 @@ typedef struct ShahdPromptCall {
   ShahdRows q, k, v, out; /* 16-byte aligned, strides multiples of 8 */
 } ShahdPromptCall;
 /* out[i] = sum over j <= i of softmax_j(scale q[i].k[j]) v[j] within each sequence. Softmax and sums in 32 bits; the
- * probabilities meet v in dtype. A value of k or v that is not finite can reach every row of its own sequence, the
- * earlier ones too, but no other sequence. */
+ * probabilities meet v in dtype. A row that sees a score of NaN or +inf is NaN; a score of -inf has weight 0, and a row that sees
+ * no other is NaN. A value of v that is not finite can reach every row of its own sequence, the earlier ones too, but no other
+ * sequence. */
 int shahd_prompt_attention(const ShahdPromptCall* call, void* stream);
 
 /* ---- attention of drafted token trees over the cache (verify passes; one node per sequence is a decode step) ---- */
@@ -434,8 +435,8 @@ typedef struct ShahdTreeCall {
 int64_t shahd_tree_attention_workspace(const ShahdTreeCall* call);
 /* out[i] = sum of softmax(scale q[i].k[j]) v[j] over the cached positions of the row's sequence and the rows of its mask;
  * a row that attends to nothing gives 0. Positions at or beyond the length are never used, whatever their pages
- * hold. A value of the nodes' or the cached k or v that is not finite can reach every row of its own sequence, masked rows
- * too, but no other sequence. */
+ * hold. Scores that are not finite: as in shahd_prompt_attention. A value of the nodes' or the cached v that is not finite
+ * can reach every row of its own sequence, masked rows too, but no other sequence. */
 int shahd_tree_attention(const ShahdTreeCall* call, void* stream);
 
 /* ---- verification of drafted trees (SpeculativeSample, SpeculativeSampling.ts:82-112, for trees and device rows) ---- */

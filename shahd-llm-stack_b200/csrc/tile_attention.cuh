@@ -163,9 +163,10 @@ __device__ __forceinline__ f32x2 Add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The largest of three, NaN if one of them is.
 __device__ __forceinline__ float Max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -179,7 +180,8 @@ __device__ __forceinline__ float Exp2(float x) {
 // a 128 x 128 block of scores wants 16384 of them next to products of 1024 (head_dim 128) or 512 clocks. x = n + f with n the
 // nearest integer (adding 1.5 * 2^23 leaves n in the low bits), 2^f by the degree-4 polynomial of least greatest relative
 // error on [-1/2, 1/2] (Remez exchange; 2.7e-6 in 32 bits, a thousandth of a bf16 rounding), n added to the exponent.
-// x is cut at -126: what is smaller becomes 2^-126, nothing next to a sum that holds at least one 2^-8.
+// x is cut at -126: what is smaller becomes 2^-126, nothing next to a sum that holds at least one 2^-8. NaN and infinite x give
+// numbers that mean nothing: Spoil() sees to the rows that have them.
 __device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
   const f32x2 magic = Two(12582912.f, 12582912.f), x = Two(fmaxf(a, -126.f), fmaxf(b, -126.f));
   const f32x2 r = Add2(x, magic);
@@ -193,6 +195,11 @@ __device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
   Split(r, r0, r1);
   return Two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23)));
 }
+
+// What a row's maximum adds to its sum: NaN where scores that are not finite (or leave 32 bits by the scale) make the row's weights
+// meaningless, else 0. Carried by the maximum, such scores cost nothing per key, and the row comes out NaN whichever way its
+// exponentials are formed. -inf stands for no key yet, or only ones of weight 0; what these add is told apart at the end.
+__device__ __forceinline__ float Spoil(float m, float scale) { return m == -INFINITY ? 0.f : m * scale * 0.f; }
 
 // 32 bytes at once: a whole sector, where 16-byte stores of lanes that lie a row apart write halves.
 __device__ __forceinline__ void Store32B(float* p, const float* v) {
@@ -964,17 +971,18 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             }
             most(0, KEYS);
           }
-          const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          const float mx = Max3(Max3(x[0], x[1], x[2]), x[3], x[3]);
           if (t == 0) {
             m = mx;
-          } else if (__any_sync(0xffffffffu, mine && (mx - m) * sc > kTaLazy)) {
+            l = Spoil(m, sc);
+          } else if (__any_sync(0xffffffffu, mine && !((mx - m) * sc <= kTaLazy))) {  // a NaN moves the maximum too
             // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
             // or a result's last bits would hang on them)
             // step t-1's products are complete: S of step t was issued behind them
-            const float mn = fmaxf(m, mx);
+            const float mn = Max3(m, mx, mx);
             const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
             m = mn;
-            l *= alpha;
+            l = fmaf(l, alpha, Spoil(m, sc));
 #pragma unroll 1
             for (int c = 0; c < D / 16; c++) {
               uint32_t o[16];
@@ -1031,6 +1039,24 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       done += w.Blocks(i);
       const bool merge = TREE && w.turns == kTurns && w.blocks1 > 0;
       if (w.Blocks(i) > 0) ok = TaWait(sh, &sh->o_full[i], (i ? outs1 : outs0) & 1) && ok;
+      // No score above -inf: the row saw no key, or (the sum is then 1, and the row NaN) none of a weight.
+      if (m == -INFINITY) {
+        bool saw = !TREE && mine;
+        if constexpr (TREE) {
+#pragma unroll 1
+          for (int t = 0; t < w.Blocks(i) && mine && !saw; t++) {
+            const int b = blk.Index(i, t);
+            if (b < w.cache_blocks) {
+              const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
+              saw = (unsigned)tb[0] < (unsigned)A.pages || (KEYS == 128 && blk.Keys(b) > 64 && (unsigned)tb[1] < (unsigned)A.pages);
+            } else {
+              const unsigned long long bits = A.masks[w.start + tok0 + token];
+              saw = (w.nodes < 64 ? bits & ((1ull << w.nodes) - 1) : bits) != 0;
+            }
+          }
+        }
+        l = saw ? 1.f : 0.f;
+      }
       if (merge && i == 1) {
         // the same rows' other key blocks: tile 0's threads read this accumulator, in the same lanes, too
         sml[r] = m;
@@ -1038,7 +1064,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         MbarArrive(&sh->ml_full);
         ok = TaWait(sh, &sh->ml_free, merges & 1) && ok;  // before the next segment's products may write over it
       } else if (!(w.turns == kTurns && i == 1)) {
-        float a0 = 1.f, a1 = 0.f;
+        float a0 = 1.f, a1 = 1.f;
         if (merge) {
           ok = TaWait(sh, &sh->ml_full, merges & 1) && ok;
           ok = TaWait(sh, &sh->o_full[1], outs1 & 1) && ok;
@@ -1054,11 +1080,11 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           TcgenFenceAfter();
           const bool parts = RANGES && w.part >= 0;
           if (!parts) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
+            const float inv = m != -INFINITY ? 1.f / l : l == 0.f ? 0.f : NAN;  // nothing seen: 0
             a0 *= inv;
             a1 *= inv;
           }
-          const bool zero = !parts && l == 0.f;
+          const bool zero = !parts && m == -INFINITY && l == 0.f;
           const int node = tok0 + token;
           uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
           const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
@@ -1135,17 +1161,19 @@ __global__ void __launch_bounds__(256) TreeJoinKernel(const __grid_constant__ Ta
 #pragma unroll 2
   for (int c = c0; c <= c1; c++) {
     const float2 ml = A.part_ml[slot(c)];
-    const float a = m == -INFINITY ? 0.f : Exp2(ml.x - m);
+    const float a = m == -INFINITY ? 1.f : Exp2(ml.x - m);
     l = fmaf(ml.y, a, l);
     const float* o = A.part_o + slot(c) * D + lane * (D / 32);
 #pragma unroll
     for (int j = 0; j < D / 32; j++) v[j] = fmaf(o[j], a, v[j]);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  // a part whose maximum is NaN has a sum of NaN, which this sum takes over
+  const float inv = m != -INFINITY ? 1.f / l : NAN;
+  const bool zero = m == -INFINITY && l == 0.f;
   uint16_t* out = A.out + (long long)row * A.out_row + (long long)h * A.out_head + lane * (D / 32);
 #pragma unroll
   for (int j = 0; j < D / 32; j++) {
-    const float x = l == 0.f ? 0.f : v[j] * inv;
+    const float x = zero ? 0.f : v[j] * inv;
     out[j] = (uint16_t)Pack2<F16>(x, 0.f);
   }
 }
