@@ -347,7 +347,7 @@ typedef struct ShahdKvCache {
  * been told so. */
 int shahd_attention_cache(ShahdAttention* a, ShahdKvCache* out);
 /* Sets the cached positions of sequences 0..n-1 (host lengths, 0 .. capacity), in the order of `stream` (0 = the operator's
- * own stream). */
+ * own stream). The lengths are taken over before the call returns, whatever host memory they lie in. */
 int shahd_attention_set_lengths(ShahdAttention* a, const int32_t* lengths, int32_t n, void* stream);
 
 /* ---- rotary positions (ApplyRope, RotaryEmbedding.ts:63-75, with further layouts and scalings) ---- */

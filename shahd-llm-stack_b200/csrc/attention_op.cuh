@@ -84,6 +84,16 @@ __global__ void AttnAdvanceKernel(int* len, int n) {
   if (i < n) len[i] += 1;
 }
 
+// Lengths that travel with the launch: the host's array may be reused as soon as the call returns, in whatever memory it lies.
+constexpr int kAttnLengths = 512;
+struct AttnLengths {
+  int v[kAttnLengths];
+};
+__global__ void AttnSetLengthsKernel(int* len, const __grid_constant__ AttnLengths from, int n) {
+  const int i = threadIdx.x;
+  if (i < n) len[i] = from.v[i];
+}
+
 template <class T>
 int OpAlloc(AttentionOp* a, T** p, size_t count) {
   void* v = nullptr;
@@ -366,7 +376,11 @@ int shahd_attention_set_lengths(ShahdAttention* a, const int32_t* lengths, int32
       return SHAHD_EINVAL;
     }
   std::lock_guard<std::mutex> g(a->mu);
-  SHAHD_CUDA_TRY(cudaSetDevice(a->device));
+  DeviceScope scope(a->device);
+  if (!scope.ok) {
+    SetError("shahd_attention_set_lengths: device %d could not be made current", a->device);
+    return SHAHD_ECUDA;
+  }
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : a->stream;
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   SHAHD_CUDA_TRY(cudaStreamIsCapturing(st, &capturing));
@@ -374,9 +388,15 @@ int shahd_attention_set_lengths(ShahdAttention* a, const int32_t* lengths, int32
     SetError("shahd_attention_set_lengths: the operator's host lengths cannot be part of a captured graph");
     return SHAHD_EINVAL;
   }
-  // from pageable memory: the call returns with the lengths taken over
-  SHAHD_CUDA_TRY(cudaMemcpyAsync(a->d_len, lengths, sizeof(int) * (size_t)n, cudaMemcpyHostToDevice, st));
-  for (int i = 0; i < n; i++) a->h_len[i] = lengths[i];
+  for (int i = 0; i < n; i += kAttnLengths) {
+    AttnLengths part;
+    const int m = std::min(n - i, kAttnLengths);
+    std::copy(lengths + i, lengths + i + m, part.v);
+    AttnSetLengthsKernel<<<1, kAttnLengths, 0, st>>>(a->d_len + i, part, m);
+  }
+  const int rc = CheckLaunch("shahd_attention_set_lengths");
+  if (rc != SHAHD_OK) return rc;
+  std::copy(lengths, lengths + n, a->h_len.begin());
   return SHAHD_OK;
 }
 

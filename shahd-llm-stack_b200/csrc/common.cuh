@@ -26,6 +26,20 @@ void ClearError();
     }                                                                                             \
   } while (0)
 
+// Makes `device` current for the scope of a call and the caller's device current again after it.
+struct DeviceScope {
+  int before = -1;
+  bool ok = true;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before == device) before = -1;
+    else ok = cudaSetDevice(device) == cudaSuccess;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 using bf16 = __nv_bfloat16;
 
 // Kernel launches of a decode step use programmatic dependent launch: the next kernel is scheduled while

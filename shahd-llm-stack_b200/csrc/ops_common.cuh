@@ -23,20 +23,6 @@ static __device__ int g_ops_device_error;  // 0, or the first kOpsErr* recorded 
 
 inline size_t TypeBytes(int dtype) { return dtype == SHAHD_F32 ? 4 : 2; }
 
-// Makes `device` current for the scope of a call and the caller's device current again after it.
-struct DeviceScope {
-  int before = -1;
-  bool ok = true;
-  explicit DeviceScope(int device) {
-    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-    if (before == device) before = -1;
-    else ok = cudaSetDevice(device) == cudaSuccess;
-  }
-  ~DeviceScope() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
-
 // The device that every buffer of a call lives on. Add() takes the call's pointers one by one; a host pointer, an
 // address that no allocation holds or a buffer of another device makes the call fail before anything is launched.
 struct BufferCheck {

@@ -40,3 +40,13 @@ def test_set_lengths_does_not_read_the_array_after_it_returned(pinned, n):
             w = torch.einsum("hl,lhd->hd", p, vv)
             # the operator's own bar: 2e-2 of the output's range
             assert float((got[i].double() - w).abs().max()) < 2e-2 * float(w.max() - w.min())
+
+
+def test_set_lengths_leaves_the_current_device():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    with pkg.FusedAttention(2, 2, 2, 32, 64, device=1) as op:
+        torch.cuda.set_device(0)
+        op.set_lengths([3, 4])
+        assert torch.cuda.current_device() == 0
+        assert (op.length(0), op.length(1)) == (3, 4)
