@@ -87,7 +87,7 @@ struct TaArgs {
   // has room for two, [2 c] for a pair that it does not begin and [2 c + 1] for one that it does not end.
   int least, part_rows;
   float* part_o;    // [2 grid, part_rows, D]
-  float2* part_ml;  // [2 grid, part_rows]: running maximum (of scaled log2 scores) and sum
+  float2* part_ml;  // [2 grid, part_rows]: -Offset() of the running maximum, and the sum
   int* plan;        // the ranges' length, then for every sequence the blocks of all before it, and their total
 };
 
@@ -196,10 +196,19 @@ __device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
   return Two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23)));
 }
 
-// What a row's maximum adds to its sum: NaN where scores that are not finite (or leave 32 bits by the scale) make the row's weights
-// meaningless, else 0. Carried by the maximum, such scores cost nothing per key, and the row comes out NaN whichever way its
+// A probability is 2^(s * scale + Offset(m)), one fused step per score. The offset is rounded, by up to 2^-24 of m * scale: a factor
+// of all the row's probabilities, which leaves with the division by their sum as long as every place that changes from one
+// maximum to another takes the difference of the rounded offsets.
+__device__ __forceinline__ float Offset(float m, float scale, float bias) { return fmaf(-m, scale, bias); }
+// What a row's maximum adds to its sum: 0, or NaN where the row's weights mean nothing or that factor could leave the range
+// that P has: scores that are not finite, or so large that it reaches 2^64 (bf16, at 2^30) or a quarter (fp16, whose P may grow to
+// 2^15, at 2^23). Carried by the maximum, such scores cost nothing per key, and the row comes out NaN whichever way its
 // exponentials are formed. -inf stands for no key yet, or only ones of weight 0; what these add is told apart at the end.
-__device__ __forceinline__ float Spoil(float m, float scale) { return m == -INFINITY ? 0.f : m * scale * 0.f; }
+template <bool F16>
+__device__ __forceinline__ float Spoil(float m, float scale) {
+  constexpr float kMost = F16 ? 8388608.f : 1073741824.f;
+  return m == -INFINITY || fabsf(m * scale) < kMost ? 0.f : NAN;
+}
 
 // 32 bytes at once: a whole sector, where 16-byte stores of lanes that lie a row apart write halves.
 __device__ __forceinline__ void Store32B(float* p, const float* v) {
@@ -974,15 +983,15 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           const float mx = Max3(Max3(x[0], x[1], x[2]), x[3], x[3]);
           if (t == 0) {
             m = mx;
-            l = Spoil(m, sc);
+            l = Spoil<F16>(m, sc);
           } else if (__any_sync(0xffffffffu, mine && !((mx - m) * sc <= kTaLazy))) {  // a NaN moves the maximum too
             // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
             // or a result's last bits would hang on them)
             // step t-1's products are complete: S of step t was issued behind them
             const float mn = Max3(m, mx, mx);
-            const float alpha = mn == -INFINITY ? 1.f : Exp2((m - mn) * sc);
+            const float alpha = mn == -INFINITY ? 1.f : Exp2(Offset(mn, sc, kBias) - Offset(m, sc, kBias));
             m = mn;
-            l = fmaf(l, alpha, Spoil(m, sc));
+            l = fmaf(l, alpha, Spoil<F16>(m, sc));
 #pragma unroll 1
             for (int c = 0; c < D / 16; c++) {
               uint32_t o[16];
@@ -993,7 +1002,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
               TmemStore16(ocol + 16u * c, o);
             }
           }
-          const float neg = m == -INFINITY ? 0.f : kBias - m * sc;
+          const float neg = m == -INFINITY ? 0.f : Offset(m, sc, kBias);
           const f32x2 sc2 = Two(sc, sc), neg2 = Two(neg, neg);
           f32x2 sum[2] = {0, 0};
           // 32 keys: the probabilities, their sum, and the 16-bit pairs into TMEM
@@ -1070,8 +1079,9 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           ok = TaWait(sh, &sh->o_full[1], outs1 & 1) && ok;
           const float m2 = sml[r], l2 = sml[128 + r], mn = fmaxf(m, m2);
           if (mn != -INFINITY) {
-            a0 = Exp2((m - mn) * sc);
-            a1 = Exp2((m2 - mn) * sc);
+            const float to = Offset(mn, sc, kBias);
+            a0 = Exp2(to - Offset(m, sc, kBias));
+            a1 = Exp2(to - Offset(m2, sc, kBias));
           }
           m = mn;
           l = l * a0 + l2 * a1;
@@ -1117,7 +1127,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
               }
             }
           }
-          if (parts && mine && ok) A.part_ml[slot] = make_float2(m * sc, l);
+          if (parts && mine && ok) A.part_ml[slot] = make_float2(-Offset(m, sc, kBias), l);
         }
         if (merge) {
           TcgenFenceBefore();

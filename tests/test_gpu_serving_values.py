@@ -91,3 +91,60 @@ def test_tree_rows_that_see_a_score_that_is_not_finite(H, Hk, d, nodes, wide, dt
         spoiled += _check_rows(out[b:e], q[b:e], torch.cat([cached[0], k[b:e]]), torch.cat([cached[1], v[b:e]]), seen, dtype)
     assert spoiled > keys
     assert bool((out[off[keys + 3] + 1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("how", ["prompt", "pairs", "ranges"])
+def test_large_scores_that_lie_close_to_each_other(how, d, dtype):
+    """Scores of 2^27 (bf16) and 2^24 (fp16), exact in 32 bits, that grow along the keys by a few units in the last place, so that the
+    maximum moves again and again, over blocks, tiles by turns and parts.
+
+    The weights are right to 2^-13 although the product of a maximum with the scale is rounded by up to 1 and 1/8 in log2: an exponent
+    of at most 150 is rounded once (2^-17), an exponential is good to 2.7e-6, and so is each of at most 40 changes of the maximum
+    (2^-24 of a difference of offsets below 150, 2^-22 of its exponential)."""
+    g, L = _gen(65), 290
+    j = torch.arange(L, device="cuda")
+    base, step = (2.0 ** 13, 16.0) if dtype == BF16 else (2.0 ** 12, 2.0)
+    n = j // 5 + torch.randint(0, 3, (L,), generator=g, device="cuda") if dtype == BF16 else j + torch.randint(0, 8, (L,), generator=g, device="cuda")
+    q, k, v = torch.zeros(L, 2, d, dtype=dtype, device="cuda"), torch.zeros(L, 1, d, dtype=dtype, device="cuda"), _normal(g, L, 1, d, dtype=dtype)
+    q[:, 0, 0], q[:, 0, 1], k[:, 0, 0], k[:, 0, 1] = base, step, 2 * base if dtype == BF16 else base, n.to(dtype)
+    q[:, 1] = -q[:, 0]
+    scores = q[:, 0].double() @ k[:, 0].double().T
+    assert torch.equal(scores.float().double(), scores) and torch.equal(scores[0], scores[0, 0] + step * (n - n[0]).double())
+    scale = 0.125
+    if how == "prompt":
+        out, want, bound, rows = _prompt(q, k, v, [L], dtype, scale=scale), *_close(q, k, v, torch.ones(L, L, device="cuda").tril().bool(), scale, dtype), L
+    else:
+        rows = 70  # sequence s: the first 220 + s keys in the cache, the next one its own row
+        pool, table, cache = _cache_of([L], 1, d, dtype, g)
+        for p in range(L):
+            pool[table[0, p // 64], -1, 0, 0, p % 64], pool[table[0, p // 64], -1, 0, 1, p % 64] = k[p, 0], v[p, 0]
+        held = torch.full((rows, 1200 if how == "ranges" else table.shape[1]), -1, dtype=torch.int32, device="cuda")
+        held[:, :table.shape[1]] = table
+        cache = pkg.KvCache(cache.pool, cache.page_stride, held.data_ptr(), held.shape[1], cache.pages, 1, d)
+        assert (pkg.tree_attention_workspace(rows, 1, 2, cache) > 0) == (how == "ranges")
+        own = slice(220, 290)
+        out = _tree(q[own], k[own], v[own], cache, list(range(220, 290)), torch.ones(rows, dtype=torch.int64, device="cuda"), [1] * rows, dtype, scale=scale)
+        want, bound = _close(q[own], k, v, torch.ones(L, L, device="cuda").tril().bool()[own], scale, dtype)
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
+def _close(q, k, v, seen, scale, dtype):
+    want, _ = R.attend(q, k, v, seen, scale, dtype)
+    mass, _ = R.attend(q, k, v.abs(), seen, scale, dtype)
+    u = R.HALF_STEP[dtype]
+    # fp16 probabilities have a fixed step below 2^-14 of 2^7 times the largest, rounded offset included
+    return want, u * want.abs() + mass * (u + 2.0 ** -12) + (2.0 ** -31 * v.abs().double().sum() + 2.0 ** -25 if dtype == F16 else 0.0)
+
+
+@pytest.mark.parametrize("dtype,most", [(BF16, 2.0 ** 30), (F16, 2.0 ** 23)], ids=["bf16", "f16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_beyond_the_range_give_nan(dtype, most, sign):
+    """Rows that see one key, of a score at the range's end (in log2) and just below it."""
+    g = _gen(66)
+    q, k, v = torch.zeros(2, 1, 64, dtype=dtype, device="cuda"), torch.zeros(2, 1, 64, dtype=dtype, device="cuda"), _normal(g, 2, 1, 64, dtype=dtype)
+    q[:, 0, 3] = 2.0 ** 15
+    k[0, 0, 3], k[1, 0, 3] = sign * most / 2 ** 15, sign * most / 2 ** 15 * (1 - 2.0 ** -7)
+    out = _prompt(q, k, v, [1, 1], dtype, scale=1 / math.log2(math.e))
+    assert bool(out[0].isnan().all()) and torch.equal(out[1], v[1])
