@@ -342,13 +342,14 @@ int shahd_rope_create(const ShahdRopeCfg* cfg, ShahdRope** out) {
     return SHAHD_EINVAL;
   }
   const bool scaled = cfg->scaling != SHAHD_ROPE_UNSCALED;
-  if (!(cfg->base > 1) || !std::isfinite(cfg->base) || !std::isfinite(cfg->magnitude) || cfg->magnitude == 0 ||
+  const float magnitude = (float)cfg->magnitude;
+  if (!(cfg->base > 1) || !std::isfinite(cfg->base) || !std::isfinite(magnitude) || magnitude == 0 ||
       (scaled && (!(cfg->factor >= 1) || !std::isfinite(cfg->factor)))) {
-    SetError("%s: need a finite base > 1, a finite magnitude other than 0 and, for a scaling, a finite factor >= 1 (got "
+    SetError("%s: need a finite base > 1, a magnitude that is finite and not 0 in 32 bits and, for a scaling, a finite factor >= 1 (got "
              "base=%g magnitude=%g factor=%g)", op, cfg->base, cfg->magnitude, cfg->factor);
     return SHAHD_EINVAL;
   }
-  double low = 0, high = 0;
+  double low = 0, high = 0, base = cfg->base;
   switch (cfg->scaling) {
     case SHAHD_ROPE_UNSCALED:
     case SHAHD_ROPE_LINEAR:
@@ -356,6 +357,11 @@ int shahd_rope_create(const ShahdRopeCfg* cfg, ShahdRope** out) {
     case SHAHD_ROPE_STRETCHED:
       if (r < 4) {
         SetError("%s: SHAHD_ROPE_STRETCHED needs rotary_dim >= 4, got %d", op, r);
+        return SHAHD_EINVAL;
+      }
+      base *= std::pow(cfg->factor, r / (r - 2.0));
+      if (!std::isfinite(base)) {
+        SetError("%s: the stretched base %g * %g^(r/(r-2)) is not finite", op, cfg->base, cfg->factor);
         return SHAHD_EINVAL;
       }
       break;
@@ -386,9 +392,7 @@ int shahd_rope_create(const ShahdRopeCfg* cfg, ShahdRope** out) {
   p->head_dim = cfg->head_dim;
   p->rotary = r;
   p->layout = cfg->layout;
-  p->magnitude = (float)cfg->magnitude;
-  const double base =
-      cfg->scaling == SHAHD_ROPE_STRETCHED ? cfg->base * std::pow(cfg->factor, r / (r - 2.0)) : cfg->base;
+  p->magnitude = magnitude;
   for (int i = 0; i < r / 2; i++) {
     double f = std::pow(base, -2.0 * i / r);
     if (cfg->scaling == SHAHD_ROPE_LINEAR) f /= cfg->factor;

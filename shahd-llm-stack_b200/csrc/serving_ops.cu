@@ -60,11 +60,11 @@ bool CheckHeads(const char* op, int H, int Hk, int d) {
 
 bool ScaleOf(const char* op, double scale, int d, float* log2) {
   if (scale == 0) scale = 1.0 / std::sqrt((double)d);
-  if (!(scale > 0) || !std::isfinite(scale)) {
-    SetError("%s: scale must be positive and finite, or 0 for 1/sqrt(head_dim)", op);
+  *log2 = (float)(scale * M_LOG2E);
+  if (!(*log2 > 0) || !std::isfinite(*log2)) {  // in 32 bits, too: masked scores are -inf times it
+    SetError("%s: scale must be positive and finite in 32 bits, or 0 for 1/sqrt(head_dim) (got %g)", op, scale);
     return false;
   }
-  *log2 = (float)(scale * M_LOG2E);
   return true;
 }
 
