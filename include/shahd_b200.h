@@ -106,7 +106,9 @@ void ShahdSetFusedAttentionBlock(int enable);
  * or 128 x 128 tiles) after a per-row norm-statistics pass; 0 keeps one 128 x 128 tile per CTA. Results agree
  * within the parity tolerance. Process-wide tuning hook; no counterpart in the reference. */
 void ShahdSetPersistentPrefillProjections(int enable);
-/* First error code a kernel recorded for a bounded device-side wait that gave up (0 = none). */
+/* First error code a kernel recorded for a bounded device-side wait that gave up (0 = none, -1 = a flag could not be read): the
+ * current device's of sections 1 and 2, and for the operators of section 3 every device's that they have run on. Waits for nothing but
+ * the legacy stream: synchronise with the calls' streams before. */
 int ShahdDeviceErrorFlag(void);
 /* Device-pointer MatMulNT on the tensor cores: out[M,N] (+)= a[M,K] @ btᵀ with a, bt bf16 row-major
  * on the device, out fp32; tcgen05/TMEM tiles fed by TMA. K must be a multiple of 8 and the three
@@ -314,7 +316,8 @@ const char* shahd_last_error(void);
  *    into CUDA graphs. Sequences are packed: rows offsets[s] .. offsets[s+1]-1 are sequence s (offsets int32 [n+1] on the
  *    device, ascending, offsets[n] <= rows; empty sequences are allowed). Rows behind the last sequence are neither
  *    read nor written. Operands and results must not overlap unless a function says so. At most 2^30 rows and sequences; a result's rows
- *    lie apart by all its heads, or its heads by all its rows.
+ *    lie apart by all its heads, or its heads by all its rows. A kernel's wait that gives up (it should not) ends the call with some
+ *    rows of its result undefined; the call has returned by then, and ShahdDeviceErrorFlag tells.
  * ============================================================================================== */
 
 #define SHAHD_BF16 0

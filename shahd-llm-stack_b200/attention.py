@@ -10,6 +10,8 @@ Next to it, attention on the caller's own buffers: prompt_attention for prompts 
 call, tree_attention for drafted token trees (or single new tokens) against a paged cache, such as FusedAttention's own
 (FusedAttention.cache). They keep no state: calls on different streams or devices do not meet, and both can be
 captured into CUDA graphs. A stream of 0 is the legacy default stream there.
+A wait inside a kernel that gives up leaves rows undefined and is recorded: _lib.load().ShahdDeviceErrorFlag() is 0 as long
+as none has.
 """
 from __future__ import annotations
 

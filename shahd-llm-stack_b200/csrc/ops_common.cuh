@@ -19,7 +19,7 @@ constexpr int kOpsPage = 64;                     // positions of a cache page
 constexpr uint32_t kOpsWaitLimit = 1u << 22;     // barrier probes before a wait gives up
 constexpr int kOpsErrTimeout = 6;                // a bounded wait of the tile attention gave up
 
-static __device__ int g_ops_device_error;  // 0, or the first kOpsErr* recorded on the device
+static __device__ int g_ops_device_error;  // 0, or the first kOpsErr* recorded on this device
 
 inline size_t TypeBytes(int dtype) { return dtype == SHAHD_F32 ? 4 : 2; }
 

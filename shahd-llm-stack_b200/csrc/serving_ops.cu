@@ -4,6 +4,7 @@
 #include <new>
 #include <type_traits>
 
+#include "device_flags.h"
 #include "ops_common.cuh"
 #include "rope.cuh"
 #include "tile_attention.cuh"
@@ -11,13 +12,17 @@
 
 namespace shahd {
 
+// The operators run where their buffers are, so a wait that gave up may have been recorded on any device that a kernel with waits
+// (the tile attention) has been launched on.
+static DeviceSet g_waiting_devices;
+
 int OpsDeviceError() {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_ops_device_error, sizeof v) != cudaSuccess) {
+  return FirstFlag(g_waiting_devices, [](int device, int* flag) {
+    DeviceScope scope(device);
+    if (scope.ok && cudaMemcpyFromSymbol(flag, g_ops_device_error, sizeof *flag) == cudaSuccess) return true;
     cudaGetLastError();
-    return 0;
-  }
-  return v;
+    return false;
+  });
 }
 
 namespace {
@@ -200,6 +205,7 @@ int shahd_prompt_attention(const ShahdPromptCall* c, void* stream) {
   a.H = H;
   a.Hk = Hk;
   TakeLaunchError(nullptr);
+  g_waiting_devices.Add(b.device);
   LaunchTiles<kPrompt>(d, c->dtype, a, (unsigned)blocks, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);
 }
@@ -296,6 +302,7 @@ int shahd_tree_attention(const ShahdTreeCall* c, void* stream) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * lay.grid * lay.part_rows * d);
   }
   TakeLaunchError(nullptr);
+  g_waiting_devices.Add(b.device);
   if (lay.least > 0) LaunchTiles<kTreeRanges>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
   else LaunchTiles<kTreePairs>(d, c->dtype, a, (unsigned)lay.grid, static_cast<cudaStream_t>(stream));
   return LaunchStatus(op);

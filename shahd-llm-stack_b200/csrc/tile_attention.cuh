@@ -237,6 +237,10 @@ __device__ __forceinline__ bool TaWait(TaShared* sh, uint64_t* bar, uint32_t par
   sh->abort = 1;
   return false;
 }
+// At the end of a block, whatever has given up before: what is in flight into the block's memory is waited for, within the limit.
+__device__ __forceinline__ void TaDrain(uint64_t* bar, uint32_t parity) {
+  if (!MbarWaitBounded(bar, parity, kOpsWaitLimit)) atomicCAS(&g_ops_device_error, 0, kOpsErrTimeout);
+}
 // The same for a whole warp, with one answer for all lanes.
 __device__ __forceinline__ bool TaWaitWarp(TaShared* sh, uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
@@ -728,8 +732,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           }
       } while (RANGES && ok && w.more);
       // every copy lands before the block may leave: the last phase of each unit's barrier
-      if (segment > 0) MbarWaitBounded(&sh->q_full, (segment - 1) & 1, kOpsWaitLimit);
-      for (int v = max(0, issued - U); v < issued; v++) MbarWaitBounded(&sh->full[v % U], (uint32_t)((v / U) & 1), kOpsWaitLimit);
+      if (segment > 0) TaDrain(&sh->q_full, (segment - 1) & 1);
+      for (int v = max(0, issued - U); v < issued; v++) TaDrain(&sh->full[v % U], (uint32_t)((v / U) & 1));
     } else if (warp == 8) {
       // The whole warp follows the same path, one lane of it issues.
       constexpr uint32_t kTypes = F16 ? 0u : (1u << 7) | (1u << 10);
@@ -883,7 +887,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       }
       UmmaIssueCommit(&sh->drained);
       __syncwarp();
-      MbarWaitBounded(&sh->drained, 0, kOpsWaitLimit);  // no product reads shared memory or TMEM after this
+      TaDrain(&sh->drained, 0);  // no product reads shared memory or TMEM after this
     }
   } else {
     if constexpr (Cfg::kWide) RegsUp<kTaRegsSoftmax>();
