@@ -412,8 +412,9 @@ typedef struct ShahdPromptCall {
 } ShahdPromptCall;
 /* out[i] = sum over j <= i of softmax_j(scale q[i].k[j]) v[j] within each sequence. Softmax and sums in 32 bits; the
  * probabilities meet v in dtype. A row that sees a score of NaN or +inf is NaN; a score of -inf has weight 0, and a row that sees
- * no other is NaN. So is a row whose largest score, scale included, has a magnitude of 7.4e8 (bf16) or 5.8e6 (fp16) and more. A
- * value of v that is not finite can reach every row of its own sequence, the earlier ones too, but no other sequence. */
+ * no other is NaN. Scores of a magnitude, scale included, of 7.4e8 (bf16) or 5.8e6 (fp16) and more can make a row that sees them
+ * NaN, and do if its largest one is such. A value of v that is not finite can reach every row of its own sequence, the earlier
+ * ones too, but no other sequence. */
 int shahd_prompt_attention(const ShahdPromptCall* call, void* stream);
 
 /* ---- attention of drafted token trees over the cache (verify passes; one node per sequence is a decode step) ---- */

@@ -200,14 +200,15 @@ __device__ __forceinline__ f32x2 Exp2Poly(float a, float b) {
 // of all the row's probabilities, which leaves with the division by their sum as long as every place that changes from one
 // maximum to another takes the difference of the rounded offsets.
 __device__ __forceinline__ float Offset(float m, float scale, float bias) { return fmaf(-m, scale, bias); }
-// What a row's maximum adds to its sum: 0, or NaN where the row's weights mean nothing or that factor could leave the range
-// that P has: scores that are not finite, or so large that it reaches 2^64 (bf16, at 2^30) or a quarter (fp16, whose P may grow to
-// 2^15, at 2^23). Carried by the maximum, such scores cost nothing per key, and the row comes out NaN whichever way its
-// exponentials are formed. -inf stands for no key yet, or only ones of weight 0; what these add is told apart at the end.
+// What a row's maximum adds to its sum at the end: 0, or NaN where the row's weights mean nothing or that factor could leave the
+// range that P has: scores that are not finite, or so large that it reaches 2^64 (bf16, at 2^30) or a quarter (fp16, whose P may
+// grow to 2^15, at 2^23). Carried by the maximum, which a NaN or +inf never leaves again, such scores cost nothing per step, and the row
+// comes out NaN whichever way its exponentials are formed. What a maximum below that range leaves behind when it moves up is
+// multiplied by 2^-inf: gone, or NaN where it was infinite. -inf stands for no key yet, or only ones of weight 0, told apart at the end.
 template <bool F16>
 __device__ __forceinline__ float Spoil(float m, float scale) {
   constexpr float kMost = F16 ? 8388608.f : 1073741824.f;
-  return m == -INFINITY || fabsf(m * scale) < kMost ? 0.f : NAN;
+  return fabsf(m * scale) < kMost ? 0.f : NAN;
 }
 
 // 32 bytes at once: a whole sector, where 16-byte stores of lanes that lie a row apart write halves.
@@ -987,7 +988,6 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           const float mx = Max3(Max3(x[0], x[1], x[2]), x[3], x[3]);
           if (t == 0) {
             m = mx;
-            l = Spoil<F16>(m, sc);
           } else if (__any_sync(0xffffffffu, mine && !((mx - m) * sc <= kTaLazy))) {  // a NaN moves the maximum too
             // (lanes without a row hold other sequences' scores, or what shared memory held: they do not move the others' maxima,
             // or a result's last bits would hang on them)
@@ -995,7 +995,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             const float mn = Max3(m, mx, mx);
             const float alpha = mn == -INFINITY ? 1.f : Exp2(Offset(mn, sc, kBias) - Offset(m, sc, kBias));
             m = mn;
-            l = fmaf(l, alpha, Spoil<F16>(m, sc));
+            l *= alpha;
 #pragma unroll 1
             for (int c = 0; c < D / 16; c++) {
               uint32_t o[16];
@@ -1069,6 +1069,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           }
         }
         l = saw ? 1.f : 0.f;
+      } else {
+        l += Spoil<F16>(m, sc);
       }
       if (merge && i == 1) {
         // the same rows' other key blocks: tile 0's threads read this accumulator, in the same lanes, too

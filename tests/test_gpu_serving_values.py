@@ -148,3 +148,21 @@ def test_scores_beyond_the_range_give_nan(dtype, most, sign):
     k[0, 0, 3], k[1, 0, 3] = sign * most / 2 ** 15, sign * most / 2 ** 15 * (1 - 2.0 ** -7)
     out = _prompt(q, k, v, [1, 1], dtype, scale=1 / math.log2(math.e))
     assert bool(out[0].isnan().all()) and torch.equal(out[1], v[1])
+
+
+@pytest.mark.parametrize("size", [2.0 ** 24, 2.0 ** 31, 2.0 ** 41, 2.0 ** 100])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_that_leave_scores_beyond_the_range_are_right_or_nan(d, size):
+    """A whole block of keys of scores far below the range, then ordinary ones: the weights of the first are 0."""
+    g, L, keys = _gen(67), 3 * KEYS[d] + 5, KEYS[d]
+    q, k, v = (_normal(g, L, h, d, dtype=BF16) for h in (2, 1, 1))
+    q[:, :, 0], k[:, :, 0] = 0.0, 0.0
+    q[:, :, 0], k[:keys, :, 0] = size ** 0.5 * 1.37, -(size ** 0.5) * (1 + torch.rand(keys, 1, generator=g, device="cuda"))
+    out = _prompt(q, k, v, [L], BF16)
+    seen = torch.ones(L, L, device="cuda").tril().bool()
+    seen[keys:, :keys] = False
+    want, bound = R.attend(q[keys:], k, v, seen[keys:], d ** -0.5, BF16)
+    off = (out[keys:].double() - want).abs()
+    assert bool((out[keys:].isnan() | (off <= bound)).all())
+    if size <= 2.0 ** 24:
+        assert bool(out.isfinite().all())
