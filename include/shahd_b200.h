@@ -347,7 +347,9 @@ typedef struct ShahdKvCache {
 
 /* The cache of a FusedAttention operator (bf16; sequence s is its slot s), for the operators below. It belongs to `a` and
  * ends with it. Rows appended through it count for shahd_attention_decode once shahd_attention_set_lengths has
- * been told so. */
+ * been told so. That function turns its q and k itself, by SHAHD_ROPE_INTERLEAVED pairs of the whole head_dim at the operator's
+ * rope_base, unscaled: keys that were appended must have been turned the same way. For any other rotation create the operator
+ * with rope_base 0, and turn its q and k by shahd_rope_apply before. */
 int shahd_attention_cache(ShahdAttention* a, ShahdKvCache* out);
 /* Sets the cached positions of sequences 0..n-1 (host lengths, 0 .. capacity), in the order of `stream` (0 = the operator's
  * own stream). The lengths are taken over before the call returns, whatever host memory they lie in. */

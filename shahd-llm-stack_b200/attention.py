@@ -70,7 +70,9 @@ class FusedAttention:
         _lib.check(self.lib.shahd_attention_decode(self.handle, q, k, v, n, out, stream or None))
 
     def cache(self) -> KvCache:
-        """This operator's cache (bf16, one layer) as rope.apply and tree_attention take it; valid until close()."""
+        """This operator's cache (bf16, one layer) as rope.apply and tree_attention take it; valid until close(). Keys appended
+        to it must be turned as this operator turns its own (Rope(head_dim, base=rope_base)) if its decode steps are to read
+        them; with rope_base 0 it turns nothing, and q and k are turned by any Rope before they get here."""
         out = KvCache()
         _lib.check(self.lib.shahd_attention_cache(self.handle, ctypes.byref(out)))
         return out
