@@ -150,13 +150,15 @@ __global__ void __launch_bounds__(kVerThreads, kVerPerSm) VerifyTreeKernel(const
     float x[VerifyRows<T>::PER];
     const uint4* vp = reinterpret_cast<const uint4*>(rows.p - rows.mis);
     const uint4* vq = reinterpret_cast<const uint4*>(rows.q - rows.mis);
-    for (int c = rows.whole0 + lane; c < rows.whole1; c += 128) {  // four pieces of each row in flight
+    // Four pieces of each row in flight. By ordinary loads: the rows are the kernel's before this one to write, and with programmatic
+    // launches this kernel may have begun by then, which loads through the read-only path do not allow for.
+    for (int c = rows.whole0 + lane; c < rows.whole1; c += 128) {
       uint4 u[4], v[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const bool in = c + 32 * k < rows.whole1;
-        u[k] = in ? LoadNc16(vp + c + 32 * k) : make_uint4(0, 0, 0, 0);
-        v[k] = in && w != 0 ? LoadNc16(vq + c + 32 * k) : make_uint4(0, 0, 0, 0);
+        u[k] = in ? vp[c + 32 * k] : make_uint4(0, 0, 0, 0);
+        v[k] = in && w != 0 ? vq[c + 32 * k] : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
