@@ -437,7 +437,8 @@ typedef struct ShahdTreeCall {
   int64_t workspace_bytes;
 } ShahdTreeCall;
 /* Bytes of workspace for a call with these n, num_heads, max_nodes and cache sizes (0: none), or a negative status; dtype,
- * pointers, rows and scale are not looked at, and no device is asked. */
+ * pointers, rows and scale are not looked at, and no device is asked. The cache's max_blocks stands for the lengths, which lie on the
+ * device: with a table as wide as the longest sequence needs, the call takes the layout that suits it best. */
 int64_t shahd_tree_attention_workspace(const ShahdTreeCall* call);
 /* out[i] = sum of softmax(scale q[i].k[j]) v[j] over the cached positions of the row's sequence and the rows of its mask;
  * a row that attends to nothing gives 0. Positions at or beyond the length are never used, whatever their pages
@@ -468,7 +469,9 @@ typedef struct ShahdVerifyCall {
 /* Each child x of the current node, in index order, is taken with probability min(1, p(x)/q(x)); a refusal replaces p by
  * max(0, p - q) over its sum. The next token is drawn from what p is at the end (the target's row itself when nothing is
  * left), in index order against the root's number. Values that are not positive numbers count as 0; a row without mass, or
- * with an infinite value, draws token 0; nodes whose token is outside the vocabulary or whose parent is not below them are passed over. */
+ * with an infinite value, draws token 0; nodes whose token is outside the vocabulary or whose parent is not below them are passed over.
+ * Decisions are formed in 64 bits from the rows' own values; of a token's max(0, p - a q) and of the up to eight that share 16 bytes
+ * the sum is in 32 bits, above that in 64: a number within some 10^-9 of a border between two tokens may fall on either side. */
 int shahd_verify_tree(const ShahdVerifyCall* call, void* stream);
 
 #ifdef __cplusplus

@@ -13,8 +13,8 @@
 // in all heads, so a lane goes over heads with up to eight 16-byte loads in flight. Where pairs do not
 // fill whole pieces, a lane's eight values find their partners in shared memory, where the warp puts the heads it has loaded.
 // Operands whose address or strides do not allow pieces go value by value. (Blocks of 256 threads over batches of rows, with a table per batch, lost a
-// fifth to a third of the time at the barriers: 56 K rows of 32 + 8 heads of 128 in f16, 1.15 GB, took 265 us; now 197, a plain
-// copy 182.)
+// fifth of the time at the barriers: 59402 rows of 32 + 8 heads of 128 in f16, 1.22 GB, took 265 us where a warp per row took
+// 209, now 206; 57344 rows, 1.17 GB, take 199 us, a plain copy of as much 180.)
 #pragma once
 
 #include "ops_common.cuh"
@@ -31,8 +31,8 @@ constexpr int kRopeWarps = 8;   // of a block, at most
 // One pair per thread; pieces of either layout; pieces whose values find their partners in shared memory.
 enum RopeMode { kRopeValues = 0, kRopeInterleaved = 1, kRopeHalf = 2, kRopeStaged = 3 };
 // Blocks of a multiprocessor: in the half layout a lane holds two pieces and their eight (cos, sin), 16-bit ones twice, which spills
-// at 80 registers (265 us instead of 196 for 56 K rows of 32 + 8 heads of 128), and so do staged pieces (296 us instead of 254,
-// 126 of the 128 values turned).
+// at 80 registers (274 us instead of 199 for 57344 rows of 32 + 8 heads of 128), and so do staged pieces (268 us instead of 227,
+// 126 of the 128 values turned). Interleaved 16-bit pieces spill a little (116 bytes) with three: 211 us, 205 with two.
 template <class T, int MODE>
 constexpr int kRopePerSm = (MODE == kRopeHalf && sizeof(T) == 2) || MODE == kRopeStaged ? 2 : 3;
 
@@ -474,8 +474,8 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
   RopeArgs a = {};
   // 16-byte pieces of 8 values need every address and stride in use a multiple of 16 bytes. With whole pieces on both sides of
   // the rotated part's end and of the pairs' halves a lane holds both values of its pairs; otherwise shared memory brings
-  // them together (56 K f16 rows of 32 + 8 heads of 128 with 126 values turned: 254 us, value by value 866;
-  // with 54 272 and 1377).
+  // them together (57344 f16 rows of 32 + 8 heads of 128 with 126 values turned: 227 us, value by value 862;
+  // with 54 243 and 1363).
   bool vec = d % 8 == 0;
   const bool whole = rope->layout == SHAHD_ROPE_HALF ? d % 16 == 0 && rope->rotary % 16 == 0 : rope->rotary % 8 == 0;
   const auto operand = [&](const ShahdRows& in, const ShahdRows& out, int heads) {

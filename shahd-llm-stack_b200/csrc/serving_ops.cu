@@ -106,7 +106,9 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
 // 12/4 heads of 64, up to 254 positions: ranges 29 us, pairs 10.9; 8 single tokens, 32/8 heads of 128, up to 2000 positions: 25.9
 // and 21.6; one tree of 24 over 2047 positions, 16/4 heads of 64: 13.5 and 23.3). 16 trees over 20 to 32 thousand positions, 8
 // kv heads of 128, kernel alone: a block of threads for each pair 490 us, parts of 2048 keys 513, ranges 427; but 512 pairs of
-// 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as 256 pairs of heads.
+// 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as 256 pairs of heads. The lengths lie on the device, so the table's width
+// stands for them: in one much wider than its sequences are long a call may take the slower layout (256 single tokens, 8/2 heads of
+// 64, 400 to 576 positions: 19 us in a table of 9 pages, 45 in one of 64 or 512; 72 trees as above, one of them over 32000 positions: 311).
 constexpr int kTaSms = 148;  // of a B200: the layout, and so the workspace, does not hang on a device being there
 struct TreeLayout {
   int pairs, two_heads, least, part_rows;

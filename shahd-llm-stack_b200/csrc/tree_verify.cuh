@@ -10,11 +10,11 @@
 // Unrolled, p_k = max(0, p - a_k q) / Z_k with a_0 = 0, Z_0 = 1, a_{k+1} = a_k + Z_k and Z_k = sum max(0, p - a_k q):
 // a refusal costs one pass over the two rows and no row is written. The test u q(x) Z < max(0, p(x) - a q(x)) is formed in 64
 // bits from the rows' own values. In a pass, max(0, p - a q) of one token is two fused 32-bit steps (a as the sum of two
-// floats; each rounds relative to its own result, so nothing cancels: off by 2^-23 of itself), a 16-byte piece's tokens are
-// added in 32 bits and the pieces in 64, in a fixed order: a running mass is good to about 2^-23 over the root of the
+// floats; each rounds relative to its own result: off by 2^-23 of itself, or, where the second step cancels what the first has left,
+// by less than 2^-47 a q), a 16-byte piece's tokens are added in 32 bits and the pieces in 64, in a fixed order: a running mass is good to about 2^-23 over the root of the
 // number of pieces, 10^-9 in a row of 32768, and a run repeats bit for bit. (Element by element in 64 bits the conversions
 // alone, 16 a clock, took twice as long as the rows from memory, and the registers left one block per multiprocessor: 64
-// trees over 32768 tokens 30 us, 128 over 50257 in bf16 61 us; now 16.6 and 26.5.)
+// trees over 32768 tokens 30 us, 128 over 50257 in bf16 61 us; now 15.5 and 26.)
 //
 // Bound by latency: a walk is a chain of decisions. What the decisions read, p and q at each node's token in its parent's
 // rows, does not hang on the walk, so a block's threads fetch it for 256 nodes at once into shared memory, and the walk
