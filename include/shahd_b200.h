@@ -416,7 +416,8 @@ typedef struct ShahdPromptCall {
  * probabilities meet v in dtype. A row that sees a score of NaN or +inf is NaN; a score of -inf has weight 0, and a row that sees
  * no other is NaN. Scores of a magnitude, scale included, of 7.4e8 (bf16) or 5.8e6 (fp16) and more can make a row that sees them
  * NaN, and do if its largest one is such. A value of v that is not finite can reach every row of its own sequence, the earlier
- * ones too, but no other sequence. */
+ * ones too, but no other sequence. Weights times v are summed before the division by the weights' sum: bf16 values beyond 1e29
+ * can overflow to infinity there. */
 int shahd_prompt_attention(const ShahdPromptCall* call, void* stream);
 
 /* ---- attention of drafted token trees over the cache (verify passes; one node per sequence is a decode step) ---- */
