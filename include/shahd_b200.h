@@ -475,6 +475,143 @@ typedef struct ShahdVerifyCall {
  * the sum is in 32 bits, above that in 64: a number within some 10^-9 of a border between two tokens may fall on either side. */
 int shahd_verify_tree(const ShahdVerifyCall* call, void* stream);
 
+/* ================================================================================================
+ * 4. A serving step over shared pages. The common rules of section 3 hold. The operators fit together, and with those above:
+ *      shahd_pages_fork (new sequences go on from earlier ones) -> shahd_norm_rope_apply or shahd_rope_apply (the step's rows; k, v into
+ *      the cache) -> shahd_chunk_attention -> (the model's logits) -> shahd_adjust_logits -> sampling,
+ *    and shahd_pages_compact now and then.
+ * ============================================================================================== */
+
+/* ---- pages shared between sequences ---- */
+/* The memory of a paged cache over all its layers: layer l of page p is [kv_heads][K|V][64][head_dim] 16-bit values at
+ * data + p * page_stride + l * layer_stride (elements; multiples of 8, data 16-byte aligned): the pool of a ShahdKvCache per layer. Layers
+ * of a page, or pages of a layer, lie together; layer_stride is not looked at for one layer. */
+typedef struct ShahdPagePool {
+  void* data;
+  int64_t page_stride;
+  int64_t layer_stride;
+  int32_t layers;
+  int32_t pages;    /* 1 .. 2^24 */
+  int32_t kv_heads;
+  int32_t head_dim; /* a multiple of 8, up to 256 */
+} ShahdPagePool;
+
+typedef struct ShahdForkCall {
+  ShahdPagePool pool;
+  int32_t n;          /* sequences of the table, 0 .. 2^20 */
+  int32_t new_n;      /* sequences of the new table */
+  int32_t max_blocks; /* of both tables; at most 2^30 entries */
+  int32_t reserved;
+  const int32_t* table;   /* [n, max_blocks] */
+  const int32_t* lengths; /* [n] cached positions (values are cut to 0 .. max_blocks * 64) */
+  const int32_t* parents; /* [new_n] the sequence that each goes on from; outside 0 .. n-1: none, it begins empty */
+  const int32_t* keep;    /* [new_n] positions it keeps (cut to 0 .. the parent's length) */
+  const int32_t* need;    /* [new_n] positions it is to have pages for (at least those it keeps) */
+  int32_t* new_table;     /* [new_n, max_blocks] out; must not overlap table */
+  int32_t* missing;       /* [new_n] out: pages that it was to have and has not (0: all is well) */
+  void* workspace;        /* 16-byte aligned, shahd_pages_workspace(pool.pages, new_n) bytes; in use until the call has run */
+  int64_t workspace_bytes;
+} ShahdForkCall;
+/* Bytes of workspace for a fork (or, with new_n 0, for shahd_pages_compact), or a negative status; no device is asked. */
+int64_t shahd_pages_workspace(int32_t pages, int32_t new_n);
+/* New sequence i keeps the first keep[i] positions of parents[i] and gets pages for positions up to need[i]. A page is held when some
+ * sequence of the old table names it among its first ceil(length / 64) entries; the others are free. Kept pages are shared by
+ * number. A page that is partly filled, in which a sequence is to go on (need > keep, keep no multiple of 64), stays with it when
+ * every new sequence that names the page goes on in it, and it is the first of them; otherwise it gets a copy of the positions it
+ * keeps. Fresh pages, copies' among them, are the free ones in ascending order, dealt out sequence by sequence, each one's in
+ * the order of its positions; where they run out, entries are -1 and missing counts them, with the pages that max_blocks has no
+ * place for. A copy that is missing means that the sequence has lost its last positions: the old table and its pages are as they
+ * were, fork fewer sequences from it. Other entries of the new table are -1; kept entries that name no page stay as they are. What no
+ * new sequence goes on with is free for the next call that is given the new table. Not for the pool of a FusedAttention
+ * operator, whose slots own their pages. */
+int shahd_pages_fork(const ShahdForkCall* call, void* stream);
+
+typedef struct ShahdCompactCall {
+  ShahdPagePool pool;
+  int32_t n;
+  int32_t max_blocks;
+  const int32_t* table;   /* [n, max_blocks] */
+  const int32_t* lengths; /* [n] */
+  int32_t* new_table;     /* [n, max_blocks] out; may be table */
+  int32_t* used;          /* [1] out: held pages U */
+  void* workspace;        /* 16-byte aligned, shahd_pages_workspace(pool.pages, 0) bytes; in use until the call has run */
+  int64_t workspace_bytes;
+} ShahdCompactCall;
+/* Moves the held pages together: those numbered U and up go, in ascending order, to the free ones below U, in ascending order. Entries of
+ * the new table behind a sequence's length, and those that name no page, are -1. */
+int shahd_pages_compact(const ShahdCompactCall* call, void* stream);
+
+/* ---- norms of the query and key heads, with the rotary positions and the append (NormRow, CachedRowMath.ts:25-56, on heads) ---- */
+#define SHAHD_NORM_RMS 0   /* x / sqrt(mean(x^2) + eps) * weight */
+#define SHAHD_NORM_LAYER 1 /* (x - mean) / sqrt(var + eps) * weight + bias, var the mean of the squared differences */
+typedef struct ShahdHeadNorm {
+  int32_t kind;
+  int32_t weight_dtype; /* of the weights and biases: SHAHD_BF16, SHAHD_F16 or SHAHD_F32 */
+  double eps;           /* positive */
+  const void *q_weight, *k_weight; /* [head_dim], for all heads; null: 1 */
+  const void *q_bias, *k_bias;     /* [head_dim], SHAHD_NORM_LAYER only; null: 0 */
+} ShahdHeadNorm;
+/* shahd_rope_apply on the normalised heads of q and k: every value is read once, and rounded once, at the end. Sums are in 32 bits:
+ * heads with values beyond some 1e18 come out 0 or NaN. The append, the rows that are passed over and the alignment rules are those of
+ * shahd_rope_apply. */
+int shahd_norm_rope_apply(const ShahdRope* rope, const ShahdRopeCall* call, const ShahdHeadNorm* norm, void* stream);
+
+/* ---- attention of chunks of new tokens over the paged cache ---- */
+typedef struct ShahdChunkCall {
+  int32_t dtype;     /* of q, out and the cache: SHAHD_BF16 or SHAHD_F16 */
+  int32_t rows;
+  int32_t n;
+  int32_t num_heads; /* kv_heads and head_dim (32, 64 or 128) are the cache's; at most 8 query heads per kv head */
+  int32_t max_rows;  /* no sequence has more rows than this (rows beyond it would be left as they are) */
+  int32_t reserved;
+  double scale;      /* 0: 1/sqrt(head_dim) */
+  const int32_t* offsets;
+  const int32_t* lengths; /* [n] positions before the chunk (values are cut to 0 .. max_blocks * 64): row i of sequence s is position
+                             lengths[s] + i */
+  ShahdRows q, out;       /* 16-byte aligned, strides multiples of 8 */
+  ShahdKvCache cache;     /* holds the chunk's own keys and values too */
+  void* workspace;        /* 32-byte aligned, shahd_chunk_attention_workspace bytes; in use until the call has run */
+  int64_t workspace_bytes;
+} ShahdChunkCall;
+/* Bytes of workspace for a call with these rows, n, num_heads, max_rows and cache sizes (0: none), or a negative status; dtype, pointers and
+ * scale are not looked at, and no device is asked. */
+int64_t shahd_chunk_attention_workspace(const ShahdChunkCall* call);
+/* out[i] = sum over positions j <= lengths[s] + i of softmax_j(scale q[i].k[j]) v[j] over the cache of the row's sequence: parts of
+ * prompts, and decode steps as chunks of one row, in one call. Positions at or beyond max_blocks * 64 and those on no page are not
+ * attended to; a row that attends to nothing gives 0. Positions behind the chunk are never used, whatever their pages hold. Scores that
+ * are not finite: as in shahd_prompt_attention. A value of the cached v that is not finite can reach every row of its own
+ * sequence, the earlier ones too, but no other sequence. */
+int shahd_chunk_attention(const ShahdChunkCall* call, void* stream);
+
+/* ---- penalties, biases and grammar masks on logits (before SampleFromLogits, Sampler.ts:16-27) ---- */
+typedef struct ShahdLogitsCall {
+  int32_t dtype;  /* of logits and out: SHAHD_BF16, SHAHD_F16 or SHAHD_F32 */
+  int32_t rows;   /* 0 .. 2^20 */
+  int32_t n;      /* sequences, 0 .. 2^20 */
+  int32_t vocab;  /* 1 .. 2^24 */
+  const void* logits;  /* [rows, vocab] */
+  void* out;           /* [rows, vocab]; may be logits, with the same stride */
+  int64_t logits_stride, out_stride; /* elements between rows, at least vocab */
+  const int32_t* sequences;          /* [rows] the row's sequence; null: row r is sequence r. A row whose number is not in 0 .. n-1 is left as it is */
+  const int32_t* history;            /* [n, history_stride] tokens of the prompt and then the generated ones; null: no penalties. Tokens outside
+                                        the vocabulary are passed over */
+  int64_t history_stride;            /* 0 .. 2^30 */
+  const int32_t* history_lengths;    /* [n] (cut to 0 .. history_stride) */
+  const int32_t* prompt_lengths;     /* [n] the history's tokens before this place are the prompt's; null: all are generated */
+  const float *repetition, *presence, *frequency; /* [n]; null: 1, 0, 0 */
+  const int32_t* bias_offsets;       /* [n+1] sequence s has entries bias_offsets[s] .. bias_offsets[s+1]-1; null: no biases */
+  const int32_t* bias_tokens;        /* [bias_entries]; of a token that is there twice the last entry counts */
+  const float* bias_values;          /* [bias_entries] */
+  int32_t bias_entries;
+  int32_t mask_count;
+  const uint32_t* masks;             /* [mask_count, mask_stride]: bit v % 32 of word v / 32 is set where token v is allowed; null: no masks */
+  int64_t mask_stride;               /* words, at least ceil(vocab / 32) */
+  const int32_t* mask_rows;          /* [rows] the row's mask; not in 0 .. mask_count-1: none. Null: row r has mask r */
+} ShahdLogitsCall;
+/* x = logit of token v. With v in the sequence's history: x > 0 ? x / repetition : x * repetition; generated c times, c > 0: x -=
+ * c * frequency + presence; x += bias; not allowed by the mask: -inf. In 32 bits, rounded once. */
+int shahd_adjust_logits(const ShahdLogitsCall* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,43 @@ class ShahdVerifyCall(ctypes.Structure):
                 ("new_lengths", _vp)]
 
 
+class ShahdPagePool(ctypes.Structure):
+    """The memory of a paged cache over all its layers: layer l of page p at data + p * page_stride + l * layer_stride (elements)."""
+
+    _fields_ = [("data", _vp), ("page_stride", _i64), ("layer_stride", _i64), ("layers", _i32), ("pages", _i32), ("kv_heads", _i32),
+                ("head_dim", _i32)]
+
+
+class ShahdForkCall(ctypes.Structure):
+    _fields_ = [("pool", ShahdPagePool), ("n", _i32), ("new_n", _i32), ("max_blocks", _i32), ("reserved", _i32), ("table", _vp),
+                ("lengths", _vp), ("parents", _vp), ("keep", _vp), ("need", _vp), ("new_table", _vp), ("missing", _vp),
+                ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+class ShahdCompactCall(ctypes.Structure):
+    _fields_ = [("pool", ShahdPagePool), ("n", _i32), ("max_blocks", _i32), ("table", _vp), ("lengths", _vp), ("new_table", _vp),
+                ("used", _vp), ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+class ShahdHeadNorm(ctypes.Structure):
+    _fields_ = [("kind", _i32), ("weight_dtype", _i32), ("eps", ctypes.c_double), ("q_weight", _vp), ("k_weight", _vp),
+                ("q_bias", _vp), ("k_bias", _vp)]
+
+
+class ShahdChunkCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("n", _i32), ("num_heads", _i32), ("max_rows", _i32), ("reserved", _i32),
+                ("scale", ctypes.c_double), ("offsets", _vp), ("lengths", _vp), ("q", ShahdRows), ("out", ShahdRows),
+                ("cache", ShahdKvCache), ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+class ShahdLogitsCall(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("n", _i32), ("vocab", _i32), ("logits", _vp), ("out", _vp),
+                ("logits_stride", _i64), ("out_stride", _i64), ("sequences", _vp), ("history", _vp), ("history_stride", _i64),
+                ("history_lengths", _vp), ("prompt_lengths", _vp), ("repetition", _vp), ("presence", _vp), ("frequency", _vp),
+                ("bias_offsets", _vp), ("bias_tokens", _vp), ("bias_values", _vp), ("bias_entries", _i32), ("mask_count", _i32),
+                ("masks", _vp), ("mask_stride", _i64), ("mask_rows", _vp)]
+
+
 # name -> (restype, argtypes); every symbol include/shahd_b200.h declares
 SIGNATURES = {
     "MatMulF64": (None, [_dp, _dp, _dp, _i32, _i32, _i32]),
@@ -156,6 +193,13 @@ SIGNATURES = {
     "shahd_tree_attention_workspace": (_i64, [ctypes.POINTER(ShahdTreeCall)]),
     "shahd_tree_attention": (ctypes.c_int, [ctypes.POINTER(ShahdTreeCall), _vp]),
     "shahd_verify_tree": (ctypes.c_int, [ctypes.POINTER(ShahdVerifyCall), _vp]),
+    "shahd_pages_workspace": (_i64, [_i32, _i32]),
+    "shahd_pages_fork": (ctypes.c_int, [ctypes.POINTER(ShahdForkCall), _vp]),
+    "shahd_pages_compact": (ctypes.c_int, [ctypes.POINTER(ShahdCompactCall), _vp]),
+    "shahd_norm_rope_apply": (ctypes.c_int, [_vp, ctypes.POINTER(ShahdRopeCall), ctypes.POINTER(ShahdHeadNorm), _vp]),
+    "shahd_chunk_attention_workspace": (_i64, [ctypes.POINTER(ShahdChunkCall)]),
+    "shahd_chunk_attention": (ctypes.c_int, [ctypes.POINTER(ShahdChunkCall), _vp]),
+    "shahd_adjust_logits": (ctypes.c_int, [ctypes.POINTER(ShahdLogitsCall), _vp]),
     "shahd_last_error": (ctypes.c_char_p, []),
 }
 

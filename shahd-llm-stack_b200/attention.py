@@ -8,8 +8,8 @@ stream has reached the call, so pass torch's current stream when torch owns them
 
 Next to it, attention on the caller's own buffers: prompt_attention for prompts of different lengths packed into one
 call, tree_attention for drafted token trees (or single new tokens) against a paged cache, such as FusedAttention's own
-(FusedAttention.cache). They keep no state: calls on different streams or devices do not meet, and both can be
-captured into CUDA graphs. A stream of 0 is the legacy default stream there.
+(FusedAttention.cache), chunk_attention for further parts of prompts, and decode steps among them, over what is cached. They keep no
+state: calls on different streams or devices do not meet, and all can be captured into CUDA graphs. A stream of 0 is the legacy default stream there.
 A wait inside a kernel that gives up leaves rows undefined and is recorded: _lib.load().ShahdDeviceErrorFlag() is 0 as long
 as none has.
 """
@@ -110,6 +110,24 @@ def tree_attention(dtype: int, q: Rows, k: Rows, v: Rows, out: Rows, cache: KvCa
     call = _lib.ShahdTreeCall(dtype, rows, n, num_heads, max_nodes, 0, scale, offsets, lengths, masks, q, k, v, out, cache,
                               workspace, workspace_bytes)
     _lib.check(_lib.load().shahd_tree_attention(ctypes.byref(call), stream or None))
+
+
+def chunk_attention_workspace(n: int, rows: int, max_rows: int, num_heads: int, cache: KvCache) -> int:
+    """Bytes of device workspace that chunk_attention needs for these sizes (0: none)."""
+    call = _lib.ShahdChunkCall(n=n, rows=rows, max_rows=max_rows, num_heads=num_heads, cache=cache)
+    size = int(_lib.load().shahd_chunk_attention_workspace(ctypes.byref(call)))
+    if size < 0:
+        _lib.check(size)
+    return size
+
+
+def chunk_attention(dtype: int, q: Rows, out: Rows, cache: KvCache, lengths: int, offsets: int, n: int, rows: int, max_rows: int,
+                    num_heads: int, scale: float = 0.0, workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+    """Attention of the next rows of each sequence over the paged cache, which holds their keys and values already: row i of
+    sequence s is position lengths[s] + i and sees the positions up to its own. Parts of prompts and decode steps (one row) in one
+    call; no sequence has more than max_rows rows. q, out [rows, num_heads, head_dim], BF16 or F16."""
+    call = _lib.ShahdChunkCall(dtype, rows, n, num_heads, max_rows, 0, scale, offsets, lengths, q, out, cache, workspace, workspace_bytes)
+    _lib.check(_lib.load().shahd_chunk_attention(ctypes.byref(call), stream or None))
 
 
 def tree_masks(parents) -> np.ndarray:

@@ -18,7 +18,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
 ]
 # each a translation unit with its own device module; compiled at the same time
-UNITS = ["shahd_b200.cu", "serving_ops.cu"]
+UNITS = ["shahd_b200.cu", "serving_ops.cu", "step_ops.cu", "chunk_attention.cu"]
 
 
 def _sources() -> list[str]:

@@ -17,13 +17,7 @@
 // 209, now 206; 57344 rows, 1.17 GB, take 199 us, a plain copy of as much 180.)
 #pragma once
 
-#include "ops_common.cuh"
-
-struct ShahdRope {
-  int head_dim, rotary, layout;
-  float magnitude;
-  double turns[128];  // f_i / 2pi
-};
+#include "rope_call.cuh"
 
 namespace shahd {
 
@@ -35,76 +29,6 @@ enum RopeMode { kRopeValues = 0, kRopeInterleaved = 1, kRopeHalf = 2, kRopeStage
 // 126 of the 128 values turned). Interleaved 16-bit pieces spill a little (116 bytes) with three: 211 us, 205 with two.
 template <class T, int MODE>
 constexpr int kRopePerSm = (MODE == kRopeHalf && sizeof(T) == 2) || MODE == kRopeStaged ? 2 : 3;
-
-struct RopeOperand {
-  const void* in;
-  void* out;
-  long long in_row, in_head, out_row, out_head;
-  int heads;
-};
-
-struct RopeArgs {
-  RopeOperand q, k, v;  // v.out is never set: values only go to the cache
-  const int* positions;
-  const int* offsets;  // null: every row counts
-  int n, rows, d, half, interleaved, pieces;
-  float magnitude;
-  uint16_t* pool;  // null: no cache
-  long long page_stride;
-  const int* table;
-  int max_blocks, pages;
-  double turns[128];
-};
-
-template <class T>
-__device__ __forceinline__ float ToFloat(T x) {
-  return float(x);
-}
-template <class T>
-__device__ __forceinline__ T FromFloat(float x) {
-  if constexpr (sizeof(T) == 4) return x;
-  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
-  else return __float2bfloat16_rn(x);
-}
-
-// Eight values as they lie in memory, and as floats.
-template <class T>
-struct Raw8 {
-  uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void Load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) u[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void Get(float (&v)[8]) const {
-    const T* h = reinterpret_cast<const T*>(u);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = ToFloat(h[i]);
-  }
-};
-template <class T>
-__device__ __forceinline__ void Store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint4 u;
-    T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = FromFloat<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = u;
-  }
-}
-
-// The sequence that holds packed row `row`: the last s with offsets[s] <= row (empty sequences before it share its start).
-__device__ __forceinline__ int SequenceOf(const int* offsets, int n, int row) {
-  int lo = 0, hi = n;  // offsets[lo] <= row < offsets[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (offsets[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 // T: the operands' type, C: the cache's.
 template <class T, class C, int MODE>
@@ -419,92 +343,19 @@ int shahd_rope_apply(const ShahdRope* rope, const ShahdRopeCall* c, void* stream
     SetError("%s: null argument", op);
     return SHAHD_EINVAL;
   }
-  if (!CheckType(op, c->dtype, true)) return SHAHD_EINVAL;
-  const bool q = c->num_heads > 0, k = c->kv_heads > 0, cache = c->cache.pool != nullptr;
-  const int d = rope->head_dim;
-  if (c->rows < 0 || c->num_heads < 0 || c->kv_heads < 0 || c->num_heads > (1 << 16) || c->kv_heads > (1 << 16) || !(q || k)) {
-    SetError("%s: need rows >= 0 and num_heads or kv_heads (got rows=%d num_heads=%d kv_heads=%d)", op, c->rows, c->num_heads,
-             c->kv_heads);
-    return SHAHD_EINVAL;
-  }
-  if (c->n > kOpsMaxRows) {
-    SetError("%s: too many sequences: %d, at most 2^30", op, c->n);
-    return SHAHD_EINVAL;
-  }
-  if (c->n < 0 || (cache && (c->n < 1 || !c->offsets)) || (c->offsets && c->n < 1)) {
-    SetError("%s: offsets, and so a cache, need n >= 1 sequences (got n=%d)", op, c->n);
-    return SHAHD_EINVAL;
-  }
-  if (cache && (!k || !CheckCache(op, c->cache, c->kv_heads, d))) {
-    if (!k) SetError("%s: a cache needs kv_heads", op);
-    return SHAHD_EINVAL;
-  }
-  if (k && !cache && !c->k_out.data) {
-    SetError("%s: keys need k_out or a cache", op);
-    return SHAHD_EINVAL;
-  }
-  if ((q && (!CheckRows(op, "q", c->q, c->rows, c->num_heads, d, 1) || !CheckRows(op, "q_out", c->q_out, c->rows, c->num_heads, d, 1, true))) ||
-      (k && !CheckRows(op, "k", c->k, c->rows, c->kv_heads, d, 1)) ||
-      (k && c->k_out.data && !CheckRows(op, "k_out", c->k_out, c->rows, c->kv_heads, d, 1, true)) ||
-      (cache && !CheckRows(op, "v", c->v, c->rows, c->kv_heads, d, 1)))
-    return SHAHD_EINVAL;
-  if (c->rows == 0) return SHAHD_OK;
-  const size_t size = TypeBytes(c->dtype);
-  BufferCheck b(op);
-  b.Add("positions", c->positions, 4);
-  if (c->offsets) b.Add("offsets", c->offsets, 4);
-  if (q) {
-    b.Add("q", c->q.data, size);
-    b.Add("q_out", c->q_out.data, size);
-  }
-  if (k) b.Add("k", c->k.data, size);
-  if (k && c->k_out.data) b.Add("k_out", c->k_out.data, size);
-  if (cache) {
-    b.Add("v", c->v.data, size);
-    b.Add("cache.pool", c->cache.pool, 16);
-    b.Add("cache.block_table", c->cache.block_table, 4);
-  }
-  if (b.rc != SHAHD_OK) return b.rc;
-  const DeviceInfo info = InfoOf(b.device);
-  DeviceScope scope(b.device);
-  if (!info.usable || !scope.ok) {
-    SetError("%s: device %d is not a usable sm_100 device", op, b.device);
+  RopeArgs a;
+  RopePieces p;
+  DeviceInfo info;
+  int device = -1;
+  const int rc = PrepareRope(op, rope, c, nullptr, 0, &a, &p, &info, &device);
+  if (rc != SHAHD_OK || c->rows == 0) return rc;
+  DeviceScope scope(device);
+  if (!scope.ok) {
+    SetError("%s: device %d is not a usable sm_100 device", op, device);
     return SHAHD_ENODEV;
   }
-  RopeArgs a = {};
-  // 16-byte pieces of 8 values need every address and stride in use a multiple of 16 bytes. With whole pieces on both sides of
-  // the rotated part's end and of the pairs' halves a lane holds both values of its pairs; otherwise shared memory brings
-  // them together (57344 f16 rows of 32 + 8 heads of 128 with 126 values turned: 227 us, value by value 862;
-  // with 54 243 and 1363).
-  bool vec = d % 8 == 0;
-  const bool whole = rope->layout == SHAHD_ROPE_HALF ? d % 16 == 0 && rope->rotary % 16 == 0 : rope->rotary % 8 == 0;
-  const auto operand = [&](const ShahdRows& in, const ShahdRows& out, int heads) {
-    for (const ShahdRows* r : {&in, &out})
-      if (r->data)
-        vec = vec && reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
-    return RopeOperand{in.data, out.data, in.row_stride, in.head_stride, out.row_stride, out.head_stride, heads};
-  };
-  if (q) a.q = operand(c->q, c->q_out, c->num_heads);
-  if (k) a.k = operand(c->k, c->k_out, c->kv_heads);
-  if (cache) a.v = operand(c->v, ShahdRows{}, c->kv_heads);
-  a.positions = c->positions;
-  a.offsets = c->offsets;
-  a.n = c->n;
-  a.rows = c->rows;
-  a.d = d;
-  a.half = rope->rotary / 2;
-  a.interleaved = rope->layout == SHAHD_ROPE_INTERLEAVED;
-  a.magnitude = rope->magnitude;
-  if (cache) {
-    a.pool = static_cast<uint16_t*>(c->cache.pool);
-    a.page_stride = c->cache.page_stride;
-    a.table = c->cache.block_table;
-    a.max_blocks = c->cache.max_blocks;
-    a.pages = c->cache.pages;
-  }
-  std::copy(rope->turns, rope->turns + a.half, a.turns);
-  const int mode = !vec ? kRopeValues : !whole ? kRopeStaged : a.interleaved ? kRopeInterleaved : kRopeHalf;
-  a.pieces = mode == kRopeValues ? d - a.half : mode == kRopeHalf ? d / 16 : d / 8;
+  const int mode = !p.vec ? kRopeValues : !p.whole ? kRopeStaged : a.interleaved ? kRopeInterleaved : kRopeHalf;
+  a.pieces = mode == kRopeValues ? a.d - a.half : mode == kRopeHalf ? a.d / 16 : a.d / 8;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   TakeLaunchError(nullptr);
   if (c->dtype == SHAHD_F32) LaunchRope<float, bf16>(a, mode, info.sms, st);

@@ -4,74 +4,16 @@
 #include <new>
 #include <type_traits>
 
-#include "device_flags.h"
 #include "ops_common.cuh"
 #include "rope.cuh"
-#include "tile_attention.cuh"
+#include "tile_host.cuh"
 #include "tree_verify.cuh"
 
 namespace shahd {
 
-// The operators run where their buffers are, so a wait that gave up may have been recorded on any device that a kernel with waits
-// (the tile attention) has been launched on.
-static DeviceSet g_waiting_devices;
-
-int OpsDeviceError() {
-  return FirstFlag(g_waiting_devices, [](int device, int* flag) {
-    DeviceScope scope(device);
-    if (scope.ok && cudaMemcpyFromSymbol(flag, g_ops_device_error, sizeof *flag) == cudaSuccess) return true;
-    cudaGetLastError();
-    return false;
-  });
-}
+int OpsDeviceError() { return TileDeviceError(); }
 
 namespace {
-
-typedef CUresult (*OpsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-OpsEncodeFn OpsEncode() {
-  static const OpsEncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<OpsEncodeFn>(p);
-  }();
-  return fn;
-}
-
-// A map of 16-bit values (x, y, z) with 128-byte swizzle and boxes of 64 x by x bz. Made for every call: it is a
-// computation of the call's own pointers and strides, a fraction of a microsecond.
-bool MakeMap(int dtype, const void* p, uint64_t nx, uint64_t ny, uint64_t nz, int64_t sy, int64_t sz, int by, int bz, CUtensorMap* m) {
-  const OpsEncodeFn enc = OpsEncode();
-  if (!enc) return false;
-  if (ny == 1) sy = (int64_t)nx;  // the stride of a single row or head is free: TMA wants one that it could use
-  if (nz == 1) sz = (int64_t)nx;
-  const cuuint64_t dims[3] = {nx, ny, nz}, strides[2] = {(cuuint64_t)sy * 2, (cuuint64_t)sz * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)by, (cuuint32_t)bz}, step[3] = {1, 1, 1};
-  return enc(m, dtype == SHAHD_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims,
-             strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-bool CheckHeads(const char* op, int H, int Hk, int d) {
-  if (H >= 1 && Hk >= 1 && H % Hk == 0 && H / Hk <= 8 && H <= (1 << 16) && (d == 32 || d == 64 || d == 128)) return true;
-  SetError("%s: need kv_heads dividing num_heads with at most 8 query heads per kv head and head_dim 32, 64 or 128 (got "
-           "num_heads=%d kv_heads=%d head_dim=%d)", op, H, Hk, d);
-  return false;
-}
-
-bool ScaleOf(const char* op, double scale, int d, float* log2) {
-  if (scale == 0) scale = 1.0 / std::sqrt((double)d);
-  *log2 = (float)(scale * M_LOG2E);
-  if (!(*log2 > 0) || !std::isfinite(*log2)) {  // in 32 bits, too: masked scores are -inf times it
-    SetError("%s: scale must be positive and finite in 32 bits, or 0 for 1/sqrt(head_dim) (got %g)", op, scale);
-    return false;
-  }
-  return true;
-}
 
 template <int D, bool F16, int KIND>
 void LaunchTiles(const TaArgs& a, unsigned blocks, cudaStream_t st) {
@@ -109,7 +51,6 @@ bool MakeRowMaps(const char* op, int dtype, int d, int H, int Hk, int rows, cons
 // 400 to 576 positions, 1.7 for each place: 33 us and 42, 31 as 256 pairs of heads. The lengths lie on the device, so the table's width
 // stands for them: in one much wider than its sequences are long a call may take the slower layout (256 single tokens, 8/2 heads of
 // 64, 400 to 576 positions: 19 us in a table of 9 pages, 45 in one of 64 or 512; 72 trees as above, one of them over 32000 positions: 311).
-constexpr int kTaSms = 148;  // of a B200: the layout, and so the workspace, does not hang on a device being there
 struct TreeLayout {
   int pairs, two_heads, least, part_rows;
   long long grid;

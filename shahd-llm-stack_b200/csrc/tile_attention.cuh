@@ -1,7 +1,8 @@
-// Attention of 128-row query tiles on the tensor cores, for two operators:
+// Attention of 128-row query tiles on the tensor cores, for three operators:
 //   packed prompts  out[i] = sum_{j <= i} softmax_j(scale q[i].k[j]) v[j] within each sequence (MultiHeadAttention.ts:46-74,
-//                   CausalSoftmax.ts:17-33, for sequences of different lengths in one call), and
-//   trees           the drafted nodes of a sequence against its cached positions and against each other by a bit mask.
+//                   CausalSoftmax.ts:17-33, for sequences of different lengths in one call),
+//   trees           the drafted nodes of a sequence against its cached positions and against each other by a bit mask, and
+//   chunks          further rows of a sequence against the cache, which holds their own keys and values too: causal by position.
 //
 // A tile's rows are (token, query head of one kv head) pairs, tokens outside: 128/G tokens times G heads, so the G heads
 // that share keys sit in one tile, a decode step of few rows fills what it can, and a tile's last key block is cut close to
@@ -26,7 +27,7 @@
 
 
 #include "ops_common.cuh"
-#include "rope.cuh"
+#include "rows.cuh"
 
 namespace shahd {
 
@@ -62,10 +63,10 @@ constexpr int kTaRegsSoftmax = 216, kTaRegsIssue = 72;
 struct TaShared {
   uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], ml_full, ml_free, drained;
   uint64_t work_full[4], work_read[4];
-  int4 work[4][4];  // trees: what the block works on, by turns; the loading warp writes it
+  int4 work[4][4];  // ranges: what the block works on, by turns; the loading warp writes it
   uint32_t tmem;
   volatile int abort;
-  int found_seq, found_at, sums[12];  // trees: where the block's range begins
+  int found_seq, found_at, sums[12];  // ranges: where the block's begins
 };
 static_assert(sizeof(TaShared) <= 768, "TaShared");
 
@@ -88,7 +89,8 @@ struct TaArgs {
   int least, part_rows;
   float* part_o;    // [2 grid, part_rows, D]
   float2* part_ml;  // [2 grid, part_rows]: -Offset() of the running maximum, and the sum
-  int* plan;        // the ranges' length, then for every sequence the blocks of all before it, and their total
+  int* plan;        // trees: the ranges' length, then for every sequence the blocks of all before it, and their total
+  int4* cuts;       // chunks: [grid] the pair that block of threads c begins and does not end: first row, kv head, tokens (0: none), parts
 };
 
 __device__ __forceinline__ void TmaLoad3D(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -274,11 +276,11 @@ struct TaWork {
   int blocks0, blocks1;  // key blocks of the tiles
   int turns;            // kShared, kTurns or kHeads
   int first;            // trees: first key block
-  int cached;           // trees: cached positions
-  int cache_blocks;     // trees: key blocks of the cache
-  int nodes;            // trees: rows of the sequence; prompts: tokens of the sequence
-  int part;             // trees: the place of the results among the block's parts, or -1: these are all key blocks
-  int more;             // trees: there is another pair behind this one
+  int cached;           // trees: cached positions; chunks: the same, the chunk's own among them
+  int cache_blocks;     // trees: key blocks of the cache; chunks: positions before the chunk
+  int nodes;            // trees, chunks: rows of the sequence; prompts: tokens of the sequence
+  int part;             // ranges: the place of the results among the block's parts, or -1: these are all key blocks
+  int more;             // ranges: there is another pair behind this one
   __device__ __forceinline__ int Tokens(int i) const { return i ? tokens1 : tokens0; }
   __device__ __forceinline__ int Blocks(int i) const { return i ? blocks1 : blocks0; }
 };
@@ -500,6 +502,184 @@ __device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& se
   }
 }
 
+// Sum of floor((a j + b) / m) over j = 0 .. n-1: the lattice points under a line, counted by turns from either axis, which shrinks the
+// numbers as Euclid's algorithm does (Graham, Knuth and Patashnik, Concrete Mathematics, 3.5). The sum is below 2^30.
+__device__ __forceinline__ int FloorSum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  uint32_t sum = 0;
+#pragma unroll 1
+  while (n > 0) {
+    if (a >= m) {
+      sum += (uint32_t)((unsigned long long)n * (n - 1) / 2 * (a / m));
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const uint32_t top = a * n + b;  // n is at most 2^23, m at most 256
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const uint32_t old = m;
+    m = a;
+    a = old;
+  }
+  return (int)sum;
+}
+
+// A sequence of a chunk call: its rows, the positions before them and in all, tile pairs, and their key blocks: causal, so a later pair
+// has more of them.
+template <int KEYS>
+struct ChunkSeq {
+  int start, nodes, past, total, most, pairs, span;
+  __device__ __forceinline__ ChunkSeq(const TaArgs& A, int s) {
+    start = min(max(A.offsets[s], 0), A.rows);
+    nodes = min(min(max(A.offsets[s + 1], start), A.rows) - start, A.max_nodes);
+    most = A.max_blocks * kOpsPage;
+    past = min(max(A.lengths[s], 0), most);
+    total = min(past + nodes, most);
+    span = 2 * A.TB;
+    pairs = (nodes + span - 1) / span;
+  }
+  // Key blocks of pair p, and of all pairs before it (p <= pairs).
+  __device__ __forceinline__ int Blocks(int p) const { return (min(past + min((p + 1) * span, nodes), most) + KEYS - 1) / KEYS; }
+  __device__ __forceinline__ int Before(int p) const {
+    if (p == 0) return 0;
+    // pairs up to the last but one are whole; from the table's end on all see the same
+    const int q = p == pairs ? p - 1 : p, inside = min(q, (most - past) / span);
+    const int sum = FloorSum(inside, KEYS, span, past + span + KEYS - 1) + (q - inside) * ((most + KEYS - 1) / KEYS);
+    return p == pairs ? sum + Blocks(q) : sum;
+  }
+};
+
+// The key blocks of a chunk call that this block of threads takes, pair by pair: sequence after sequence, kv head after kv head.
+template <int KEYS>
+struct ChunkWalk {
+  const TaArgs& A;
+  ChunkSeq<KEYS> q;             // of `seq`
+  int seq, head, pair, at, pos, end;  // the next pair and its first block; the range that is left
+  int cut_row, cut_head, cut_tokens, cut_from, cut_blocks;  // the pair that the range begins and does not end
+  // From block `at_` of sequence seq_'s on, pos_ in the line, to end_. The whole warp takes part.
+  __device__ __forceinline__ ChunkWalk(const TaArgs& a, int seq_, int at_, int pos_, int end_) : A(a), q(a, seq_), seq(seq_), pos(pos_), end(end_) {
+    cut_tokens = 0;
+    const int line = q.Before(q.pairs);
+    head = at_ / line;
+    const int x = at_ - head * line;
+    // the last pair with no more than x blocks before it
+    int lo = 0, cnt = q.pairs;
+    while (cnt > 1) {
+      const int step = (cnt + 31) / 32, k = (threadIdx.x & 31) * step;
+      const unsigned hit = __ballot_sync(0xffffffffu, k < cnt && q.Before(lo + k) <= x);
+      const int to = (31 - __clz(hit)) * step;  // lane 0's always holds
+      lo += to;
+      cnt = min(step, cnt - to);
+    }
+    pair = lo;
+    at = x - q.Before(lo);
+  }
+  // The next pair's work; there is one (pos < end).
+  __device__ __forceinline__ TaWork Take() {
+    TaWork w;
+    const int blocks = q.Blocks(pair), count = min(blocks - at, end - pos);
+    w.seq = seq;
+    w.start = q.start;
+    w.nodes = q.nodes;
+    w.cached = q.total;
+    w.cache_blocks = q.past;
+    w.head = head;
+    w.q0 = pair * q.span;
+    w.tokens0 = min(q.nodes - w.q0, A.TB);
+    w.tokens1 = min(max(q.nodes - w.q0 - A.TB, 0), A.TB);
+    w.first = at;
+    w.part = count == blocks ? -1 : 2 * (int)blockIdx.x + (at > 0 ? 0 : 1);
+    if (w.tokens1 == 0) {
+      w.turns = kTurns;
+      w.tokens1 = w.tokens0;
+      w.blocks0 = (count + 1) / 2;
+      w.blocks1 = count / 2;
+    } else {
+      w.turns = kShared;
+      w.blocks0 = min(max((min(q.past + w.q0 + w.tokens0, q.most) + KEYS - 1) / KEYS - at, 0), count);
+      w.blocks1 = count;
+    }
+    if (at == 0 && count < blocks) {
+      cut_row = q.start + w.q0;
+      cut_head = head;
+      cut_tokens = min(q.nodes - w.q0, q.span);
+      cut_from = pos;
+      cut_blocks = blocks;
+    }
+    pos += count;
+    w.more = pos < end;
+    if (w.more) {
+      at = 0;
+      if (++pair == q.pairs) {
+        pair = 0;
+        head++;
+        while (head == A.Hk || q.pairs == 0) {  // also past sequences without rows
+          head = 0;
+          q = ChunkSeq<KEYS>(A, ++seq);
+        }
+      }
+    }
+    return w;
+  }
+  __device__ __forceinline__ int4 Cut(int per) const {
+    return make_int4(cut_row, cut_head, cut_tokens, cut_tokens > 0 ? (cut_from + cut_blocks - 1) / per - (int)blockIdx.x + 1 : 0);
+  }
+};
+
+// Where this block of threads begins, as TreeBegin finds it; per: the ranges' length.
+template <int KEYS>
+__device__ __forceinline__ bool ChunkBegin(const TaArgs& A, TaShared* sh, int& seq, int& at, int& pos, int& end, int& per) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto work = [&](int s) {
+    if (s >= A.n) return 0;
+    const ChunkSeq<KEYS> q(A, s);
+    return A.Hk * q.Before(q.pairs);
+  };
+  const int first = work(threadIdx.x);
+  int sum = first;
+  for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sh->sums[warp] = sum;
+  __syncthreads();
+  int total = 0;
+  for (int k = 0; k < warps; k++) total += sh->sums[k];
+  per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  pos = (int)min((long long)blockIdx.x * per, (long long)total);
+  end = min(pos + per, total);
+  if (pos >= end) return false;
+  int before = 0;
+  for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) sh->sums[warp] = incl;
+    __syncthreads();
+    int ahead = before;
+    for (int k = 0; k < warps; k++) {
+      if (k < warp) ahead += sh->sums[k];
+      before += sh->sums[k];
+    }
+    ahead += incl - mine;
+    if (ahead <= pos && pos < ahead + mine) {
+      sh->found_seq = s;
+      sh->found_at = pos - ahead;
+    }
+  }
+  __syncthreads();
+  seq = sh->found_seq;
+  at = sh->found_at;
+  return true;
+}
+
 __device__ __forceinline__ void PutWork(TaShared* sh, int slot, const TaWork& w) {
   sh->work[slot][0] = make_int4(w.seq, w.start, w.head, w.q0);
   sh->work[slot][1] = make_int4(w.tokens0, w.tokens1, w.blocks0, w.blocks1);
@@ -525,32 +705,37 @@ __device__ __forceinline__ void GetWork(const TaShared* sh, int slot, TaWork& w)
   w.more = Uniform(d.z);
 }
 
-template <int KEYS, bool TREE>
+template <int KEYS, bool TREE, bool CHUNK>
 struct TaBlocks {
   const TaArgs& A;
   const TaWork& w;
   // The key block of step t of tile i.
   __device__ __forceinline__ int Index(int i, int t) const { return TREE ? (w.turns == kTurns ? w.first + 2 * t + i : w.first + t) : t; }
+  // Whether a block lies in the cache.
+  __device__ __forceinline__ bool Cached(int b) const { return CHUNK || (TREE && b < w.cache_blocks); }
   // Keys of a block that belong to the sequence (1 .. KEYS).
   __device__ __forceinline__ int Keys(int b) const {
-    if constexpr (TREE) return b < w.cache_blocks ? min(KEYS, w.cached - KEYS * b) : w.nodes;
+    if constexpr (CHUNK) return min(KEYS, w.cached - KEYS * b);
+    else if constexpr (TREE) return b < w.cache_blocks ? min(KEYS, w.cached - KEYS * b) : w.nodes;
     else return min(KEYS, w.nodes - KEYS * b);
   }
   // Keys of a block that some row of tile i may see.
   __device__ __forceinline__ int Seen(int i, int b) const {
-    if constexpr (TREE) return Keys(b);
+    if constexpr (CHUNK) return min(Keys(b), w.cache_blocks + w.q0 + (w.turns == kShared ? i * A.TB : 0) + w.Tokens(i) - KEYS * b);
+    else if constexpr (TREE) return Keys(b);
     else return min(KEYS, w.q0 + i * A.TB + w.Tokens(i) - KEYS * b);
   }
 };
 
-// Prompts; trees with a block of threads for every tile pair; trees with a range of key blocks for every block of threads, pair after
-// pair. (Pairs on their own are worth a kernel: what goes on from one pair to the next takes registers that head_dim 64
+// Prompts; trees with a block of threads for every tile pair; trees, and chunks, with a range of key blocks for every block of
+// threads, pair after pair. (Pairs on their own are worth a kernel: what goes on from one pair to the next takes registers that head_dim 64
 // does not have, and 256 single tokens over 512 positions took 27 us instead of 21.)
-enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2 };
+enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2, kChunkRanges = 3 };
 
 template <int D, bool F16, int KIND>
 __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAttentionKernel(const __grid_constant__ TaArgs A) {
-  constexpr bool TREE = KIND != kPrompt, RANGES = KIND == kTreeRanges;
+  // TREE: keys come from the cache's pages (all of them for CHUNK)
+  constexpr bool TREE = KIND != kPrompt, CHUNK = KIND == kChunkRanges, RANGES = KIND == kTreeRanges || CHUNK;
   using Cfg = TaCfg<D>;
   constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
   extern __shared__ uint8_t ta_raw[];
@@ -559,11 +744,17 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   uint8_t* ring = base + 2 * Cfg::kQTile;
   TaShared* sh = reinterpret_cast<TaShared*>(ring + U * Cfg::kUnit);
   const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (warp == 9 && lane < (TREE ? 4 : 3)) PrefetchTmaDesc(lane == 0 ? &A.qmap : lane == 1 ? &A.kmap : lane == 2 ? &A.vmap : &A.pool);
+  if (CHUNK ? warp == 9 && lane < 2 : warp == 9 && lane < (TREE ? 4 : 3))
+    PrefetchTmaDesc(lane == 0 ? &A.qmap : CHUNK ? &A.pool : lane == 1 ? &A.kmap : lane == 2 ? &A.vmap : &A.pool);
   GridDepWait();
   TaWork w;
-  int begin_seq = 0, begin_at = 0, begin_pos = 0, begin_end = 0;
-  if constexpr (TREE) {
+  int begin_seq = 0, begin_at = 0, begin_pos = 0, begin_end = 0, per = 0;
+  if constexpr (CHUNK) {
+    if (!ChunkBegin<KEYS>(A, sh, begin_seq, begin_at, begin_pos, begin_end, per)) {
+      if (threadIdx.x == 0) A.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
+  } else if constexpr (TREE) {
     if (!TreeBegin<KEYS, RANGES>(A, sh, begin_seq, begin_at, begin_pos, begin_end)) return;
     if constexpr (!RANGES) {
       w = TreeWalk<KEYS>(A, begin_seq, begin_at, begin_pos, begin_end).Take();
@@ -589,7 +780,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     w.cache_blocks = Uniform(w.cache_blocks);
     w.nodes = Uniform(w.nodes);
   }
-  const TaBlocks<KEYS, TREE> blk{A, w};
+  const TaBlocks<KEYS, TREE, CHUNK> blk{A, w};
 
   if (warp == 0) {
     if (lane < U) {
@@ -667,10 +858,10 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         uint8_t* dst = ring + st * Cfg::kUnit;
         const int boxes = keys > 64 ? 2 : 1;
         if (lane == 0) MbarArriveExpectTx(&sh->full[st], boxes * Cfg::kHalves * kTaBox);
-        if (TREE && b < w.cache_blocks && b * kPages + boxes > held + 32) hold((b - 2) * kPages);  // by turns, a block before the last one can follow it
+        if (blk.Cached(b) && b * kPages + boxes > held + 32) hold((b - 2) * kPages);  // by turns, a block before the last one can follow it
 #pragma unroll 1
         for (int x = 0; x < boxes; x++) {
-          if (TREE && b < w.cache_blocks) {
+          if (blk.Cached(b)) {
             const int page = __shfl_sync(0xffffffffu, ids, b * kPages + x - held);
             if (lane == 0)
               for (int h = 0; h < Cfg::kHalves; h++)
@@ -692,7 +883,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       // both tiles at once or, by turns, for each
       bool ok = true;
       uint32_t segment = 0;
-      typename std::conditional<RANGES, TreeWalk<KEYS>, NoWalk>::type walk(A, begin_seq, begin_at, begin_pos, begin_end);
+      typename std::conditional<CHUNK, ChunkWalk<KEYS>, typename std::conditional<RANGES, TreeWalk<KEYS>, NoWalk>::type>::type walk(
+          A, begin_seq, begin_at, begin_pos, begin_end);
       do {
         if (segment > 0) ok = TaWaitWarp(sh, &sh->q_empty, (segment - 1) & 1);
         if (!ok) break;
@@ -732,6 +924,9 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             one(i, t + 1, false);
           }
       } while (RANGES && ok && w.more);
+      if constexpr (CHUNK) {
+        if (lane == 0) A.cuts[blockIdx.x] = walk.Cut(per);
+      }
       // every copy lands before the block may leave: the last phase of each unit's barrier
       if (segment > 0) TaDrain(&sh->q_full, (segment - 1) & 1);
       for (int v = max(0, issued - U); v < issued; v++) TaDrain(&sh->full[v % U], (uint32_t)((v / U) & 1));
@@ -916,7 +1111,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
         int page0 = 0, page1 = 0;           // read ahead of the wait, looked at behind it
         if constexpr (TREE) {
-          if (b < w.cache_blocks) {
+          if (blk.Cached(b)) {
             const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
             page0 = tb[0];
             if (KEYS == 128 && seen > 64) page1 = tb[1];
@@ -929,7 +1124,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         if constexpr (TREE) {
           gone0 = (unsigned)page0 >= (unsigned)A.pages;
           gone1 = (unsigned)page1 >= (unsigned)A.pages;
-          cut = seen < KEYS || b >= w.cache_blocks || __any_sync(0xffffffffu, gone0 || gone1);
+          cut = seen < KEYS || !blk.Cached(b) || __any_sync(0xffffffffu, gone0 || gone1);
+          if constexpr (CHUNK) cut = cut || w.cache_blocks + tok0 < KEYS * b + KEYS - 1;
         } else {
           cut = tok0 < KEYS * b + KEYS - 1 || seen < KEYS;
         }
@@ -966,11 +1162,11 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             TmemWaitLd();
             // columns this row sees: 0 .. lim-1, or the bits of its mask
             unsigned long long m0, m1 = 0;
-            if (TREE && b >= w.cache_blocks) {
+            if (TREE && !blk.Cached(b)) {
               m0 = mine ? A.masks[w.start + tok0 + token] : 0;
               if (w.nodes < 64) m0 &= (1ull << w.nodes) - 1;
             } else {
-              const int lim = TREE ? seen : min(seen, tok0 + token - KEYS * b + 1);
+              const int lim = CHUNK ? min(seen, w.cache_blocks + tok0 + token - KEYS * b + 1) : TREE ? seen : min(seen, tok0 + token - KEYS * b + 1);
               m0 = lim >= 64 ? ~0ull : lim > 0 ? (1ull << lim) - 1 : 0;
               if (KEYS == 128) m1 = lim >= 128 ? ~0ull : lim > 64 ? (1ull << (lim - 64)) - 1 : 0;
               if (gone0) m0 = 0;
@@ -1059,7 +1255,11 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
 #pragma unroll 1
           for (int t = 0; t < w.Blocks(i) && mine && !saw; t++) {
             const int b = blk.Index(i, t);
-            if (b < w.cache_blocks) {
+            if constexpr (CHUNK) {
+              const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
+              const int lim = min(blk.Keys(b), w.cache_blocks + tok0 + token - KEYS * b + 1);
+              saw = (lim > 0 && (unsigned)tb[0] < (unsigned)A.pages) || (KEYS == 128 && lim > 64 && (unsigned)tb[1] < (unsigned)A.pages);
+            } else if (b < w.cache_blocks) {
               const int* tb = A.table + (long long)w.seq * A.max_blocks + b * (KEYS / 64);
               saw = (unsigned)tb[0] < (unsigned)A.pages || (KEYS == 128 && blk.Keys(b) > 64 && (unsigned)tb[1] < (unsigned)A.pages);
             } else {
@@ -1100,7 +1300,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             a0 *= inv;
             a1 *= inv;
           }
-          const bool zero = !parts && m == -INFINITY && l == 0.f;
+          // (a part of a pair of chunk tiles may hold no key of the first of them: nothing has been accumulated)
+          const bool zero = (!parts && m == -INFINITY && l == 0.f) || (CHUNK && w.Blocks(i) == 0);
           const int node = tok0 + token;
           uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
           const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
@@ -1187,6 +1388,40 @@ __global__ void __launch_bounds__(256) TreeJoinKernel(const __grid_constant__ Ta
   const float inv = m != -INFINITY ? 1.f / l : NAN;
   const bool zero = m == -INFINITY && l == 0.f;
   uint16_t* out = A.out + (long long)row * A.out_row + (long long)h * A.out_head + lane * (D / 32);
+#pragma unroll
+  for (int j = 0; j < D / 32; j++) {
+    const float x = zero ? 0.f : v[j] * inv;
+    out[j] = (uint16_t)Pack2<F16>(x, 0.f);
+  }
+}
+
+// Joins the parts of a chunk call's rows that a range cuts: for block of threads c of the attention the pair that it begins and does not
+// end, one warp per (row, query head), D / 32 values per lane.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) ChunkJoinKernel(const __grid_constant__ TaArgs A) {
+  GridDepWait();
+  const int warps = (A.part_rows + 7) / 8, c = blockIdx.x / warps, local = (blockIdx.x - c * warps) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int4 cut = A.cuts[c];
+  if (local >= cut.z * A.G) return;
+  const int token = local / A.G, g = local - token * A.G;
+  // the block of threads that begins the pair holds its part in its second place, the others in their first
+  const auto slot = [&](int k) { return (long long)(2 * (c + k) + (k == 0 ? 1 : 0)) * A.part_rows + local; };
+  float m = -INFINITY;
+  for (int k = 0; k < cut.w; k++) m = fmaxf(m, A.part_ml[slot(k)].x);
+  float l = 0.f, v[D / 32] = {};
+#pragma unroll 2
+  for (int k = 0; k < cut.w; k++) {
+    const float2 ml = A.part_ml[slot(k)];
+    const float a = m == -INFINITY ? 1.f : Exp2(ml.x - m);
+    l = fmaf(ml.y, a, l);
+    const float* o = A.part_o + slot(k) * D + lane * (D / 32);
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) v[j] = fmaf(o[j], a, v[j]);
+  }
+  // a part whose maximum is NaN has a sum of NaN, which this sum takes over
+  const float inv = m != -INFINITY ? 1.f / l : NAN;
+  const bool zero = m == -INFINITY && l == 0.f;
+  uint16_t* out = A.out + (long long)(cut.x + token) * A.out_row + (long long)(cut.y * A.G + g) * A.out_head + lane * (D / 32);
 #pragma unroll
   for (int j = 0; j < D / 32; j++) {
     const float x = zero ? 0.f : v[j] * inv;
