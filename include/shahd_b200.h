@@ -595,7 +595,7 @@ typedef struct ShahdLogitsCall {
   const int32_t* sequences;          /* [rows] the row's sequence; null: row r is sequence r. A row whose number is not in 0 .. n-1 is left as it is */
   const int32_t* history;            /* [n, history_stride] tokens of the prompt and then the generated ones; null: no penalties. Tokens outside
                                         the vocabulary are passed over */
-  int64_t history_stride;            /* 0 .. 2^30 */
+  int64_t history_stride;            /* 0 .. 2^30 - 1 */
   const int32_t* history_lengths;    /* [n] (cut to 0 .. history_stride) */
   const int32_t* prompt_lengths;     /* [n] the history's tokens before this place are the prompt's; null: all are generated */
   const float *repetition, *presence, *frequency; /* [n]; null: 1, 0, 0 */

@@ -23,6 +23,30 @@ static __device__ int g_ops_device_error;  // 0, or the first kOpsErr* recorded 
 
 inline size_t TypeBytes(int dtype) { return dtype == SHAHD_F32 ? 4 : 2; }
 
+// The device of an address in a device's own memory; false for any other address, and where the driver cannot be asked: then the
+// runtime is, which tells more and takes longer (0.39 us an address, the driver 0.03; a call has up to fourteen).
+inline bool DeviceOfAddress(const void* p, int* device) {
+  typedef CUresult (*Fn)(unsigned int, CUpointer_attribute*, void**, CUdeviceptr);
+  static const Fn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<Fn>(f);
+  }();
+  if (!fn) return false;
+  unsigned int type = 0, managed = 1;
+  int ordinal = -1;
+  CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+  void* to[3] = {&type, &managed, &ordinal};
+  if (fn(3, what, to, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return false;
+  if (type != CU_MEMORYTYPE_DEVICE || managed != 0 || ordinal < 0) return false;
+  *device = ordinal;
+  return true;
+}
+
 // The device that every buffer of a call lives on. Add() takes the call's pointers one by one; a host pointer, an
 // address that no allocation holds or a buffer of another device makes the call fail before anything is launched.
 struct BufferCheck {
@@ -42,27 +66,31 @@ struct BufferCheck {
       rc = SHAHD_EINVAL;
       return;
     }
-    cudaPointerAttributes at = {};
-    const cudaError_t e = cudaPointerGetAttributes(&at, p);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) {
-        SetError("%s: no usable sm_100 device", op);
-        rc = SHAHD_ENODEV;
-      } else {
-        SetError("%s: %s is not a device address (%s)", op, name, cudaGetErrorString(e));
-        rc = SHAHD_EINVAL;
+    int where = -1;
+    if (!DeviceOfAddress(p, &where)) {
+      cudaPointerAttributes at = {};
+      const cudaError_t e = cudaPointerGetAttributes(&at, p);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) {
+          SetError("%s: no usable sm_100 device", op);
+          rc = SHAHD_ENODEV;
+        } else {
+          SetError("%s: %s is not a device address (%s)", op, name, cudaGetErrorString(e));
+          rc = SHAHD_EINVAL;
+        }
+        return;
       }
-      return;
+      if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) {
+        SetError("%s: %s is not a device address", op, name);
+        rc = SHAHD_EINVAL;
+        return;
+      }
+      where = at.device;
     }
-    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) {
-      SetError("%s: %s is not a device address", op, name);
-      rc = SHAHD_EINVAL;
-      return;
-    }
-    if (device < 0) device = at.device;
-    if (at.device != device) {
-      SetError("%s: %s is on device %d, other buffers are on device %d", op, name, at.device, device);
+    if (device < 0) device = where;
+    if (where != device) {
+      SetError("%s: %s is on device %d, other buffers are on device %d", op, name, where, device);
       rc = SHAHD_EINVAL;
     }
   }
