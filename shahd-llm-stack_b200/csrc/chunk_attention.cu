@@ -10,15 +10,34 @@ namespace {
 
 template <int D, bool F16>
 void LaunchChunks(const TaArgs& a, unsigned blocks, cudaStream_t st) {
+  if (a.split > 1) {
+    if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, kChunkSplit>, TaCfg<D>::kSmem)) return;
+    LaunchPdlCluster(TileAttentionKernel<D, F16, kChunkSplit>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, dim3((unsigned)a.split), st, a);
+    return;
+  }
+  if (a.least == 0) {
+    if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, kChunkPairs>, TaCfg<D>::kSmem)) return;
+    LaunchPdl(TileAttentionKernel<D, F16, kChunkPairs>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
+    return;
+  }
   if (!EnsureKernelAttrs((const void*)TileAttentionKernel<D, F16, kChunkRanges>, TaCfg<D>::kSmem)) return;
   LaunchPdl(TileAttentionKernel<D, F16, kChunkRanges>, dim3(blocks), dim3(TaCfg<D>::kThreads), TaCfg<D>::kSmem, st, a);
-  LaunchPdl(ChunkJoinKernel<D, F16>, dim3(blocks * CeilDiv(a.part_rows, 8)), dim3(256), 0, st, a);
+  LaunchPdl(ChunkJoinKernel<D, F16>, dim3(blocks * CeilDiv(a.part_rows, kJoinRows<D>)), dim3(256), 0, st, a);
 }
 
-// How a call's work is laid out: as many blocks of threads as run at once take ranges of equal length out of all key blocks of all tile
-// pairs, 256 keys at least, and the pairs that a range cuts are joined by a second kernel.
+// How a call's work is laid out; times are of one graph, 16/4 heads of 64 if nothing else is said.
+//   Pairs: a block of threads for every tile pair, longest first. Where there are many, or enough with short caches. 16 chunks of 300 to
+//     2048 rows from position 0: 127 us, ranges 154; 256 single tokens, 8/2 heads, 400 to 576 positions: 17.7 and 35; 48 sequences, six
+//     of them with 200 to 512 rows, 0 to 1500 positions: 44.4 and 45.8 (the longest pair is 38 of them).
+//   Split: a cluster of 2 to 8 blocks of threads for every pair, where that leaves multiprocessors for all and the steps are few: one
+//     launch, no second kernel. 96 rows over 1700 positions: 13.4 us, ranges 20, pairs 36.
+//   Ranges: as many blocks of threads as run at once take ranges of equal cost out of the line of all pairs, and what a range cuts is joined
+//     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 167 us, pairs 219, split in
+//     two 219; 2 chunks of 1024 over 12000, 32/8 heads of 128: 440 and 510. The second kernel and the parts cost about eight steps.
+// The lengths lie on the device, so the table's width stands for them, and a table much wider than its sequences are long may get the
+// layout for longer ones.
 struct ChunkLayout {
-  int least, part_rows;
+  int least, part_rows, two_heads, split;
   long long grid;
   int64_t cut_bytes, bytes;
 };
@@ -32,18 +51,35 @@ int LayChunks(const char* op, const ShahdChunkCall* c, ChunkLayout* out) {
   }
   const int G = H / Hk, span = 2 * (128 / G), keys = d == 128 ? 128 : 64;
   const long long pairs = std::min((long long)c->rows / span + c->n, (long long)c->n * CeilDiv(std::min(c->max_rows, 1 << 30), span));
-  const long long most = pairs * Hk * CeilDiv(c->cache.max_blocks, keys / 64);  // key blocks of all pairs, if all sequences were as long
+  const long long most = pairs * Hk * (CeilDiv(c->cache.max_blocks, keys / 64) + kPairCost);  // what all pairs cost, if all sequences were as long
   if (c->rows > kOpsMaxRows || pairs > (1 << 23) || most > 0x3fffffffLL) {
     SetError("%s: too many rows or key blocks: %d rows, %d sequences, %d pages each", op, c->rows, c->n, c->cache.max_blocks);
     return SHAHD_EINVAL;
   }
   ChunkLayout l = {};
   const long long slots = kTaSms * (d == 128 ? 1 : 2);
-  l.least = 256 / keys;
-  l.grid = std::max(1LL, std::min(slots, (most + l.least - 1) / l.least));
+  const long long places = (long long)c->rows / span + c->n, tiles = pairs * Hk, blocks = CeilDiv(c->cache.max_blocks, keys / 64);
+  if (places * Hk > 0x3fffffff) {
+    SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
+    return SHAHD_EINVAL;
+  }
   l.part_rows = std::min(c->max_rows, span) * G;
-  l.cut_bytes = (l.grid * (int64_t)sizeof(int4) + 255) / 256 * 256;
-  l.bytes = l.cut_bytes + 2 * l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
+  l.split = 1;
+  while (l.split < 8 && tiles * l.split * 2 <= slots) l.split *= 2;
+  const bool ranges = tiles >= 4 * slots ? false : tiles >= slots ? blocks >= 64 : blocks / l.split > tiles * blocks / slots + 8;
+  if (ranges) {
+    l.split = 1;
+    l.least = 256 / keys + kPairCost;
+    l.grid = std::max(1LL, std::min(slots, (most + l.least - 1) / l.least));
+    l.cut_bytes = (l.grid * (int64_t)sizeof(int4) + 255) / 256 * 256;
+    l.bytes = l.cut_bytes + 2 * l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
+  } else if (l.split > 1) {
+    l.grid = places * Hk * l.split;
+    l.bytes = l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
+  } else {  // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge
+    l.two_heads = c->max_rows <= span / 2 && Hk % 2 == 0;
+    l.grid = l.two_heads ? places * Hk / 2 : places * Hk;
+  }
   *out = l;
   return SHAHD_OK;
 }
@@ -93,7 +129,7 @@ int shahd_chunk_attention(const ShahdChunkCall* c, void* stream) {
   b.Add("out", c->out.data, 16);
   b.Add("cache.pool", c->cache.pool, 16);
   b.Add("cache.block_table", c->cache.block_table, 4);
-  b.Add("workspace", c->workspace, 32);
+  if (lay.bytes > 0) b.Add("workspace", c->workspace, 32);
   if (b.rc != SHAHD_OK) return b.rc;
   const DeviceInfo info = InfoOf(b.device);
   DeviceScope scope(b.device);
@@ -122,10 +158,14 @@ int shahd_chunk_attention(const ShahdChunkCall* c, void* stream) {
   a.pages = c->cache.pages;
   a.max_nodes = c->max_rows;
   a.least = lay.least;
-  a.part_rows = lay.part_rows;
-  a.cuts = static_cast<int4*>(c->workspace);
-  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(c->workspace) + lay.cut_bytes);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * lay.grid * lay.part_rows * d);
+  a.two_heads = lay.two_heads;
+  a.split = lay.split;
+  if (lay.bytes > 0) {
+    a.part_rows = lay.part_rows;
+    a.cuts = static_cast<int4*>(c->workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(c->workspace) + lay.cut_bytes);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (lay.split > 1 ? 1 : 2) * lay.grid * lay.part_rows * d);
+  }
   TakeLaunchError(nullptr);
   g_waiting_devices.Add(b.device);
   const unsigned blocks = (unsigned)lay.grid;

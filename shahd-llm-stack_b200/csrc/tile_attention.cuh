@@ -82,12 +82,12 @@ struct TaArgs {
   const unsigned long long* masks;
   const int* lengths;
   const int* table;
-  int max_blocks, pages, max_nodes, pairs, two_heads;  // two_heads: the pair's tiles are those of two kv heads
+  int max_blocks, pages, max_nodes, pairs, split, two_heads;  // split: blocks of threads that share a pair; two_heads: the pair's tiles are those of two kv heads
   // All key blocks of all tile pairs in one line, dealt out to the blocks of threads in ranges of equal length, at least
   // `least`: 0 where every pair has a block of threads of its own instead. A pair that a range cuts leaves parts: block of threads c
   // has room for two, [2 c] for a pair that it does not begin and [2 c + 1] for one that it does not end.
   int least, part_rows;
-  float* part_o;    // [2 grid, part_rows, D]
+  float* part_o;    // [2 grid, part_rows, D] (split: [grid, part_rows, D])
   float2* part_ml;  // [2 grid, part_rows]: -Offset() of the running maximum, and the sum
   int* plan;        // trees: the ranges' length, then for every sequence the blocks of all before it, and their total
   int4* cuts;       // chunks: [grid] the pair that block of threads c begins and does not end: first row, kv head, tokens (0: none), parts
@@ -280,7 +280,7 @@ struct TaWork {
   int cache_blocks;     // trees: key blocks of the cache; chunks: positions before the chunk
   int nodes;            // trees, chunks: rows of the sequence; prompts: tokens of the sequence
   int part;             // ranges: the place of the results among the block's parts, or -1: these are all key blocks
-  int more;             // ranges: there is another pair behind this one
+  int more;             // ranges: there is another pair behind this one; split: the pair's shares
   __device__ __forceinline__ int Tokens(int i) const { return i ? tokens1 : tokens0; }
   __device__ __forceinline__ int Blocks(int i) const { return i ? blocks1 : blocks0; }
 };
@@ -503,32 +503,33 @@ __device__ __forceinline__ bool TreeBegin(const TaArgs& A, TaShared* sh, int& se
 }
 
 // Sum of floor((a j + b) / m) over j = 0 .. n-1: the lattice points under a line, counted by turns from either axis, which shrinks the
-// numbers as Euclid's algorithm does (Graham, Knuth and Patashnik, Concrete Mathematics, 3.5). The sum is below 2^30.
-__device__ __forceinline__ int FloorSum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  uint32_t sum = 0;
+// numbers as Euclid's algorithm does (Graham, Knuth and Patashnik, Concrete Mathematics, 3.5). The sum is below 2^30. The first turn's
+// divisor is known: two shifts, and where it divides a, all there is to do.
+template <uint32_t M>
+__device__ __forceinline__ int FloorSum(uint32_t n, uint32_t a, uint32_t b) {
+  if (n == 0) return 0;
+  uint32_t sum = (uint32_t)((unsigned long long)n * (n - 1) / 2 * (a / M)) + n * (b / M), m = M;
+  a %= M;
+  b %= M;
 #pragma unroll 1
-  while (n > 0) {
-    if (a >= m) {
-      sum += (uint32_t)((unsigned long long)n * (n - 1) / 2 * (a / m));
-      a %= m;
-    }
-    if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
-    }
-    const uint32_t top = a * n + b;  // n is at most 2^23, m at most 256
-    if (top < m) break;
+  while (a * n + b >= m) {  // n is at most 2^23, m at most 256
+    const uint32_t top = a * n + b, old = m;
     n = top / m;
     b = top % m;
-    const uint32_t old = m;
     m = a;
     a = old;
+    sum += (uint32_t)((unsigned long long)n * (n - 1) / 2 * (a / m)) + n * (b / m);
+    a %= m;
+    b %= m;
   }
   return (int)sum;
 }
 
 // A sequence of a chunk call: its rows, the positions before them and in all, tile pairs, and their key blocks: causal, so a later pair
-// has more of them.
+// has more of them. What a pair costs is counted in steps: a key block for both tiles, or two blocks by turns; and kPairCost of them
+// for what a pair takes besides (its queries, the ends of the chain, its results: 4 to 5 us next to steps of 1.2 to 1.9). Those stand
+// before a pair's other steps in the line and belong to the block of threads that has the first of these.
+constexpr int kPairCost = 3;
 template <int KEYS>
 struct ChunkSeq {
   int start, nodes, past, total, most, pairs, span;
@@ -541,31 +542,70 @@ struct ChunkSeq {
     span = 2 * A.TB;
     pairs = (nodes + span - 1) / span;
   }
-  // Key blocks of pair p, and of all pairs before it (p <= pairs).
+  // Key blocks and steps of pair p, and what all pairs before it cost (p <= pairs).
   __device__ __forceinline__ int Blocks(int p) const { return (min(past + min((p + 1) * span, nodes), most) + KEYS - 1) / KEYS; }
+  __device__ __forceinline__ bool Turns(int p) const { return nodes - p * span <= span / 2; }
+  __device__ __forceinline__ int Steps(int p) const {
+    const int blocks = Blocks(p);
+    return Turns(p) ? (blocks + 1) / 2 : blocks;
+  }
   __device__ __forceinline__ int Before(int p) const {
     if (p == 0) return 0;
     // pairs up to the last but one are whole; from the table's end on all see the same
     const int q = p == pairs ? p - 1 : p, inside = min(q, (most - past) / span);
-    const int sum = FloorSum(inside, KEYS, span, past + span + KEYS - 1) + (q - inside) * ((most + KEYS - 1) / KEYS);
-    return p == pairs ? sum + Blocks(q) : sum;
+    const int sum = FloorSum<KEYS>(inside, span, past + span + KEYS - 1) + (q - inside) * ((most + KEYS - 1) / KEYS) + p * kPairCost;
+    return p == pairs ? sum + Steps(q) : sum;
   }
 };
 
-// The key blocks of a chunk call that this block of threads takes, pair by pair: sequence after sequence, kv head after kv head.
+// The pair of tiles that a block of threads takes, as PromptWork finds it: the chunks' own rows count for the order, not what is cached. Of
+// its key blocks this is the share of number `place` of `split`, two blocks at least; w.more: shares that there are.
+template <int KEYS>
+__device__ __forceinline__ bool ChunkWork(const TaArgs& A, int rank, int all, int split, int place, TaWork& w) {
+  if (!PromptWork<KEYS>(A, rank, all, w)) return false;
+  const ChunkSeq<KEYS> q(A, w.seq);
+  if (w.q0 >= q.nodes) return false;
+  w.nodes = q.nodes;
+  w.cached = q.total;
+  w.cache_blocks = q.past;
+  w.tokens0 = min(q.nodes - w.q0, A.TB);
+  w.tokens1 = min(max(q.nodes - w.q0 - A.TB, 0), A.TB);
+  const int blocks = q.Blocks(w.q0 / q.span), per = max((blocks + split - 1) / split, min(blocks, 2));
+  w.first = place * per;
+  const int count = min(max(blocks - w.first, 0), per);
+  w.more = (blocks + per - 1) / per;
+  w.part = w.more > 1 ? (int)blockIdx.x : -1;
+  if (A.two_heads) {
+    w.turns = kHeads;
+    w.tokens1 = w.tokens0;
+    w.blocks0 = w.blocks1 = count;
+  } else if (w.tokens1 == 0) {
+    w.turns = kTurns;
+    w.tokens1 = w.tokens0;
+    w.blocks0 = (count + 1) / 2;
+    w.blocks1 = count / 2;
+  } else {
+    w.turns = kShared;
+    w.blocks0 = min(max((min(q.past + w.q0 + w.tokens0, q.most) + KEYS - 1) / KEYS - w.first, 0), count);
+    w.blocks1 = count;
+  }
+  return true;
+}
+
+// The steps of a chunk call that this block of threads takes, pair by pair: sequence after sequence, kv head after kv head.
 template <int KEYS>
 struct ChunkWalk {
   const TaArgs& A;
-  ChunkSeq<KEYS> q;             // of `seq`
-  int seq, head, pair, at, pos, end;  // the next pair and its first block; the range that is left
-  int cut_row, cut_head, cut_tokens, cut_from, cut_blocks;  // the pair that the range begins and does not end
-  // From block `at_` of sequence seq_'s on, pos_ in the line, to end_. The whole warp takes part.
+  ChunkSeq<KEYS> q;                   // of `seq`
+  int seq, head, pair, at, pos, end;  // the next pair and how much of its cost lies behind; the range that is left
+  int cut_row, cut_head, cut_tokens, cut_from, cut_steps;  // the pair that the range begins and does not end
+  // From place `at_` of sequence seq_'s on, pos_ in the line, to end_. The whole warp takes part.
   __device__ __forceinline__ ChunkWalk(const TaArgs& a, int seq_, int at_, int pos_, int end_) : A(a), q(a, seq_), seq(seq_), pos(pos_), end(end_) {
     cut_tokens = 0;
     const int line = q.Before(q.pairs);
     head = at_ / line;
     const int x = at_ - head * line;
-    // the last pair with no more than x blocks before it
+    // the last pair with no more than x before it
     int lo = 0, cnt = q.pairs;
     while (cnt > 1) {
       const int step = (cnt + 31) / 32, k = (threadIdx.x & 31) * step;
@@ -577,10 +617,12 @@ struct ChunkWalk {
     pair = lo;
     at = x - q.Before(lo);
   }
-  // The next pair's work; there is one (pos < end).
+  // The next pair's work; there is some: ranges are longer than kPairCost, and the last one goes to a pair's end.
   __device__ __forceinline__ TaWork Take() {
     TaWork w;
-    const int blocks = q.Blocks(pair), count = min(blocks - at, end - pos);
+    const int steps = q.Steps(pair), blocks = q.Blocks(pair), length = min(steps + kPairCost - at, end - pos);
+    const int first = max(at - kPairCost, 0), last = at + length - kPairCost;
+    const bool turns = q.Turns(pair);
     w.seq = seq;
     w.start = q.start;
     w.nodes = q.nodes;
@@ -589,28 +631,30 @@ struct ChunkWalk {
     w.head = head;
     w.q0 = pair * q.span;
     w.tokens0 = min(q.nodes - w.q0, A.TB);
-    w.tokens1 = min(max(q.nodes - w.q0 - A.TB, 0), A.TB);
-    w.first = at;
-    w.part = count == blocks ? -1 : 2 * (int)blockIdx.x + (at > 0 ? 0 : 1);
-    if (w.tokens1 == 0) {
+    w.tokens1 = turns ? w.tokens0 : q.nodes - w.q0 - w.tokens0;
+    if (!turns) w.tokens1 = min(w.tokens1, A.TB);
+    w.part = first == 0 && last == steps ? -1 : 2 * (int)blockIdx.x + (first > 0 ? 0 : 1);
+    if (turns) {
+      const int count = min(2 * last, blocks) - 2 * first;
       w.turns = kTurns;
-      w.tokens1 = w.tokens0;
+      w.first = 2 * first;
       w.blocks0 = (count + 1) / 2;
       w.blocks1 = count / 2;
     } else {
       w.turns = kShared;
-      w.blocks0 = min(max((min(q.past + w.q0 + w.tokens0, q.most) + KEYS - 1) / KEYS - at, 0), count);
-      w.blocks1 = count;
+      w.first = first;
+      w.blocks1 = last - first;
+      w.blocks0 = min(max((min(q.past + w.q0 + w.tokens0, q.most) + KEYS - 1) / KEYS - first, 0), w.blocks1);
     }
-    if (at == 0 && count < blocks) {
+    if (first == 0 && last < steps) {
       cut_row = q.start + w.q0;
       cut_head = head;
       cut_tokens = min(q.nodes - w.q0, q.span);
-      cut_from = pos;
-      cut_blocks = blocks;
+      cut_from = pos - at + kPairCost;
+      cut_steps = steps;
     }
-    pos += count;
-    w.more = pos < end;
+    pos += length;
+    w.more = end - pos > kPairCost;
     if (w.more) {
       at = 0;
       if (++pair == q.pairs) {
@@ -625,7 +669,7 @@ struct ChunkWalk {
     return w;
   }
   __device__ __forceinline__ int4 Cut(int per) const {
-    return make_int4(cut_row, cut_head, cut_tokens, cut_tokens > 0 ? (cut_from + cut_blocks - 1) / per - (int)blockIdx.x + 1 : 0);
+    return make_int4(cut_row, cut_head, cut_tokens, cut_tokens > 0 ? (cut_from + cut_steps - 1) / per - (int)blockIdx.x + 1 : 0);
   }
 };
 
@@ -641,37 +685,51 @@ __device__ __forceinline__ bool ChunkBegin(const TaArgs& A, TaShared* sh, int& s
   const int first = work(threadIdx.x);
   int sum = first;
   for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
+  const bool one = A.n <= (int)blockDim.x;  // a sequence a thread: one scan gives the total, too
+  int incl = sum;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) sh->sums[warp] = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh->sums[warp] = incl;
   __syncthreads();
-  int total = 0;
-  for (int k = 0; k < warps; k++) total += sh->sums[k];
+  int total = 0, ahead = incl - sum;
+  for (int k = 0; k < warps; k++) {
+    if (k < warp) ahead += sh->sums[k];
+    total += sh->sums[k];
+  }
   per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   pos = (int)min((long long)blockIdx.x * per, (long long)total);
   end = min(pos + per, total);
   if (pos >= end) return false;
-  int before = 0;
-  for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    __syncthreads();
-    if (lane == 31) sh->sums[warp] = incl;
-    __syncthreads();
-    int ahead = before;
-    for (int k = 0; k < warps; k++) {
-      if (k < warp) ahead += sh->sums[k];
-      before += sh->sums[k];
-    }
-    ahead += incl - mine;
-    if (ahead <= pos && pos < ahead + mine) {
+  const auto look = [&](int s, int from, int mine) {
+    if (from <= pos && pos < from + mine) {
       sh->found_seq = s;
-      sh->found_at = pos - ahead;
+      sh->found_at = pos - from;
+    }
+  };
+  if (one) {
+    look(threadIdx.x, ahead, first);
+  } else {
+    int before = 0;
+    for (int s0 = 0; s0 < A.n; s0 += blockDim.x) {
+      const int s = s0 + threadIdx.x, mine = s0 == 0 ? first : work(s);
+      incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      __syncthreads();
+      if (lane == 31) sh->sums[warp] = incl;
+      __syncthreads();
+      int from = before;
+      for (int k = 0; k < warps; k++) {
+        if (k < warp) from += sh->sums[k];
+        before += sh->sums[k];
+      }
+      look(s, from + incl - mine, mine);
     }
   }
   __syncthreads();
@@ -705,6 +763,12 @@ __device__ __forceinline__ void GetWork(const TaShared* sh, int slot, TaWork& w)
   w.more = Uniform(d.z);
 }
 
+// The same into ordinary registers.
+__device__ __forceinline__ void ReadWork(const TaShared* sh, int slot, TaWork& w) {
+  const int4 a = sh->work[slot][0], b = sh->work[slot][1], c = sh->work[slot][2], d = sh->work[slot][3];
+  w = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w, d.x, d.y, d.z};
+}
+
 template <int KEYS, bool TREE, bool CHUNK>
 struct TaBlocks {
   const TaArgs& A;
@@ -727,17 +791,87 @@ struct TaBlocks {
   }
 };
 
-// Prompts; trees with a block of threads for every tile pair; trees, and chunks, with a range of key blocks for every block of
+// Joins the parts of rows of a chunk call: `parts` of them in the places first, first + 1, .. of the parts, or, where they are a range's, in
+// the second place of block of threads `first` and the first places of those behind it. A warp takes R groups of rows from local0 on,
+// 16 bytes of a row a lane, with K parts of each in flight.
+template <int D, bool F16, int R, int K>
+__device__ __forceinline__ void JoinRows(const TaArgs& A, int first, bool ranges, int parts, int local0, int rows, int row0, int head) {
+  constexpr int kLanes = D / 4, kGroup = 32 / kLanes;  // lanes of a row, rows of a group
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, piece = lane % kLanes;
+  float m[R], l[R], v[R][4];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    m[r] = -INFINITY;
+    l[r] = v[r][0] = v[r][1] = v[r][2] = v[r][3] = 0.f;
+  }
+#pragma unroll 1
+  for (int k0 = 0; k0 < parts; k0 += K) {
+    float2 ml[R][K];
+    float4 o[R][K];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int local = local0 + r * kGroup + sub, part = k0 + k;
+        ml[r][k] = make_float2(-INFINITY, 0.f);
+        o[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (part < parts && local < rows) {
+          const long long slot = (long long)(ranges ? 2 * (first + part) + (part == 0 ? 1 : 0) : first + part) * A.part_rows + local;
+          ml[r][k] = A.part_ml[slot];
+          o[r][k] = reinterpret_cast<const float4*>(A.part_o + slot * D)[piece];
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float most = m[r];
+#pragma unroll
+      for (int k = 0; k < K; k++) most = fmaxf(most, ml[r][k].x);
+      const float was = most == -INFINITY ? 1.f : Exp2(m[r] - most);
+      m[r] = most;
+      l[r] *= was;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[r][j] *= was;
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const float a = most == -INFINITY ? 1.f : Exp2(ml[r][k].x - most);
+        l[r] = fmaf(ml[r][k].y, a, l[r]);
+        v[r][0] = fmaf(o[r][k].x, a, v[r][0]);
+        v[r][1] = fmaf(o[r][k].y, a, v[r][1]);
+        v[r][2] = fmaf(o[r][k].z, a, v[r][2]);
+        v[r][3] = fmaf(o[r][k].w, a, v[r][3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int local = local0 + r * kGroup + sub;
+    if (local >= rows) break;
+    const int token = local / A.G, g = local - token * A.G;
+    // a part whose maximum is NaN has a sum of NaN, which this sum takes over
+    const float inv = m[r] != -INFINITY ? 1.f / l[r] : NAN;
+    const bool zero = m[r] == -INFINITY && l[r] == 0.f;
+    uint16_t* out = A.out + (long long)(row0 + token) * A.out_row + (long long)(head * A.G + g) * A.out_head + 4 * piece;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[r][j] = zero ? 0.f : v[r][j] * inv;
+    *reinterpret_cast<uint2*>(out) = make_uint2(Pack2<F16>(v[r][0], v[r][1]), Pack2<F16>(v[r][2], v[r][3]));
+  }
+}
+
+// Prompts; trees, and chunks, with a block of threads for every tile pair, or with a range of key blocks for every block of
 // threads, pair after pair. (Pairs on their own are worth a kernel: what goes on from one pair to the next takes registers that head_dim 64
 // does not have, and 256 single tokens over 512 positions took 27 us instead of 21.)
-enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2, kChunkRanges = 3 };
+// Chunks also with a cluster of blocks of threads for every tile pair, which split its key blocks and join their parts at the end.
+enum TaKind { kPrompt = 0, kTreePairs = 1, kTreeRanges = 2, kChunkPairs = 3, kChunkRanges = 4, kChunkSplit = 5 };
 
 template <int D, bool F16, int KIND>
 __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAttentionKernel(const __grid_constant__ TaArgs A) {
   // TREE: keys come from the cache's pages (all of them for CHUNK)
-  constexpr bool TREE = KIND != kPrompt, CHUNK = KIND == kChunkRanges, RANGES = KIND == kTreeRanges || CHUNK;
+  constexpr bool TREE = KIND != kPrompt, SPLIT = KIND == kChunkSplit, CHUNK = KIND == kChunkPairs || KIND == kChunkRanges || SPLIT, RANGES = KIND == kTreeRanges || KIND == kChunkRanges;
   using Cfg = TaCfg<D>;
   constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
+  // The softmax warps read what they work on from shared memory at every step instead of holding it in registers, which two blocks of
+  // threads on a multiprocessor do not have: the steps of 64 keys are a chain of latencies, and what is spilled lengthens it.
+  constexpr bool RELOAD = KIND == kChunkRanges && !TaCfg<D>::kWide;
   extern __shared__ uint8_t ta_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = base;
@@ -749,10 +883,17 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   GridDepWait();
   TaWork w;
   int begin_seq = 0, begin_at = 0, begin_pos = 0, begin_end = 0, per = 0;
-  if constexpr (CHUNK) {
+  if constexpr (KIND == kChunkRanges) {
     if (!ChunkBegin<KEYS>(A, sh, begin_seq, begin_at, begin_pos, begin_end, per)) {
       if (threadIdx.x == 0) A.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);
       return;
+    }
+  } else if constexpr (KIND == kChunkPairs || SPLIT) {
+    if (warp == 9) {
+      const int heads = A.two_heads ? A.Hk / 2 : A.Hk, split = SPLIT ? A.split : 1, tile = blockIdx.x / split;
+      if (!ChunkWork<KEYS>(A, tile / heads, gridDim.x / split / heads, split, blockIdx.x - tile * split, w)) w.nodes = 0;
+      w.head = tile % heads * (A.two_heads ? 2 : 1);
+      if (lane == 0) PutWork(sh, 0, w);
     }
   } else if constexpr (TREE) {
     if (!TreeBegin<KEYS, RANGES>(A, sh, begin_seq, begin_at, begin_pos, begin_end)) return;
@@ -813,11 +954,12 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   __syncthreads();
   TcgenFenceAfter();
   const uint32_t tmem = (uint32_t)Uniform((int)sh->tmem);
-  if constexpr (KIND == kPrompt) {
+  if constexpr (KIND == kPrompt || KIND == kChunkPairs || SPLIT) {
     GetWork(sh, 0, w);
-    w.turns = w.first = w.cached = w.cache_blocks = 0;
-    w.part = -1;
-    if (w.nodes == 0) {
+    if (KIND == kPrompt) w.turns = w.cached = w.cache_blocks = 0;
+    if (!SPLIT) w.first = 0;
+    if (!SPLIT) w.part = -1;
+    if (w.nodes == 0) {  // a whole cluster
       if (warp == 8) TmemDealloc(tmem, Cfg::kCols);
       return;
     }
@@ -830,14 +972,16 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     ok = ok && got;
     if (got) {
       GetWork(sh, segment & 3, w);
-      if (lane == 0) MbarArrive(&sh->work_read[segment & 3]);
+      if (lane == 0 && !(RELOAD && warp < 8)) MbarArrive(&sh->work_read[segment & 3]);
     }
     return got;
   };
   GridDepLaunch();  // after this block holds its TMEM
   float* const sml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 768);  // tile 1's maxima and sums, for a merge
 
-  if (warp >= 8) {
+  const bool idle = SPLIT && w.blocks0 + w.blocks1 == 0;  // the pair has fewer blocks than the cluster would take
+  if (idle) {
+  } else if (warp >= 8) {
     if constexpr (Cfg::kWide) RegsDown<kTaRegsIssue>();
     if (warp == 9) {
       // The whole warp follows the same path, lane 0 issues. Lane l holds the l-th page of the 32 that come next.
@@ -883,7 +1027,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       // both tiles at once or, by turns, for each
       bool ok = true;
       uint32_t segment = 0;
-      typename std::conditional<CHUNK, ChunkWalk<KEYS>, typename std::conditional<RANGES, TreeWalk<KEYS>, NoWalk>::type>::type walk(
+      typename std::conditional<KIND == kChunkRanges, ChunkWalk<KEYS>, typename std::conditional<RANGES, TreeWalk<KEYS>, NoWalk>::type>::type walk(
           A, begin_seq, begin_at, begin_pos, begin_end);
       do {
         if (segment > 0) ok = TaWaitWarp(sh, &sh->q_empty, (segment - 1) & 1);
@@ -924,7 +1068,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
             one(i, t + 1, false);
           }
       } while (RANGES && ok && w.more);
-      if constexpr (CHUNK) {
+      if constexpr (KIND == kChunkRanges) {
         if (lane == 0) A.cuts[blockIdx.x] = walk.Cut(per);
       }
       // every copy lands before the block may leave: the last phase of each unit's barrier
@@ -1031,7 +1175,8 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           values(i, t, vunit);
           if (ok && (w.turns || i == last)) release(vunit);
         };
-        // prompts: V of step t and K of step t + 1, under one wait
+        // prompts and chunks: V of step t and K of step t + 1, under one wait
+        const bool both = !TREE || (CHUNK && !w.turns);
         int vnext = 0, knext = 0;
         const auto acquire_step = [&](int t) {
           if (t >= steps) return;
@@ -1059,10 +1204,10 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         next_scores(0, 0);
         next_scores(1, 0);
         if (steps == 1 && ok) UmmaIssueCommit(&sh->q_empty);
-        if (!TREE) acquire_step(0);
+        if (both) acquire_step(0);
 #pragma unroll 1
         for (int t = 0; t < steps && ok; t++) {
-          if (!TREE) {
+          if (both) {
             vunit = vnext;
             kunit = knext;
             trim(blk.Index(0, t), vunit);
@@ -1073,7 +1218,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           }
           next_values(0, t);
           next_scores(0, t + 1);
-          if (!TREE) acquire_step(t + 1);  // under the products just issued
+          if (both) acquire_step(t + 1);  // under the products just issued
           next_values(1, t);
           next_scores(1, t + 1);
           if (t + 2 == steps && ok) UmmaIssueCommit(&sh->q_empty);  // the last scores: Q may be replaced behind them
@@ -1100,12 +1245,21 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     if constexpr (RANGES) w.more = 1;
     while ((segment == 0 && !RANGES) || next(segment, ok)) {
       segment++;
-      const int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
-      const bool mine = token < w.Tokens(i);
-      const bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
+      int tok0 = w.q0 + (w.turns ? 0 : i * A.TB);  // the tile's first token
+      bool mine = token < w.Tokens(i);
+      bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
+      const auto again = [&]() {
+        if constexpr (RELOAD) {
+          ReadWork(sh, (segment - 1) & 3, w);
+          tok0 = w.q0 + (w.turns ? 0 : i * A.TB);
+          mine = token < w.Tokens(i);
+          busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;
+        }
+      };
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int t = 0; t < w.Blocks(i); t++) {
+        again();
         const int b = blk.Index(i, t), seen = blk.Seen(i, b);
         bool cut;  // some row does not see all keys of a whole block
         bool gone0 = false, gone1 = false;  // trees: cache pages of the block that are not there
@@ -1245,6 +1399,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         MbarArrive(&sh->p_full[i]);
       }
       // ---- the rows' results ----
+      again();
       done += w.Blocks(i);
       const bool merge = TREE && w.turns == kTurns && w.blocks1 > 0;
       if (w.Blocks(i) > 0) ok = TaWait(sh, &sh->o_full[i], (i ? outs1 : outs0) & 1) && ok;
@@ -1294,7 +1449,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
         }
         if (busy) {
           TcgenFenceAfter();
-          const bool parts = RANGES && w.part >= 0;
+          const bool parts = (RANGES || SPLIT) && w.part >= 0;
           if (!parts) {
             const float inv = m != -INFINITY ? 1.f / l : l == 0.f ? 0.f : NAN;  // nothing seen: 0
             a0 *= inv;
@@ -1306,7 +1461,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
           uint16_t* out = A.out + (long long)(w.start + node) * A.out_row + (long long)((w.head + (w.turns == kHeads ? i : 0)) * A.G + g) * A.out_head;
           const long long slot = parts ? (long long)w.part * A.part_rows + (node - w.q0) * A.G + g : 0;
           // 16 columns at a time, 8 where registers are few
-          constexpr int kCols = Cfg::kWide || !TREE ? 16 : 8;
+          constexpr int kCols = Cfg::kWide || !TREE || CHUNK ? 16 : 8;
           const auto columns = [](uint32_t addr, uint32_t* v) {
             if constexpr (kCols == 16) TmemLoad16(addr, v);
             else TmemLoad8(addr, v);
@@ -1344,12 +1499,26 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       outs0 += w.blocks0 > 0;
       outs1 += w.blocks1 > 0;
       merges += merge;
+      if constexpr (RELOAD) {  // only now the place may be written again
+        __syncwarp();
+        if (lane == 0) MbarArrive(&sh->work_read[(segment - 1) & 3]);
+      }
     }
   }
   TcgenFenceBefore();
   __syncthreads();
   TcgenFenceAfter();
   if (warp == 8) TmemDealloc(tmem, Cfg::kCols);
+  if constexpr (SPLIT) {
+    if (w.more < 2) return;  // the whole cluster: one block of threads has it all
+    ClusterSync();           // all parts are written
+    if (warp < 8) {          // (at head_dim 128 the others have given registers away)
+      const int tokens = min(w.nodes - w.q0, 2 * A.TB), rank = blockIdx.x % A.split;
+      constexpr int kGroup = 128 / D;
+      for (int local = (rank * 8 + warp) * kGroup; local < tokens * A.G; local += A.split * 8 * kGroup)
+        JoinRows<D, F16, 1, 8>(A, (int)blockIdx.x - rank, false, w.more, local, tokens * A.G, w.start + w.q0, w.head);
+    }
+  }
 }
 
 // Joins the parts of a tree call's rows: one warp per (row, query head), D / 32 values per lane. Rows whose tile pair was not
@@ -1396,37 +1565,16 @@ __global__ void __launch_bounds__(256) TreeJoinKernel(const __grid_constant__ Ta
 }
 
 // Joins the parts of a chunk call's rows that a range cuts: for block of threads c of the attention the pair that it begins and does not
-// end, one warp per (row, query head), D / 32 values per lane.
+// end. (A row a warp took 17 to 30 us for the cuts of 296 ranges: 75 thousand rows in eight rounds of latency.)
+template <int D>
+constexpr int kJoinRows = 8 * 4 * 128 / D;  // of a block of threads
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) ChunkJoinKernel(const __grid_constant__ TaArgs A) {
   GridDepWait();
-  const int warps = (A.part_rows + 7) / 8, c = blockIdx.x / warps, local = (blockIdx.x - c * warps) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int blocks = (A.part_rows + kJoinRows<D> - 1) / kJoinRows<D>, c = blockIdx.x / blocks;
+  const int local = (blockIdx.x - c * blocks) * kJoinRows<D> + (threadIdx.x >> 5) * (kJoinRows<D> / 8);
   const int4 cut = A.cuts[c];
-  if (local >= cut.z * A.G) return;
-  const int token = local / A.G, g = local - token * A.G;
-  // the block of threads that begins the pair holds its part in its second place, the others in their first
-  const auto slot = [&](int k) { return (long long)(2 * (c + k) + (k == 0 ? 1 : 0)) * A.part_rows + local; };
-  float m = -INFINITY;
-  for (int k = 0; k < cut.w; k++) m = fmaxf(m, A.part_ml[slot(k)].x);
-  float l = 0.f, v[D / 32] = {};
-#pragma unroll 2
-  for (int k = 0; k < cut.w; k++) {
-    const float2 ml = A.part_ml[slot(k)];
-    const float a = m == -INFINITY ? 1.f : Exp2(ml.x - m);
-    l = fmaf(ml.y, a, l);
-    const float* o = A.part_o + slot(k) * D + lane * (D / 32);
-#pragma unroll
-    for (int j = 0; j < D / 32; j++) v[j] = fmaf(o[j], a, v[j]);
-  }
-  // a part whose maximum is NaN has a sum of NaN, which this sum takes over
-  const float inv = m != -INFINITY ? 1.f / l : NAN;
-  const bool zero = m == -INFINITY && l == 0.f;
-  uint16_t* out = A.out + (long long)(cut.x + token) * A.out_row + (long long)(cut.y * A.G + g) * A.out_head + lane * (D / 32);
-#pragma unroll
-  for (int j = 0; j < D / 32; j++) {
-    const float x = zero ? 0.f : v[j] * inv;
-    out[j] = (uint16_t)Pack2<F16>(x, 0.f);
-  }
+  if (local < cut.z * A.G) JoinRows<D, F16, 4, 2>(A, c, true, cut.w, local, cut.z * A.G, cut.x, cut.y);
 }
 
 }  // namespace shahd

@@ -443,6 +443,37 @@ def test_chunk_attention_many_sequences(n, heads, most_rows, most):
     _check_chunk(q, pool, table, lengths, rows, _chunk(q, cache, lengths, rows, BF16, max_rows=5000), BF16, seqs=set(rng.integers(0, n, 9).tolist()))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("lengths,rows", [
+    ([0, 1, 63, 64, 65, 127, 128, 129], [1, 1, 1, 1, 1, 1, 1, 1]), ([0, 0, 700, 5, 130], [3, 1, 17, 0, 64]), ([100, 900, 0, 64], [1, 260, 513, 1]),
+    ([0], [1]), ([0, 300, 0], [0, 2, 0]), ([5000], [3]), ([3000, 17, 2000], [1, 1, 130]),
+], ids=str)
+def test_chunk_attention_short_lengths_in_a_long_table(dtype, heads, lengths, rows):
+    """Room for 2000 pages a sequence: the work goes in ranges, which cut pairs where they like."""
+    q, pool, table, cache = _chunk_case(_gen(17), lengths, rows, heads, dtype)
+    wide = torch.cat([table, torch.full((len(rows), 2000 - table.shape[1]), 2**31 - 1, dtype=torch.int32, device="cuda")], 1)
+    cache = pkg.KvCache(cache.pool, cache.page_stride, wide.data_ptr(), 2000, cache.pages, heads[1], heads[2])
+    out = _chunk(q, cache, lengths, rows, dtype)
+    _check_chunk(q, pool, table, lengths, rows, out, dtype)
+    assert bool((out[sum(rows):] == 7.0).all())
+    assert torch.equal(out, _chunk(q, cache, lengths, rows, dtype))
+
+
+@pytest.mark.parametrize("heads", [(4, 4, 64), (10, 2, 32), (16, 4, 128), (7, 1, 128), (6, 2, 64)], ids=str)
+@pytest.mark.parametrize("blocks", [None, 2000])
+def test_chunk_attention_ranges_over_many_pairs(heads, blocks):
+    """Rows that make several pairs a sequence, of which the last has one tile or two: whole tables and wide ones."""
+    rng = np.random.default_rng(heads[0])
+    rows = [1, 700, 33, 0, 512, 2, 190, 65, 1, 1, 300]
+    lengths = rng.integers(0, 2500, len(rows)).tolist()
+    q, pool, table, cache = _chunk_case(_gen(18), lengths, rows, heads, BF16, spread=1)
+    if blocks:
+        table = torch.cat([table, torch.full((len(rows), blocks - table.shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+        cache = pkg.KvCache(cache.pool, cache.page_stride, table.data_ptr(), blocks, cache.pages, heads[1], heads[2])
+    _check_chunk(q, pool, table, lengths, rows, _chunk(q, cache, lengths, rows, BF16), BF16)
+
+
 @pytest.mark.parametrize("heads", [(4, 4, 64), (16, 4, 128), (10, 2, 32)], ids=str)
 def test_chunk_attention_pages_that_are_not_there(heads):
     g, lengths, rows = _gen(21), [300, 0, 64, 500], [70, 40, 1, 200]

@@ -52,7 +52,13 @@ def test_chunk_calls():
     _refused("too many rows or key blocks", pkg.chunk_attention_workspace, 100, 10**6, 10**6, 2, pkg.KvCache(AT, PAGE, AT, 1 << 24, 9, 2, 64))
     call(**{**ok, "n": 0})
     call(**{**ok, "rows": 0})
-    assert pkg.chunk_attention_workspace(256, 256, 1, 8, CACHE) > 0 and pkg.chunk_attention_workspace(0, 0, 1, 8, CACHE) >= 0
+    # a block of threads for every pair of tiles where there are many, or enough over short caches: no workspace
+    wide = lambda blocks: pkg.KvCache(AT, PAGE, AT, blocks, 9, 2, 64)  # noqa: E731
+    assert pkg.chunk_attention_workspace(256, 256, 1, 8, wide(9)) == 0 and pkg.chunk_attention_workspace(256, 256, 1, 8, wide(900)) > 0
+    assert pkg.chunk_attention_workspace(1000, 1000, 1, 8, wide(900)) == 0
+    # a few pairs: clusters share them, ranges where that leaves too many steps
+    assert 0 < pkg.chunk_attention_workspace(1, 64, 64, 8, wide(30)) != pkg.chunk_attention_workspace(1, 64, 64, 8, wide(3000))
+    assert pkg.chunk_attention_workspace(0, 0, 1, 8, CACHE) >= 0
 
 
 def test_head_norms():
