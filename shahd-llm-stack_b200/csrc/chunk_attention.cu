@@ -34,10 +34,13 @@ void LaunchChunks(const TaArgs& a, unsigned blocks, cudaStream_t st) {
 //   Ranges: as many blocks of threads as run at once take ranges of equal cost out of the line of all pairs, and what a range cuts is joined
 //     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 167 us, pairs 219, split in
 //     two 219; 2 chunks of 1024 over 12000, 32/8 heads of 128: 440 and 510. The second kernel and the parts cost about eight steps.
+// Pairs go longest first over all kv heads; where the keys and values do not fit the L2 cache, head after head, so that the blocks of threads that
+// run at a time read the same ones (4 chunks of 1500 to 2048 rows over 10 to 24 thousand positions, 32/8 heads of 128, 427 MB: 2820 us and
+// 2511; but 2 of 7000 to 8192 from position 0, 16/2 heads of 128, 16 MB: 467 and 513).
 // The lengths lie on the device, so the table's width stands for them, and a table much wider than its sequences are long may get the
 // layout for longer ones.
 struct ChunkLayout {
-  int least, part_rows, two_heads, split;
+  int least, part_rows, two_heads, split, by_heads;
   long long grid;
   int64_t cut_bytes, bytes;
 };
@@ -78,6 +81,7 @@ int LayChunks(const char* op, const ShahdChunkCall* c, ChunkLayout* out) {
     l.bytes = l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
   } else {  // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge
     l.two_heads = c->max_rows <= span / 2 && Hk % 2 == 0;
+    l.by_heads = (double)c->n * c->cache.max_blocks * kOpsPage * Hk * 2 * d * 2 > 126e6;
     l.grid = l.two_heads ? places * Hk / 2 : places * Hk;
   }
   *out = l;
@@ -160,6 +164,7 @@ int shahd_chunk_attention(const ShahdChunkCall* c, void* stream) {
   a.least = lay.least;
   a.two_heads = lay.two_heads;
   a.split = lay.split;
+  a.by_heads = lay.by_heads;
   if (lay.bytes > 0) {
     a.part_rows = lay.part_rows;
     a.cuts = static_cast<int4*>(c->workspace);

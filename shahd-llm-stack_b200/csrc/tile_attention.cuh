@@ -82,6 +82,7 @@ struct TaArgs {
   const unsigned long long* masks;
   const int* lengths;
   const int* table;
+  int by_heads;  // chunks: one kv head's pairs after another's
   int max_blocks, pages, max_nodes, pairs, split, two_heads;  // split: blocks of threads that share a pair; two_heads: the pair's tiles are those of two kv heads
   // All key blocks of all tile pairs in one line, dealt out to the blocks of threads in ranges of equal length, at least
   // `least`: 0 where every pair has a block of threads of its own instead. A pair that a range cuts leaves parts: block of threads c
@@ -871,7 +872,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
   // The softmax warps read what they work on from shared memory at every step instead of holding it in registers, which two blocks of
   // threads on a multiprocessor do not have: the steps of 64 keys are a chain of latencies, and what is spilled lengthens it.
-  constexpr bool RELOAD = KIND == kChunkRanges && !TaCfg<D>::kWide;
+  constexpr bool RELOAD = CHUNK && RANGES != TaCfg<D>::kWide;
   extern __shared__ uint8_t ta_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = base;
@@ -891,8 +892,9 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   } else if constexpr (KIND == kChunkPairs || SPLIT) {
     if (warp == 9) {
       const int heads = A.two_heads ? A.Hk / 2 : A.Hk, split = SPLIT ? A.split : 1, tile = blockIdx.x / split;
-      if (!ChunkWork<KEYS>(A, tile / heads, gridDim.x / split / heads, split, blockIdx.x - tile * split, w)) w.nodes = 0;
-      w.head = tile % heads * (A.two_heads ? 2 : 1);
+      const int places = gridDim.x / split / heads, head = A.by_heads ? tile / places : tile % heads;
+      if (!ChunkWork<KEYS>(A, A.by_heads ? tile - head * places : tile / heads, places, split, blockIdx.x - tile * split, w)) w.nodes = 0;
+      w.head = head * (A.two_heads ? 2 : 1);
       if (lane == 0) PutWork(sh, 0, w);
     }
   } else if constexpr (TREE) {
@@ -1250,7 +1252,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       bool busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;  // some row of this warp is in use
       const auto again = [&]() {
         if constexpr (RELOAD) {
-          ReadWork(sh, (segment - 1) & 3, w);
+          ReadWork(sh, RANGES ? (segment - 1) & 3 : 0, w);
           tok0 = w.q0 + (w.turns ? 0 : i * A.TB);
           mine = token < w.Tokens(i);
           busy = ((warp & 3) << 5) < w.Tokens(i) * A.G;
@@ -1499,7 +1501,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
       outs0 += w.blocks0 > 0;
       outs1 += w.blocks1 > 0;
       merges += merge;
-      if constexpr (RELOAD) {  // only now the place may be written again
+      if constexpr (RELOAD && RANGES) {  // only now the place may be written again
         __syncwarp();
         if (lane == 0) MbarArrive(&sh->work_read[(segment - 1) & 3]);
       }
