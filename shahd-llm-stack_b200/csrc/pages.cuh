@@ -8,8 +8,10 @@
 //     one: so no copy reads what another one writes.
 // Compact: of U held pages those numbered U and up move into the holes below U, both in ascending order.
 //
-// The numbers are found by one cluster of blocks of threads in a few steps (mark, look through, deal out) with cluster barriers
-// between them: latency. The copies are bound by memory, in a second kernel over all multiprocessors.
+// The numbers are found in a few steps (mark, look through, deal out): latency. Up to 32768 pages and table entries one block of threads does it,
+// with all that it keeps in shared memory; larger ones take a cluster of blocks of threads with cluster barriers between the steps
+// and the workspace for what is kept (32 beams over 320 pages, copies included: 6.4 us, as a cluster 10.5; 256 sequences, 4200 pages: 12.2 and 15.7). The copies are bound by memory, in a second kernel over all
+// multiprocessors.
 #pragma once
 
 #include "rows.cuh"
@@ -21,7 +23,7 @@ constexpr int kPagesCluster = 8;
 constexpr int kCopyThreads = 256;
 
 struct PageCopy {
-  int from, to, lines;  // lines: positions of the page; 0: nothing to copy
+  int from, to, lines;  // lines: positions of the page; 0: nothing to copy (to = -1: there was no page for it)
 };
 
 struct PagesArgs {
@@ -32,7 +34,7 @@ struct PagesArgs {
   uint32_t *held, *read;  // bits of pages
   int* first;             // [pages] fork: the first new sequence that would write into a page; compact: where a page goes
   int* order;             // [pages] fork: free pages in order; compact: the holes
-  int* start;             // [new_n] fork: number of the first fresh page of a new sequence
+  int* start;             // [new_n] fork: number of the first fresh page of a new sequence, in `order`
   int* count;             // [2] fork: free pages; compact: held pages, pages that move
   PageCopy* copies;       // [new_n], or [pages]
 };
@@ -180,44 +182,168 @@ __global__ void __launch_bounds__(kPagesThreads) PlanPagesKernel(const __grid_co
   }
   ClusterSync();
   GridDepLaunch();
-  // ---- the new tables and what is to be copied ----
+  // ---- what is to be copied ----
   if constexpr (FORK) {
     const int free = __ldcg(a.count);
-    const auto fresh = [&](int k) { return k < free ? __ldcg(&a.order[k]) : -1; };
-    for (long long e = t; e < new_entries; e += all) {
-      const int i = (int)(e / a.max_blocks), b = (int)(e - (long long)i * a.max_blocks);
+    for (int i = t; i < a.new_n; i += all) {
       const Fork f(a, i);
       const bool copies = Copies(a, i, f);
-      const int start = __ldcg(&a.start[i]);
-      int page = -1;
-      if (b < f.kept - (copies ? 1 : 0)) page = a.table[(long long)f.parent * a.max_blocks + b];
-      else if (b < f.kept) page = fresh(start);
-      else if (b < f.upto) page = fresh(start + (copies ? 1 : 0) + b - f.kept);
-      a.new_table[e] = page;
-      if (b == 0) {
-        const int wants = f.upto - f.kept + (copies ? 1 : 0);
-        a.missing[i] = wants - min(max(free - start, 0), wants) + f.beyond;
-        const int to = copies ? fresh(start) : -1;
-        a.copies[i] = to >= 0 ? PageCopy{a.table[(long long)f.parent * a.max_blocks + f.kept - 1], to, f.keep % kOpsPage} : PageCopy{0, 0, 0};
+      const int start = __ldcg(&a.start[i]), wants = f.upto - f.kept + (copies ? 1 : 0);
+      a.missing[i] = wants - min(max(free - start, 0), wants) + f.beyond;
+      PageCopy c = {0, 0, 0};
+      if (copies) {
+        if (start < free) c = {a.table[(long long)f.parent * a.max_blocks + f.kept - 1], __ldcg(&a.order[start]), f.keep % kOpsPage};
+        else c.to = -1;
       }
+      a.copies[i] = c;
     }
   } else {
-    const int used = __ldcg(&a.count[0]), moved = __ldcg(&a.count[1]);
+    const int moved = __ldcg(&a.count[1]);
     for (int m = t; m < moved; m += all) {
       const int to = __ldcg(&a.order[m]), from = __ldcg(&a.copies[m].from);
       a.copies[m].to = to;
       a.first[from] = to;
     }
-    ClusterSync();
-    for (long long e = t; e < old_entries; e += all) {
-      const int s = (int)(e / a.max_blocks), b = (int)(e - (long long)s * a.max_blocks);
-      int page = -1;
-      if (b < Blocks(min(max(a.lengths[s], 0), a.max_blocks * kOpsPage))) {
-        page = a.table[e];
-        if ((unsigned)page >= (unsigned)a.pages) page = -1;
-        else if (page >= used) page = __ldcg(&a.first[page]);
+  }
+}
+
+constexpr int kPagesSmall = 32768;  // pages, and entries of either table, that one block of threads sees to
+constexpr int kPagesSmallRows = 1024;
+
+// What one block of threads holds in shared memory.
+struct PagesShared {
+  uint32_t held[kPagesSmall / 32], read[kPagesSmall / 32];
+  int ahead[kPagesSmall / 32];  // free pages before a word's; compact: holes below U
+  int4 rows[kPagesSmallRows];   // fork: of the new sequences the parent's place in the table, whether it goes on in a page, kept blocks, blocks to have
+  int start[kPagesSmall / 32];  // compact: rank of a word's first held page among those that move
+  int warps[32];
+  int first[1];                 // [pages] fork: the first new sequence that would write into a page
+};
+
+// The k-th (from 0) set bit of `bits`.
+__device__ __forceinline__ int NthBit(uint32_t bits, int k) {
+  int at = 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const int below = __popc(bits & ((1u << o) - 1));
+    if (k >= below) {
+      k -= below;
+      bits >>= o;
+      at += o;
+    }
+  }
+  return at;
+}
+
+// The k-th free page; there is one. ahead: of `words` words of pages.
+__device__ __forceinline__ int NthFree(const PagesShared& s, int words, int k) {
+  int lo = 0, hi = words;  // ahead[lo] <= k
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s.ahead[mid] <= k) lo = mid;
+    else hi = mid;
+  }
+  return lo * 32 + NthBit(~s.held[lo], k - s.ahead[lo]);
+}
+
+template <bool FORK>
+__global__ void __launch_bounds__(kPagesThreads) PlanPagesSmallKernel(const __grid_constant__ PagesArgs a) {
+  extern __shared__ __align__(16) uint8_t pages_raw[];
+  PagesShared& s = *reinterpret_cast<PagesShared*>(pages_raw);
+  const int t = threadIdx.x, most = a.max_blocks * kOpsPage, old_entries = a.n * a.max_blocks, new_entries = a.new_n * a.max_blocks;
+  const float per = 1.f / (float)a.max_blocks;
+  // e / max_blocks, exact for e below 2^21: (e + 1/2) / max_blocks is further from whole numbers than its rounding
+  const auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * per); };
+  for (int w = t; w < a.words; w += kPagesThreads) s.held[w] = s.read[w] = 0;
+  if (FORK)
+    for (int p = t; p < a.pages; p += kPagesThreads) s.first[p] = 0x7fffffff;
+  GridDepWait();
+  int4 mine = make_int4(0, 0, 0, 0);  // fork: of new sequence t
+  bool writes = false;
+  int keep = 0, beyond = 0;
+  if (FORK && t < a.new_n) {
+    const Fork f(a, t);
+    writes = f.writes;
+    keep = f.keep;
+    beyond = f.beyond;
+    mine = make_int4(f.parent * a.max_blocks, writes, f.kept, f.upto);
+    s.rows[t] = mine;
+  }
+  __syncthreads();
+  // ---- which pages are held, and which of them somebody reads without writing ----
+#pragma unroll 4
+  for (int e = t; e < old_entries; e += kPagesThreads) {
+    const int q = row_of(e), b = e - q * a.max_blocks, page = a.table[e];
+    if (b < Blocks(min(max(a.lengths[q], 0), most)) && (unsigned)page < (unsigned)a.pages) atomicOr(&s.held[page >> 5], 1u << (page & 31));
+  }
+  if constexpr (FORK) {
+#pragma unroll 4
+    for (int e = t; e < new_entries; e += kPagesThreads) {
+      const int i = row_of(e), b = e - i * a.max_blocks;
+      const int4 f = s.rows[i];
+      if (b >= f.z) continue;
+      const int page = a.table[f.x + b];
+      if ((unsigned)page >= (unsigned)a.pages) continue;
+      if (f.y && b == f.z - 1) atomicMin(&s.first[page], i);
+      else atomicOr(&s.read[page >> 5], 1u << (page & 31));
+    }
+  }
+  __syncthreads();
+  // ---- free pages in order; what the new sequences want of them, and what is to be copied ----
+  uint32_t bits = 0, there = 0;
+  if (t < a.words) {
+    bits = s.held[t];
+    there = a.pages - 32 * t < 32 ? (1u << (a.pages - 32 * t)) - 1 : 0xffffffffu;
+  }
+  int free = 0, used = 0;
+  if constexpr (!FORK) {
+    BlockScan(__popc(bits), s.warps, used);
+    const int base = 32 * t;  // holes: free pages below U
+    there = used <= base ? 0 : used - base < 32 ? there & ((1u << (used - base)) - 1) : there;
+  }
+  const int ahead = BlockScan(__popc(~bits & there), s.warps, free);
+  if (t < a.words) s.ahead[t] = ahead;
+  if constexpr (FORK) {
+    int page = -1;
+    if (writes) page = a.table[mine.x + mine.z - 1];
+    const bool copy = writes && (unsigned)page < (unsigned)a.pages && ((s.read[page >> 5] >> (page & 31) & 1) != 0 || s.first[page] != t);
+    const int wants = mine.w - mine.z + (copy ? 1 : 0);
+    int total = 0;
+    const int start = BlockScan(wants, s.warps, total);  // (s.ahead is there behind its barriers)
+    GridDepLaunch();
+    if (t < a.new_n) {
+      a.start[t] = start;
+      a.missing[t] = wants - min(max(free - start, 0), wants) + beyond;
+      PageCopy c = {0, 0, 0};
+      if (copy) {
+        if (start < free) c = {page, NthFree(s, a.words, start), keep % kOpsPage};
+        else c.to = -1;
       }
-      a.new_table[e] = page;
+      a.copies[t] = c;
+    }
+    if (t == 0) a.count[0] = free;
+    // the free pages that are wanted, in order
+    uint32_t left = ~bits & there;
+    for (int k = ahead; left != 0 && k < total; left &= left - 1) a.order[k++] = 32 * t + __ffs(left) - 1;
+  } else {
+    // held pages from U on, by their rank among them: those in front of each word (the word that U lies in has some below U, too)
+    const uint32_t behind = t < a.words ? bits & ~there : 0;
+    int all = 0;
+    const int rank = BlockScan(__popc(behind), s.warps, all);
+    if (t < a.words) s.start[t] = rank - __popc(bits & there);
+    __syncthreads();
+    GridDepLaunch();
+    if (t == 0) {
+      a.count[0] = used;
+      a.count[1] = free;  // as many pages move as there are holes
+      *a.used = used;
+    }
+    for (int p = used + t; p < a.pages; p += kPagesThreads) {
+      const int w = p >> 5;
+      if (!(s.held[w] >> (p & 31) & 1)) continue;
+      const int m = s.start[w] + __popc(s.held[w] & ((1u << (p & 31)) - 1)), to = NthFree(s, a.words, m);
+      a.copies[m] = PageCopy{p, to, kOpsPage};
+      a.first[p] = to;
     }
   }
 }
@@ -231,10 +357,32 @@ struct CopyArgs {
   int most, split;   // split: blocks of threads that share a layer of a copy
 };
 
-// Copies the first `lines` positions of every part of a page.
-__global__ void __launch_bounds__(kCopyThreads) CopyPagesKernel(const __grid_constant__ CopyArgs a) {
+// The entries of the new tables, and copies of the first `lines` positions of every part of a page.
+template <bool FORK>
+__global__ void __launch_bounds__(kCopyThreads) CopyPagesKernel(const __grid_constant__ CopyArgs a, const __grid_constant__ PagesArgs p) {
   GridDepWait();
   GridDepLaunch();
+  const long long entries = (long long)(FORK ? p.new_n : p.n) * p.max_blocks;
+  for (long long e = (long long)blockIdx.x * kCopyThreads + threadIdx.x; e < entries; e += (long long)gridDim.x * kCopyThreads) {
+    const int i = (int)(e / p.max_blocks), b = (int)(e - (long long)i * p.max_blocks);
+    int page = -1;
+    if constexpr (FORK) {
+      const Fork f(p, i);
+      const PageCopy c = p.copies[i];
+      const int copies = c.lines != 0 || c.to < 0;
+      if (b < f.kept - copies) page = p.table[(long long)f.parent * p.max_blocks + b];
+      else if (b < f.kept) page = c.to;
+      else if (b < f.upto) {
+        const int k = p.start[i] + copies + b - f.kept;
+        if (k < p.count[0]) page = p.order[k];
+      }
+    } else if (b < Blocks(min(max(p.lengths[i], 0), p.max_blocks * kOpsPage))) {
+      page = p.table[e];
+      if ((unsigned)page >= (unsigned)p.pages) page = -1;
+      else if (page >= p.count[0]) page = p.first[page];
+    }
+    p.new_table[e] = page;
+  }
   const long long items = (long long)(a.count ? *a.count : a.most) * a.layers * a.split;
   const int row16 = a.d / 8;  // 16-byte pieces of a position
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
@@ -336,11 +484,18 @@ int LaunchPages(const char* op, const ShahdPagePool& pool, PagesArgs a, void* wo
   c.copies = a.copies;
   c.count = FORK ? nullptr : a.count + 1;
   c.most = FORK ? a.new_n : a.pages;
-  c.split = std::max(1, c.parts * c.d * 8 / (4 * kCopyThreads * 4));  // 64 KiB of a layer at most
+  c.split = 1;  // a layer of a page is shared by blocks of threads down to 16 KiB, while there are few
+  while (c.split * 1024 < c.parts * c.d * 8 && (long long)c.most * c.layers * c.split < 4 * sms) c.split *= 2;
   TakeLaunchError(nullptr);
-  LaunchPdlCluster(PlanPagesKernel<FORK>, dim3(kPagesCluster), dim3(kPagesThreads), 0, dim3(kPagesCluster), st, a);
+  if (a.pages <= kPagesSmall && std::max(a.n, a.new_n) * (long long)a.max_blocks <= kPagesSmall && a.new_n <= kPagesSmallRows) {
+    const size_t smem = sizeof(PagesShared) + (FORK ? 4 * (size_t)a.pages : 0);
+    if (EnsureKernelAttrs((const void*)PlanPagesSmallKernel<FORK>, (int)smem)) LaunchPdl(PlanPagesSmallKernel<FORK>, dim3(1), dim3(kPagesThreads), smem, st, a);
+  } else {
+    LaunchPdlCluster(PlanPagesKernel<FORK>, dim3(kPagesCluster), dim3(kPagesThreads), 0, dim3(kPagesCluster), st, a);
+  }
   const long long items = (long long)c.most * c.layers * c.split;
-  LaunchPdl(CopyPagesKernel, dim3((unsigned)std::min<long long>(items, 8LL * sms)), dim3(kCopyThreads), 0, st, c);
+  const long long entries = (long long)(FORK ? a.new_n : a.n) * a.max_blocks;
+  LaunchPdl(CopyPagesKernel<FORK>, dim3((unsigned)std::min<long long>(std::max(items, entries / kCopyThreads + 1), 8LL * sms)), dim3(kCopyThreads), 0, st, c, a);
   return LaunchStatus(op);
 }
 
