@@ -60,6 +60,21 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
     j0 += half;
     apart = d / 2 - half;
   }
+  // The next heads' values are on their way while these are worked on, from one operand to the next and from a row to the next.
+  Raw8<T> na[kDeep], nb[kDeep];
+  const auto load = [&](const RopeOperand& o, long long r, int h) {
+    const T* in = static_cast<const T*>(o.in) + r * o.in_row + j0;
+#pragma unroll
+    for (int k = 0; k < kDeep; k++) {
+      const int hk = h + n0 + k * lanes;
+      if (hk < o.heads) {
+        na[k].Load(in + hk * o.in_head);
+        if (MODE == kNormHalf) nb[k].Load(in + hk * o.in_head + apart);
+      }
+    }
+  };
+  const RopeOperand& begin = a.q.heads > 0 ? a.q : a.k;  // the first operand
+  long long loaded = -1;                                 // the row whose first heads have been asked for
   const int first = a.offsets ? a.offsets[0] : 0, end = a.offsets ? a.offsets[a.n] : a.rows;
   const long long step = (long long)gridDim.x * (blockDim.x >> 5);
   long long row = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
@@ -68,6 +83,7 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
     const int p = next;
     next = row + step < a.rows ? a.positions[row + step] : -1;  // ahead of this row's values
     if (p < 0 || row < first || row >= end) continue;
+    if (MODE != kNormValues && loaded != row) load(begin, row, 0);
     long long at = -1;  // the row's place in the cache (kv head 0, K)
     if (a.pool && (p >> 6) < a.max_blocks) {
       const int page = a.table[(long long)SequenceOf(a.offsets, a.n, (int)row) * a.max_blocks + (p >> 6)];
@@ -170,8 +186,7 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
         for (int q = 0; q < kPer / 2; q++) cs[q] = from[q * (half / kPer)];
       }
       // one operand's heads; kv: 0 for keys, 1 for values, -1 for queries
-      const auto heads = [&](const RopeOperand& o, int kv) {
-        const T* in = static_cast<const T*>(o.in) + row * o.in_row + j0;
+      const auto heads = [&](const RopeOperand& o, int kv, const RopeOperand& then, long long then_row) {
         T* out = o.out ? static_cast<T*>(o.out) + row * o.out_row + j0 : nullptr;
         C* cache = kv >= 0 && at >= 0 ? reinterpret_cast<C*>(a.pool) + at + (long long)kv * kOpsPage * d + j0 : nullptr;
         const float *w = weights[kv < 0 ? 0 : 1] + j0, *b = biases[kv < 0 ? 0 : 1] + j0;
@@ -181,12 +196,11 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
           Raw8<T> ra[kDeep], rb[kDeep];
 #pragma unroll
           for (int k = 0; k < kDeep; k++) {
-            const int hk = h + n0 + k * lanes;
-            if (hk < o.heads) {
-              ra[k].Load(in + hk * o.in_head);
-              if (MODE == kNormHalf) rb[k].Load(in + hk * o.in_head + apart);
-            }
+            ra[k] = na[k];
+            if (MODE == kNormHalf) rb[k] = nb[k];
           }
+          if (h + kDeep * lanes < o.heads) load(o, row, h + kDeep * lanes);
+          else load(then, then_row, 0);
           float mu[kDeep], scale[kDeep];
           if (kv != 1) {
             const auto all = [&](float (&s)[kDeep]) {  // sums over the lanes of a head
@@ -222,11 +236,11 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
               float x[8];
               ra[k].Get(x);
 #pragma unroll
-              for (int i = 0; i < 8; i++) scale[k] = fmaf(x[i] - mu[k], x[i] - mu[k], scale[k]);
+              for (int i = 0; i < 8; i++) scale[k] = LAYER ? fmaf(x[i] - mu[k], x[i] - mu[k], scale[k]) : fmaf(x[i], x[i], scale[k]);
               if (MODE == kNormHalf) {
                 rb[k].Get(x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) scale[k] = fmaf(x[i] - mu[k], x[i] - mu[k], scale[k]);
+                for (int i = 0; i < 8; i++) scale[k] = LAYER ? fmaf(x[i] - mu[k], x[i] - mu[k], scale[k]) : fmaf(x[i], x[i], scale[k]);
               }
             }
             all(scale);
@@ -238,10 +252,10 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
             for (int i = 0; i < 8; i += 4) {
               const float4 wv = *reinterpret_cast<const float4*>(w + from + i);
               const float4 bv = LAYER ? *reinterpret_cast<const float4*>(b + from + i) : make_float4(0, 0, 0, 0);
-              x[i] = fmaf((x[i] - mu[k]) * scale[k], wv.x, bv.x);
-              x[i + 1] = fmaf((x[i + 1] - mu[k]) * scale[k], wv.y, bv.y);
-              x[i + 2] = fmaf((x[i + 2] - mu[k]) * scale[k], wv.z, bv.z);
-              x[i + 3] = fmaf((x[i + 3] - mu[k]) * scale[k], wv.w, bv.w);
+              x[i] = LAYER ? fmaf((x[i] - mu[k]) * scale[k], wv.x, bv.x) : x[i] * scale[k] * wv.x;
+              x[i + 1] = LAYER ? fmaf((x[i + 1] - mu[k]) * scale[k], wv.y, bv.y) : x[i + 1] * scale[k] * wv.y;
+              x[i + 2] = LAYER ? fmaf((x[i + 2] - mu[k]) * scale[k], wv.z, bv.z) : x[i + 2] * scale[k] * wv.z;
+              x[i + 3] = LAYER ? fmaf((x[i + 3] - mu[k]) * scale[k], wv.w, bv.w) : x[i + 3] * scale[k] * wv.w;
             }
           };
           if constexpr (MODE == kNormStaged) {
@@ -309,9 +323,12 @@ __global__ void __launch_bounds__(kNormWarps * 32, 2) NormRopeKernel(const __gri
           }
         }
       };
-      heads(a.q, -1);
-      heads(a.k, 0);
-      heads(a.v, 1);
+      // (an operand that there is not has no heads: nothing is done and nothing loaded)
+      const long long next_row = next >= 0 && row + step < end ? row + step : row;  // no other rows are read
+      if (a.q.heads > 0) heads(a.q, -1, a.k.heads > 0 ? a.k : a.q, a.k.heads > 0 ? row : next_row);
+      if (a.k.heads > 0) heads(a.k, 0, a.v.heads > 0 ? a.v : begin, a.v.heads > 0 ? row : next_row);
+      if (a.v.heads > 0) heads(a.v, 1, begin, next_row);
+      loaded = next_row;
     }
   }
 }
