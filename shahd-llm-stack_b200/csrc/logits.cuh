@@ -3,12 +3,13 @@
 //   known: x > 0 ? x / repetition : x * repetition;  x -= c frequency + [c > 0] presence;  x += bias of v;  not allowed: -inf.
 // Formed in 32 bits, rounded once.
 //
-// Bound by memory: a row is read once and written once. A block of threads takes a slice of the tokens of a few rows into shared memory
-// (asynchronous copies), and while it comes counts the history's tokens of the slice there: whole numbers, so the order of the atomics
-// does not matter. Few tokens of a vocabulary are in a history or a list of biases: each warp looks through a part of the counts, makes a
-// list of those that are, and does what is to be done for its list; then the rows go out in 16-byte pieces as the masks leave them.
-// Rows of one sequence (drafted rows) share counts and lists. The history is read by every slice's block, from the cache but for the
-// first: 4 bytes a token, four a load where it is aligned.
+// Bound by memory, next to it by instructions: a row is read once and written once. A block of threads takes a slice of the tokens of a
+// few rows into shared memory (asynchronous copies). While it comes, each warp looks through a part of the history, puts the tokens that
+// lie in the slice on a list of its own, and counts them: whole numbers, so the order of the atomics does not matter. Behind a barrier
+// it takes its list's counts out of the table, which empties it, and does what is to be done for those that it found there:
+// of all that meet a token one. Then the rows go out in 16-byte pieces as the masks leave them. Rows of one sequence (drafted rows) share
+// counts and lists. The history is read by every slice's block, from the cache but for the first: 4 bytes a token, four a load where it
+// is aligned.
 #pragma once
 
 #include "rows.cuh"
@@ -19,7 +20,8 @@ constexpr int kLogThreads = 256;
 constexpr int kLogWarps = kLogThreads / 32;
 constexpr int kLogGroup = 4;     // rows of a block of threads, at most
 constexpr int kLogDeep = 3;      // loads of the history of a thread in flight
-constexpr int kLogTable = 4096;  // tokens of a slice's table, at most
+constexpr int kLogTable = 3968;  // tokens of a slice's table, at most: four blocks of threads on a multiprocessor, with four 16-bit rows each
+constexpr int kLogList = 384;    // tokens of a warp's list
 
 struct LogitsArgs {
   const void* in;
@@ -40,16 +42,25 @@ struct LogitsArgs {
   int mask_count;
 };
 
-// Two 16-bit or one 32-bit value, -inf where a token's bit is not set.
+// A piece with -inf where a token's bit is not set. Of 16-bit values a word's two bits are brought to the beginnings of its halves, and each
+// times 0xffff fills its half.
 template <class T>
-__device__ __forceinline__ uint32_t Masked(uint32_t u, uint32_t bits) {
+__device__ __forceinline__ uint4 Masked(const uint4& u, uint32_t bits) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t r[4];
   if constexpr (sizeof(T) == 4) {
-    return bits & 1 ? u : 0xff800000u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = bits >> i & 1 ? w[i] : 0xff800000u;
   } else {
-    constexpr uint32_t kLow = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
-    const uint32_t keep = (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
-    return (u & keep) | ((kLow << 16 | kLow) & ~keep);
+    constexpr uint32_t kLow = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    const uint32_t both = (bits & 0xffu) | bits << 15;  // the odd bits, 16 above the even ones that they go with
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t keep = (both >> 2 * i & 0x10001u) * 0xffffu;
+      r[i] = (w[i] & keep) | (kLow & ~keep);
+    }
   }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 // Cells of a table in shared memory: 32 bits, or 16, two of which share a word that atomics work on.
@@ -73,30 +84,20 @@ struct LogCells {
       }
     }
   }
-  // Which of the eight cells from t on are not 0.
-  __device__ __forceinline__ uint32_t Eight(int t) const {
-    uint32_t some = 0;
-#pragma unroll
-    for (int j = 0; j < (WIDE ? 2 : 1); j++) {
-      const uint4 u = reinterpret_cast<const uint4*>(at + t)[j];
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (WIDE) some |= (w[i] != 0 ? 1u : 0u) << (4 * j + i);
-        else some |= ((w[i] & 0xffffu) != 0 ? 1u << 2 * i : 0u) | (w[i] >> 16 != 0 ? 2u << 2 * i : 0u);
-      }
-    }
-    return some;
+  // What a cell holds, which is 0 after that.
+  __device__ __forceinline__ uint32_t Take(uint32_t t) const {
+    if constexpr (WIDE) return atomicExch(Word(t), 0u);
+    else return atomicAnd(Word(t), ~(0xffffu << Shift(t))) >> Shift(t) & 0xffffu;
   }
 };
 
-// A token's count: 2 x times generated + whether the prompt has it.
+// A token's count: 4 x times generated + 2 where it has a bias + 1 where the prompt has it.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __grid_constant__ LogitsArgs a) {
   typedef typename LogCells<WIDE>::Cell Cell;
   constexpr int PER = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t log_raw[];
-  __shared__ int seqs[kLogGroup], mask_rows[kLogGroup], lead[kLogGroup];  // lead: values between a 16-byte boundary and the row's beginning
+  __shared__ int overflow, seqs[kLogGroup], mask_rows[kLogGroup], lead[kLogGroup];  // lead: values between a 16-byte boundary and the row's beginning
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = blockIdx.x / a.slices * a.group, sl = blockIdx.x % a.slices, rows = min(a.group, a.rows - first);
   // Pieces begin at 16-byte boundaries, rows where they like: slices are whole pieces, and a row reaches up to PER - 1 tokens into the
@@ -106,13 +107,14 @@ __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __gri
   T* const held_rows = reinterpret_cast<T*>(log_raw);                                                         // [group][pitch]
   uint32_t* const held_masks = reinterpret_cast<uint32_t*>(log_raw + (size_t)a.group * pitch * sizeof(T));    // [group][mask_words]
   const LogCells<WIDE> table{reinterpret_cast<Cell*>(held_masks + (a.group * mask_words + 3) / 4 * 4)};
-  const LogCells<WIDE> entry{table.at + (counts ? a.table : 0)};  // place of a token's last entry + 1
-  uint16_t* const list = reinterpret_cast<uint16_t*>(entry.at + (biases ? a.table : 0)) + warp * 256;
+  const LogCells<WIDE> entry{table.at + a.table};  // place of a token's last entry + 1
+  uint16_t* const list = reinterpret_cast<uint16_t*>(entry.at + (biases ? a.table : 0)) + warp * kLogList;
   if (counts || biases)
     for (uint4* p = reinterpret_cast<uint4*>(table.at) + threadIdx.x; p < reinterpret_cast<uint4*>(entry.at + (biases ? a.table : 0)); p += kLogThreads)
       *p = make_uint4(0, 0, 0, 0);
   GridDepWait();
   GridDepLaunch();
+  if (threadIdx.x == 0) overflow = 0;
   if ((int)threadIdx.x < rows) {
     seqs[threadIdx.x] = a.seqs ? a.seqs[first + threadIdx.x] : first + (int)threadIdx.x;
     mask_rows[threadIdx.x] = a.mask_rows ? a.mask_rows[first + threadIdx.x] : first + (int)threadIdx.x;
@@ -146,16 +148,43 @@ __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __gri
     while (r < rows && seqs[r] == seq) r++;
     if ((unsigned)seq >= (unsigned)a.n) continue;
     // ---- the tokens that there are: the table is empty ----
+    int listed = 0;  // on the warp's list
+    const unsigned below = (1u << lane) - 1;
+    // All lanes: N tokens each are put on the list, those with a place in the table; false where they have not all room there.
+    const auto enlist = [&](auto n, const uint32_t* t, const uint32_t* flag) {
+      constexpr int N = decltype(n)::value;
+      unsigned who[N];
+      int all = 0;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        who[j] = __ballot_sync(0xffffffffu, t[j] < (uint32_t)a.table);
+        all += __popc(who[j]);
+      }
+      if (listed + all > kLogList) return false;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        if (t[j] < (uint32_t)a.table) list[listed + __popc(who[j] & below)] = (uint16_t)(t[j] | flag[j]);
+        listed += __popc(who[j]);
+      }
+      return true;
+    };
     int b0 = 0;
     if (biases) {
       b0 = min(max(a.bias_offsets[seq], 0), a.bias_entries);
       const int count = min(max(a.bias_offsets[seq + 1], b0), a.bias_entries) - b0;
-      for (int i = threadIdx.x; i < count; i += kLogThreads) {
+      for (int i0 = warp * 32; i0 < count; i0 += kLogThreads) {
+        const int i = i0 + lane;
         // in unsigned numbers, which wrap: any value may stand there
-        const uint32_t t = (uint32_t)a.bias_tokens[b0 + i] - (uint32_t)base;
-        if (t < (uint32_t)a.table) entry.Max(t, (uint32_t)i + 1u);
+        const uint32_t t = i < count ? (uint32_t)a.bias_tokens[b0 + i] - (uint32_t)base : 0xffffffffu;
+        if (t < (uint32_t)a.table) {
+          entry.Max(t, (uint32_t)i + 1u);
+          table.Or(t, 2);
+        }
+        const uint32_t none = 0;
+        if (!enlist(std::integral_constant<int, 1>(), &t, &none)) overflow = 1;
       }
     }
+    const int biased = listed;
     float rep = 1.f, inv = 1.f, freq = 0.f, pres = 0.f;
     if (counts) {
       const int* h = a.history + seq * a.history_stride;
@@ -164,79 +193,84 @@ __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __gri
       inv = 1.f / rep;  // a division for a row instead of one for a token: half a step more
       freq = a.frequency ? a.frequency[seq] : 0.f;
       pres = a.presence ? a.presence[seq] : 0.f;
-      const auto meet = [&](int token, int i) {
-        const uint32_t t = (uint32_t)token - (uint32_t)base;
-        if (t < (uint32_t)a.table) {
-          if (i < prompt) table.Or(t, 1);
-          else table.Add(t, 2);
+      const auto count = [&](uint32_t t, bool of_prompt) {
+        if (of_prompt) table.Or(t, 1);
+        else table.Add(t, 4);
+      };
+      constexpr uint32_t kPrompt = 0x8000u;
+      // four tokens a lane, from place i[j] of the history each (INT32_MIN is no token of any table)
+      const auto meet = [&](const int (&token)[4], const int (&i)[4]) {
+        uint32_t t[4], flag[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          t[j] = (uint32_t)token[j] - (uint32_t)base;
+          flag[j] = i[j] < prompt ? kPrompt : 0u;
         }
+        if (enlist(std::integral_constant<int, 4>(), t, flag)) return;
+        overflow = 1;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (t[j] < (uint32_t)a.table) count(t[j], flag[j] != 0);
       };
       const int fours = reinterpret_cast<uintptr_t>(h) % 16 == 0 ? length / 4 : 0;
 #pragma unroll 1
-      for (int i0 = threadIdx.x; i0 < fours; i0 += kLogDeep * kLogThreads) {
+      for (int i0 = warp * 32; i0 < fours; i0 += kLogDeep * kLogThreads) {
         int4 u[kLogDeep];
 #pragma unroll
-        for (int k = 0; k < kLogDeep; k++)
-          if (i0 + k * kLogThreads < fours) u[k] = reinterpret_cast<const int4*>(h)[i0 + k * kLogThreads];
+        for (int k = 0; k < kLogDeep; k++) {
+          const int i = i0 + k * kLogThreads + lane;
+          u[k] = i < fours ? reinterpret_cast<const int4*>(h)[i] : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+        }
 #pragma unroll
         for (int k = 0; k < kLogDeep; k++) {
-          const int i = i0 + k * kLogThreads;
-          if (i >= fours) break;
-          meet(u[k].x, 4 * i);
-          meet(u[k].y, 4 * i + 1);
-          meet(u[k].z, 4 * i + 2);
-          meet(u[k].w, 4 * i + 3);
+          if (i0 + k * kLogThreads >= fours) break;
+          const int i = 4 * (i0 + k * kLogThreads + lane);
+          meet({u[k].x, u[k].y, u[k].z, u[k].w}, {i, i + 1, i + 2, i + 3});
         }
       }
 #pragma unroll 1
-      for (int i0 = 4 * fours + (int)threadIdx.x; i0 < length; i0 += 4 * kLogThreads) {
-        int u[4];
+      for (int i0 = 4 * fours + warp * 32; i0 < length; i0 += 4 * kLogThreads) {
+        int u[4], i[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (i0 + k * kLogThreads < length) u[k] = h[i0 + k * kLogThreads];
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (i0 + k * kLogThreads < length) meet(u[k], i0 + k * kLogThreads);
+        for (int k = 0; k < 4; k++) {
+          i[k] = i0 + k * kLogThreads + lane;
+          u[k] = i[k] < length ? h[i[k]] : INT32_MIN;
+        }
+        meet(u, i);
       }
+      __syncwarp();
+      for (int i = biased + lane; i < listed; i += 32) count(list[i] & ~kPrompt, list[i] & kPrompt);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    // ---- this warp's part of them: tokens 256 k + .. of every kLogWarps-th k ----
-#pragma unroll 1
-    for (int t0 = warp * 256; t0 < a.table; t0 += kLogWarps * 256) {
-      const int t = t0 + 8 * lane;
-      uint32_t some = 0;  // bit j: token t + j is there
-      if (counts) some |= table.Eight(t);
-      if (biases) some |= entry.Eight(t);
-      int upto = __popc(some);  // of the lanes up to this one
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += u;
+    const auto adjust = [&](int t, uint32_t w) {
+      uint32_t e = 0;
+      if (w & 2) {
+        e = entry.at[t];
+        entry.at[t] = 0;
       }
-      const int listed = __shfl_sync(0xffffffffu, upto, 31);
-      int at = upto - __popc(some);
-      __syncwarp();  // the last list has been read
-      for (; some != 0; some &= some - 1) list[at++] = (uint16_t)(t + __ffs(some) - 1);
-      __syncwarp();
-#pragma unroll 1
-      for (int i = lane; i < listed; i += 32) {
-        const int t = list[i];
-        const uint32_t w = counts ? table.at[t] : 0, e = biases ? entry.at[t] : 0, times = w >> 1;
-        const float bias = e != 0 ? a.bias_values[b0 + (int)e - 1] : 0.f, fine = times != 0 ? fmaf((float)times, freq, pres) : 0.f;
-        for (int k = from; k < r; k++) {
-          T* at = held_rows + k * pitch + lead[k] + t;
-          float x = ToFloat(*at);
-          if (w != 0) x = x > 0.f ? x * inv : x * rep;
-          if (times != 0) x -= fine;
-          if (e != 0) x += bias;
-          *at = FromFloat<T>(x);
-        }
-        if (r < rows) {  // empty again
-          if (counts) table.at[t] = 0;
-          if (biases) entry.at[t] = 0;
-        }
+      const float bias = e != 0 ? a.bias_values[b0 + (int)e - 1] : 0.f, fine = w > 3 ? fmaf((float)(w >> 2), freq, pres) : 0.f;
+      for (int k = from; k < r; k++) {
+        T* at = held_rows + k * pitch + lead[k] + t;
+        float x = ToFloat(*at);
+        if (w & ~2u) x = x > 0.f ? x * inv : x * rep;
+        if (w > 3) x -= fine;
+        if (e != 0) x += bias;
+        *at = FromFloat<T>(x);
       }
+    };
+    for (int i = lane; i < listed; i += 32) {
+      const int t = list[i] & 0x7fff;
+      const uint32_t w = table.Take(t);
+      if (w != 0) adjust(t, w);
+    }
+    if (overflow) {  // some token is on no list
+      __syncthreads();
+      for (int t = threadIdx.x; t < a.table; t += kLogThreads)
+        if (table.at[t] != 0) adjust(t, table.at[t]);
+      __syncthreads();
+      for (int t = threadIdx.x; t < a.table; t += kLogThreads) table.at[t] = 0;
+      if (threadIdx.x == 0) overflow = 0;
     }
     if (r < rows) __syncthreads();
   }
@@ -251,9 +285,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __gri
     const int v = c * PER - mis;
     uint4 u = *reinterpret_cast<const uint4*>(held + v);
     if (masked) {
-      constexpr int kTwo = PER / 4;  // tokens of a word
-      const uint32_t allowed = __funnelshift_r(bits[(v >> 5) - word0], bits[((v + PER - 1) >> 5) - word0], v & 31);
-      u = make_uint4(Masked<T>(u.x, allowed), Masked<T>(u.y, allowed >> kTwo), Masked<T>(u.z, allowed >> 2 * kTwo), Masked<T>(u.w, allowed >> 3 * kTwo));
+      u = Masked<T>(u, __funnelshift_r(bits[(v >> 5) - word0], bits[((v + PER - 1) >> 5) - word0], v & 31));
     }
     *reinterpret_cast<uint4*>(out + v) = u;
   }
@@ -356,23 +388,22 @@ int shahd_adjust_logits(const ShahdLogitsCall* c, void* stream) {
   a.mask_stride = c->mask_stride;
   a.mask_rows = c->mask_rows;
   a.mask_count = c->mask_count;
-  // Slices of whole pieces, as many as give every multiprocessor a few blocks of threads; rows in groups where they share sequences and enough are left.
-  const auto lay = [&](int table) {
-    a.table = table;
-    a.slices = CeilDiv(c->vocab + 7, table - 8);  // a row that does not begin at a boundary reaches up to 7 values further
-  };
-  lay(kLogTable);
-  while (a.table > 1024 && (long long)c->rows * a.slices < 4 * info.sms) lay(a.table / 2);
+  // Slices of whole pieces and of one size, as many as give every multiprocessor a few blocks of threads, a thousand tokens at least; rows in
+  // groups where they share sequences and enough are left. (A row that does not begin at a boundary reaches up to 7 values further.)
+  const int reach = c->vocab + 7, wanted = std::max(CeilDiv(reach, kLogTable - 8), std::min(CeilDiv(4 * info.sms, c->rows), CeilDiv(reach, 1016)));
+  const int slice = RoundUp(CeilDiv(reach, wanted), 8);
+  a.table = slice + 8;
+  a.slices = CeilDiv(reach, slice);
   a.group = 1;
   while (c->rows / c->n >= 2 * a.group && a.group < kLogGroup && (long long)c->rows / (2 * a.group) * a.slices >= 4 * info.sms) a.group *= 2;
   if ((long long)a.rows * a.slices > 0x7fffffffLL) {
     SetError("%s: too many rows of this vocabulary: %d of %d", op, c->rows, c->vocab);
     return SHAHD_EINVAL;
   }
-  const bool wide = (a.history && a.history_stride > 0x7fff) || a.bias_entries > 0xfffe;  // a cell of 16 bits holds 2 x 2^15 - 1, and 2^16 - 1
+  const bool wide = (a.history && a.history_stride > 0x3fff) || a.bias_entries > 0xfffe;  // a cell of 16 bits holds 4 x 2^14 - 1, and 2^16 - 1
   // rows, masks, counts, entries, lists
   const int smem = a.group * (a.table + 8) * (int)size + RoundUp(a.group * (a.table / 32 + 2), 4) * 4 +
-                   (a.history || a.bias_tokens ? a.table * ((a.history ? 1 : 0) + (a.bias_tokens ? 1 : 0)) * (wide ? 4 : 2) + kLogWarps * 512 : 0);
+                   (a.history || a.bias_tokens ? a.table * (a.bias_tokens ? 2 : 1) * (wide ? 4 : 2) + kLogWarps * kLogList * 2 : 0);
   TakeLaunchError(nullptr);
   if (c->dtype == SHAHD_F32) LaunchLogits<float>(a, wide, smem, static_cast<cudaStream_t>(stream));
   else if (c->dtype == SHAHD_F16) LaunchLogits<__half>(a, wide, smem, static_cast<cudaStream_t>(stream));
