@@ -538,7 +538,8 @@ typedef struct ShahdCompactCall {
   int64_t workspace_bytes;
 } ShahdCompactCall;
 /* Moves the held pages together: those numbered U and up go, in ascending order, to the free ones below U, in ascending order. Entries of
- * the new table behind a sequence's length, and those that name no page, are -1. */
+ * the new table behind a sequence's length, and those that name no page, are -1: where a fork gave pages for positions that are still to
+ * come, the lengths given here count those positions. */
 int shahd_pages_compact(const ShahdCompactCall* call, void* stream);
 
 /* ---- norms of the query and key heads, with the rotary positions and the append (NormRow, CachedRowMath.ts:25-56, on heads) ---- */
