@@ -37,12 +37,12 @@ inline bool DeviceOfAddress(const void* p, int* device) {
     return reinterpret_cast<Fn>(f);
   }();
   if (!fn) return false;
-  unsigned int type = 0, managed = 1;
+  unsigned int type = 0;
   int ordinal = -1;
-  CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
-  void* to[3] = {&type, &managed, &ordinal};
-  if (fn(3, what, to, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return false;
-  if (type != CU_MEMORYTYPE_DEVICE || managed != 0 || ordinal < 0) return false;
+  CUpointer_attribute what[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+  void* to[2] = {&type, &ordinal};
+  if (fn(2, what, to, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return false;
+  if (type != CU_MEMORYTYPE_DEVICE || ordinal < 0) return false;
   *device = ordinal;
   return true;
 }

@@ -662,6 +662,10 @@ struct ChunkWalk {
         pair = 0;
         head++;
         while (head == A.Hk || q.pairs == 0) {  // also past sequences without rows
+          if (seq + 1 >= A.n) {                 // (the line does not end here as long as its offsets and lengths stay)
+            w.more = 0;
+            break;
+          }
           head = 0;
           q = ChunkSeq<KEYS>(A, ++seq);
         }
@@ -674,7 +678,10 @@ struct ChunkWalk {
   }
 };
 
-// Where this block of threads begins, as TreeBegin finds it; per: the ranges' length.
+// Where this block of threads begins, as TreeBegin finds it; per: the ranges' length. Sums stop at kLineMost, which is more than the host lets
+// a call's cost be: only offsets that do not ascend get there, and then nothing is done.
+constexpr int kLineMost = 1 << 30;
+__device__ __forceinline__ int LineAdd(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)kLineMost); }
 template <int KEYS>
 __device__ __forceinline__ bool ChunkBegin(const TaArgs& A, TaShared* sh, int& seq, int& at, int& pos, int& end, int& per) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -685,21 +692,22 @@ __device__ __forceinline__ bool ChunkBegin(const TaArgs& A, TaShared* sh, int& s
   };
   const int first = work(threadIdx.x);
   int sum = first;
-  for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum += work(s);
+  for (int s = threadIdx.x + blockDim.x; s < A.n; s += blockDim.x) sum = LineAdd(sum, work(s));
   const bool one = A.n <= (int)blockDim.x;  // a sequence a thread: one scan gives the total, too
   int incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    if (lane >= o) incl = LineAdd(incl, v);
   }
   if (lane == 31) sh->sums[warp] = incl;
   __syncthreads();
   int total = 0, ahead = incl - sum;
   for (int k = 0; k < warps; k++) {
-    if (k < warp) ahead += sh->sums[k];
-    total += sh->sums[k];
+    if (k < warp) ahead = LineAdd(ahead, sh->sums[k]);
+    total = LineAdd(total, sh->sums[k]);
   }
+  if (total >= kLineMost) return false;
   per = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   pos = (int)min((long long)blockIdx.x * per, (long long)total);
   end = min(pos + per, total);

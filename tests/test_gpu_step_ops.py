@@ -571,3 +571,76 @@ def test_chunk_attention_of_one_row_is_a_decode_step():
     pkg.tree_attention(pkg.BF16, _rows(q), _rows(own[0]), _rows(own[1]), _rows(other), cache, ln.data_ptr(), masks.data_ptr(), off.data_ptr(), n, n, 1, H,
                        workspace=ws.data_ptr(), workspace_bytes=size, stream=_stream())
     assert float((out.float() - other.float()).abs().max()) <= 4 * 2.0 ** -8 * float(out.float().abs().max())
+
+
+@pytest.mark.parametrize("blocks", [9, 3000])
+def test_chunk_attention_offsets_and_lengths_that_make_no_sense(blocks):
+    """Nothing outside the buffers is read or written, whatever the offsets and lengths on the device are; a later call is not harmed."""
+    g, n, H, Hk, d, N = _gen(28), 40, 4, 2, 64, 300
+    q = _normal(g, N, H, d, dtype=BF16)
+    pool = _normal(g, 30, 1, Hk, 2, 64, d, dtype=BF16)
+    table = torch.randint(-5, 35, (n, blocks), generator=g, device="cuda", dtype=torch.int32)
+    cache = pkg.KvCache(pool.data_ptr(), pool.stride(0), table.data_ptr(), blocks, 30, Hk, d)
+    size = pkg.chunk_attention_workspace(n, N, N, H, cache)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    guard = torch.full((N + 64, H, d), 7.0, dtype=BF16, device="cuda")
+    out = guard[32:32 + N]
+    for seed in range(6):
+        rng = np.random.default_rng(seed)
+        off = _ints(rng.integers(-2**31, 2**31, n + 1) if seed % 3 == 0 else rng.integers(-10, N + 10, n + 1) if seed % 3 == 1 else [0, N] * (n // 2) + [0])
+        ln = _ints(rng.integers(-2**31, 2**31, n) if seed % 2 else rng.integers(0, 64 * blocks, n))
+        pkg.chunk_attention(pkg.BF16, _rows(q), _rows(out), cache, ln.data_ptr(), off.data_ptr(), n, N, N, H, workspace=ws.data_ptr(), workspace_bytes=size, stream=_stream())
+        torch.cuda.synchronize()
+        assert bool((guard[:32] == 7.0).all()) and bool((guard[32 + N:] == 7.0).all())
+    off, ln = _ints([0, 100] + [100] * (n - 1)), _ints([60] * n)
+    table.clamp_(0, 29)
+    pkg.chunk_attention(pkg.BF16, _rows(q), _rows(out), cache, ln.data_ptr(), off.data_ptr(), n, N, N, H, workspace=ws.data_ptr(), workspace_bytes=size, stream=_stream())
+    torch.cuda.synchronize()
+    _check_chunk(q, pool, table, [60] * n, [100] + [0] * (n - 1), out, BF16)
+
+
+def test_adjust_logits_long_histories_with_many_biases():
+    """Histories and lists of biases beyond what 16-bit cells hold; a slice whose tokens are on no list, there are too many of them."""
+    g, V, held = _gen(29), 5000, 40000
+    rng = np.random.default_rng(29)
+    history = rng.integers(0, V, (2, held))
+    history[1, :30000] = 17
+    bt, bv = rng.integers(-5, V + 5, 70000), rng.normal(size=70000).astype(np.float32)
+    bo = [0, 60000, 70000]
+    x = _normal(g, 6, V, dtype=F16)
+    out, seqs = torch.empty_like(x), [0, 0, 1, 1, 1, 0]
+    lens, prompt = [held, held - 7], [100, 30001]
+    dev = [_ints(history.ravel()), _ints(lens), _ints(prompt), _ints(seqs), _ints(bo), _ints(bt), torch.tensor(bv, device="cuda")]
+    rep, pres, freq = (torch.tensor(v, device="cuda") for v in ([1.2, 0.9], [0.3, -0.2], [0.01, 0.5]))
+    pkg.adjust_logits(pkg.F16, x.data_ptr(), out.data_ptr(), 6, V, 2, sequences=dev[3].data_ptr(), history=dev[0].data_ptr(), history_stride=held,
+                      history_lengths=dev[1].data_ptr(), prompt_lengths=dev[2].data_ptr(), repetition=rep.data_ptr(), presence=pres.data_ptr(), frequency=freq.data_ptr(),
+                      bias_offsets=dev[4].data_ptr(), bias_tokens=dev[5].data_ptr(), bias_values=dev[6].data_ptr(), bias_entries=70000, stream=_stream())
+    for i, s in enumerate(seqs):
+        want, bound = S.adjust(x[i].double(), history[s, : lens[s]].tolist(), prompt[s], rep[s].double(), pres[s].double(), freq[s].double(),
+                               list(zip(bt[bo[s]:bo[s + 1]].tolist(), bv[bo[s]:bo[s + 1]].tolist())), None, F16)
+        _within(out[i], want, bound)
+    # the same without biases, in 16-bit cells and as many tokens as a slice has
+    short = _ints(np.stack([rng.permutation(V), rng.permutation(V)]).ravel())
+    ln = _ints([V, V])
+    pkg.adjust_logits(pkg.F16, x.data_ptr(), out.data_ptr(), 6, V, 2, sequences=dev[3].data_ptr(), history=short.data_ptr(), history_stride=V, history_lengths=ln.data_ptr(),
+                      presence=pres.data_ptr(), stream=_stream())
+    for i, s in enumerate(seqs):
+        want, bound = S.adjust(x[i].double(), list(range(V)), 0, torch.ones((), device="cuda").double(), pres[s].double(), torch.zeros((), device="cuda").double(), [], None,
+                               F16)
+        _within(out[i], want, bound)
+
+
+def test_operators_with_nothing_to_do():
+    """Sequences without rows, rows without sequences, vocabularies of one token."""
+    q = torch.full((4, 2, 64), 7.0, dtype=BF16, device="cuda")
+    pool, table = torch.zeros(2, 1, 2, 2, 64, 64, dtype=BF16, device="cuda"), _ints([0, 1])
+    cache = pkg.KvCache(pool.data_ptr(), pool.stride(0), table.data_ptr(), 1, 2, 2, 64)
+    size = pkg.chunk_attention_workspace(2, 4, 3, 2, cache)
+    ws, off, ln = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda"), _ints([0, 0, 0]), _ints([5, 0])
+    pkg.chunk_attention(pkg.BF16, _rows(q), _rows(q), cache, ln.data_ptr(), off.data_ptr(), 2, 4, 3, 2, workspace=ws.data_ptr(), workspace_bytes=size, stream=_stream())
+    assert bool((q == 7.0).all())
+    x, seqs, held = torch.ones(3, 1, device="cuda"), _ints([0, -1, 5]), _ints([3])
+    history, pres = _ints([0, 0, 9]), torch.ones(1, device="cuda")
+    pkg.adjust_logits(pkg.F32, x.data_ptr(), x.data_ptr(), 3, 1, 1, sequences=seqs.data_ptr(), history=history.data_ptr(), history_stride=3, history_lengths=held.data_ptr(),
+                      presence=pres.data_ptr(), stream=_stream())
+    assert x.tolist() == [[0.0], [1.0], [1.0]]
