@@ -16,12 +16,10 @@
 
 namespace shahd {
 
-constexpr int kLogThreads = 256;
-constexpr int kLogWarps = kLogThreads / 32;
 constexpr int kLogGroup = 4;     // rows of a block of threads, at most
 constexpr int kLogDeep = 3;      // loads of the history of a thread in flight
 constexpr int kLogTable = 3968;  // tokens of a slice's table, at most: four blocks of threads on a multiprocessor, with four 16-bit rows each
-constexpr int kLogList = 384;    // tokens of a warp's list
+constexpr int kLogLists = 3072;  // tokens of the lists of a block's warps
 
 struct LogitsArgs {
   const void* in;
@@ -92,8 +90,9 @@ struct LogCells {
 };
 
 // A token's count: 4 x times generated + 2 where it has a bias + 1 where the prompt has it.
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __grid_constant__ LogitsArgs a) {
+template <class T, bool WIDE, int kLogThreads>
+__global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsKernel(const __grid_constant__ LogitsArgs a) {
+  constexpr int kLogWarps = kLogThreads / 32, kLogList = kLogLists / kLogWarps;
   typedef typename LogCells<WIDE>::Cell Cell;
   constexpr int PER = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t log_raw[];
@@ -295,11 +294,18 @@ __global__ void __launch_bounds__(kLogThreads, 4) AdjustLogitsKernel(const __gri
     for (int v = tail + begin; v < v1; v += step) single(v);
 }
 
+// Rows on their own: blocks of 128 threads, twice as many at a time, so that the steps of one run under the copies of others (256 rows of 32768
+// f32: 20.9 us, with 256 threads 24.3). Groups: 256 threads, since four rows take the shared memory (512 rows of 50257 bf16: 44.7 us, with 128 60).
+template <class T, bool WIDE, int THREADS>
+void LaunchLogitsAs(const LogitsArgs& a, int smem, cudaStream_t st) {
+  if (!EnsureKernelAttrs((const void*)AdjustLogitsKernel<T, WIDE, THREADS>, smem)) return;
+  LaunchPdl(AdjustLogitsKernel<T, WIDE, THREADS>, dim3((unsigned)(CeilDiv(a.rows, a.group) * a.slices)), dim3(THREADS), (size_t)smem, st, a);
+}
+
 template <class T>
 void LaunchLogits(const LogitsArgs& a, bool wide, int smem, cudaStream_t st) {
-  const auto kernel = wide ? AdjustLogitsKernel<T, true> : AdjustLogitsKernel<T, false>;
-  if (!EnsureKernelAttrs((const void*)kernel, smem)) return;
-  LaunchPdl(kernel, dim3((unsigned)(CeilDiv(a.rows, a.group) * a.slices)), dim3(kLogThreads), (size_t)smem, st, a);
+  if (a.group > 1) wide ? LaunchLogitsAs<T, true, 256>(a, smem, st) : LaunchLogitsAs<T, false, 256>(a, smem, st);
+  else wide ? LaunchLogitsAs<T, true, 128>(a, smem, st) : LaunchLogitsAs<T, false, 128>(a, smem, st);
 }
 
 }  // namespace shahd
@@ -403,7 +409,7 @@ int shahd_adjust_logits(const ShahdLogitsCall* c, void* stream) {
   const bool wide = (a.history && a.history_stride > 0x3fff) || a.bias_entries > 0xfffe;  // a cell of 16 bits holds 4 x 2^14 - 1, and 2^16 - 1
   // rows, masks, counts, entries, lists
   const int smem = a.group * (a.table + 8) * (int)size + RoundUp(a.group * (a.table / 32 + 2), 4) * 4 +
-                   (a.history || a.bias_tokens ? a.table * (a.bias_tokens ? 2 : 1) * (wide ? 4 : 2) + kLogWarps * kLogList * 2 : 0);
+                   (a.history || a.bias_tokens ? a.table * (a.bias_tokens ? 2 : 1) * (wide ? 4 : 2) + kLogLists * 2 : 0);
   TakeLaunchError(nullptr);
   if (c->dtype == SHAHD_F32) LaunchLogits<float>(a, wide, smem, static_cast<cudaStream_t>(stream));
   else if (c->dtype == SHAHD_F16) LaunchLogits<__half>(a, wide, smem, static_cast<cudaStream_t>(stream));
