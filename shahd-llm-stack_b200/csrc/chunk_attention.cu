@@ -26,21 +26,24 @@ void LaunchChunks(const TaArgs& a, unsigned blocks, cudaStream_t st) {
 }
 
 // How a call's work is laid out; times are of one graph, 16/4 heads of 64 if nothing else is said.
-//   Pairs: a block of threads for every tile pair, longest first. Where there are many, or enough with short caches. 16 chunks of 300 to
-//     2048 rows from position 0: 127 us, ranges 154; 256 single tokens, 8/2 heads, 400 to 576 positions: 17.7 and 35; 48 sequences, six
-//     of them with 200 to 512 rows, 0 to 1500 positions: 44.4 and 45.8 (the longest pair is 38 of them).
-//   Split: a cluster of 2 to 8 blocks of threads for every pair, where that leaves multiprocessors for all and the steps are few: one
-//     launch, no second kernel. 96 rows over 1700 positions: 13.4 us, ranges 20, pairs 36.
+//   Pairs: a block of threads for every pair of tiles, longest first, where there are many of them. 16 chunks of 300 to 2048 rows from position
+//     0: 121 us, ranges 154, tiles 151.
+//   Tiles: a block of threads for every tile, its key blocks by turns: half as many steps, at twice the loads. Where pairs are few enough that
+//     the longest is what is waited for: 48 sequences, six of them with 200 to 512 rows, 0 to 1500 positions: 39 us, pairs 44, ranges 46; 8192
+//     rows from position 0: 198, pairs 208, ranges 218. At head_dim 128 the loads tell: 2 chunks of 1024 over 12000, 32/8 heads: 500, pairs and
+//     ranges 440 to 470.
+//   Split: a cluster of 2 to 8 blocks of threads for every tile, where that leaves multiprocessors for all and the steps are few: one
+//     launch, no second kernel. 96 rows over 1700 positions: 11.2 us, pairs split in eight 13.4, ranges 20, pairs 36.
 //   Ranges: as many blocks of threads as run at once take ranges of equal cost out of the line of all pairs, and what a range cuts is joined
-//     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 167 us, pairs 219, split in
-//     two 219; 2 chunks of 1024 over 12000, 32/8 heads of 128: 440 and 510. The second kernel and the parts cost about eight steps.
+//     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 166 us, tiles 202, pairs 220. The
+//     second kernel and the parts cost about eight steps.
 // Pairs go longest first over all kv heads; where the keys and values do not fit the L2 cache, head after head, so that the blocks of threads that
 // run at a time read the same ones (4 chunks of 1500 to 2048 rows over 10 to 24 thousand positions, 32/8 heads of 128, 427 MB: 2820 us and
 // 2511; but 2 of 7000 to 8192 from position 0, 16/2 heads of 128, 16 MB: 467 and 513).
 // The lengths lie on the device, so the table's width stands for them, and a table much wider than its sequences are long may get the
 // layout for longer ones.
 struct ChunkLayout {
-  int least, part_rows, two_heads, split, by_heads;
+  int span, least, part_rows, two_heads, split, by_heads;
   long long grid;
   int64_t cut_bytes, bytes;
 };
@@ -52,24 +55,26 @@ int LayChunks(const char* op, const ShahdChunkCall* c, ChunkLayout* out) {
     SetError("%s: need n, rows >= 0 and max_rows >= 1 (got n=%d rows=%d max_rows=%d)", op, c->n, c->rows, c->max_rows);
     return SHAHD_EINVAL;
   }
-  const int G = H / Hk, span = 2 * (128 / G), keys = d == 128 ? 128 : 64;
-  const long long pairs = std::min((long long)c->rows / span + c->n, (long long)c->n * CeilDiv(std::min(c->max_rows, 1 << 30), span));
-  const long long most = pairs * Hk * (CeilDiv(c->cache.max_blocks, keys / 64) + kPairCost);  // what all pairs cost, if all sequences were as long
-  if (c->rows > kOpsMaxRows || pairs > (1 << 23) || most > 0x3fffffffLL) {
+  const int G = H / Hk, TB = 128 / G, keys = d == 128 ? 128 : 64;
+  // tiles of all sequences together, `span` tokens each, at most
+  const auto tiles_of = [&](int span) { return std::min((long long)c->rows / span + c->n, (long long)c->n * CeilDiv(std::min(c->max_rows, 1 << 30), span)) * Hk; };
+  const long long pairs = tiles_of(2 * TB), blocks = CeilDiv(c->cache.max_blocks, keys / 64);
+  const long long most = pairs * (blocks + kPairCost);  // what all pairs cost, if all sequences were as long
+  const long long places = (long long)c->rows / TB + c->n;
+  if (c->rows > kOpsMaxRows || pairs / Hk > (1 << 23) || most > 0x3fffffffLL || places * Hk > 0x3fffffff) {
     SetError("%s: too many rows or key blocks: %d rows, %d sequences, %d pages each", op, c->rows, c->n, c->cache.max_blocks);
     return SHAHD_EINVAL;
   }
   ChunkLayout l = {};
   const long long slots = kTaSms * (d == 128 ? 1 : 2);
-  const long long places = (long long)c->rows / span + c->n, tiles = pairs * Hk, blocks = CeilDiv(c->cache.max_blocks, keys / 64);
-  if (places * Hk > 0x3fffffff) {
-    SetError("%s: too many rows and sequences (%d and %d)", op, c->rows, c->n);
-    return SHAHD_EINVAL;
-  }
-  l.part_rows = std::min(c->max_rows, span) * G;
   l.split = 1;
+  const long long tiles = tiles_of(TB);
   while (l.split < 8 && tiles * l.split * 2 <= slots) l.split *= 2;
-  const bool ranges = tiles >= 4 * slots ? false : tiles >= slots ? blocks >= 64 : blocks / l.split > tiles * blocks / slots + 8;
+  const bool many = pairs >= 4 * slots;
+  const bool ranges = !many && (pairs >= slots ? blocks >= 64 && (d == 128 || tiles < 3 * slots)
+                                               : (tiles * l.split + slots - 1) / slots * blocks / (2 * l.split) > pairs * blocks / slots + 8);
+  l.span = many || ranges ? 2 * TB : TB;
+  l.part_rows = std::min(c->max_rows, l.span) * G;
   if (ranges) {
     l.split = 1;
     l.least = 256 / keys + kPairCost;
@@ -79,10 +84,10 @@ int LayChunks(const char* op, const ShahdChunkCall* c, ChunkLayout* out) {
   } else if (l.split > 1) {
     l.grid = places * Hk * l.split;
     l.bytes = l.grid * l.part_rows * (d + 2) * (int64_t)sizeof(float);
-  } else {  // one tile of rows: those of two kv heads together take half as many blocks of threads as one by turns, and no merge
-    l.two_heads = c->max_rows <= span / 2 && Hk % 2 == 0;
+  } else {  // one tile of rows: those of two kv heads together take half as many blocks of threads, and no merge
+    l.two_heads = c->max_rows <= TB && Hk % 2 == 0;
     l.by_heads = (double)c->n * c->cache.max_blocks * kOpsPage * Hk * 2 * d * 2 > 126e6;
-    l.grid = l.two_heads ? places * Hk / 2 : places * Hk;
+    l.grid = ((long long)c->rows / l.span + c->n) * Hk / (l.two_heads ? 2 : 1);
   }
   *out = l;
   return SHAHD_OK;
@@ -162,6 +167,7 @@ int shahd_chunk_attention(const ShahdChunkCall* c, void* stream) {
   a.pages = c->cache.pages;
   a.max_nodes = c->max_rows;
   a.least = lay.least;
+  a.span = lay.span;
   a.two_heads = lay.two_heads;
   a.split = lay.split;
   a.by_heads = lay.by_heads;

@@ -82,6 +82,7 @@ struct TaArgs {
   const unsigned long long* masks;
   const int* lengths;
   const int* table;
+  int span;      // chunks: tokens of a pair of tiles (ranges: always), or of one tile where each goes by turns on its own
   int by_heads;  // chunks: one kv head's pairs after another's
   int max_blocks, pages, max_nodes, pairs, split, two_heads;  // split: blocks of threads that share a pair; two_heads: the pair's tiles are those of two kv heads
   // All key blocks of all tile pairs in one line, dealt out to the blocks of threads in ranges of equal length, at least
@@ -295,8 +296,8 @@ struct TaWork {
 // sequences: s owns places offsets[s] / span + s .. offsets[s+1] / span + s, at least as many as it needs, which a search in
 // the offsets finds.
 template <int KEYS>
-__device__ __forceinline__ bool PromptWork(const TaArgs& A, int rank, int all, TaWork& w) {
-  const int lane = threadIdx.x & 31, span = 2 * A.TB;
+__device__ __forceinline__ bool PromptWork(const TaArgs& A, int rank, int all, int span, TaWork& w) {
+  const int lane = threadIdx.x & 31;
   const auto off = [&](int s) { return min(max(A.offsets[s], 0), A.rows); };
   int seq, local;
   if (A.n > 1 && A.n <= 128) {
@@ -533,19 +534,20 @@ __device__ __forceinline__ int FloorSum(uint32_t n, uint32_t a, uint32_t b) {
 constexpr int kPairCost = 3;
 template <int KEYS>
 struct ChunkSeq {
-  int start, nodes, past, total, most, pairs, span;
-  __device__ __forceinline__ ChunkSeq(const TaArgs& A, int s) {
+  int start, nodes, past, total, most, pairs, span, turns;  // turns: rows of a tile; up to so many go by turns
+  __device__ __forceinline__ ChunkSeq(const TaArgs& A, int s, int span_) {
     start = min(max(A.offsets[s], 0), A.rows);
     nodes = min(min(max(A.offsets[s + 1], start), A.rows) - start, A.max_nodes);
     most = A.max_blocks * kOpsPage;
     past = min(max(A.lengths[s], 0), most);
     total = min(past + nodes, most);
-    span = 2 * A.TB;
+    span = span_;
+    turns = A.TB;
     pairs = (nodes + span - 1) / span;
   }
-  // Key blocks and steps of pair p, and what all pairs before it cost (p <= pairs).
+  // Key blocks and steps of pair p, and what all pairs before it cost (p <= pairs; of pairs of two tiles, whose steps are their blocks).
   __device__ __forceinline__ int Blocks(int p) const { return (min(past + min((p + 1) * span, nodes), most) + KEYS - 1) / KEYS; }
-  __device__ __forceinline__ bool Turns(int p) const { return nodes - p * span <= span / 2; }
+  __device__ __forceinline__ bool Turns(int p) const { return min(nodes - p * span, span) <= turns; }
   __device__ __forceinline__ int Steps(int p) const {
     const int blocks = Blocks(p);
     return Turns(p) ? (blocks + 1) / 2 : blocks;
@@ -563,14 +565,14 @@ struct ChunkSeq {
 // its key blocks this is the share of number `place` of `split`, two blocks at least; w.more: shares that there are.
 template <int KEYS>
 __device__ __forceinline__ bool ChunkWork(const TaArgs& A, int rank, int all, int split, int place, TaWork& w) {
-  if (!PromptWork<KEYS>(A, rank, all, w)) return false;
-  const ChunkSeq<KEYS> q(A, w.seq);
+  if (!PromptWork<KEYS>(A, rank, all, A.span, w)) return false;
+  const ChunkSeq<KEYS> q(A, w.seq, A.span);
   if (w.q0 >= q.nodes) return false;
   w.nodes = q.nodes;
   w.cached = q.total;
   w.cache_blocks = q.past;
   w.tokens0 = min(q.nodes - w.q0, A.TB);
-  w.tokens1 = min(max(q.nodes - w.q0 - A.TB, 0), A.TB);
+  w.tokens1 = min(max(min(q.nodes - w.q0, q.span) - A.TB, 0), A.TB);
   const int blocks = q.Blocks(w.q0 / q.span), per = max((blocks + split - 1) / split, min(blocks, 2));
   w.first = place * per;
   const int count = min(max(blocks - w.first, 0), per);
@@ -601,7 +603,7 @@ struct ChunkWalk {
   int seq, head, pair, at, pos, end;  // the next pair and how much of its cost lies behind; the range that is left
   int cut_row, cut_head, cut_tokens, cut_from, cut_steps;  // the pair that the range begins and does not end
   // From place `at_` of sequence seq_'s on, pos_ in the line, to end_. The whole warp takes part.
-  __device__ __forceinline__ ChunkWalk(const TaArgs& a, int seq_, int at_, int pos_, int end_) : A(a), q(a, seq_), seq(seq_), pos(pos_), end(end_) {
+  __device__ __forceinline__ ChunkWalk(const TaArgs& a, int seq_, int at_, int pos_, int end_) : A(a), q(a, seq_, 2 * a.TB), seq(seq_), pos(pos_), end(end_) {
     cut_tokens = 0;
     const int line = q.Before(q.pairs);
     head = at_ / line;
@@ -667,7 +669,7 @@ struct ChunkWalk {
             break;
           }
           head = 0;
-          q = ChunkSeq<KEYS>(A, ++seq);
+          q = ChunkSeq<KEYS>(A, ++seq, 2 * A.TB);
         }
       }
     }
@@ -687,7 +689,7 @@ __device__ __forceinline__ bool ChunkBegin(const TaArgs& A, TaShared* sh, int& s
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto work = [&](int s) {
     if (s >= A.n) return 0;
-    const ChunkSeq<KEYS> q(A, s);
+    const ChunkSeq<KEYS> q(A, s, 2 * A.TB);
     return A.Hk * q.Before(q.pairs);
   };
   const int first = work(threadIdx.x);
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     }
   } else if (warp == 9) {  // one warp looks, the others prepare meanwhile
     w.head = blockIdx.x % A.Hk;
-    if (!PromptWork<KEYS>(A, blockIdx.x / A.Hk, gridDim.x / A.Hk, w)) w.nodes = 0;
+    if (!PromptWork<KEYS>(A, blockIdx.x / A.Hk, gridDim.x / A.Hk, 2 * A.TB, w)) w.nodes = 0;
     if (lane == 0) PutWork(sh, 0, w);
   }
   if constexpr (KIND == kTreePairs) {
@@ -1523,7 +1525,7 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
     if (w.more < 2) return;  // the whole cluster: one block of threads has it all
     ClusterSync();           // all parts are written
     if (warp < 8) {          // (at head_dim 128 the others have given registers away)
-      const int tokens = min(w.nodes - w.q0, 2 * A.TB), rank = blockIdx.x % A.split;
+      const int tokens = min(w.nodes - w.q0, A.span), rank = blockIdx.x % A.split;
       constexpr int kGroup = 128 / D;
       for (int local = (rank * 8 + warp) * kGroup; local < tokens * A.G; local += A.split * 8 * kGroup)
         JoinRows<D, F16, 1, 8>(A, (int)blockIdx.x - rank, false, w.more, local, tokens * A.G, w.start + w.q0, w.head);
