@@ -10,6 +10,11 @@
 // of all that meet a token one. Then the rows go out in 16-byte pieces as the masks leave them. Rows of one sequence (drafted rows) share
 // counts and lists. The history is read by every slice's block, from the cache but for the first: 4 bytes a token, four a load where it
 // is aligned.
+//
+// Measured, in one graph: 512 rows of 50257 bf16, four to a sequence of 4000 to 8000 tokens: 44.2 us for 108 MB, and half of the issue slots: 13 blocks
+// look through each history. 256 rows of 32768 f32 with histories of 1000 to 2000: 20.9 us for 69 MB. What else was timed on the first: a look into the
+// table for every value that goes out 54 us, the few values put right in global memory behind the copy 78, tables of 2048 or 8192 tokens and
+// blocks of 512 threads slower than 44.2, all of the history in flight no faster. 64 rows of 4096 f32: 4.0 us, latency.
 #pragma once
 
 #include "rows.cuh"
@@ -19,7 +24,7 @@ namespace shahd {
 constexpr int kLogGroup = 4;     // rows of a block of threads, at most
 constexpr int kLogDeep = 3;      // loads of the history of a thread in flight
 constexpr int kLogTable = 3968;  // tokens of a slice's table, at most: four blocks of threads on a multiprocessor, with four 16-bit rows each
-constexpr int kLogLists = 3072;  // tokens of the lists of a block's warps
+constexpr int kLogLists = 3200;  // tokens of the lists of a block's warps
 
 struct LogitsArgs {
   const void* in;

@@ -6,7 +6,13 @@
 // reads nothing); one rounding, at the end.
 //
 // Bound by memory: each value is read once and written once. Lanes take pieces of heads as in rope.cuh; the lanes that hold one
-// head's pieces lie side by side and add up their shares by shuffles, for all the heads in flight at once.
+// head's pieces lie side by side and add up their shares by shuffles, for all the heads in flight at once. Two blocks of threads on a
+// multiprocessor, 128 registers a thread: the next heads' values come in while these are summed, which the third block's registers would
+// be taken from.
+//
+// Measured, in one graph: 59402 rows of 32+8 f16 heads of 128 into the cache, 1.46 GB: 247 us, 5.9 TB/s; without the next heads' loads ahead
+// 293, with three blocks, whose values spill, 394. 13872 rows of 16+4 f32 heads of 64, layer norm, 159 MB: 35 us, 4.5 TB/s: sums, shuffles and the
+// sines of a row's positions take four of ten issue slots, and the rows are few for each warp. One token of 64 users: 6.4 us, latency.
 #pragma once
 
 #include "rope_call.cuh"
