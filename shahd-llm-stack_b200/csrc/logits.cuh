@@ -94,10 +94,14 @@ struct LogCells {
   }
 };
 
+// Threads of a block.
+template <bool GROUPS>
+constexpr int kLogThreadsOf = GROUPS ? 256 : 128;
+
 // A token's count: 4 x times generated + 2 where it has a bias + 1 where the prompt has it.
-template <class T, bool WIDE, int kLogThreads>
-__global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsKernel(const __grid_constant__ LogitsArgs a) {
-  constexpr int kLogWarps = kLogThreads / 32, kLogList = kLogLists / kLogWarps;
+template <class T, bool WIDE, bool GROUPS>
+__global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GROUPS>) AdjustLogitsKernel(const __grid_constant__ LogitsArgs a) {
+  constexpr int kLogThreads = kLogThreadsOf<GROUPS>, kLogWarps = kLogThreads / 32, kLogList = kLogLists / kLogWarps, kCells = WIDE ? 4 : 8;
   typedef typename LogCells<WIDE>::Cell Cell;
   constexpr int PER = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t log_raw[];
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsK
           table.Or(t, 2);
         }
         const uint32_t none = 0;
-        if (!enlist(std::integral_constant<int, 1>(), &t, &none)) overflow = 1;
+        if (!GROUPS && !enlist(std::integral_constant<int, 1>(), &t, &none)) overflow = 1;
       }
     }
     const int biased = listed;
@@ -205,6 +209,14 @@ __global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsK
       // four tokens a lane, from place i[j] of the history each (INT32_MIN is no token of any table)
       const auto meet = [&](const int (&token)[4], const int (&i)[4]) {
         uint32_t t[4], flag[4];
+        if constexpr (GROUPS) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint32_t at = (uint32_t)token[j] - (uint32_t)base;
+            if (at < (uint32_t)a.table) count(at, i[j] < prompt);
+          }
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           t[j] = (uint32_t)token[j] - (uint32_t)base;
@@ -243,7 +255,8 @@ __global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsK
         meet(u, i);
       }
       __syncwarp();
-      for (int i = biased + lane; i < listed; i += 32) count(list[i] & ~kPrompt, list[i] & kPrompt);
+      for (int i = biased + lane; i < listed; i += 32)  // none in groups
+        count(list[i] & ~kPrompt, list[i] & kPrompt);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
@@ -263,12 +276,45 @@ __global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsK
         *at = FromFloat<T>(x);
       }
     };
-    for (int i = lane; i < listed; i += 32) {
-      const int t = list[i] & 0x7fff;
-      const uint32_t w = table.Take(t);
-      if (w != 0) adjust(t, w);
+    const auto see_to = [&] {
+      for (int i = lane; i < listed; i += 32) {
+        const int t = list[i] & 0x7fff;
+        const uint32_t w = table.Take(t);
+        if (w != 0) adjust(t, w);
+      }
+    };
+    if constexpr (GROUPS) {
+      // each warp lists the tokens of its part of the table: one for a lane at a time
+      for (int c0 = warp * 32; c0 < a.table / kCells; c0 += kLogThreads) {
+        const int c = c0 + lane;
+        const uint4 u = c < a.table / kCells ? reinterpret_cast<const uint4*>(table.at)[c] : make_uint4(0, 0, 0, 0);
+        const uint32_t words[4] = {u.x, u.y, u.z, u.w};
+        uint32_t there = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (WIDE) there |= (uint32_t)(words[i] != 0) << i;
+          else there |= (uint32_t)((words[i] & 0xffffu) != 0) << 2 * i | (uint32_t)(words[i] > 0xffffu) << (2 * i + 1);
+        }
+        int upto = __popc(there);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const int all = __shfl_sync(0xffffffffu, upto, 31);
+        if (listed + all > kLogList) {
+          __syncwarp();
+          see_to();
+          __syncwarp();
+          listed = 0;
+        }
+        for (uint16_t* p = list + listed + upto - __popc(there); there != 0; there &= there - 1) *p++ = (uint16_t)(c * kCells + __ffs(there) - 1);
+        listed += all;
+      }
+      __syncwarp();
     }
-    if (overflow) {  // some token is on no list
+    see_to();
+    if (!GROUPS && overflow) {  // some token is on no list
       __syncthreads();
       for (int t = threadIdx.x; t < a.table; t += kLogThreads)
         if (table.at[t] != 0) adjust(t, table.at[t]);
@@ -299,18 +345,20 @@ __global__ void __launch_bounds__(kLogThreads, 1024 / kLogThreads) AdjustLogitsK
     for (int v = tail + begin; v < v1; v += step) single(v);
 }
 
-// Rows on their own: blocks of 128 threads, twice as many at a time, so that the steps of one run under the copies of others (256 rows of 32768
-// f32: 20.9 us, with 256 threads 24.3). Groups: 256 threads, since four rows take the shared memory (512 rows of 50257 bf16: 44.7 us, with 128 60).
-template <class T, bool WIDE, int THREADS>
+// Rows on their own: blocks of 128 threads, twice as many at a time, so that the steps of one run under the copies of others, and each
+// warp lists the history's tokens that it met, since a row meets few (256 rows of 32768 f32: 20.9 us; with 256 threads 24.3; looking for them
+// in the table 25.5). Groups: 256 threads, since four rows take the shared memory (512 rows of 50257 bf16: with 128 60 us), and
+// the tokens are looked for in the table, which costs a lane less than a list of all that it met (39.5 us, with such lists 44.4).
+template <class T, bool WIDE, bool GROUPS>
 void LaunchLogitsAs(const LogitsArgs& a, int smem, cudaStream_t st) {
-  if (!EnsureKernelAttrs((const void*)AdjustLogitsKernel<T, WIDE, THREADS>, smem)) return;
-  LaunchPdl(AdjustLogitsKernel<T, WIDE, THREADS>, dim3((unsigned)(CeilDiv(a.rows, a.group) * a.slices)), dim3(THREADS), (size_t)smem, st, a);
+  if (!EnsureKernelAttrs((const void*)AdjustLogitsKernel<T, WIDE, GROUPS>, smem)) return;
+  LaunchPdl(AdjustLogitsKernel<T, WIDE, GROUPS>, dim3((unsigned)(CeilDiv(a.rows, a.group) * a.slices)), dim3(kLogThreadsOf<GROUPS>), (size_t)smem, st, a);
 }
 
 template <class T>
 void LaunchLogits(const LogitsArgs& a, bool wide, int smem, cudaStream_t st) {
-  if (a.group > 1) wide ? LaunchLogitsAs<T, true, 256>(a, smem, st) : LaunchLogitsAs<T, false, 256>(a, smem, st);
-  else wide ? LaunchLogitsAs<T, true, 128>(a, smem, st) : LaunchLogitsAs<T, false, 128>(a, smem, st);
+  if (a.group > 1) wide ? LaunchLogitsAs<T, true, true>(a, smem, st) : LaunchLogitsAs<T, false, true>(a, smem, st);
+  else wide ? LaunchLogitsAs<T, true, false>(a, smem, st) : LaunchLogitsAs<T, false, false>(a, smem, st);
 }
 
 }  // namespace shahd

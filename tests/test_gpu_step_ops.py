@@ -630,6 +630,31 @@ def test_adjust_logits_long_histories_with_many_biases():
         _within(out[i], want, bound)
 
 
+@pytest.mark.parametrize("held", [5000, 17000])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_adjust_logits_many_rows_of_a_sequence_that_has_most_tokens(held, dtype):
+    """Rows that go four together, sequences that end inside such a group, histories with nearly every token, in 16-bit and 32-bit cells."""
+    g, V, rows, n = _gen(31), 5000, 1200, 290
+    rng = np.random.default_rng(held)
+    history = np.stack([rng.permutation(held) % V for _ in range(n)])
+    seqs = np.arange(rows) * n // rows
+    seqs[5], seqs[6] = -1, 9
+    lens, prompt = rng.integers(held - 9, held + 1, n), rng.integers(0, held, n)
+    bt, bv = rng.integers(0, V, 3 * n), rng.normal(size=3 * n).astype(np.float32)
+    x = _normal(g, rows, V, dtype=dtype)
+    out = torch.empty_like(x)
+    rep, pres, freq = (torch.tensor(rng.uniform(a, b, n), dtype=F32, device="cuda") for a, b in ((0.7, 1.5), (-1, 1), (-0.5, 0.5)))
+    dev = [_ints(history.ravel()), _ints(lens), _ints(prompt), _ints(seqs), _ints(3 * np.arange(n + 1)), _ints(bt), torch.tensor(bv, device="cuda")]
+    pkg.adjust_logits(CODE[dtype], x.data_ptr(), out.data_ptr(), rows, V, n, sequences=dev[3].data_ptr(), history=dev[0].data_ptr(), history_stride=held,
+                      history_lengths=dev[1].data_ptr(), prompt_lengths=dev[2].data_ptr(), repetition=rep.data_ptr(), presence=pres.data_ptr(), frequency=freq.data_ptr(),
+                      bias_offsets=dev[4].data_ptr(), bias_tokens=dev[5].data_ptr(), bias_values=dev[6].data_ptr(), bias_entries=3 * n, stream=_stream())
+    for i in [0, 1, 2, 3, 4, 6, 7, 8, 601, 1198, 1199]:
+        s = int(seqs[i])
+        want, bound = S.adjust(x[i].double(), history[s, : lens[s]].tolist(), int(prompt[s]), rep[s].double(), pres[s].double(), freq[s].double(),
+                               list(zip(bt[3 * s:3 * s + 3].tolist(), bv[3 * s:3 * s + 3].tolist())), None, dtype)
+        _within(out[i], want, bound)
+
+
 def test_operators_with_nothing_to_do():
     """Sequences without rows, rows without sequences, vocabularies of one token."""
     q = torch.full((4, 2, 64), 7.0, dtype=BF16, device="cuda")
