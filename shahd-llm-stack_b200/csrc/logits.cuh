@@ -94,6 +94,12 @@ struct LogCells {
   }
 };
 
+// Values between a 16-byte boundary and a row's beginning.
+template <class T>
+__device__ __forceinline__ int LeadOf(const LogitsArgs& a, int row) {
+  return (int)((reinterpret_cast<uintptr_t>(a.in) + (uintptr_t)(row * a.in_row) * sizeof(T)) % 16 / sizeof(T));
+}
+
 // Threads of a block.
 template <bool GROUPS>
 constexpr int kLogThreadsOf = GROUPS ? 256 : 128;
@@ -126,30 +132,30 @@ __global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GR
   if ((int)threadIdx.x < rows) {
     seqs[threadIdx.x] = a.seqs ? a.seqs[first + threadIdx.x] : first + (int)threadIdx.x;
     mask_rows[threadIdx.x] = a.mask_rows ? a.mask_rows[first + threadIdx.x] : first + (int)threadIdx.x;
-    lead[threadIdx.x] = (int)((reinterpret_cast<uintptr_t>(a.in) + (uintptr_t)((first + threadIdx.x) * a.in_row) * sizeof(T)) % 16 / sizeof(T));
+    lead[threadIdx.x] = LeadOf<T>(a, first + (int)threadIdx.x);
   }
-  __syncthreads();
   // The warps are dealt out to the rows: this one's row, its tokens v0 .. v1-1 of this slice, their whole pieces p0 .. p1-1 (inside the
   // row) and the values before and behind them; the warp takes every `step`-th 32 of what there is.
   const int mine = warp & (a.group - 1), begin = (warp / a.group) * 32 + lane, step = kLogThreads / a.group;
-  const bool busy = mine < rows && (unsigned)seqs[min(mine, rows - 1)] < (unsigned)a.n;
-  const int mis = lead[min(mine, rows - 1)], v0 = max(sl * slice - mis, 0), v1 = min((sl + 1) * slice - mis, a.vocab);
+  const int mis = LeadOf<T>(a, first + min(mine, rows - 1)), v0 = max(sl * slice - mis, 0), v1 = min((sl + 1) * slice - mis, a.vocab);
   const int p0 = (v0 + mis + PER - 1) / PER, p1 = max((v1 + mis) / PER, p0), head = min(p0 * PER - mis, v1), tail = max(p1 * PER - mis, head);
   T* const held = held_rows + mine * pitch + 8 + mis - sl * slice;  // held[v]: token v
   uint32_t* const bits = held_masks + mine * mask_words;            // from the word of v0 on
-  const bool masked = busy && a.masks && (unsigned)mask_rows[mine] < (unsigned)a.mask_count && v0 < v1;
-  if (busy) {
+  if (mine < rows) {  // also where the row will turn out to be nobody's: its values do not wait for its sequence's number
     const T* in = static_cast<const T*>(a.in) + (first + mine) * a.in_row;
     for (int c = p0 + begin; c < p1; c += step)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(SmemAddr(held + c * PER - mis)), "l"(in + c * PER - mis) : "memory");
     for (int v = v0 + begin; v < head; v += step) held[v] = in[v];
     for (int v = tail + begin; v < v1; v += step) held[v] = in[v];
-    if (masked) {
-      const uint32_t* mask = a.masks + mask_rows[mine] * a.mask_stride + (v0 >> 5);
-      const int words = ((v1 - 1) >> 5) - (v0 >> 5) + 1;
-      for (int i = begin; i < words; i += step)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(SmemAddr(bits + i)), "l"(mask + i) : "memory");
-    }
+  }
+  __syncthreads();
+  const bool busy = mine < rows && (unsigned)seqs[min(mine, rows - 1)] < (unsigned)a.n;
+  const bool masked = busy && a.masks && (unsigned)mask_rows[mine] < (unsigned)a.mask_count && v0 < v1;
+  if (masked) {
+    const uint32_t* mask = a.masks + mask_rows[mine] * a.mask_stride + (v0 >> 5);
+    const int words = ((v1 - 1) >> 5) - (v0 >> 5) + 1;
+    for (int i = begin; i < words; i += step)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(SmemAddr(bits + i)), "l"(mask + i) : "memory");
   }
   for (int r = 0; (counts || biases) && r < rows;) {
     const int seq = seqs[r], from = r;
