@@ -655,6 +655,23 @@ def test_adjust_logits_many_rows_of_a_sequence_that_has_most_tokens(held, dtype)
         _within(out[i], want, bound)
 
 
+def test_adjust_logits_rows_beyond_32_bits():
+    """Rows, and histories, whose places pass 2^31 elements."""
+    g, V, apart = _gen(37), 1000, (1 << 31) + 40
+    x, h = torch.empty(2 * apart + V, dtype=BF16, device="cuda"), torch.empty((1 << 30) - 1 + 64, dtype=torch.int32, device="cuda")
+    rows = x.as_strided((3, V), (apart, 1))
+    rows.copy_(_normal(g, 3, V))
+    before, hold = rows.clone(), (1 << 30) - 1
+    h[:64], h[hold:] = 5, 9
+    held, seqs, pres = _ints([64, 64]), _ints([1, 0, 1]), torch.ones(2, device="cuda")
+    pkg.adjust_logits(pkg.BF16, x.data_ptr(), x.data_ptr(), 3, V, 2, sequences=seqs.data_ptr(), history=h.data_ptr(), history_stride=hold, history_lengths=held.data_ptr(),
+                      frequency=pres.data_ptr(), logits_stride=apart, out_stride=apart, stream=_stream())
+    want = before.clone()
+    for i, t in enumerate((9, 5, 9)):
+        want[i, t] = (before[i, t].float() - 64).to(BF16)  # the same two roundings: to 32 bits, to the type
+    assert torch.equal(rows, want)
+
+
 def test_operators_with_nothing_to_do():
     """Sequences without rows, rows without sequences, vocabularies of one token."""
     q = torch.full((4, 2, 64), 7.0, dtype=BF16, device="cuda")
