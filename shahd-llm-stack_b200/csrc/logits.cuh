@@ -4,17 +4,19 @@
 // Formed in 32 bits, rounded once.
 //
 // Bound by memory, next to it by instructions: a row is read once and written once. A block of threads takes a slice of the tokens of a
-// few rows into shared memory (asynchronous copies). While it comes, each warp looks through a part of the history, puts the tokens that
-// lie in the slice on a list of its own, and counts them: whole numbers, so the order of the atomics does not matter. Behind a barrier
-// it takes its list's counts out of the table, which empties it, and does what is to be done for those that it found there:
-// of all that meet a token one. Then the rows go out in 16-byte pieces as the masks leave them. Rows of one sequence (drafted rows) share
-// counts and lists. The history is read by every slice's block, from the cache but for the first: 4 bytes a token, four a load where it
-// is aligned.
+// few rows into shared memory (asynchronous copies). While it comes, each warp looks through a part of the history and counts the tokens that
+// lie in the slice in a table: whole numbers, so the order of the atomics does not matter. Where rows are on their own it puts them on a
+// list of its own first; in groups it lists, behind a barrier, what its part of the table holds. Then it takes its list's counts out of the
+// table, which empties it, and does what is to be done for those that it found there: of all that meet a token one. Then the rows
+// go out in 16-byte pieces as the masks leave them. Rows of one sequence (drafted rows) share counts and lists. The history is read by every
+// slice's block, from the cache but for the first: 4 bytes a token, four a load where it is aligned.
 //
-// Measured, in one graph: 512 rows of 50257 bf16, four to a sequence of 4000 to 8000 tokens: 44.2 us for 108 MB, and half of the issue slots: 13 blocks
-// look through each history. 256 rows of 32768 f32 with histories of 1000 to 2000: 20.9 us for 69 MB. What else was timed on the first: a look into the
-// table for every value that goes out 54 us, the few values put right in global memory behind the copy 78, tables of 2048 or 8192 tokens and
-// blocks of 512 threads slower than 44.2, all of the history in flight no faster. 64 rows of 4096 f32: 4.0 us, latency.
+// Measured, in one graph, data from memory: 512 rows of 50257 bf16, four to a sequence of 4000 to 8000 tokens: 41 us for 108 MB, without the
+// history 27: 13 blocks look through each. 256 rows of 32768 f32 with histories of 1000 to 2000: 26.7 us for 69 MB, without the history
+// 19. From the cache: 39.8 and 20.9. What else was timed on the first, from the cache: a look into the table for every value that goes
+// out 54 us, the few values put right in global memory behind the copy 78, all that it met on lists 44.4, tables of 2048 or 8192
+// tokens and blocks of 512 threads slower than that, all of the history in flight no faster, a cluster's blocks that share the history
+// and count in one another's tables 57. 64 rows of 4096 f32: 4.0 us, latency.
 #pragma once
 
 #include "rows.cuh"
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GR
 }
 
 // Rows on their own: blocks of 128 threads, twice as many at a time, so that the steps of one run under the copies of others, and each
-// warp lists the history's tokens that it met, since a row meets few (256 rows of 32768 f32: 20.9 us; with 256 threads 24.3; looking for them
+// warp lists the history's tokens that it met, since a row meets few (256 rows of 32768 f32, all from the cache: 20.9 us; with 256 threads 24.3; looking for them
 // in the table 25.5). Groups: 256 threads, since four rows take the shared memory (512 rows of 50257 bf16: with 128 60 us), and
 // the tokens are looked for in the table, which costs a lane less than a list of all that it met (39.5 us, with such lists 44.4).
 template <class T, bool WIDE, bool GROUPS>

@@ -10,9 +10,9 @@
 //
 // The numbers are found in a few steps (mark, look through, deal out): latency. Up to 32768 pages and table entries one block of
 // threads does it, with all that it keeps in shared memory; larger ones take a cluster of blocks of threads with cluster barriers between
-// the steps and the workspace for what is kept (32 beams over 320 pages, copies included: 6.4 us, as a cluster 10.5; 256 sequences,
+// the steps and the workspace for what is kept (from the cache: 32 beams over 320 pages, copies included: 6.4 us, as a cluster 10.5; 256 sequences,
 // 4200 pages: 12.2 and 15.7). The copies are bound by memory, in a second kernel over all multiprocessors (112 partly filled
-// pages of 1 MiB, 112 MB moved, calls in a row, so that much of it stays in the L2 cache: 19.2 us the whole call, 5.8 TB/s).
+// pages of 1 MiB, 112 MB moved: 21.0 us the whole call, 5.3 TB/s, 19.3 where the L2 cache holds them).
 #pragma once
 
 #include "rows.cuh"
