@@ -521,7 +521,7 @@ int64_t shahd_pages_workspace(int32_t pages, int32_t new_n);
  * keeps. Fresh pages, copies' among them, are the free ones in ascending order, dealt out sequence by sequence, each one's in
  * the order of its positions; where they run out, entries are -1 and missing counts them, with the pages that max_blocks has no
  * place for. A copy that is missing means that the sequence has lost its last positions: the old table and its pages are as they
- * were, fork fewer sequences from it. Other entries of the new table are -1; kept entries that name no page stay as they are. What no
+ * were, fork fewer sequences from it. Neither new_table nor missing may overlap what is read. Other entries of the new table are -1; kept entries that name no page stay as they are. What no
  * new sequence goes on with is free for the next call that is given the new table. Not for the pool of a FusedAttention
  * operator, whose slots own their pages. */
 int shahd_pages_fork(const ShahdForkCall* call, void* stream);

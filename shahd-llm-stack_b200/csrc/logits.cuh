@@ -216,25 +216,25 @@ __global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GR
       constexpr uint32_t kPrompt = 0x8000u;
       // four tokens a lane, from place i[j] of the history each (INT32_MIN is no token of any table)
       const auto meet = [&](const int (&token)[4], const int (&i)[4]) {
-        uint32_t t[4], flag[4];
         if constexpr (GROUPS) {
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const uint32_t at = (uint32_t)token[j] - (uint32_t)base;
             if (at < (uint32_t)a.table) count(at, i[j] < prompt);
           }
-          return;
-        }
+        } else {
+          uint32_t t[4], flag[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          t[j] = (uint32_t)token[j] - (uint32_t)base;
-          flag[j] = i[j] < prompt ? kPrompt : 0u;
-        }
-        if (enlist(std::integral_constant<int, 4>(), t, flag)) return;
-        overflow = 1;
+          for (int j = 0; j < 4; j++) {
+            t[j] = (uint32_t)token[j] - (uint32_t)base;
+            flag[j] = i[j] < prompt ? kPrompt : 0u;
+          }
+          if (enlist(std::integral_constant<int, 4>(), t, flag)) return;
+          overflow = 1;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (t[j] < (uint32_t)a.table) count(t[j], flag[j] != 0);
+          for (int j = 0; j < 4; j++)
+            if (t[j] < (uint32_t)a.table) count(t[j], flag[j] != 0);
+        }
       };
       const int fours = reinterpret_cast<uintptr_t>(h) % 16 == 0 ? length / 4 : 0;
 #pragma unroll 1
