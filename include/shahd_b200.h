@@ -515,15 +515,14 @@ typedef struct ShahdForkCall {
 /* Bytes of workspace for a fork (or, with new_n 0, for shahd_pages_compact), or a negative status; no device is asked. */
 int64_t shahd_pages_workspace(int32_t pages, int32_t new_n);
 /* New sequence i keeps the first keep[i] positions of parents[i] and gets pages for positions up to need[i]. A page is held when some
- * sequence of the old table names it among its first ceil(length / 64) entries; the others are free. Kept pages are shared by
- * number. A page that is partly filled, in which a sequence is to go on (need > keep, keep no multiple of 64), stays with it when
- * every new sequence that names the page goes on in it, and it is the first of them; otherwise it gets a copy of the positions it
- * keeps. Fresh pages, copies' among them, are the free ones in ascending order, dealt out sequence by sequence, each one's in
- * the order of its positions; where they run out, entries are -1 and missing counts them, with the pages that max_blocks has no
- * place for. A copy that is missing means that the sequence has lost its last positions: the old table and its pages are as they
- * were, fork fewer sequences from it. Neither new_table nor missing may overlap what is read. Other entries of the new table are -1; kept entries that name no page stay as they are. What no
- * new sequence goes on with is free for the next call that is given the new table. Not for the pool of a FusedAttention
- * operator, whose slots own their pages. */
+ * sequence of the old table names it among its first ceil(length / 64) entries; the others are free. Kept pages are shared by number. A page
+ * that is partly filled, in which a sequence is to go on (need > keep, keep no multiple of 64), stays with it when every new sequence that
+ * names the page goes on in it, and it is the first of them; otherwise it gets a copy of the positions it keeps. Fresh pages, copies' among
+ * them, are the free ones in ascending order, dealt out sequence by sequence, each one's in the order of its positions; where they run out,
+ * entries are -1 and missing counts them, with the pages that max_blocks has no place for. A copy that is missing means that the sequence
+ * has lost its last positions: the old table and its pages are as they were, fork fewer sequences from it. Neither new_table nor missing may
+ * overlap what is read. Other entries of the new table are -1; kept entries that name no page stay as they are. What no new sequence goes on
+ * with is free for the next call that is given the new table. Not for the pool of a FusedAttention operator, whose slots own their pages. */
 int shahd_pages_fork(const ShahdForkCall* call, void* stream);
 
 typedef struct ShahdCompactCall {

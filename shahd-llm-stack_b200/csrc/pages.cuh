@@ -8,11 +8,14 @@
 //     one: so no copy reads what another one writes.
 // Compact: of U held pages those numbered U and up move into the holes below U, both in ascending order.
 //
-// The numbers are found in a few steps (mark, look through, deal out): latency. Up to 32768 pages and table entries one block of
-// threads does it, with all that it keeps in shared memory; larger ones take a cluster of blocks of threads with cluster barriers between
-// the steps and the workspace for what is kept (from the cache: 32 beams over 320 pages, copies included: 6.4 us, as a cluster 10.5; 256 sequences,
-// 4200 pages: 12.2 and 15.7). The copies are bound by memory, in a second kernel over all multiprocessors (112 partly filled
-// pages of 1 MiB, 112 MB moved: 21.0 us the whole call, 5.3 TB/s, 19.3 where the L2 cache holds them).
+// The numbers are found in a few steps (mark, look through, deal out): latency; the copies are bound by memory. Up to 32768 pages and table
+// entries a fork is one kernel, in which every block of threads finds all the numbers for itself, in shared memory, then writes its share of
+// the table and copies its share of the pages (32 beams over 320 pages, copies included: 4.2 us, with the numbers found by one block and the
+// copies in a second kernel 6.3; 112 partly filled pages of 1 MiB, 112 MB moved: 17.9 us, 6.3 TB/s, and 21.0). Larger ones take a
+// cluster of blocks of threads with cluster barriers between the steps, the workspace for what is kept, and a second kernel that
+// copies (10.5 us for the beams). Compactions: one block of threads finds the numbers, or the cluster, and a second kernel copies, since
+// a table that is compacted in place cannot be read by one block while another writes it (256 sequences, 4200 pages: 17.4 us, from the cache
+// 12.2 and 15.7).
 #pragma once
 
 #include "rows.cuh"
@@ -210,13 +213,17 @@ __global__ void __launch_bounds__(kPagesThreads) PlanPagesKernel(const __grid_co
 
 constexpr int kPagesSmall = 32768;  // pages, and entries of either table, that one block of threads sees to
 constexpr int kPagesSmallRows = 1024;
+constexpr int kNoCopy = -2;
 
 // What one block of threads holds in shared memory.
 struct PagesShared {
   uint32_t held[kPagesSmall / 32], read[kPagesSmall / 32];
   int ahead[kPagesSmall / 32];  // free pages before a word's; compact: holes below U
   int4 rows[kPagesSmallRows];   // fork: of the new sequences the parent's place in the table, whether it goes on in a page, kept blocks, blocks to have
-  int start[kPagesSmall / 32];  // compact: rank of a word's first held page among those that move
+  int start[kPagesSmall / 32];  // compact: rank of a word's first held page among those that move; fork: number of a new sequence's first fresh page
+  int to[kPagesSmallRows];      // fork: where a new sequence's page is copied to; -1: there is none for it, kNoCopy: nothing to copy
+  int from[kPagesSmallRows];    // fork: that page
+  int copying[kPagesSmallRows];  // fork: the new sequences that copy
   int warps[32];
   int first[1];                 // [pages] fork: the first new sequence that would write into a page
 };
@@ -247,22 +254,84 @@ __device__ __forceinline__ int NthFree(const PagesShared& s, int words, int k) {
   return lo * 32 + NthBit(~s.held[lo], k - s.ahead[lo]);
 }
 
-template <bool FORK>
-__global__ void __launch_bounds__(kPagesThreads) PlanPagesSmallKernel(const __grid_constant__ PagesArgs a) {
+// e / blocks, exact for e below 2^21: (e + 1/2) / blocks is further from whole numbers than its rounding.
+struct RowOf {
+  float per;
+  __device__ __forceinline__ RowOf(int blocks) : per(1.f / (float)blocks) {}
+  __device__ __forceinline__ int operator()(int e) const { return (int)(((float)e + 0.5f) * per); }
+};
+
+__global__ void __launch_bounds__(kPagesThreads) PlanCompactSmallKernel(const __grid_constant__ PagesArgs a) {
+  extern __shared__ __align__(16) uint8_t pages_raw[];
+  PagesShared& s = *reinterpret_cast<PagesShared*>(pages_raw);
+  const int t = threadIdx.x, most = a.max_blocks * kOpsPage, entries = a.n * a.max_blocks;
+  const RowOf row_of(a.max_blocks);
+  for (int w = t; w < a.words; w += kPagesThreads) s.held[w] = 0;
+  GridDepWait();
+  __syncthreads();
+  // ---- which pages are held ----
+#pragma unroll 4
+  for (int e = t; e < entries; e += kPagesThreads) {
+    const int q = row_of(e), b = e - q * a.max_blocks, page = a.table[e];
+    if (b < Blocks(min(max(a.lengths[q], 0), most)) && (unsigned)page < (unsigned)a.pages) atomicOr(&s.held[page >> 5], 1u << (page & 31));
+  }
+  __syncthreads();
+  // ---- holes below U in order, and the held pages that go there ----
+  uint32_t bits = 0, there = 0;
+  if (t < a.words) {
+    bits = s.held[t];
+    there = a.pages - 32 * t < 32 ? (1u << (a.pages - 32 * t)) - 1 : 0xffffffffu;
+  }
+  int free = 0, used = 0;
+  BlockScan(__popc(bits), s.warps, used);
+  const int base = 32 * t;  // holes: free pages below U
+  there = used <= base ? 0 : used - base < 32 ? there & ((1u << (used - base)) - 1) : there;
+  const int ahead = BlockScan(__popc(~bits & there), s.warps, free);
+  if (t < a.words) s.ahead[t] = ahead;
+  // held pages from U on, by their rank among them: those in front of each word (the word that U lies in has some below U, too)
+  const uint32_t behind = t < a.words ? bits & ~there : 0;
+  int all = 0;
+  const int rank = BlockScan(__popc(behind), s.warps, all);
+  if (t < a.words) s.start[t] = rank - __popc(bits & there);
+  __syncthreads();
+  GridDepLaunch();
+  if (t == 0) {
+    a.count[0] = used;
+    a.count[1] = free;  // as many pages move as there are holes
+    *a.used = used;
+  }
+  for (int p = used + t; p < a.pages; p += kPagesThreads) {
+    const int w = p >> 5;
+    if (!(s.held[w] >> (p & 31) & 1)) continue;
+    const int m = s.start[w] + __popc(s.held[w] & ((1u << (p & 31)) - 1)), to = NthFree(s, a.words, m);
+    a.copies[m] = PageCopy{p, to, kOpsPage};
+    a.first[p] = to;
+  }
+}
+
+struct CopyArgs {
+  uint16_t* pool;
+  long long page_stride, layer_stride;  // values
+  int layers, parts, d;                 // parts: blocks of 64 positions of a layer (K and V of each head)
+  const PageCopy* copies;
+  const int* count;  // copies in all, or null: `most`
+  int most, split;   // split: blocks of threads that share a layer of a copy
+};
+
+// A fork that one block of threads can plan: every block plans all of it for itself, then writes its share of the table and copies its share
+// of the pages, a part (64 positions of a layer's head) a warp. Nothing passes between blocks of threads.
+__global__ void __launch_bounds__(kPagesThreads) ForkPagesSmallKernel(const __grid_constant__ CopyArgs c, const __grid_constant__ PagesArgs a) {
   extern __shared__ __align__(16) uint8_t pages_raw[];
   PagesShared& s = *reinterpret_cast<PagesShared*>(pages_raw);
   const int t = threadIdx.x, most = a.max_blocks * kOpsPage, old_entries = a.n * a.max_blocks, new_entries = a.new_n * a.max_blocks;
-  const float per = 1.f / (float)a.max_blocks;
-  // e / max_blocks, exact for e below 2^21: (e + 1/2) / max_blocks is further from whole numbers than its rounding
-  const auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * per); };
+  const RowOf row_of(a.max_blocks);
   for (int w = t; w < a.words; w += kPagesThreads) s.held[w] = s.read[w] = 0;
-  if (FORK)
-    for (int p = t; p < a.pages; p += kPagesThreads) s.first[p] = 0x7fffffff;
+  for (int p = t; p < a.pages; p += kPagesThreads) s.first[p] = 0x7fffffff;
   GridDepWait();
-  int4 mine = make_int4(0, 0, 0, 0);  // fork: of new sequence t
+  int4 mine = make_int4(0, 0, 0, 0);  // of new sequence t
   bool writes = false;
   int keep = 0, beyond = 0;
-  if (FORK && t < a.new_n) {
+  if (t < a.new_n) {
     const Fork f(a, t);
     writes = f.writes;
     keep = f.keep;
@@ -277,17 +346,15 @@ __global__ void __launch_bounds__(kPagesThreads) PlanPagesSmallKernel(const __gr
     const int q = row_of(e), b = e - q * a.max_blocks, page = a.table[e];
     if (b < Blocks(min(max(a.lengths[q], 0), most)) && (unsigned)page < (unsigned)a.pages) atomicOr(&s.held[page >> 5], 1u << (page & 31));
   }
-  if constexpr (FORK) {
 #pragma unroll 4
-    for (int e = t; e < new_entries; e += kPagesThreads) {
-      const int i = row_of(e), b = e - i * a.max_blocks;
-      const int4 f = s.rows[i];
-      if (b >= f.z) continue;
-      const int page = a.table[f.x + b];
-      if ((unsigned)page >= (unsigned)a.pages) continue;
-      if (f.y && b == f.z - 1) atomicMin(&s.first[page], i);
-      else atomicOr(&s.read[page >> 5], 1u << (page & 31));
-    }
+  for (int e = t; e < new_entries; e += kPagesThreads) {
+    const int i = row_of(e), b = e - i * a.max_blocks;
+    const int4 f = s.rows[i];
+    if (b >= f.z) continue;
+    const int page = a.table[f.x + b];
+    if ((unsigned)page >= (unsigned)a.pages) continue;
+    if (f.y && b == f.z - 1) atomicMin(&s.first[page], i);
+    else atomicOr(&s.read[page >> 5], 1u << (page & 31));
   }
   __syncthreads();
   // ---- free pages in order; what the new sequences want of them, and what is to be copied ----
@@ -296,67 +363,62 @@ __global__ void __launch_bounds__(kPagesThreads) PlanPagesSmallKernel(const __gr
     bits = s.held[t];
     there = a.pages - 32 * t < 32 ? (1u << (a.pages - 32 * t)) - 1 : 0xffffffffu;
   }
-  int free = 0, used = 0;
-  if constexpr (!FORK) {
-    BlockScan(__popc(bits), s.warps, used);
-    const int base = 32 * t;  // holes: free pages below U
-    there = used <= base ? 0 : used - base < 32 ? there & ((1u << (used - base)) - 1) : there;
-  }
+  int free = 0, total = 0;
   const int ahead = BlockScan(__popc(~bits & there), s.warps, free);
   if (t < a.words) s.ahead[t] = ahead;
-  if constexpr (FORK) {
-    int page = -1;
-    if (writes) page = a.table[mine.x + mine.z - 1];
-    const bool copy = writes && (unsigned)page < (unsigned)a.pages && ((s.read[page >> 5] >> (page & 31) & 1) != 0 || s.first[page] != t);
-    const int wants = mine.w - mine.z + (copy ? 1 : 0);
-    int total = 0;
-    const int start = BlockScan(wants, s.warps, total);  // (s.ahead is there behind its barriers)
-    GridDepLaunch();
-    if (t < a.new_n) {
-      a.start[t] = start;
-      a.missing[t] = wants - min(max(free - start, 0), wants) + beyond;
-      PageCopy c = {0, 0, 0};
-      if (copy) {
-        if (start < free) c = {page, NthFree(s, a.words, start), keep % kOpsPage};
-        else c.to = -1;
-      }
-      a.copies[t] = c;
+  int page = -1;
+  if (writes) page = a.table[mine.x + mine.z - 1];
+  const bool copy = writes && (unsigned)page < (unsigned)a.pages && ((s.read[page >> 5] >> (page & 31) & 1) != 0 || s.first[page] != t);
+  const int wants = mine.w - mine.z + (copy ? 1 : 0);
+  constexpr int kOne = 1 << 20;  // more than all that is wanted: 32768 entries and 1024 copies
+  const int before = BlockScan(wants + (copy ? kOne : 0), s.warps, total), start = before % kOne, copies = total / kOne;
+  GridDepLaunch();
+  if (t < a.new_n) {
+    s.start[t] = start;
+    s.to[t] = !copy ? kNoCopy : start < free ? NthFree(s, a.words, start) : -1;
+    s.from[t] = page;
+    if (copy) s.copying[before / kOne] = t;
+    if (blockIdx.x == 0) a.missing[t] = wants - min(max(free - start, 0), wants) + beyond;
+    s.rows[t].y = keep % kOpsPage;
+  }
+  __syncthreads();
+  // ---- this block's share of the table, and of the copies ----
+  for (int e = (int)blockIdx.x * kPagesThreads + t; e < new_entries; e += (int)gridDim.x * kPagesThreads) {
+    const int i = row_of(e), b = e - i * a.max_blocks, to = s.to[i], copied = to != kNoCopy;
+    const int4 f = s.rows[i];
+    int entry = -1;
+    if (b < f.z - copied) entry = a.table[f.x + b];
+    else if (b < f.z) entry = to;
+    else if (b < f.w) {
+      const int k = s.start[i] + copied + b - f.z;
+      if (k < free) entry = NthFree(s, a.words, k);
     }
-    if (t == 0) a.count[0] = free;
-    // the free pages that are wanted, in order
-    uint32_t left = ~bits & there;
-    for (int k = ahead; left != 0 && k < total; left &= left - 1) a.order[k++] = 32 * t + __ffs(left) - 1;
-  } else {
-    // held pages from U on, by their rank among them: those in front of each word (the word that U lies in has some below U, too)
-    const uint32_t behind = t < a.words ? bits & ~there : 0;
-    int all = 0;
-    const int rank = BlockScan(__popc(behind), s.warps, all);
-    if (t < a.words) s.start[t] = rank - __popc(bits & there);
-    __syncthreads();
-    GridDepLaunch();
-    if (t == 0) {
-      a.count[0] = used;
-      a.count[1] = free;  // as many pages move as there are holes
-      *a.used = used;
-    }
-    for (int p = used + t; p < a.pages; p += kPagesThreads) {
-      const int w = p >> 5;
-      if (!(s.held[w] >> (p & 31) & 1)) continue;
-      const int m = s.start[w] + __popc(s.held[w] & ((1u << (p & 31)) - 1)), to = NthFree(s, a.words, m);
-      a.copies[m] = PageCopy{p, to, kOpsPage};
-      a.first[p] = to;
+    a.new_table[e] = entry;
+  }
+  const uint32_t row16 = c.d / 8, warps = gridDim.x * (kPagesThreads / 32);  // row16: 16-byte pieces of a position
+  const uint32_t parts = c.parts, all = (uint32_t)copies * c.layers * parts;
+  uint32_t split = 1;  // warps that share a part, where there are more of them
+  while (split < 4 && 2 * split * all <= warps) split *= 2;
+  for (uint32_t u = (t >> 5) * gridDim.x + blockIdx.x; u < all * split; u += warps) {
+    const uint32_t share = u % split, whole = u / split, part = whole % parts, rest = whole / parts, which = rest / c.layers;
+    const int i = s.copying[which], to = s.to[i];
+    if (to < 0) continue;
+    const int4 f = s.rows[i];
+    const long long in_page = (rest - which * c.layers) * c.layer_stride + (long long)part * kOpsPage * c.d;
+    const uint4* in = reinterpret_cast<const uint4*>(c.pool + s.from[i] * c.page_stride + in_page);
+    uint4* out = reinterpret_cast<uint4*>(c.pool + to * c.page_stride + in_page);
+    const uint32_t run = f.y * row16;
+    for (uint32_t j = share * 128 + (t & 31); j < run; j += 128 * split) {
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (j + 32 * k < run) v[k] = in[j + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (j + 32 * k < run) out[j + 32 * k] = v[k];
     }
   }
 }
-
-struct CopyArgs {
-  uint16_t* pool;
-  long long page_stride, layer_stride;  // values
-  int layers, parts, d;                 // parts: blocks of 64 positions of a layer (K and V of each head)
-  const PageCopy* copies;
-  const int* count;  // copies in all, or null: `most`
-  int most, split;   // split: blocks of threads that share a layer of a copy
-};
 
 // The entries of the new tables, and copies of the first `lines` positions of every part of a page.
 template <bool FORK>
@@ -462,7 +524,7 @@ inline bool CheckPool(const char* op, const ShahdPagePool& p) {
   return true;
 }
 
-// The cluster that finds the numbers, then the copies.
+// One kernel for a fork that blocks of threads can plan each for itself; else the numbers, then the copies.
 template <bool FORK>
 int LaunchPages(const char* op, const ShahdPagePool& pool, PagesArgs a, void* workspace, int sms, cudaStream_t st) {
   const PagesLayout l = LayPages(a.pages, a.new_n);
@@ -488,14 +550,22 @@ int LaunchPages(const char* op, const ShahdPagePool& pool, PagesArgs a, void* wo
   c.split = 1;  // a layer of a page is shared by blocks of threads down to 16 KiB, while there are few
   while (c.split * 1024 < c.parts * c.d * 8 && (long long)c.most * c.layers * c.split < 4 * sms) c.split *= 2;
   TakeLaunchError(nullptr);
-  if (a.pages <= kPagesSmall && std::max(a.n, a.new_n) * (long long)a.max_blocks <= kPagesSmall && a.new_n <= kPagesSmallRows) {
-    const size_t smem = sizeof(PagesShared) + (FORK ? 4 * (size_t)a.pages : 0);
-    if (EnsureKernelAttrs((const void*)PlanPagesSmallKernel<FORK>, (int)smem)) LaunchPdl(PlanPagesSmallKernel<FORK>, dim3(1), dim3(kPagesThreads), smem, st, a);
+  const long long entries = (long long)(FORK ? a.new_n : a.n) * a.max_blocks;
+  const long long units = (long long)a.new_n * c.layers * c.parts;  // of a fork's copies, at most
+  const bool small = a.pages <= kPagesSmall && std::max(a.n, a.new_n) * (long long)a.max_blocks <= kPagesSmall && a.new_n <= kPagesSmallRows && units < (1 << 28);
+  if (FORK && small) {  // eight units, four warps each, or a thousand entries a block of threads, and no more blocks than multiprocessors
+    const int smem = (int)sizeof(PagesShared) + 4 * a.pages;
+    const int blocks = (int)std::min<long long>(std::max(units / 8 + 1, (entries + kPagesThreads - 1) / kPagesThreads), sms);
+    if (EnsureKernelAttrs((const void*)ForkPagesSmallKernel, smem)) LaunchPdl(ForkPagesSmallKernel, dim3(blocks), dim3(kPagesThreads), (size_t)smem, st, c, a);
+    return LaunchStatus(op);
+  }
+  if (small) {
+    if (EnsureKernelAttrs((const void*)PlanCompactSmallKernel, (int)sizeof(PagesShared)))
+      LaunchPdl(PlanCompactSmallKernel, dim3(1), dim3(kPagesThreads), sizeof(PagesShared), st, a);
   } else {
     LaunchPdlCluster(PlanPagesKernel<FORK>, dim3(kPagesCluster), dim3(kPagesThreads), 0, dim3(kPagesCluster), st, a);
   }
   const long long items = (long long)c.most * c.layers * c.split;
-  const long long entries = (long long)(FORK ? a.new_n : a.n) * a.max_blocks;
   LaunchPdl(CopyPagesKernel<FORK>, dim3((unsigned)std::min<long long>(std::max(items, entries / kCopyThreads + 1), 8LL * sms)), dim3(kCopyThreads), 0, st, c, a);
   return LaunchStatus(op);
 }
