@@ -9,13 +9,12 @@
 // Compact: of U held pages those numbered U and up move into the holes below U, both in ascending order.
 //
 // The numbers are found in a few steps (mark, look through, deal out): latency; the copies are bound by memory. Up to 32768 pages and table
-// entries a fork is one kernel, in which every block of threads finds all the numbers for itself, in shared memory, then writes its share of
-// the table and copies its share of the pages (32 beams over 320 pages, copies included: 4.2 us, with the numbers found by one block and the
-// copies in a second kernel 6.3; 112 partly filled pages of 1 MiB, 112 MB moved: 17.9 us, 6.3 TB/s, and 21.0). Larger ones take a
-// cluster of blocks of threads with cluster barriers between the steps, the workspace for what is kept, and a second kernel that
-// copies (10.5 us for the beams). Compactions: one block of threads finds the numbers, or the cluster, and a second kernel copies, since
-// a table that is compacted in place cannot be read by one block while another writes it (256 sequences, 4200 pages: 17.4 us, from the cache
-// 12.2 and 15.7).
+// entries a call is one kernel, in which every block of threads finds all the numbers for itself, in shared memory, then writes its share of
+// the table and copies its share of the pages: 32 beams over 320 pages 4.2 us, with the numbers found by one block and the copies in a
+// second kernel 6.3; 112 partly filled pages of 1 MiB, 112 MB moved, 17.9 us, 6.3 TB/s, and 21.0; a compaction of 256 sequences over 4200
+// pages 15.7 and 17.4. Larger ones take a cluster of blocks of threads with cluster barriers between the steps, the workspace for what is
+// kept, and a second kernel that copies (10.5 us for the beams), and so do compactions in place, whose table one block cannot read while
+// another writes it.
 #pragma once
 
 #include "rows.cuh"
@@ -225,7 +224,7 @@ struct PagesShared {
   int from[kPagesSmallRows];    // fork: that page
   int copying[kPagesSmallRows];  // fork: the new sequences that copy
   int warps[32];
-  int first[1];                 // [pages] fork: the first new sequence that would write into a page
+  int first[1];                 // [pages] fork: the first new sequence that would write into a page; compact: what moves, and where it goes
 };
 
 // The k-th (from 0) set bit of `bits`.
@@ -261,54 +260,6 @@ struct RowOf {
   __device__ __forceinline__ int operator()(int e) const { return (int)(((float)e + 0.5f) * per); }
 };
 
-__global__ void __launch_bounds__(kPagesThreads) PlanCompactSmallKernel(const __grid_constant__ PagesArgs a) {
-  extern __shared__ __align__(16) uint8_t pages_raw[];
-  PagesShared& s = *reinterpret_cast<PagesShared*>(pages_raw);
-  const int t = threadIdx.x, most = a.max_blocks * kOpsPage, entries = a.n * a.max_blocks;
-  const RowOf row_of(a.max_blocks);
-  for (int w = t; w < a.words; w += kPagesThreads) s.held[w] = 0;
-  GridDepWait();
-  __syncthreads();
-  // ---- which pages are held ----
-#pragma unroll 4
-  for (int e = t; e < entries; e += kPagesThreads) {
-    const int q = row_of(e), b = e - q * a.max_blocks, page = a.table[e];
-    if (b < Blocks(min(max(a.lengths[q], 0), most)) && (unsigned)page < (unsigned)a.pages) atomicOr(&s.held[page >> 5], 1u << (page & 31));
-  }
-  __syncthreads();
-  // ---- holes below U in order, and the held pages that go there ----
-  uint32_t bits = 0, there = 0;
-  if (t < a.words) {
-    bits = s.held[t];
-    there = a.pages - 32 * t < 32 ? (1u << (a.pages - 32 * t)) - 1 : 0xffffffffu;
-  }
-  int free = 0, used = 0;
-  BlockScan(__popc(bits), s.warps, used);
-  const int base = 32 * t;  // holes: free pages below U
-  there = used <= base ? 0 : used - base < 32 ? there & ((1u << (used - base)) - 1) : there;
-  const int ahead = BlockScan(__popc(~bits & there), s.warps, free);
-  if (t < a.words) s.ahead[t] = ahead;
-  // held pages from U on, by their rank among them: those in front of each word (the word that U lies in has some below U, too)
-  const uint32_t behind = t < a.words ? bits & ~there : 0;
-  int all = 0;
-  const int rank = BlockScan(__popc(behind), s.warps, all);
-  if (t < a.words) s.start[t] = rank - __popc(bits & there);
-  __syncthreads();
-  GridDepLaunch();
-  if (t == 0) {
-    a.count[0] = used;
-    a.count[1] = free;  // as many pages move as there are holes
-    *a.used = used;
-  }
-  for (int p = used + t; p < a.pages; p += kPagesThreads) {
-    const int w = p >> 5;
-    if (!(s.held[w] >> (p & 31) & 1)) continue;
-    const int m = s.start[w] + __popc(s.held[w] & ((1u << (p & 31)) - 1)), to = NthFree(s, a.words, m);
-    a.copies[m] = PageCopy{p, to, kOpsPage};
-    a.first[p] = to;
-  }
-}
-
 struct CopyArgs {
   uint16_t* pool;
   long long page_stride, layer_stride;  // values
@@ -317,6 +268,33 @@ struct CopyArgs {
   const int* count;  // copies in all, or null: `most`
   int most, split;   // split: blocks of threads that share a layer of a copy
 };
+
+// This block's share of `copies` copies, which copy_of numbers; a part (64 positions of a layer's head) a warp.
+template <class F>
+__device__ __forceinline__ void CopyParts(const CopyArgs& c, int copies, const F& copy_of) {
+  const uint32_t row16 = c.d / 8, warps = gridDim.x * (blockDim.x / 32);  // row16: 16-byte pieces of a position
+  const uint32_t parts = c.parts, all = (uint32_t)copies * c.layers * parts;
+  uint32_t split = 1;  // warps that share a part, where there are more of them
+  while (split < 4 && 2 * split * all <= warps) split *= 2;
+  for (uint32_t u = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; u < all * split; u += warps) {
+    const uint32_t share = u % split, whole = u / split, part = whole % parts, rest = whole / parts, which = rest / c.layers;
+    const PageCopy copy = copy_of(which);
+    if (copy.to < 0) continue;
+    const long long in_page = (rest - which * c.layers) * c.layer_stride + (long long)part * kOpsPage * c.d;
+    const uint4* in = reinterpret_cast<const uint4*>(c.pool + copy.from * c.page_stride + in_page);
+    uint4* out = reinterpret_cast<uint4*>(c.pool + copy.to * c.page_stride + in_page);
+    const uint32_t run = copy.lines * row16;
+    for (uint32_t j = share * 128 + (threadIdx.x & 31); j < run; j += 128 * split) {
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (j + 32 * k < run) v[k] = in[j + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (j + 32 * k < run) out[j + 32 * k] = v[k];
+    }
+  }
+}
 
 // A fork that one block of threads can plan: every block plans all of it for itself, then writes its share of the table and copies its share
 // of the pages, a part (64 positions of a layer's head) a warp. Nothing passes between blocks of threads.
@@ -395,29 +373,66 @@ __global__ void __launch_bounds__(kPagesThreads) ForkPagesSmallKernel(const __gr
     }
     a.new_table[e] = entry;
   }
-  const uint32_t row16 = c.d / 8, warps = gridDim.x * (kPagesThreads / 32);  // row16: 16-byte pieces of a position
-  const uint32_t parts = c.parts, all = (uint32_t)copies * c.layers * parts;
-  uint32_t split = 1;  // warps that share a part, where there are more of them
-  while (split < 4 && 2 * split * all <= warps) split *= 2;
-  for (uint32_t u = (t >> 5) * gridDim.x + blockIdx.x; u < all * split; u += warps) {
-    const uint32_t share = u % split, whole = u / split, part = whole % parts, rest = whole / parts, which = rest / c.layers;
-    const int i = s.copying[which], to = s.to[i];
-    if (to < 0) continue;
-    const int4 f = s.rows[i];
-    const long long in_page = (rest - which * c.layers) * c.layer_stride + (long long)part * kOpsPage * c.d;
-    const uint4* in = reinterpret_cast<const uint4*>(c.pool + s.from[i] * c.page_stride + in_page);
-    uint4* out = reinterpret_cast<uint4*>(c.pool + to * c.page_stride + in_page);
-    const uint32_t run = f.y * row16;
-    for (uint32_t j = share * 128 + (t & 31); j < run; j += 128 * split) {
-      uint4 v[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (j + 32 * k < run) v[k] = in[j + 32 * k];
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (j + 32 * k < run) out[j + 32 * k] = v[k];
-    }
+  CopyParts(c, copies, [&](uint32_t which) {
+    const int i = s.copying[which];
+    return PageCopy{s.from[i], s.to[i], s.rows[i].y};
+  });
+}
+
+// A compaction that one block of threads can plan, into another table, in the same manner.
+__global__ void __launch_bounds__(kPagesThreads) CompactPagesSmallKernel(const __grid_constant__ CopyArgs c, const __grid_constant__ PagesArgs a) {
+  extern __shared__ __align__(16) uint8_t pages_raw[];
+  PagesShared& s = *reinterpret_cast<PagesShared*>(pages_raw);
+  const int t = threadIdx.x, most = a.max_blocks * kOpsPage, entries = a.n * a.max_blocks;
+  const RowOf row_of(a.max_blocks);
+  for (int w = t; w < a.words; w += kPagesThreads) s.held[w] = 0;
+  GridDepWait();
+  __syncthreads();
+  // ---- which pages are held ----
+#pragma unroll 4
+  for (int e = t; e < entries; e += kPagesThreads) {
+    const int q = row_of(e), b = e - q * a.max_blocks, page = a.table[e];
+    if (b < Blocks(min(max(a.lengths[q], 0), most)) && (unsigned)page < (unsigned)a.pages) atomicOr(&s.held[page >> 5], 1u << (page & 31));
   }
+  __syncthreads();
+  // ---- holes below U in order, and the held pages that go there ----
+  uint32_t bits = 0, there = 0;
+  if (t < a.words) {
+    bits = s.held[t];
+    there = a.pages - 32 * t < 32 ? (1u << (a.pages - 32 * t)) - 1 : 0xffffffffu;
+  }
+  int free = 0, used = 0;
+  BlockScan(__popc(bits), s.warps, used);
+  const int base = 32 * t;  // holes: free pages below U
+  there = used <= base ? 0 : used - base < 32 ? there & ((1u << (used - base)) - 1) : there;
+  const int ahead = BlockScan(__popc(~bits & there), s.warps, free);
+  if (t < a.words) s.ahead[t] = ahead;
+  // held pages from U on, by their rank among them: those in front of each word (the word that U lies in has some below U, too)
+  const uint32_t behind = t < a.words ? bits & ~there : 0;
+  int all = 0;
+  const int rank = BlockScan(__popc(behind), s.warps, all);
+  if (t < a.words) s.start[t] = rank - __popc(bits & there);
+  __syncthreads();
+  GridDepLaunch();
+  if (blockIdx.x == 0 && t == 0) *a.used = used;
+  // as many pages move as there are holes: from s.first[m], to s.first[free + m]; both lists together name pages once
+  const auto rank_of = [&](int p) { return s.start[p >> 5] + __popc(s.held[p >> 5] & ((1u << (p & 31)) - 1)); };
+  for (int p = used + t; p < a.pages; p += kPagesThreads) {
+    if (!(s.held[p >> 5] >> (p & 31) & 1)) continue;
+    const int m = rank_of(p);
+    s.first[m] = p;
+    s.first[free + m] = NthFree(s, a.words, m);
+  }
+  __syncthreads();
+  // ---- this block's share of the table, and of the copies ----
+  for (int e = (int)blockIdx.x * kPagesThreads + t; e < entries; e += (int)gridDim.x * kPagesThreads) {
+    const int q = row_of(e), b = e - q * a.max_blocks;
+    int page = b < Blocks(min(max(a.lengths[q], 0), most)) ? a.table[e] : -1;
+    if ((unsigned)page >= (unsigned)a.pages) page = -1;
+    else if (page >= used) page = s.first[free + rank_of(page)];
+    a.new_table[e] = page;
+  }
+  CopyParts(c, free, [&](uint32_t m) { return PageCopy{s.first[m], s.first[free + m], kOpsPage}; });
 }
 
 // The entries of the new tables, and copies of the first `lines` positions of every part of a page.
@@ -524,7 +539,7 @@ inline bool CheckPool(const char* op, const ShahdPagePool& p) {
   return true;
 }
 
-// One kernel for a fork that blocks of threads can plan each for itself; else the numbers, then the copies.
+// One kernel for what blocks of threads can plan each for itself; else the numbers, then the copies.
 template <bool FORK>
 int LaunchPages(const char* op, const ShahdPagePool& pool, PagesArgs a, void* workspace, int sms, cudaStream_t st) {
   const PagesLayout l = LayPages(a.pages, a.new_n);
@@ -551,20 +566,17 @@ int LaunchPages(const char* op, const ShahdPagePool& pool, PagesArgs a, void* wo
   while (c.split * 1024 < c.parts * c.d * 8 && (long long)c.most * c.layers * c.split < 4 * sms) c.split *= 2;
   TakeLaunchError(nullptr);
   const long long entries = (long long)(FORK ? a.new_n : a.n) * a.max_blocks;
-  const long long units = (long long)a.new_n * c.layers * c.parts;  // of a fork's copies, at most
+  const long long units = (long long)c.most * c.layers * c.parts;  // of the copies, at most
   const bool small = a.pages <= kPagesSmall && std::max(a.n, a.new_n) * (long long)a.max_blocks <= kPagesSmall && a.new_n <= kPagesSmallRows && units < (1 << 28);
-  if (FORK && small) {  // eight units, four warps each, or a thousand entries a block of threads, and no more blocks than multiprocessors
+  // eight units, four warps each, or a thousand entries a block of threads, and no more blocks than multiprocessors
+  if (small && (FORK || a.table != a.new_table)) {
     const int smem = (int)sizeof(PagesShared) + 4 * a.pages;
     const int blocks = (int)std::min<long long>(std::max(units / 8 + 1, (entries + kPagesThreads - 1) / kPagesThreads), sms);
-    if (EnsureKernelAttrs((const void*)ForkPagesSmallKernel, smem)) LaunchPdl(ForkPagesSmallKernel, dim3(blocks), dim3(kPagesThreads), (size_t)smem, st, c, a);
+    const auto kernel = FORK ? ForkPagesSmallKernel : CompactPagesSmallKernel;
+    if (EnsureKernelAttrs((const void*)kernel, smem)) LaunchPdl(kernel, dim3(blocks), dim3(kPagesThreads), (size_t)smem, st, c, a);
     return LaunchStatus(op);
   }
-  if (small) {
-    if (EnsureKernelAttrs((const void*)PlanCompactSmallKernel, (int)sizeof(PagesShared)))
-      LaunchPdl(PlanCompactSmallKernel, dim3(1), dim3(kPagesThreads), sizeof(PagesShared), st, a);
-  } else {
-    LaunchPdlCluster(PlanPagesKernel<FORK>, dim3(kPagesCluster), dim3(kPagesThreads), 0, dim3(kPagesCluster), st, a);
-  }
+  LaunchPdlCluster(PlanPagesKernel<FORK>, dim3(kPagesCluster), dim3(kPagesThreads), 0, dim3(kPagesCluster), st, a);
   const long long items = (long long)c.most * c.layers * c.split;
   LaunchPdl(CopyPagesKernel<FORK>, dim3((unsigned)std::min<long long>(std::max(items, entries / kCopyThreads + 1), 8LL * sms)), dim3(kCopyThreads), 0, st, c, a);
   return LaunchStatus(op);
