@@ -126,6 +126,20 @@ def test_fork_large(n, new_n, blocks, pages, layers):
     _check_fork(view, pool, table, lengths, parents, keep, [k + 1 for k in keep])
 
 
+@pytest.mark.parametrize("pages", [32767, 32768, 32769])
+def test_fork_and_compact_around_the_sizes_that_one_kernel_sees_to(pages):
+    """Tables of 32768 entries over as many pages, one less and one more."""
+    rng, g = np.random.default_rng(pages), _gen(17)
+    n, blocks = 64, 512
+    lengths = [int(rng.integers(0, blocks * 64 + 1)) for _ in range(n)]
+    view, pool = _pool(pages, 1, 1, 8, g)
+    table = rng.permutation(pages)[: (pages // 64) * 64].reshape(64, -1)
+    table = np.concatenate([table, np.full((n, blocks - table.shape[1]), -1)], 1) if table.shape[1] < blocks else table
+    parents, keep = rng.integers(0, n, n), rng.integers(0, blocks * 64 + 1, n)
+    _check_fork(view, pool, table, lengths, parents.tolist(), keep.tolist(), (keep + rng.integers(0, 300, n)).tolist())
+    _compact(view, pool, table, lengths)
+
+
 def test_fork_from_no_sequences_and_to_none():
     g = _gen(3)
     view, pool = _pool(5, 1, 1, 64, g)
