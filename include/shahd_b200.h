@@ -609,7 +609,8 @@ typedef struct ShahdLogitsCall {
   const int32_t* mask_rows;          /* [rows] the row's mask; not in 0 .. mask_count-1: none. Null: row r has mask r */
 } ShahdLogitsCall;
 /* x = logit of token v. With v in the sequence's history: x > 0 ? x / repetition : x * repetition; generated c times, c > 0: x -=
- * c * frequency + presence; x += bias; not allowed by the mask: -inf. In 32 bits, rounded once. */
+ * c * frequency + presence; x += bias; not allowed by the mask: -inf. Each of these steps is rounded to 32 bits (c * frequency + presence is
+ * one), the last one to dtype. */
 int shahd_adjust_logits(const ShahdLogitsCall* call, void* stream);
 
 #ifdef __cplusplus
