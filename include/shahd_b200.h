@@ -590,7 +590,7 @@ typedef struct ShahdLogitsCall {
   int32_t n;      /* sequences, 0 .. 2^20 */
   int32_t vocab;  /* 1 .. 2^24 */
   const void* logits;  /* [rows, vocab] */
-  void* out;           /* [rows, vocab]; may be logits, with the same stride */
+  void* out;           /* [rows, vocab]; may be logits, with the same stride; else no row may share memory with one of logits */
   int64_t logits_stride, out_stride; /* elements between rows, at least vocab */
   const int32_t* sequences;          /* [rows] the row's sequence; null: row r is sequence r. A row whose number is not in 0 .. n-1 is left as it is */
   const int32_t* history;            /* [n, history_stride] tokens of the prompt and then the generated ones; null: no penalties. Tokens outside

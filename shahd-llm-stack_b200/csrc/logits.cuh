@@ -374,6 +374,22 @@ void LaunchLogits(const LogitsArgs& a, bool wide, int smem, cudaStream_t st) {
   else wide ? LaunchLogitsAs<T, true, false>(a, smem, st) : LaunchLogitsAs<T, false, false>(a, smem, st);
 }
 
+// Whether some row of `out` shares bytes with some row of `in` (rows of `width` bytes, `in_row` and `out_row` apart, no row across the next one's
+// beginning). Rows that lie in the gaps of the others do not: two halves of one buffer.
+inline bool RowsOverlap(const void* in, const void* out, long long rows, long long width, long long in_row, long long out_row) {
+  const long long a = reinterpret_cast<long long>(in), b = reinterpret_cast<long long>(out);
+  if (b >= a + (rows - 1) * in_row + width || a >= b + (rows - 1) * out_row + width) return false;
+  // row i of `in` begins `ahead` bytes behind a row of `out`, and that many less than out_row before the next one
+  const long long look = in_row == out_row ? 1 : rows;  // the same for all of them
+  for (long long i = 0; i < look; i++) {
+    const long long apart = a + i * in_row - b, row = apart >= 0 ? apart / out_row : -((-apart + out_row - 1) / out_row), ahead = apart - row * out_row;
+    // with one stride, row i of `in` meets rows i + row and i + row + 1: some i has them as long as they are less than `rows` off
+    const long long least = in_row == out_row ? 1 - rows : 0;
+    if ((row >= least && row < rows && ahead < width) || (row + 1 >= least && row + 1 < rows && out_row - ahead < width)) return true;
+  }
+  return false;
+}
+
 }  // namespace shahd
 
 extern "C" {
@@ -418,6 +434,10 @@ int shahd_adjust_logits(const ShahdLogitsCall* c, void* stream) {
   }
   if (c->rows == 0 || c->n == 0) return SHAHD_OK;
   const size_t size = TypeBytes(c->dtype);
+  if (c->logits != c->out && RowsOverlap(c->logits, c->out, c->rows, (long long)c->vocab * size, c->logits_stride * size, c->out_stride * size)) {
+    SetError("%s: logits and out overlap; they may be one", op);
+    return SHAHD_EINVAL;
+  }
   BufferCheck b(op);
   b.Add("logits", c->logits, size);
   if (c->out != c->logits) b.Add("out", c->out, size);
