@@ -574,7 +574,9 @@ typedef struct ShahdChunkCall {
   int64_t workspace_bytes;
 } ShahdChunkCall;
 /* Bytes of workspace for a call with these rows, n, num_heads, max_rows and cache sizes (0: none), or a negative status; dtype, pointers and
- * scale are not looked at, and no device is asked. */
+ * scale are not looked at, and no device is asked. They do not grow with the sizes: a smaller call may be laid out in another way that needs
+ * more. No call with rows <= n * max_rows needs more than SHAHD_CHUNK_WORKSPACE_MOST. */
+#define SHAHD_CHUNK_WORKSPACE_MOST (40LL << 20)
 int64_t shahd_chunk_attention_workspace(const ShahdChunkCall* call);
 /* out[i] = sum over positions j <= lengths[s] + i of softmax_j(scale q[i].k[j]) v[j] over the cache of the row's sequence: parts of
  * prompts, and decode steps as chunks of one row, in one call. Positions at or beyond max_blocks * 64 and those on no page are not

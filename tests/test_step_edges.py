@@ -1,5 +1,6 @@
 """Refusals and sizes of the operators of a serving step over shared pages that the other tests do not reach, without a GPU."""
 import itertools
+import random
 
 import pytest
 
@@ -36,3 +37,22 @@ def test_logits_and_results_of_other_strides_that_share_memory():
             _refused("overlap", pkg.adjust_logits, **args)
         else:
             _no_device(pkg.adjust_logits, **args)
+
+
+def test_chunk_workspaces_of_any_size_fit_what_the_header_says():
+    """Steps of any n, rows and max_rows over tables of any width; smaller calls may need more than larger ones, none more than this."""
+    rng, most, some = random.Random(5), 40 << 20, 0
+    for _ in range(20000):
+        d, Hk, G = rng.choice((32, 64, 128)), rng.randint(1, 16), rng.randint(1, 8)
+        n, longest = int(2 ** rng.uniform(0, 11)), int(2 ** rng.uniform(0, 14))
+        rows, blocks = rng.randint(1, n * longest) if rng.random() < 0.7 else min(n * longest, n + rng.randint(0, 300)), int(2 ** rng.uniform(0, 12))
+        try:
+            size = pkg.chunk_attention_workspace(n, rows, longest, Hk * G, pkg.KvCache(AT, Hk * 2 * 64 * d, AT, blocks, 9, Hk, d))
+        except pkg._lib.ShahdError as e:
+            assert "too many rows or key blocks" in str(e)
+            continue
+        assert 0 <= size <= most, (d, Hk, G, n, longest, rows, blocks, size)
+        some += size > most // 2
+    assert some > 20  # the bound is not far above what there is
+    grows = [pkg.chunk_attention_workspace(n, rows, longest, 16, pkg.KvCache(AT, 4 * 2 * 64 * 64, AT, 64, 9, 4, 64)) for n, rows, longest in ((16, 32768, 2048), (1, 96, 96))]
+    assert grows[0] < grows[1]
