@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 from tests import serving_refs as R  # noqa: E402
 from tests import step_refs as S  # noqa: E402
 from tests.test_gpu_serving_ops import BF16, CODE, F16, F32, _cache_of, _gen, _held, _ints, _normal, _offsets, _rows, _stream, _within  # noqa: E402
-from tests.test_gpu_step_ops import _check_chunk, _chunk, _chunk_case  # noqa: E402
+from tests.test_gpu_step_ops import _check_chunk, _check_fork, _chunk, _chunk_case, _pool  # noqa: E402
 
 
 @pytest.fixture(autouse=True)
@@ -190,3 +190,20 @@ def test_chunks_of_many_pairs_of_tiles(heads, n, most_rows, blocks):
     _check_chunk(q, pool, table, lengths, rows, out, dtype, seqs={0, 2, 3, 4, 5, 6, n - 1})
     assert bool((out[sum(rows):] == 7.0).all())
     assert torch.equal(out, _chunk(q, cache, lengths, rows, dtype))
+
+
+# ---- pages ---------------------------------------------------------------------------------------------------------
+
+
+def test_room_that_a_fork_gave_is_free_again_unless_the_lengths_cover_it():
+    view, pool = _pool(12, 2, 1, 64, _gen(44))
+    table, missing_room = np.full((1, 6), -1, np.int64), [64, 64]
+    table[0, 0] = 5
+    room, _ = _check_fork(view, pool, table, [64], [0, 0], missing_room, [200, 300])
+    assert room.tolist() == [[5, 0, 1, 2, -1, -1], [5, 3, 4, 6, 7, -1]]
+    # by their cached positions alone the pages beyond are free, although the table names them
+    again, _ = _check_fork(view, pool, room, [64, 64], [1, 0], [64, 64], [128, 128])
+    assert again.tolist() == [[5, 0, -1, -1, -1, -1], [5, 1, -1, -1, -1, -1]]
+    # by lengths that cover the room they are held, and go with those that keep them
+    kept, _ = _check_fork(view, pool, room, [200, 300], [1, 0], [300, 200], [300, 384])
+    assert kept.tolist() == [[5, 3, 4, 6, 7, -1], [5, 0, 1, 2, 8, 9]]
