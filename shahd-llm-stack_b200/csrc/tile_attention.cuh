@@ -880,9 +880,13 @@ __global__ void __launch_bounds__(TaCfg<D>::kThreads, TaCfg<D>::kPerSm) TileAtte
   constexpr bool TREE = KIND != kPrompt, SPLIT = KIND == kChunkSplit, CHUNK = KIND == kChunkPairs || KIND == kChunkRanges || SPLIT, RANGES = KIND == kTreeRanges || KIND == kChunkRanges;
   using Cfg = TaCfg<D>;
   constexpr int U = Cfg::kUnits, KEYS = Cfg::kKeys;
-  // The softmax warps read what they work on from shared memory at every step instead of holding it in registers, which two blocks of
-  // threads on a multiprocessor do not have: the steps of 64 keys are a chain of latencies, and what is spilled lengthens it.
-  constexpr bool RELOAD = CHUNK && RANGES != TaCfg<D>::kWide;
+  // The softmax warps read what they work on from shared memory at every step instead of holding it in registers: at wide heads, whose rows
+  // of scores take them, and in ranges, which hold the walk's state besides. Pairs and clusters of narrow heads hold it: their steps of 64
+  // keys are a chain of latencies, which the reads lengthen. With reloads and without, in one graph: head_dim 64, ranges (4 chunks of 500 to
+  // 1024 over 3000 to 9000) 143 us and 157, pairs (16 chunks of 300 to 2048 from position 0) 118 and 110, tiles (the mixed step) 42.2 and 39.8, a
+  // cluster (96 rows over 1700) 11.7 and 11.2; head_dim 128, ranges (2 of 1024 over 12000) 454 and 497, pairs (4 of 2048 over 6000) 829 and
+  // 837, a cluster (96 rows over 1700) 19.8 and 21.2.
+  constexpr bool RELOAD = CHUNK && (RANGES || TaCfg<D>::kWide);
   extern __shared__ uint8_t ta_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = base;
