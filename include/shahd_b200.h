@@ -478,8 +478,9 @@ int shahd_verify_tree(const ShahdVerifyCall* call, void* stream);
 /* ================================================================================================
  * 4. A serving step over shared pages. The common rules of section 3 hold. The operators fit together, and with those above:
  *      shahd_pages_fork (new sequences go on from earlier ones) -> shahd_norm_rope_apply or shahd_rope_apply (the step's rows; k, v into
- *      the cache) -> shahd_chunk_attention -> (the model's logits) -> shahd_adjust_logits -> sampling,
- *    and shahd_pages_compact now and then.
+ *      the cache) -> shahd_chunk_attention -> (the model's logits) -> shahd_adjust_logits -> (sampling),
+ *    and shahd_pages_compact now and then. What stands in brackets is the caller's: shahd_sample_logits takes its rows from the host, in 32 bits,
+ *    and waits. They serve a model of the caller's own; a session's cache and logits stay inside it.
  * ============================================================================================== */
 
 /* ---- pages shared between sequences ---- */
