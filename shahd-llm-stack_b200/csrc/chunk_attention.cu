@@ -29,13 +29,13 @@ void LaunchChunks(const TaArgs& a, unsigned blocks, cudaStream_t st) {
 //   Pairs: a block of threads for every pair of tiles, longest first, where there are many of them. 16 chunks of 300 to 2048 rows from position
 //     0: 121 us, ranges 154, tiles 151.
 //   Tiles: a block of threads for every tile, its key blocks by turns: half as many steps, at twice the loads. Where pairs are few enough that
-//     the longest is what is waited for: 48 sequences, six of them with 200 to 512 rows, 0 to 1500 positions: 39 us, pairs 44, ranges 46; 8192
+//     the longest is what is waited for: 48 sequences, six of them with 200 to 512 rows, 0 to 1500 positions: 40 us, pairs 44, ranges 46; 8192
 //     rows from position 0: 198, pairs 208, ranges 218. At head_dim 128 the loads tell: 2 chunks of 1024 over 12000, 32/8 heads: 500, pairs and
-//     ranges 440 to 470.
+//     ranges 440 to 470 (454).
 //   Split: a cluster of 2 to 8 blocks of threads for every tile, where that leaves multiprocessors for all and the steps are few: one
 //     launch, no second kernel. 96 rows over 1700 positions: 11.2 us, pairs split in eight 13.4, ranges 20, pairs 36.
 //   Ranges: as many blocks of threads as run at once take ranges of equal cost out of the line of all pairs, and what a range cuts is joined
-//     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 166 us, tiles 202, pairs 220. The
+//     by a second kernel. Long caches and few pairs: 4 chunks of 500 to 1024 rows over 3000 to 9000 positions: 143 to 166 us, tiles 202, pairs 220. The
 //     second kernel and the parts cost about eight steps.
 // Pairs go longest first over all kv heads; where the keys and values do not fit the L2 cache, head after head, so that the blocks of threads that
 // run at a time read the same ones (4 chunks of 1500 to 2048 rows over 10 to 24 thousand positions, 32/8 heads of 128, 427 MB: 2820 us and

@@ -12,9 +12,9 @@
 // go out in 16-byte pieces as the masks leave them. Rows of one sequence (drafted rows) share counts and lists. The history is read by every
 // slice's block, from the cache but for the first: 4 bytes a token, four a load where it is aligned.
 //
-// Measured, in one graph, data from memory: 512 rows of 50257 bf16, four to a sequence of 4000 to 8000 tokens: 41 us for 108 MB, without the
-// history 27: 13 blocks look through each. 256 rows of 32768 f32 with histories of 1000 to 2000: 26.7 us for 69 MB, without the history
-// 19. From the cache: 39.8 and 20.9. What else was timed on the first, from the cache: a look into the table for every value that goes
+// Measured, in one graph, data from memory: 512 rows of 50257 bf16, four to a sequence of 4000 to 8000 tokens: 42 us for 108 MB, without the
+// history 27: 13 blocks look through each. 256 rows of 32768 f32 with histories of 1000 to 2000: 27.1 us for 69 MB, without the history
+// 19. From the cache: 40.6 and 21.3. What else was timed on the first, from the cache, where it then took 39.8: a look into the table for every value that goes
 // out 54 us, the few values put right in global memory behind the copy 78, all that it met on lists 44.4, tables of 2048 or 8192
 // tokens and blocks of 512 threads slower than that, all of the history in flight no faster, a cluster's blocks that share the history
 // and count in one another's tables 57. 64 rows of 4096 f32: 4.0 us, latency.
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GR
       for (int i = biased + lane; i < listed; i += 32)  // none in groups
         count(list[i] & ~kPrompt, list[i] & kPrompt);
       // The quotient by a product in 64 bits, off by 2^-52 of itself: as x / rep rounds it, since a quotient of 24-bit numbers is a border between two
-      // 32-bit values, or 2^-49 of itself away from one. (A product in 32 bits is rounded twice, and inf for a rep below 2^-128. The drafted rows, from the
+      // 32-bit values, which only one below 2^-126 can be and which then goes to either side, or 2^-49 of itself away from one. (A product in 32 bits is rounded twice, and inf for a rep below 2^-128. The drafted rows, from the
       // cache: 40.4 us, with it 39.4, with a division for each token 42.4; the 64 rows of 4096: 3.9, 3.9 and 4.3.)
       inv = 1.0 / (double)rep;
     }
@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(kLogThreadsOf<GROUPS>, 1024 / kLogThreadsOf<GR
 // Rows on their own: blocks of 128 threads, twice as many at a time, so that the steps of one run under the copies of others, and each
 // warp lists the history's tokens that it met, since a row meets few (256 rows of 32768 f32, all from the cache: 20.9 us; with 256 threads 24.3; looking for them
 // in the table 25.5). Groups: 256 threads, since four rows take the shared memory (512 rows of 50257 bf16: with 128 60 us), and
-// the tokens are looked for in the table, which costs a lane less than a list of all that it met (39.5 us, with such lists 44.4).
+// the tokens are looked for in the table, which costs a lane less than a list of all that it met (39.8 us, with such lists 44.4). All before the quotient by
+// a product in 64 bits, which costs 0.4 to 1.0.
 template <class T, bool WIDE, bool GROUPS>
 void LaunchLogitsAs(const LogitsArgs& a, int smem, cudaStream_t st) {
   if (!EnsureKernelAttrs((const void*)AdjustLogitsKernel<T, WIDE, GROUPS>, smem)) return;
