@@ -16,7 +16,7 @@ def adjust_logits(dtype: int, logits: int, out: int, rows: int, vocab: int, n: i
                   frequency: int = 0, bias_offsets: int = 0, bias_tokens: int = 0, bias_values: int = 0, bias_entries: int = 0,
                   masks: int = 0, mask_rows: int = 0, mask_count: int = 0, mask_stride: int | None = None,
                   logits_stride: int | None = None, out_stride: int | None = None, stream: int = 0) -> None:
-    """Rows of logits [rows, vocab] into out (which may be logits). A row belongs to sequence sequences[row] (its own number
+    """Rows of logits [rows, vocab] into out (which may be logits; else no row of it shares memory with one of them). A row belongs to sequence sequences[row] (its own number
     without them). A token of that sequence's history [n, history_stride] (prompt first) is divided by repetition where its logit
     is positive, else multiplied; one that was generated c times loses c * frequency + presence; biases (token, value entries
     bias_offsets[s] .. bias_offsets[s+1]-1) are added; tokens whose bit the row's mask [mask_count, mask_stride words] lacks become
